@@ -1,0 +1,566 @@
+// gfx950 kernels that write the 8-bit input of a projection, codes and scales:
+//   - add_rms_norm_quant: the RMSNorm in front of it, with the residual's
+//     addition:  h = round(x + residual),  y = h r w,  r = 1/sqrt(mean(h^2) + eps);
+//   - silu_mul_quant: the gated activation of a feed-forward block, of rows
+//     gate | up:  y = g / (1 + exp(-g)) * u.
+// int8 codes have one scale per row (for int8_scaled_mm), e4m3fn codes one per
+// 128 columns (for fp8_einsum):
+//   a = max |y| under the scale,  s = a / q  (q = 127 or 448),  code = RNE(q y / a).
+//
+// The codes are those of this definition in 64 bits, every one.  In the norm r
+// cancels, so a code is the rounded quotient q h w / max |h w| and needs no
+// sum.  The fast path works on v = h w (exact in binary32 for 16-bit weights)
+// or v = y within a relative 2^-20 (float32 weights 2^-24, the activation
+// 2^-21): t = v * (q / a) in binary32 is off by less than 2^-19.4 relative, so
+// a code can be wrong only where t lies that close to the border between two
+// codes.  Those elements, one in a few thousand, are computed again in binary64
+// (with a correctly rounded division) and their bytes overwritten.  The largest
+// magnitude is settled the same way: every element within 2^-18 of the
+// binary32 maximum is computed again in binary64.  Where the binary32 values
+// leave the range in which these bounds hold (a row of zeros, of values below
+// 2^-60 or above 2^120, gates below -60 under a huge up value, NaN, infinities),
+// all elements under the scale go that way.
+//
+// Bound by memory: 7 bytes per element with a residual (x, residual, hidden,
+// code), 3 without, 5 for the activation.  A row is read once and held in
+// registers; a thread holds P pieces of 8 elements, piece j at element
+// 8 (t + LANES j), so a wave's loads are 1 KiB contiguous, and 16 consecutive
+// threads hold the 128 columns of an e4m3fn scale.  Loads and stores assume no
+// alignment beyond the element's own, so rows of any stride and width take the
+// same code.
+#include "fgv_device.h"
+#include "fgv_host.h"
+
+namespace fgv {
+namespace {
+
+enum Op { kNorm = 0, kSilu = 1 };
+constexpr int kGroup = 128;       // columns under one e4m3fn scale
+constexpr int kMaxCols = 65536;   // 1024 threads x 8 pieces x 8 elements
+
+struct QuantArgs {
+    const uint16_t* x;         // norm: x[rows, cols]; silu: gate | up [rows, 2 cols]
+    int64_t x_stride;
+    const uint16_t* residual;  // or null
+    int64_t r_stride;
+    const void* w;             // norm weights
+    uint16_t* hidden;          // with a residual
+    int64_t h_stride;
+    uint8_t* codes;
+    int64_t c_stride;
+    float* scales;
+    int64_t s_stride;
+    int64_t rows;
+    int32_t cols;
+    double eps;
+};
+
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_a1 __attribute__((ext_vector_type(2), aligned(1)));
+
+// ---- 16-bit elements ----
+
+template <bool F16>
+__device__ __forceinline__ float elem(uint16_t bits) {
+    if constexpr (F16)
+        return (float)__builtin_bit_cast(_Float16, bits);
+    else
+        return __uint_as_float((uint32_t)bits << 16);
+}
+template <bool F16>
+__device__ __forceinline__ float lo_of(uint32_t w) {
+    return F16 ? elem<true>((uint16_t)w) : bf16_lo(w);
+}
+template <bool F16>
+__device__ __forceinline__ float hi_of(uint32_t w) {
+    return F16 ? elem<true>((uint16_t)(w >> 16)) : bf16_hi(w);
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (F16) {
+        const uint32_t l = __builtin_bit_cast(uint16_t, (_Float16)a), h = __builtin_bit_cast(uint16_t, (_Float16)b);
+        return l | (h << 16);
+    } else {
+        return pack_bf16x2(a, b);
+    }
+}
+
+// Eight elements from e0 on of a row that ends at cols (zeros behind it).
+__device__ __forceinline__ u32x4_t load_piece(const uint16_t* row, int e0, int cols) {
+    if (e0 + 8 <= cols)
+        return __builtin_nontemporal_load(reinterpret_cast<const u32x4_a2*>(row + e0));
+    u32x4_t v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (e0 + i < cols)
+            v[i >> 1] |= (uint32_t)row[e0 + i] << (16 * (i & 1));
+    return v;
+}
+__device__ __forceinline__ void store_piece(uint16_t* row, int e0, int cols, u32x4_t v) {
+    if (e0 + 8 <= cols) {
+        __builtin_nontemporal_store(v, reinterpret_cast<u32x4_a2*>(row + e0));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (e0 + i < cols)
+            row[e0 + i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+}
+__device__ __forceinline__ void store_codes(uint8_t* row, int e0, int cols, uint32_t lo, uint32_t hi) {
+    if (e0 + 8 <= cols) {
+        const u32x2_t v = {lo, hi};
+        *reinterpret_cast<u32x2_a1*>(row + e0) = v;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (e0 + i < cols)
+            row[e0 + i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+}
+
+// ---- the value that is quantised ----
+
+// silu(g) u in binary32, within a relative 2^-21: the exponent g log2(e) is
+// split into an integer and a fraction known to 2^-26, so that v_exp_f32's
+// argument keeps its low bits (one rounding of g log2(e) alone would cost
+// 2^-17 at g = -88).  The exponent stops at g = +-128, where the sigmoid is 1
+// or below binary32's range.
+__device__ __forceinline__ float silu_mul32(float g, float u) {
+    constexpr float kLog2e = 0x1.715476p0f, kLog2eLo = 0x1.4ae0cp-26f;  // log2(e) = their sum to 2^-49
+    const float x = __builtin_amdgcn_fmed3f(-g, -128.f, 128.f);
+    const float n = rintf(x * kLog2e);
+    const float f = fmaf(x, kLog2eLo, fmaf(x, kLog2e, -n));
+    const float e = __builtin_ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
+    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
+
+// Element e of the row in binary64.  h is read back from hidden where there
+// is a residual (this thread wrote it).
+template <int OP, bool F16, bool WF32>
+__device__ __forceinline__ double value64(const QuantArgs& a, int64_t row, int e) {
+    if constexpr (OP == kSilu) {
+        const uint16_t* x = a.x + row * a.x_stride;
+        const double g = elem<F16>(x[e]), u = elem<F16>(x[a.cols + e]);
+        return g / (1.0 + exp(-g)) * u;
+    } else {
+        const double h = elem<F16>(a.residual ? a.hidden[row * a.h_stride + e] : a.x[row * a.x_stride + e]);
+        const double w = WF32 ? reinterpret_cast<const float*>(a.w)[e]
+                              : elem<F16>(reinterpret_cast<const uint16_t*>(a.w)[e]);
+        return h * w;
+    }
+}
+
+// The int8 code of v under the largest magnitude `most` (0 for a row of zeros
+// or one that is not finite).
+__device__ __forceinline__ uint8_t code64_i8(double v, double most) {
+    if (!(most > 0.0 && most < HUGE_VAL))
+        return 0;
+    return (uint8_t)(int8_t)(int)rint(v * 127.0 / most);
+}
+// The e4m3fn code: the quotient is rounded to binary32 towards zero with the
+// lost part kept in the last bit (to odd), so that the second rounding, to
+// e4m3fn, is the only one that counts.
+__device__ __forceinline__ uint8_t code64_fp8(double v, double most) {
+    if (!(most > 0.0 && most < HUGE_VAL))
+        return 0;
+    const double q = v * 448.0 / most;
+    const float f = (float)q;
+    const double left = q - (double)f;
+    uint32_t bits = __float_as_uint(f);
+    if (left != 0.0) {
+        if ((left > 0.0) != (q > 0.0))
+            --bits;  // |f| > |q|
+        bits |= 1u;
+    }
+    return (uint8_t)(pack_fp8x4(__uint_as_float(bits), 0.f, 0.f, 0.f) & 0xffu);
+}
+
+// ---- reductions over the LANES threads of a row ----
+
+__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+    return (uint64_t)dpp_u32<CTRL>((uint32_t)v) | ((uint64_t)dpp_u32<CTRL>((uint32_t)(v >> 32)) << 32);
+}
+__device__ __forceinline__ uint64_t row16_max64(uint64_t v) {
+    v = max64(v, dpp_u64<kDppQuadXor1>(v));
+    v = max64(v, dpp_u64<kDppQuadXor2>(v));
+    v = max64(v, dpp_u64<kDppHalfMirror>(v));
+    v = max64(v, dpp_u64<kDppMirror>(v));
+    return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = row16_sum(v);
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = row16_max(v);
+    v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+    return max(v, (uint32_t)__shfl_xor((int)v, 32));
+}
+__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
+    v = row16_max64(v);
+    v = max64(v, (uint64_t)__shfl_xor((unsigned long long)v, 16));
+    return max64(v, (uint64_t)__shfl_xor((unsigned long long)v, 32));
+}
+
+// binary32 magnitudes between these (as bits) keep the fast path's bounds
+constexpr uint32_t kLeast = (127 - 60) << 23, kMost = (127 + 120) << 23;
+constexpr float kNearMost = 1.0f - 0x1p-18f;  // nearer to the maximum than this: settled in binary64
+// distance from the next code at which a code counts as beside a border: int8
+// 0.5 - 2^-12 of a step (127 * 2^-19.4 < 2^-12); e4m3fn 0.5 - 2^-14 of a step,
+// at most 16 steps to a value (16 * 2^-19.4 < 2^-15)
+constexpr float kBorderI8 = 0.5f - 0x1p-12f, kBorderFp8 = 0.5f - 0x1p-14f;
+
+// One row per LANES threads (64: four rows to a workgroup; else one).
+template <int OP, bool F16, bool WF32, bool FP8, int LANES, int P>
+__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) act_quant_kernel(QuantArgs a) {
+    constexpr int kBlock = LANES < 256 ? 256 : LANES, kWaves = LANES / 64;
+    constexpr bool kRowScale = !FP8;                       // one scale per row, else per 16 threads and piece
+    constexpr bool kExact32 = OP == kNorm && !WF32;        // v is exact
+    __shared__ double sum_of[kWaves];
+    __shared__ uint32_t max_of[kWaves];
+    __shared__ unsigned long long best_of;
+
+    const int64_t row = (int64_t)blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
+    if (row >= a.rows)
+        return;  // (only where waves are rows: no barrier below)
+    const int t = threadIdx.x % LANES, cols = a.cols;
+    const uint16_t* xrow = a.x + row * a.x_stride;
+    uint8_t* crow = a.codes + row * a.c_stride;
+
+    // ---- one pass over the row: v, the sum of squares, the largest magnitude ----
+    float v[P][8];
+    double ss = 0.0;
+    uint32_t mx[P];
+    {
+        u32x4_t p0[P], p1[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int e0 = 8 * (t + LANES * j);
+            p0[j] = load_piece(xrow, e0, cols);
+            if constexpr (OP == kSilu)
+                p1[j] = load_piece(xrow + cols, e0, cols);
+            else if (a.residual)
+                p1[j] = load_piece(a.residual + row * a.r_stride, e0, cols);
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int e0 = 8 * (t + LANES * j);
+            mx[j] = 0;
+            if constexpr (OP == kSilu) {
+                float least = 0.f, widest = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float g = i & 1 ? hi_of<F16>(p0[j][i >> 1]) : lo_of<F16>(p0[j][i >> 1]);
+                    const float u = i & 1 ? hi_of<F16>(p1[j][i >> 1]) : lo_of<F16>(p1[j][i >> 1]);
+                    v[j][i] = silu_mul32(g, u);
+                    mx[j] = max(mx[j], __float_as_uint(fabsf(v[j][i])));
+                    least = fminf(least, g);
+                    widest = fmaxf(widest, fabsf(u));
+                }
+                // below, exp(-g) may pass binary32's range under an up value that brings the product back
+                if (least < -60.f && widest > 0x1p20f)
+                    mx[j] = 0x7fffffffu;
+            } else {
+                if (a.residual) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        p0[j][q] = pack2<F16>(lo_of<F16>(p0[j][q]) + lo_of<F16>(p1[j][q]),
+                                              hi_of<F16>(p0[j][q]) + hi_of<F16>(p1[j][q]));
+                    store_piece(a.hidden + row * a.h_stride, e0, cols, p0[j]);
+                }
+                float w[8];
+                if constexpr (WF32) {
+                    const float* wp = reinterpret_cast<const float*>(a.w) + e0;
+                    if (e0 + 8 <= cols) {
+                        const f32x4_a4 lo = *reinterpret_cast<const f32x4_a4*>(wp);
+                        const f32x4_a4 hi = *reinterpret_cast<const f32x4_a4*>(wp + 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            w[i] = lo[i];
+                            w[4 + i] = hi[i];
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            w[i] = e0 + i < cols ? wp[i] : 0.f;
+                    }
+                } else {
+                    u32x4_t wp = {0, 0, 0, 0};
+                    const uint16_t* w16 = reinterpret_cast<const uint16_t*>(a.w);
+                    if (e0 + 8 <= cols)
+                        wp = *reinterpret_cast<const u32x4_a2*>(w16 + e0);
+                    else
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (e0 + i < cols)
+                                wp[i >> 1] |= (uint32_t)w16[e0 + i] << (16 * (i & 1));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        w[i] = i & 1 ? hi_of<F16>(wp[i >> 1]) : lo_of<F16>(wp[i >> 1]);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float h = i & 1 ? hi_of<F16>(p0[j][i >> 1]) : lo_of<F16>(p0[j][i >> 1]);
+                    ss = fma((double)h, (double)h, ss);  // (the square is exact)
+                    v[j][i] = h * w[i];
+                    mx[j] = max(mx[j], __float_as_uint(fabsf(v[j][i])));
+                }
+            }
+        }
+    }
+
+    // ---- the row's sum, and its largest magnitude where it has one scale ----
+    if constexpr (OP == kNorm || kRowScale) {
+        uint32_t m = mx[0];
+#pragma unroll
+        for (int j = 1; j < P; ++j)
+            m = max(m, mx[j]);
+        if constexpr (OP == kNorm)
+            ss = wave_sum(ss);
+        if constexpr (kRowScale)
+            m = wave_max(m);
+        if constexpr (kWaves > 1) {
+            if ((threadIdx.x & 63) == 0) {
+                sum_of[threadIdx.x >> 6] = ss;
+                max_of[threadIdx.x >> 6] = m;
+            }
+            if (threadIdx.x == 0)
+                best_of = 0;
+            __syncthreads();
+            ss = sum_of[0];
+            m = max_of[0];
+#pragma unroll
+            for (int i = 1; i < kWaves; ++i) {
+                ss += sum_of[i];
+                m = max(m, max_of[i]);
+            }
+        }
+        if constexpr (kRowScale)
+            mx[0] = m;
+    }
+    double r = 1.0;
+    if constexpr (OP == kNorm) {
+        r = 1.0 / sqrt(ss / cols + a.eps);
+        if (!(ss < HUGE_VAL))
+            r = __builtin_nan("");  // a NaN or an infinity in the row
+    }
+
+    if constexpr (kRowScale) {
+        // ---- int8: one scale per row ----
+        const bool odd = !(mx[0] >= kLeast && mx[0] <= kMost);  // (the same in all threads of the row)
+        double most = __uint_as_float(mx[0]);
+        if (!kExact32 || odd) {
+            const float from = odd ? 0.f : __uint_as_float(mx[0]) * kNearMost;
+            uint64_t mask = 0, best = 0;
+#pragma unroll
+            for (int j = 0; j < P; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (8 * (t + LANES * j) + i < cols && (odd || fabsf(v[j][i]) >= from))
+                        mask |= 1ull << (8 * j + i);
+            while (mask) {
+                const int at = __builtin_ctzll(mask);
+                mask &= mask - 1;
+                const double y = fabs(value64<OP, F16, WF32>(a, row, 8 * (t + LANES * (at >> 3)) + (at & 7)));
+                best = max64(best, __builtin_bit_cast(uint64_t, y));  // (a NaN is above all)
+            }
+            best = wave_max64(best);
+            if constexpr (kWaves > 1) {
+                if ((threadIdx.x & 63) == 0 && best)
+                    atomicMax(&best_of, (unsigned long long)best);
+                __syncthreads();
+                best = best_of;
+            }
+            most = __builtin_bit_cast(double, best);
+        }
+        const bool finite = most < HUGE_VAL;
+        if (t == 0)
+            a.scales[row * a.s_stride] = finite ? (float)(most * r / 127.0) : __builtin_nanf("");
+        const float inv = (float)(127.0 / most);
+        uint64_t near = 0;
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int e0 = 8 * (t + LANES * j);
+            uint32_t m[8];
+            uint32_t mask = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low byte is the rounded value's
+                const float q = v[j][i] * inv, s = q + kMagic;
+                m[i] = __float_as_uint(s);
+                mask |= fabsf(q - (s - kMagic)) > kBorderI8 ? 1u << i : 0u;
+            }
+            const uint32_t lo = __builtin_amdgcn_perm(__builtin_amdgcn_perm(m[3], m[2], 0x0c0c0400u),
+                                                      __builtin_amdgcn_perm(m[1], m[0], 0x0c0c0400u), 0x05040100u);
+            const uint32_t hi = __builtin_amdgcn_perm(__builtin_amdgcn_perm(m[7], m[6], 0x0c0c0400u),
+                                                      __builtin_amdgcn_perm(m[5], m[4], 0x0c0c0400u), 0x05040100u);
+            store_codes(crow, e0, cols, lo, hi);
+            if (odd) {
+                const int left = cols - e0;
+                mask = left >= 8 ? 0xffu : left > 0 ? (1u << left) - 1 : 0u;
+            }
+            near |= (uint64_t)mask << (8 * j);
+        }
+        while (near) {
+            const int at = __builtin_ctzll(near);
+            near &= near - 1;
+            const int e = 8 * (t + LANES * (at >> 3)) + (at & 7);
+            crow[e] = code64_i8(value64<OP, F16, WF32>(a, row, e), most);
+        }
+    } else {
+        // ---- e4m3fn: one scale per 16 threads and piece (cols a multiple of 128: a group is whole or absent) ----
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int e0 = 8 * (t + LANES * j);
+            if (e0 >= cols)
+                continue;
+            const uint32_t m = row16_max(mx[j]);
+            const bool odd = !(m >= kLeast && m <= kMost);  // (the same in the 16 threads)
+            double most = __uint_as_float(m);
+            if (!kExact32 || odd) {
+                const float from = __uint_as_float(m) * kNearMost;
+                uint32_t mask = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    mask |= odd || fabsf(v[j][i]) >= from ? 1u << i : 0u;
+                uint64_t best = 0;
+                while (mask) {
+                    const int at = __builtin_ctz(mask);
+                    mask &= mask - 1;
+                    best = max64(best, __builtin_bit_cast(uint64_t, fabs(value64<OP, F16, WF32>(a, row, e0 + at))));
+                }
+                most = __builtin_bit_cast(double, row16_max64(best));
+            }
+            const bool finite = most < HUGE_VAL;
+            if ((t & 15) == 0)
+                a.scales[row * a.s_stride + e0 / kGroup] = finite ? (float)(most * r / 448.0) : __builtin_nanf("");
+            const float inv = (float)(448.0 / most);
+            uint32_t near = 0;
+            float q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                q[i] = v[j][i] * inv;
+                // in steps of e4m3fn at this magnitude: 8 to a binade, 2^-9 below 2^-6
+                const int e = max(__builtin_amdgcn_frexp_expf(q[i]), -5);
+                const float k = __builtin_ldexpf(q[i], 4 - e);
+                near |= fabsf(k - rintf(k)) > kBorderFp8 ? 1u << i : 0u;
+            }
+            store_codes(crow, e0, cols, pack_fp8x4(q[0], q[1], q[2], q[3]), pack_fp8x4(q[4], q[5], q[6], q[7]));
+            if (odd)
+                near = 0xffu;
+            while (near) {
+                const int at = __builtin_ctz(near);
+                near &= near - 1;
+                crow[e0 + at] = code64_fp8(value64<OP, F16, WF32>(a, row, e0 + at), most);
+            }
+        }
+    }
+}
+
+template <int OP, bool F16, bool WF32, bool FP8, int LANES, int P>
+void launch(const QuantArgs& a, hipStream_t st) {
+    constexpr int kRows = LANES < 256 ? 256 / LANES : 1;
+    hipLaunchKernelGGL((act_quant_kernel<OP, F16, WF32, FP8, LANES, P>), dim3((unsigned)((a.rows + kRows - 1) / kRows)),
+                       dim3(kRows * LANES), 0, st, a);
+}
+
+template <int OP, bool F16, bool WF32, bool FP8>
+int launch_cols(const QuantArgs& a, hipStream_t st) {
+    const int pieces = (a.cols + 7) / 8;
+    if (pieces <= 64)
+        launch<OP, F16, WF32, FP8, 64, 1>(a, st);
+    else if (pieces <= 128)
+        launch<OP, F16, WF32, FP8, 64, 2>(a, st);
+    else if (pieces <= 256)
+        launch<OP, F16, WF32, FP8, 64, 4>(a, st);
+    else if (pieces <= 512)
+        launch<OP, F16, WF32, FP8, 256, 2>(a, st);
+    else if (pieces <= 1024)
+        launch<OP, F16, WF32, FP8, 256, 4>(a, st);
+    else if (pieces <= 2048)
+        launch<OP, F16, WF32, FP8, 512, 4>(a, st);
+    else if (pieces <= 4096)
+        launch<OP, F16, WF32, FP8, 1024, 4>(a, st);
+    else
+        launch<OP, F16, WF32, FP8, 1024, 8>(a, st);
+    return launch_status();
+}
+
+int check_common(const QuantArgs& a, int x_dtype, int code_dtype) {
+    if (a.rows < 0 || a.cols <= 0)
+        return fail(FGV_E_BAD_SHAPE, "rows must not be negative and cols positive");
+    if (a.rows > 0x7fffffffLL || a.cols > kMaxCols)
+        return fail(FGV_E_TOO_LARGE, "at most 2^31 - 1 rows of 65536 columns");
+    if ((x_dtype != 0 && x_dtype != 1) || (code_dtype != 0 && code_dtype != 1))
+        return fail(FGV_E_BAD_SHAPE, "x_dtype must be 0 (bf16) or 1 (fp16), code_dtype 0 (int8) or 1 (e4m3fn)");
+    if (code_dtype == 1 && a.cols % kGroup)
+        return fail(FGV_E_BAD_SHAPE, "e4m3fn codes need cols to be a multiple of 128");
+    return FGV_OK;
+}
+
+}  // namespace
+}  // namespace fgv
+
+extern "C" int fgv_add_rms_norm_quant(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                                      const void* weight, int32_t weight_is_fp32, void* hidden, int64_t hidden_stride,
+                                      void* codes, int64_t codes_stride, float* scales, int64_t scales_stride,
+                                      int64_t rows, int64_t cols, double eps, int32_t x_dtype, int32_t code_dtype,
+                                      void* stream) {
+    using namespace fgv;
+    if (cols > kMaxCols)
+        return fail(FGV_E_TOO_LARGE, "at most 2^31 - 1 rows of 65536 columns");
+    const QuantArgs a{static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(residual), residual_stride,
+                      weight, static_cast<uint16_t*>(hidden), hidden_stride, static_cast<uint8_t*>(codes), codes_stride,
+                      scales, scales_stride, rows, (int32_t)cols, eps};
+    if (const int rc = check_common(a, x_dtype, code_dtype))
+        return rc;
+    if (!(eps > 0.0))
+        return fail(FGV_E_BAD_SHAPE, "eps must be positive");
+    if (rows == 0)
+        return FGV_OK;
+    if (!x || !weight || !codes || !scales || (residual && !hidden))
+        return fail(FGV_E_NULL_POINTER, "null tensor");
+    if (!aligned(x, 2) || !aligned(residual, 2) || !aligned(hidden, 2) || !aligned(weight, weight_is_fp32 ? 4 : 2) ||
+        !aligned(scales, 4))
+        return fail(FGV_E_MISALIGNED, "tensors must be aligned to their element size");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (x_dtype == 0) {
+        if (code_dtype == 0)
+            return weight_is_fp32 ? launch_cols<kNorm, false, true, false>(a, st)
+                                  : launch_cols<kNorm, false, false, false>(a, st);
+        return weight_is_fp32 ? launch_cols<kNorm, false, true, true>(a, st)
+                              : launch_cols<kNorm, false, false, true>(a, st);
+    }
+    if (code_dtype == 0)
+        return weight_is_fp32 ? launch_cols<kNorm, true, true, false>(a, st)
+                              : launch_cols<kNorm, true, false, false>(a, st);
+    return weight_is_fp32 ? launch_cols<kNorm, true, true, true>(a, st) : launch_cols<kNorm, true, false, true>(a, st);
+}
+
+extern "C" int fgv_silu_mul_quant(const void* x, int64_t x_stride, void* codes, int64_t codes_stride, float* scales,
+                                  int64_t scales_stride, int64_t rows, int64_t cols, int32_t x_dtype,
+                                  int32_t code_dtype, void* stream) {
+    using namespace fgv;
+    if (cols > kMaxCols)
+        return fail(FGV_E_TOO_LARGE, "at most 2^31 - 1 rows of 65536 columns");
+    const QuantArgs a{static_cast<const uint16_t*>(x), x_stride, nullptr, 0, nullptr, nullptr, 0,
+                      static_cast<uint8_t*>(codes), codes_stride, scales, scales_stride, rows, (int32_t)cols, 0.0};
+    if (const int rc = check_common(a, x_dtype, code_dtype))
+        return rc;
+    if (rows == 0)
+        return FGV_OK;
+    if (!x || !codes || !scales)
+        return fail(FGV_E_NULL_POINTER, "null tensor");
+    if (!aligned(x, 2) || !aligned(scales, 4))
+        return fail(FGV_E_MISALIGNED, "tensors must be aligned to their element size");
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (x_dtype == 0)
+        return code_dtype == 0 ? launch_cols<kSilu, false, false, false>(a, st)
+                               : launch_cols<kSilu, false, false, true>(a, st);
+    return code_dtype == 0 ? launch_cols<kSilu, true, false, false>(a, st)
+                           : launch_cols<kSilu, true, false, true>(a, st);
+}

@@ -5,7 +5,9 @@
 //     src/flaggems_vllm/ops/fused_inv_rope_fp8_quant.py:157-256)
 // and of the five ops beside them (fused_q_kv_rmsnorm,
 // dequantize_and_gather_k_cache, fused_indexer_q_rope_quant,
-// compute_slot_mapping_parallel, indexer_k_quant_and_cache).
+// compute_slot_mapping_parallel, indexer_k_quant_and_cache) and the 8-bit
+// linear ops around the layer (fused_add_rms_norm_quant,
+// fused_silu_mul_quant, int8_scaled_mm), which have no counterpart there.
 //
 // The argument checks, the output allocation and the launch run here in C++,
 // so an eager call costs a few microseconds of host time instead of the
@@ -18,8 +20,8 @@
 //   - the dispatcher ops torch.ops.flaggems_vllm.<name> (TORCH_LIBRARY_FRAGMENT;
 //     schemas mark q and k_cache written), for torch.compile and graph capture.
 //     These raise RuntimeError on any failure, as vLLM's own compiled op does.
-// The other five are module functions only; their torch.ops registrations
-// call the Python drop-ins.
+// The others are module functions only; their torch.ops registrations
+// call the Python wrappers.
 // Launches go on torch's current HIP stream of the tensors' device; nothing
 // synchronises and nothing is read back from the device.
 #include <torch/extension.h>
@@ -28,8 +30,10 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <optional>
 #include <string>
 #include <tuple>
+#include <utility>
 
 #include "flaggems_vllm_amd.h"
 
@@ -385,6 +389,182 @@ int slot_mapping(int64_t num_tokens, int64_t max_num_tokens, const at::Tensor& q
                                     cp_interleave, pad_id, current_stream(slot_mapping_out));
 }
 
+// ---- the 8-bit linear ops: norm or activation to codes and scales, int8 product ----
+
+bool takes_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+bool unit_rows(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1; }
+
+// Bytes [first, last) that a tensor of at least one element spans.
+std::pair<uintptr_t, uintptr_t> span_of(const at::Tensor& t) {
+    const auto first = reinterpret_cast<uintptr_t>(t.data_ptr());
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d)
+        last += (t.size(d) - 1) * t.stride(d);
+    return {first, first + (last + 1) * t.element_size()};
+}
+
+bool spans_meet(const at::Tensor& a, const at::Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0)
+        return false;
+    const auto x = span_of(a), y = span_of(b);
+    return x.first < y.second && y.first < x.second;
+}
+
+// Whether rows of `to` (2-D, the shape and type of `from`) may be written while
+// those of `from` are read row by row: the same rows, rows side by side in one
+// wider buffer, or other memory.
+bool rows_apart_or_same(const at::Tensor& to, const at::Tensor& from) {
+    if (!spans_meet(to, from))
+        return true;
+    const int64_t rows = to.size(0), cols = to.size(1);
+    if (to.data_ptr() == from.data_ptr())
+        return rows <= 1 || to.stride(0) == from.stride(0);
+    if (rows <= 1 || to.stride(0) != from.stride(0))
+        return false;
+    const int64_t size = to.element_size(), step = to.stride(0) * size;
+    int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(to.data_ptr()) -
+                                       reinterpret_cast<uintptr_t>(from.data_ptr())) % step;
+    if (off < 0)
+        off += step;
+    return off >= cols * size && step - off >= cols * size;
+}
+
+constexpr int64_t kQuantGroup = 128;
+constexpr int64_t kQuantMaxCols = 65536;
+
+// Checks that both producers share, and their outputs: codes [rows, cols] and
+// scales [rows, 1] (int8) or [rows, cols / 128] (e4m3fn).
+int quant_outputs(const at::Tensor& x, int64_t cols, bool int8, at::Tensor* codes, at::Tensor* scales) {
+    FGV_ASSERT(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "x must be bfloat16 or float16");
+    FGV_ASSERT(cols >= 1 && cols <= kQuantMaxCols, "rows must have 1 to 65536 columns to quantise");
+    FGV_ASSERT(int8 || cols % kQuantGroup == 0, "float8_e4m3fn codes need a multiple of 128 columns");
+    FGV_ASSERT(unit_rows(x), "x's rows must be contiguous");
+    FGV_ASSERT(x.is_cuda(), "flaggems_vllm runs on the GPU (HIP) only");
+    const int64_t rows = x.size(0);
+    *codes = at::empty({rows, cols}, x.options().dtype(int8 ? at::kChar : at::kFloat8_e4m3fn));
+    *scales = at::empty({rows, int8 ? 1 : cols / kQuantGroup}, x.options().dtype(at::kFloat));
+    return 0;
+}
+
+using NormQuantOut = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+
+int add_rms_norm_quant(const at::Tensor& x, const std::optional<at::Tensor>& residual, const at::Tensor& weight,
+                       double eps, bool int8, const std::optional<at::Tensor>& hidden_out, NormQuantOut* out) {
+    FGV_ASSERT(x.dim() == 2, "x must be 2D [num_tokens, size]");
+    FGV_ASSERT(!takes_grad(x) && !takes_grad(weight) && !(residual && takes_grad(*residual)),
+               "inference only: no input may require a gradient");
+    const int64_t rows = x.size(0), cols = x.size(1);
+    FGV_ASSERT(weight.dim() == 1 && weight.size(0) == cols && weight.is_contiguous(),
+               "weight must be [size] and contiguous");
+    FGV_ASSERT(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat,
+               "weight must have x's type or float32");
+    FGV_ASSERT(eps > 0.0, "eps must be positive");
+    FGV_ASSERT(residual || !hidden_out, "hidden_out needs a residual");
+    FGV_ASSERT(weight.device() == x.device(), "all tensors must be on x's device");
+    if (residual) {
+        FGV_ASSERT(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(),
+                   "residual must have x's shape and type");
+        FGV_ASSERT(unit_rows(*residual), "residual's rows must be contiguous");
+        FGV_ASSERT(residual->device() == x.device(), "all tensors must be on x's device");
+    }
+    if (hidden_out) {
+        const at::Tensor& h = *hidden_out;
+        FGV_ASSERT(h.sizes() == x.sizes() && h.scalar_type() == x.scalar_type() && h.device() == x.device(),
+                   "hidden_out must have x's shape, type and device");
+        FGV_ASSERT(!takes_grad(h), "inference only: no output may require a gradient");
+        FGV_ASSERT(unit_rows(h) && (rows <= 1 || h.stride(0) >= cols),
+                   "hidden_out's rows must be contiguous and apart");
+        FGV_ASSERT(rows_apart_or_same(h, x) && rows_apart_or_same(h, *residual) && !spans_meet(h, weight),
+                   "hidden_out must be x or residual itself, or apart from every input");
+    }
+    at::Tensor codes, scales;
+    if (const int rc = quant_outputs(x, cols, int8, &codes, &scales))
+        return rc;
+    const at::Tensor hidden =
+        hidden_out ? *hidden_out : residual ? at::empty({rows, cols}, x.options()) : x;
+    *out = NormQuantOut(codes, scales, hidden);
+    const c10::DeviceGuard guard(x.device());
+    return fgv_add_rms_norm_quant(x.data_ptr(), x.stride(0), residual ? residual->data_ptr() : nullptr,
+                                  residual ? residual->stride(0) : 0, weight.data_ptr(),
+                                  weight.scalar_type() == at::kFloat ? 1 : 0, residual ? hidden.data_ptr() : nullptr,
+                                  residual ? hidden.stride(0) : 0, codes.data_ptr(), codes.stride(0),
+                                  scales.data_ptr<float>(), scales.stride(0), rows, cols, eps,
+                                  x.scalar_type() == at::kHalf ? 1 : 0, int8 ? 0 : 1, current_stream(x));
+}
+
+int silu_mul_quant(const at::Tensor& x, bool int8, TensorPair* out) {
+    FGV_ASSERT(x.dim() == 2 && x.size(1) % 2 == 0, "x must be 2D [num_tokens, 2 * size], gate beside up");
+    FGV_ASSERT(!takes_grad(x), "inference only: no input may require a gradient");
+    const int64_t cols = x.size(1) / 2;
+    at::Tensor codes, scales;
+    if (const int rc = quant_outputs(x, cols, int8, &codes, &scales))
+        return rc;
+    *out = TensorPair(codes, scales);
+    const c10::DeviceGuard guard(x.device());
+    return fgv_silu_mul_quant(x.data_ptr(), x.stride(0), codes.data_ptr(), codes.stride(0), scales.data_ptr<float>(),
+                              scales.stride(0), x.size(0), cols, x.scalar_type() == at::kHalf ? 1 : 0, int8 ? 0 : 1,
+                              current_stream(x));
+}
+
+int out_code(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat ? 2 : -1; }
+
+// The stride of n scales given as [n], [n, 1], [1, n] or one scale for all (0); -1: none of these.
+int64_t scale_stride(const at::Tensor& s, int64_t n) {
+    if (s.dim() > 2 || s.scalar_type() != at::kFloat)
+        return -1;
+    if (s.numel() == 1)
+        return 0;
+    if (s.numel() != n)
+        return -1;
+    if (s.dim() == 1)
+        return s.stride(0);
+    return s.size(0) == n ? s.stride(0) : s.size(1) == n ? s.stride(1) : -1;
+}
+
+int int8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale_a, const at::Tensor& scale_b,
+            const std::optional<at::Tensor>& bias, at::ScalarType out_dtype, const std::optional<at::Tensor>& out_in,
+            at::Tensor* result) {
+    FGV_ASSERT(a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(1), "a must be [M, K] and b [N, K]");
+    FGV_ASSERT(a.scalar_type() == at::kChar && b.scalar_type() == at::kChar, "a and b must be int8");
+    const int64_t m = a.size(0), n = b.size(0), k = a.size(1);
+    FGV_ASSERT(unit_rows(a) && unit_rows(b), "a's and b's rows must be contiguous");
+    const int64_t sa = scale_stride(scale_a, m), sb = scale_stride(scale_b, n);
+    FGV_ASSERT(sa >= 0 && (scale_a.numel() == 1 || scale_a.dim() == 1 || scale_a.size(0) == m),
+               "scale_a must be float32: [M], [M, 1] or one scale");
+    FGV_ASSERT(sb >= 0, "scale_b must be float32: [N], [N, 1], [1, N] or one scale");
+    FGV_ASSERT(out_code(out_dtype) >= 0, "out_dtype must be bfloat16, float16 or float32");
+    FGV_ASSERT(!takes_grad(scale_a) && !takes_grad(scale_b) && !(bias && takes_grad(*bias)),
+               "inference only: no input may require a gradient");
+    const c10::Device dev = a.device();
+    FGV_ASSERT(b.device() == dev && scale_a.device() == dev && scale_b.device() == dev &&
+                   (!bias || bias->device() == dev) && (!out_in || out_in->device() == dev),
+               "all tensors must be on a's device");
+    if (bias) {
+        FGV_ASSERT(bias->dim() == 1 && bias->size(0) == n && bias->is_contiguous(), "bias must be [N] and contiguous");
+        FGV_ASSERT(bias->scalar_type() == at::kFloat || bias->scalar_type() == out_dtype,
+                   "bias must be float32 or have the output's type");
+    }
+    if (out_in) {
+        const at::Tensor& o = *out_in;
+        FGV_ASSERT(o.dim() == 2 && o.size(0) == m && o.size(1) == n && o.scalar_type() == out_dtype,
+                   "out must be [M, N] of out_dtype");
+        FGV_ASSERT(!takes_grad(o), "inference only: no output may require a gradient");
+        FGV_ASSERT(unit_rows(o) && (m <= 1 || o.stride(0) >= n), "out's rows must be contiguous and apart");
+        FGV_ASSERT(!spans_meet(o, a) && !spans_meet(o, b) && !spans_meet(o, scale_a) && !spans_meet(o, scale_b) &&
+                       !(bias && spans_meet(o, *bias)),
+                   "out must not overlap an input");
+    }
+    FGV_ASSERT(dev.is_cuda(), "flaggems_vllm runs on the GPU (HIP) only");
+    const at::Tensor out = out_in ? *out_in : at::empty({m, n}, a.options().dtype(out_dtype));
+    *result = out;
+    const c10::DeviceGuard guard(dev);
+    return fgv_int8_scaled_mm(a.data_ptr<int8_t>(), a.stride(0), b.data_ptr<int8_t>(), b.stride(0),
+                              scale_a.data_ptr<float>(), sa, scale_b.data_ptr<float>(), sb,
+                              bias ? bias->data_ptr() : nullptr, bias ? out_code(bias->scalar_type()) : 0,
+                              out.data_ptr(), out.stride(0), m, n, k, out_code(out_dtype), current_stream(a));
+}
+
 // ---- dispatcher ops: the same functions, failures raised as RuntimeError ----
 
 void raise_on_status(int rc, const char* op) {
@@ -433,8 +613,8 @@ TORCH_LIBRARY_IMPL(flaggems_vllm, CUDA, m) {
 
 PYBIND11_MODULE(_fgv_torch, m) {
     m.doc() = "C++ checks and launches of fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert, "
-              "fused_inv_rope_fp8_quant and the five ops beside them (status-returning; the Python drop-ins map "
-              "the status)";
+              "fused_inv_rope_fp8_quant, the five ops beside them and the 8-bit linear ops (status-returning; the "
+              "Python wrappers map the status)";
     m.attr("ASSERT_FAILED") = kAssertFailed;
     m.def("qnorm_rope_kv_insert", &qnorm_rope_kv_insert);
     m.def("inv_rope_fp8_quant",
@@ -465,5 +645,24 @@ PYBIND11_MODULE(_fgv_torch, m) {
           });
     m.def("slot_mapping", &slot_mapping);
     m.def("indexer_k_quant", &indexer_k_quant);
+    m.def("add_rms_norm_quant",
+          [](const at::Tensor& x, const std::optional<at::Tensor>& residual, const at::Tensor& weight, double eps,
+             bool int8, const std::optional<at::Tensor>& hidden_out) {
+              NormQuantOut out;
+              const int rc = add_rms_norm_quant(x, residual, weight, eps, int8, hidden_out, &out);
+              return std::make_tuple(rc, std::get<0>(out), std::get<1>(out), std::get<2>(out));
+          });
+    m.def("silu_mul_quant", [](const at::Tensor& x, bool int8) {
+        TensorPair out;
+        const int rc = silu_mul_quant(x, int8, &out);
+        return std::make_tuple(rc, std::get<0>(out), std::get<1>(out));
+    });
+    m.def("int8_mm", [](const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale_a, const at::Tensor& scale_b,
+                        const std::optional<at::Tensor>& bias, at::ScalarType out_dtype,
+                        const std::optional<at::Tensor>& out_in) {
+        at::Tensor out;
+        const int rc = int8_mm(a, b, scale_a, scale_b, bias, out_dtype, out_in, &out);
+        return std::make_tuple(rc, out);
+    });
     m.def("assert_message", []() { return g_assert_message; });
 }

@@ -8,7 +8,9 @@ and the ops either side of that path (src/flaggems_vllm/ops/__init__.py): the
 K-cache gather, q/kv RMSNorm, the sparse indexer (q quant, key cache and
 logits and their top-k per row), the index rows sparse attention reads (global
 top-k indices, top-k plus sliding window), slot mapping, sparse MLA decode, sparse MLA prefill
-(``flash_mla_sparse_fwd``) and the block-FP8 grouped output projection (``fp8_einsum``) after the sibling op.  Every op runs hand-written HIP kernels through the C ABI declared in
+(``flash_mla_sparse_fwd``) and the block-FP8 grouped output projection (``fp8_einsum``) after the sibling op.  The 8-bit linear ops around the layer (``fused_add_rms_norm_quant``,
+``fused_silu_mul_quant``, ``int8_scaled_mm``) have no counterpart in the reference package's
+exports used here.  Every op runs hand-written HIP kernels through the C ABI declared in
 include/flaggems_vllm_amd.h; there is no Triton, no vendor dispatch and no
 CPU fallback.
 """
@@ -26,12 +28,15 @@ from .ops import (  # noqa: F401
     fp8_einsum,
     fp8_fp4_mqa_logits,
     fp8_fp4_paged_mqa_logits,
+    fused_add_rms_norm_quant,
     fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert,
     fused_indexer_q_rope_quant,
     fused_inv_rope_fp8_quant,
     fused_q_kv_rmsnorm,
+    fused_silu_mul_quant,
     get_mla_metadata,
     indexer_k_quant_and_cache,
+    int8_scaled_mm,
     persistent_topk,
     top_k_per_row_decode,
     top_k_per_row_prefill,
@@ -59,7 +64,10 @@ __all__ = [
     "fp8_fp4_paged_mqa_logits",
     "get_mla_metadata",
     "dequantize_and_gather_k_cache",
+    "fused_add_rms_norm_quant",
     "fused_q_kv_rmsnorm",
+    "fused_silu_mul_quant",
+    "int8_scaled_mm",
     "fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert",
     "fused_indexer_q_rope_quant",
     "fused_inv_rope_fp8_quant",

@@ -308,6 +308,26 @@ def lib():
         _P, _I64, _I64,  # cu_seqlen, batch_size, num_tokens
         _P,  # stream
     ]
+    L.fgv_add_rms_norm_quant.restype = ctypes.c_int
+    L.fgv_add_rms_norm_quant.argtypes = [
+        _P, _I64, _P, _I64,  # x, stride, residual, stride
+        _P, ctypes.c_int32, _P, _I64,  # weight, weight_is_fp32, hidden, stride
+        _P, _I64, _P, _I64,  # codes, stride, scales, stride
+        _I64, _I64, ctypes.c_double,  # rows, cols, eps
+        ctypes.c_int32, ctypes.c_int32, _P,  # x_dtype, code_dtype, stream
+    ]
+    L.fgv_silu_mul_quant.restype = ctypes.c_int
+    L.fgv_silu_mul_quant.argtypes = [
+        _P, _I64, _P, _I64, _P, _I64,  # x, stride, codes, stride, scales, stride
+        _I64, _I64, ctypes.c_int32, ctypes.c_int32, _P,  # rows, cols, x_dtype, code_dtype, stream
+    ]
+    L.fgv_int8_scaled_mm.restype = ctypes.c_int
+    L.fgv_int8_scaled_mm.argtypes = [
+        _P, _I64, _P, _I64,  # a, stride, b, stride (bytes)
+        _P, _I64, _P, _I64,  # scale_a, stride, scale_b, stride
+        _P, ctypes.c_int32, _P, _I64,  # bias, bias_dtype, out, stride
+        _I64, _I64, _I64, ctypes.c_int32, _P,  # m, n, k, out_dtype, stream
+    ]
     _lib = L
     return _lib
 
@@ -350,4 +370,7 @@ EXPORTED_SYMBOLS = (
     "fgv_cp_gather_indexer_k_quant_cache",
     "fgv_fp8_fp4_mqa_logits",
     "fgv_fp8_fp4_paged_mqa_logits",
+    "fgv_add_rms_norm_quant",
+    "fgv_silu_mul_quant",
+    "fgv_int8_scaled_mm",
 )

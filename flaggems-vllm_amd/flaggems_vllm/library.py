@@ -8,7 +8,8 @@ opaque custom ops: the schemas declare what each op writes, namely ``q`` and
 for the gather, ``slot_mapping`` for the slot mapping, ``kv_cache`` for the
 indexer key insert and ``k_fp8`` / ``k_fp8_scale`` for its gather, ``indices`` for the top-k per row
 (``output`` and, for rows long enough to split, ``workspace`` for ``persistent_topk``),
-``out`` for ``fp8_einsum_out`` (the index-row ops, ``fp8_einsum`` and ``flash_mla_sparse_fwd`` write only what they return).  The fake (meta)
+``out`` for ``fp8_einsum_out`` (the index-row ops, ``fp8_einsum``, ``flash_mla_sparse_fwd`` and the 8-bit linear ops write only what they return, but for
+``int8_scaled_mm_out``'s ``out``).  The fake (meta)
 implementations give the output shapes and strides the real ops return.
 The main op and the sibling are C++ ops (the torch extension's
 ``torch_ops.cpp``, loaded here): the same checks and launch the Python
@@ -18,7 +19,9 @@ errors are the wrapper's.
 
 ``fused_indexer_q_rope_quant`` returns ``(q, q_scale, weights)`` here, with an
 empty ``q_scale`` for FP8, because an op schema cannot return the nested tuple
-the Python function returns for MXFP4.  ``flash_mla_with_kvcache`` takes a
+the Python function returns for MXFP4.  ``fused_add_rms_norm_quant`` returns an
+empty ``hidden`` here when there is no residual (an op must not return its
+input).  ``flash_mla_with_kvcache`` takes a
 scheduler-metadata object and is not registered.
 """
 from typing import List, Optional, Tuple
@@ -34,9 +37,12 @@ from .ops import (
     dequantize_and_gather_k_cache,
     flash_mla_sparse_fwd,
     fp8_einsum,
+    fused_add_rms_norm_quant,
     fused_indexer_q_rope_quant,
     fused_q_kv_rmsnorm,
+    fused_silu_mul_quant,
     indexer_k_quant_and_cache,
+    int8_scaled_mm,
     persistent_topk,
     top_k_per_row_decode,
     top_k_per_row_prefill,
@@ -263,6 +269,55 @@ def _(q, kv, indices, sm_scale, d_v=512, attn_sink=None, topk_length=None):
             q.new_empty((s_q, h_q), dtype=torch.float32))
 
 
+def _codes_like(x, cols, dtype):
+    blocks = 1 if dtype == torch.int8 else cols // 128
+    return x.new_empty((x.shape[0], cols), dtype=dtype), x.new_empty((x.shape[0], blocks), dtype=torch.float32)
+
+
+@_op("fused_add_rms_norm_quant")
+def _add_rms_norm_quant(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float,
+                        dtype: torch.dtype = torch.int8) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    codes, scales, hidden = fused_add_rms_norm_quant(x, residual, weight, eps, dtype)
+    return codes, scales, x.new_empty((0,)) if residual is None else hidden
+
+
+@_add_rms_norm_quant.register_fake
+def _(x, residual, weight, eps, dtype=torch.int8):
+    return (*_codes_like(x, x.shape[1], dtype), x.new_empty((0,) if residual is None else x.shape))
+
+
+@_op("fused_silu_mul_quant")
+def _silu_mul_quant(x: torch.Tensor, dtype: torch.dtype = torch.int8) -> Tuple[torch.Tensor, torch.Tensor]:
+    return fused_silu_mul_quant(x, dtype)
+
+
+@_silu_mul_quant.register_fake
+def _(x, dtype=torch.int8):
+    return _codes_like(x, x.shape[1] // 2, dtype)
+
+
+@_op("int8_scaled_mm")
+def _int8_scaled_mm(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
+                    bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    return int8_scaled_mm(a, b, scale_a, scale_b, bias, out_dtype)
+
+
+@_int8_scaled_mm.register_fake
+def _(a, b, scale_a, scale_b, bias=None, out_dtype=torch.bfloat16):
+    return a.new_empty((a.shape[0], b.shape[0]), dtype=out_dtype)
+
+
+@_op("int8_scaled_mm_out", ("out",))
+def _int8_scaled_mm_out(a: torch.Tensor, b: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
+                        bias: Optional[torch.Tensor], out: torch.Tensor) -> None:
+    int8_scaled_mm(a, b, scale_a, scale_b, bias, out.dtype, out=out)
+
+
+@_int8_scaled_mm_out.register_fake
+def _(a, b, scale_a, scale_b, bias, out):
+    return None
+
+
 REGISTERED: List[str] = [
     "fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert",
     "fused_inv_rope_fp8_quant",
@@ -280,4 +335,12 @@ REGISTERED: List[str] = [
     "fp8_einsum_out",
     "persistent_topk",
     "flash_mla_sparse_fwd",
+]
+
+# the 8-bit linear ops, which have no counterpart in the reference package
+REGISTERED_LINEAR: List[str] = [
+    "fused_add_rms_norm_quant",
+    "fused_silu_mul_quant",
+    "int8_scaled_mm",
+    "int8_scaled_mm_out",
 ]

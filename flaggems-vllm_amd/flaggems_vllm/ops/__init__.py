@@ -1,4 +1,5 @@
-"""DeepSeek-V4 attention pre-processing ops (reference: src/flaggems_vllm/ops/__init__.py:23-38, 55, 56, 57, 58-65, 78, 122, 142-143, 187, 229)."""
+"""DeepSeek-V4 attention pre-processing ops (reference: src/flaggems_vllm/ops/__init__.py:23-38, 55, 56, 57, 58-65, 78, 122, 142-143, 187, 229),
+and the 8-bit linear ops around the layer (``int8_linear``)."""
 from .cp_gather_indexer_k_quant_cache import cp_gather_indexer_k_quant_cache
 from .deepseek_v4_attention_combine_topk_swa_indices import combine_topk_swa_indices
 from .deepseek_v4_attention_compute_global_topk_indices_and_lens import compute_global_topk_indices_and_lens
@@ -14,6 +15,7 @@ from .fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert import (
 )
 from .fused_indexer_q_rope_quant import fused_indexer_q_rope_quant
 from .fused_inv_rope_fp8_quant import SUPPORTED_FP8_DTYPE, fused_inv_rope_fp8_quant
+from .int8_linear import fused_add_rms_norm_quant, fused_silu_mul_quant, int8_scaled_mm
 from .indexer_k_quant_and_cache import indexer_k_quant_and_cache
 from .persistent_topk import persistent_topk
 from .slot_mapping import compute_slot_mapping_parallel
@@ -33,6 +35,9 @@ __all__ = [
     "get_mla_metadata",
     "dequantize_and_gather_k_cache",
     "fused_q_kv_rmsnorm",
+    "fused_add_rms_norm_quant",
+    "fused_silu_mul_quant",
+    "int8_scaled_mm",
     "fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert",
     "fused_indexer_q_rope_quant",
     "fused_inv_rope_fp8_quant",

@@ -650,6 +650,59 @@ int fgv_fp8_einsum_bhr_hdr_ws(const uint8_t* x, int64_t x_stride_b, int64_t x_st
                               void* out, int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_d,
                               int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * RMSNorm in front of an 8-bit projection, with the residual's addition:
+ *   h = round(x + residual) (h = x when residual is NULL), written to hidden;
+ *   y = h * r * weight, r = 1 / sqrt(mean(h^2) + eps);
+ *   codes and scales of y: int8 (code_dtype 0) with one scale per row,
+ *   a = max |y|, scale = a / 127, code = round(127 y / a); or e4m3fn
+ *   (code_dtype 1) with one scale per 128 columns, scale = a / 448,
+ *   code = e4m3fn(448 y / a); ties to even, no code differs from this
+ *   definition in 64 bits (r cancels in it).
+ * Under a largest magnitude of 0 the scale and codes are 0; under one that is
+ * not finite the codes are 0 and the scale NaN, and a row of x that holds a
+ * NaN or an infinity has NaN in all its scales.
+ *
+ *   x, residual, hidden  [rows, cols] bf16 (x_dtype 0) or fp16 (1), unit column
+ *       stride, any row stride; hidden may be x or residual itself, and is
+ *       neither read nor written when residual is NULL.
+ *   weight  [cols] of x's type, or float32 (weight_is_fp32).
+ *   codes   [rows, cols] bytes; scales [rows, 1 or cols / 128] float32.
+ * cols from 1 to 65536, a multiple of 128 for e4m3fn; rows below 2^31; eps > 0.
+ * Rows need no alignment beyond their elements'.
+ */
+int fgv_add_rms_norm_quant(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                           const void* weight, int32_t weight_is_fp32, void* hidden, int64_t hidden_stride,
+                           void* codes, int64_t codes_stride, float* scales, int64_t scales_stride, int64_t rows,
+                           int64_t cols, double eps, int32_t x_dtype, int32_t code_dtype, void* stream);
+
+/*
+ * The gated activation of a feed-forward block as 8-bit codes and scales:
+ * y = g / (1 + exp(-g)) * u of rows x = gate | up [rows, 2 * cols], codes and
+ * scales of y as in fgv_add_rms_norm_quant.
+ */
+int fgv_silu_mul_quant(const void* x, int64_t x_stride, void* codes, int64_t codes_stride, float* scales,
+                       int64_t scales_stride, int64_t rows, int64_t cols, int32_t x_dtype, int32_t code_dtype,
+                       void* stream);
+
+/*
+ * Product of int8 codes with a scale per token and per channel:
+ *   out[m, n] = scale_a[m] * scale_b[n] * sum_k a[m, k] * b[n, k] + bias[n]
+ * with the exact integer sum, the rest in binary32 in the order
+ * (sum * scale_a) * scale_b + bias, rounded once to out.
+ *   a [m, k], b [n, k] int8, unit column stride, rows a_stride / b_stride
+ *   bytes apart, no alignment needed (16-byte aligned rows take the fast paths);
+ *   scale_a[m * scale_a_stride], scale_b[n * scale_b_stride] float32 (stride
+ *   0: one scale for all); bias [n] or NULL, in bias_dtype; out [m, n], unit
+ *   column stride.  out_dtype and bias_dtype: 0 bf16, 1 fp16, 2 fp32.
+ * k at most 131071 (the sum is an int32), m at most 2^20; k = 0 writes the
+ * bias, or zeros.
+ */
+int fgv_int8_scaled_mm(const int8_t* a, int64_t a_stride, const int8_t* b, int64_t b_stride, const float* scale_a,
+                       int64_t scale_a_stride, const float* scale_b, int64_t scale_b_stride, const void* bias,
+                       int32_t bias_dtype, void* out, int64_t out_stride, int64_t m, int64_t n, int64_t k,
+                       int32_t out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
