@@ -9,6 +9,9 @@
 // operand row c, bytes 16 g .. 16 g + 15 of the 64; the accumulator holds rows
 // 4 g .. 4 g + 3 of the first operand against row c of the second.  b is the
 // first operand, so a lane holds four neighbouring channels of one token.
+#include <algorithm>
+#include <type_traits>
+
 #include "fgv_device.h"
 #include "fgv_host.h"
 
@@ -16,6 +19,7 @@ namespace fgv {
 namespace {
 
 typedef int v4i_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef v4i_t v4i_a1 __attribute__((aligned(1)));
@@ -23,6 +27,7 @@ typedef v4i_t v4i_a1 __attribute__((aligned(1)));
 enum OutType { kOutBf16 = 0, kOutF16 = 1, kOutF32 = 2 };
 constexpr int kBlockK = 128;
 constexpr int64_t kMaxK = 131071;  // K * 2^14 fits int32
+constexpr int64_t kMaxM = 1 << 20, kMaxN = 1 << 24;
 
 struct MmArgs {
     const int8_t* a;  // a[m, k], rows a_s bytes apart
@@ -53,6 +58,18 @@ __device__ __forceinline__ float bias_at(const MmArgs& p, int n) {
     return p.bias_type == kOutF16 ? (float)__builtin_bit_cast(_Float16, v) : __uint_as_float((uint32_t)v << 16);
 }
 
+// Two outputs in one word.
+template <int OUT>
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
+    if constexpr (OUT == kOutBf16)
+        return pack_bf16x2(lo, hi);
+    // (kept apart from the product before it: the compiler would round both at
+    // once in one kernel and not in another, and results would depend on the schedule)
+    asm("" : "+v"(lo), "+v"(hi));
+    return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) |
+           ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16);
+}
+
 // Four channels n .. n + 3 of one token (those below p.n).
 template <int OUT>
 __device__ __forceinline__ void store4(const MmArgs& p, int64_t m, int n, const float v[4]) {
@@ -71,13 +88,8 @@ __device__ __forceinline__ void store4(const MmArgs& p, int64_t m, int n, const 
         uint16_t* o = reinterpret_cast<uint16_t*>(p.out) + m * p.o_s + n;
         u32x2_a2 w;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if constexpr (OUT == kOutBf16)
-                w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-            else
-                w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * i]) |
-                       ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) << 16);
-        }
+        for (int i = 0; i < 2; ++i)
+            w[i] = pack_out<OUT>(v[2 * i], v[2 * i + 1]);
         if (n + 4 <= p.n) {
             *reinterpret_cast<u32x2_a2*>(o) = w;
         } else {
@@ -209,16 +221,15 @@ __global__ void __launch_bounds__(64 * KS) int8_mm_rows_kernel(MmArgs p) {
 }
 
 // ---- many rows: tiles through LDS ----
-// Output tiles of 32 TM tokens x 32 TN channels, four waves of 16 TM x 16 TN
-// each.  The 128-byte K blocks of a's and b's rows stream through a ring of NS
-// LDS stages by LDS DMA; rows are stored unpadded, 16-byte chunk q of row r at
-// q ^ ((r >> 1) & 7), so that the 16 rows of a fragment read hit all 64 banks.
+// Output tiles of 16 TM WM tokens x 16 TN WN channels, WM x WN waves of
+// 16 TM x 16 TN each.  The 128-byte K blocks of a's and b's rows stream through
+// a ring of NS LDS stages by LDS DMA; rows are stored unpadded, 16-byte chunk q
+// of row r at q ^ ((r >> 1) & 7), so that a fragment read meets no bank conflict.
 // A block is two slices of 64 bytes (one MFMA each); a slice's operands are read
 // into registers under the MFMAs of the slice before it, in a second register
-// set, so the matrix unit only waits at the barrier that hands a block over:
-// once per block, between its two slices, when every wave holds the second
-// slice in registers, the block's stage is free for block kb + NS and block
-// kb + 1 has landed.
+// set.  Between a block's two slices stands the barrier that hands blocks over:
+// every wave holds the second slice in registers, so the stage is free for block
+// kb + NS, and block kb + 1 has landed.
 __device__ __forceinline__ int swz(int row, int chunk) { return chunk ^ ((row >> 1) & 7); }
 
 // s_waitcnt operand: vector memory operations outstanding <= n (expcnt and
@@ -233,11 +244,23 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// LDS DMA of 16 bytes per lane from row + off (row a scalar result, not a
-// v_readlane's) to lds + 16 lane, by all lanes (`lanes` ~0) or none (0: what a
-// step past the last block sends).  Counted by vmcnt.
+// A value that is the same in all lanes, in a scalar register (the builtin is
+// dropped where the compiler knows that much, and the value may stay in a vector
+// register, which the "s" operands below then get).  The VALU may have written v
+// just before: a v_readfirstlane must not follow within a wait state, which the
+// compiler does not see to inside assembly.
+__device__ __forceinline__ uint32_t scalar(uint32_t v) {
+    uint32_t r;
+    asm volatile("s_nop 1\n\tv_readfirstlane_b32 %0, %1" : "=s"(r) : "v"(v));
+    return r;
+}
+
+// LDS DMA of 16 bytes per lane from row + off to lds + 16 lane, by all lanes (`lanes` ~0) or none (0: what a
+// step past the last block sends).  Counted by vmcnt.  (The row may come from a
+// v_readfirstlane: a vector memory instruction must not read it within five wait
+// states, and the compiler does not look for that inside assembly.)
 __device__ __forceinline__ void dma16_if(const void* row, uint32_t off, uint32_t lds, uint32_t lanes) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %1, %0\n\ts_mov_b64 exec, -1" ::"s"(row),
+    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %0\n\ts_mov_b64 exec, -1" ::"s"(row),
                  "v"(off), "s"(lds), "s"(lanes)
                  : "memory", "m0");
 }
@@ -245,15 +268,11 @@ __device__ __forceinline__ void dma16_if(const void* row, uint32_t off, uint32_t
 // The tile kernels' MFMA as inline assembly, its accumulator tied in place: left
 // to itself the compiler gives the result other registers and copies the
 // 256 accumulators around (150 copies to 128 MFMAs).  It knows of no
-// wait states inside assembly: operands come from LDS or memory (whose waits it
-// does insert); where the VALU may have written them `kAfterValu` waits, and
-// mfma_done() stands before the accumulators are read.
-template <bool kAfterValu = false>
+// wait states inside assembly: the operands come from LDS (whose waits it does
+// insert), never from the VALU, and mfma_done() stands before the accumulators
+// are read.
 __device__ __forceinline__ void mfma_in_place(v4i_t& acc, v4i_t a, v4i_t b) {
-    if constexpr (kAfterValu)
-        asm volatile("s_nop 4\n\tv_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
-    else
-        asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+    asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 __device__ __forceinline__ void mfma_done() { asm volatile("s_nop 15\n\ts_nop 7" ::: "memory"); }
 
@@ -272,61 +291,98 @@ __device__ __forceinline__ void tile_of(int at, int mtiles, int ntiles, int& mt,
     nt = in / height;
 }
 
-template <int TM, int TN, int NS, int OUT>
-__global__ void __launch_bounds__(256, 1) int8_mm_tile_kernel(MmArgs p, int32_t mtiles, int32_t ntiles) {
-    constexpr int kBM = 32 * TM, kBN = 32 * TN, kABytes = kBM * kBlockK;
-    constexpr int kStage = (kBM + kBN) * kBlockK, kPer = TM + TN;  // DMAs per wave and block
+// Split K: with gridDim.y = S > 1, workgroup y takes its part of the K blocks
+// and writes its int32 tile to partial y of `part` ([S][m][part_pitch(n)]);
+// int8_mm_sum_kernel adds the partials and scales.  The sums are whole numbers,
+// so the result is the unsplit one, bit for bit.
+__host__ __device__ constexpr int64_t part_pitch(int64_t n) { return (n + 3) / 4 * 4; }
+
+template <int WM, int WN, int TM, int TN, int NS, int OUT, bool SPLIT>
+__global__ void __launch_bounds__(64 * WM * WN, 1) int8_mm_tile_kernel(MmArgs p, int32_t mtiles, int32_t ntiles,
+                                                                       int32_t* part) {
+    constexpr int kWaves = WM * WN, kBM = 16 * TM * WM, kBN = 16 * TN * WN, kABytes = kBM * kBlockK;
+    constexpr int kStage = (kBM + kBN) * kBlockK;
+    constexpr int kA = kBM / 8 / kWaves, kB = kBN / 8 / kWaves, kPer = kA + kB;  // DMAs per wave and block
+    static_assert(kBM % (8 * kWaves) == 0 && kBN % (8 * kWaves) == 0, "tile shape");
+    using Elem = std::conditional_t<OUT == kOutF32, float, uint16_t>;
+    constexpr int kRowBytes = 16 * TN * sizeof(Elem) + 16, kCornerRows = OUT == kOutF32 ? 8 : 16;
+    constexpr int kSa = (kBM + 63) / 64 * 64, kScales = kSa + (kBN + 63) / 64 * 64;
     __shared__ __attribute__((aligned(1024))) uint8_t st[NS][kStage];
+    __shared__ __attribute__((aligned(16))) float scales[SPLIT ? 4 : kScales];
 
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int c = lane & 15, g = lane >> 4, wm = wave >> 1, wn = wave & 1;
+    const int c = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
+    // the workgroup's K blocks: all, or the part blockIdx.y of them (K is a multiple of 128 here)
+    const int all = p.k / kBlockK;
+    const int kb_lo = SPLIT ? (int)((int64_t)all * blockIdx.y / gridDim.y) : 0;
+    const int nkb = SPLIT ? (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y) - kb_lo : all;
+
     int mt, nt;
     tile_of(blockIdx.x, mtiles, ntiles, mt, nt);
     const int m0 = mt * kBM, n0 = nt * kBN;
 
     // This lane's DMA sources, relative to the tile's first row: instruction j of
-    // the wave covers tile rows 8 (wave T + j) + lane / 8, physical chunk lane % 8.
+    // the wave covers 8 tile rows, lane / 8 of them, physical chunk lane % 8.
     // Rows past the end read the last one: they only feed outputs that are not stored.
-    const int8_t* const abase = p.a + (int64_t)m0 * p.a_s;
-    const int8_t* const bbase = p.b + (int64_t)n0 * p.b_s;
+    const int8_t* const abase = p.a + (int64_t)m0 * p.a_s + (int64_t)kb_lo * kBlockK;
+    const int8_t* const bbase = p.b + (int64_t)n0 * p.b_s + (int64_t)kb_lo * kBlockK;
     uint32_t src[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        const bool is_a = j < TM;
-        const int row = 8 * (is_a ? wave * TM + j : wave * TN + j - TM) + (lane >> 3);
+        const bool is_a = j < kA;
+        const int row = 8 * (is_a ? wave * kA + j : wave * kB + j - kA) + (lane >> 3);
         const int r = is_a ? min(row, p.m - 1 - m0) : min(row, p.n - 1 - n0);
         src[j] = (uint32_t)r * (uint32_t)(is_a ? p.a_s : p.b_s) + 16 * swz(row, lane & 7);
     }
-    const int nkb = p.k / kBlockK;  // whole blocks; what is left of K comes last, straight from memory
     auto issue = [&](int kb, uint32_t base, int j, uint32_t lanes) __attribute__((always_inline)) {
-        const int8_t* row = (j < TM ? abase : bbase) + (int64_t)kb * kBlockK;
-        const uint32_t to = base + (j < TM ? 1024 * (wave * TM + j) : kABytes + 1024 * (wave * TN + j - TM));
-        dma16_if(row, src[j], to, lanes);
+        const int8_t* row = (j < kA ? abase : bbase) + (int64_t)kb * kBlockK;
+        dma16_if(row, src[j], base + (j < kA ? 1024 * (wave * kA + j) : kABytes + 1024 * (wave * kB + j - kA)), lanes);
     };
-
     auto sending = [&](int kb) __attribute__((always_inline)) {
-        return (uint32_t)__builtin_amdgcn_readfirstlane((kb - nkb) >> 31);  // ~0 below nkb
+        return scalar((kb - nkb) >> 31);  // ~0 below nkb
     };
 
+    // A slice's operands: b's and a's last row in two register sets, a's other
+    // rows in one (row i is reloaded behind its own MFMAs).
     v4i_t acc[TM][TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-            acc[i][j] = v4i_t{0, 0, 0, 0};
-
-    v4i_t A[2][TM], B[2][TN];
+    v4i_t A[TM - 1], last[2], B[2][TN];
     const uint32_t lane_off = c * kBlockK + 16 * swz(c, g);
     const uint32_t aoff = wm * 16 * TM * kBlockK + lane_off, boff = kABytes + wn * 16 * TN * kBlockK + lane_off;
-    // fragment u of slice s: a's, then b's (slice 1 is chunk ^ 4)
-    auto read = [&](const uint8_t* stage, int s, int u) __attribute__((always_inline)) {
-        if (u < TM)
-            A[s][u] = *reinterpret_cast<const v4i_t*>(stage + (aoff ^ (64 * s)) + 16 * u * kBlockK);
-        else
-            B[s][u - TM] = *reinterpret_cast<const v4i_t*>(stage + (boff ^ (64 * s)) + 16 * (u - TM) * kBlockK);
+    // (slice 1 is chunk ^ 4)
+    auto read_b = [&](const uint8_t* stage, int s, int j) __attribute__((always_inline)) {
+        B[s][j] = *reinterpret_cast<const v4i_t*>(stage + (boff ^ (64 * s)) + 16 * j * kBlockK);
+    };
+    auto read_a = [&](const uint8_t* stage, int s, int i) __attribute__((always_inline)) {
+        (i < TM - 1 ? A[i] : last[s]) =
+            *reinterpret_cast<const v4i_t*>(stage + (aoff ^ (64 * s)) + 16 * i * kBlockK);
+    };
+    constexpr int kMfmas = TM * TN;
+    constexpr int kSendEvery = kMfmas >= 4 * kPer ? 4 : kMfmas >= 2 * kPer ? 2 : 1;
+    static_assert(kMfmas >= 2 * TN && kMfmas >= kPer * kSendEvery, "every read and DMA finds its MFMA");
+    // MFMA u of slice s, and behind it what it lets go of of slice s ^ 1, which is in `stage`
+    auto mfma_and_read = [&](int u, int s, const uint8_t* stage) __attribute__((always_inline)) {
+        const int i = u / TN, j = u % TN;
+        mfma_in_place(acc[i][j], B[s][j], i < TM - 1 ? A[i] : last[s]);
+        if (u == 1)
+            read_a(stage, s ^ 1, TM - 1);
+        if (u % 2 == 0 && u / 2 < TN)
+            read_b(stage, s ^ 1, u / 2);
+        if (j == TN - 1 && i < TM - 1)
+            read_a(stage, s ^ 1, i);
     };
 
+    // the tile's scales, then its first NS blocks
+    if constexpr (!SPLIT) {
+#pragma unroll
+        for (int i = 0; i < (kScales / 64 + kWaves - 1) / kWaves; ++i) {
+            const int to = 64 * (wave + kWaves * i);
+            if (to < kScales)
+                dma4(to < kSa ? p.sa + min(m0 + to + lane, p.m - 1) * p.sa_s
+                              : p.sb + min(n0 + to - kSa + lane, p.n - 1) * p.sb_s,
+                     lds_addr(scales) + 4 * to);
+        }
+    }
 #pragma unroll
     for (int b = 0; b < NS; ++b)
 #pragma unroll
@@ -337,12 +393,18 @@ __global__ void __launch_bounds__(256, 1) int8_mm_tile_kernel(MmArgs p, int32_t 
     else
         __builtin_amdgcn_s_waitcnt(wait_vm(0));
     lds_barrier();
-    constexpr int kMfmas = TM * TN;
-    static_assert(kMfmas >= 3 * kPer - 1, "every read finds its MFMA");
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            acc[i][j] = v4i_t{0, 0, 0, 0};
     if (nkb > 0) {
 #pragma unroll
-        for (int u = 0; u < kPer; ++u)
-            read(st[0], 0, u);
+        for (int j = 0; j < TN; ++j)
+            read_b(st[0], 0, j);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+            read_a(st[0], 0, i);
     }
     int at = 0;
     for (int kb = 0; kb < nkb; ++kb) {
@@ -352,10 +414,7 @@ __global__ void __launch_bounds__(256, 1) int8_mm_tile_kernel(MmArgs p, int32_t 
         const uint32_t dst = lds_addr(cur);
 #pragma unroll
         for (int u = 0; u < kMfmas; ++u) {
-            const int i = u / TN, j = u % TN;
-            mfma_in_place(acc[i][j], B[0][j], A[0][i]);
-            if (u % 2 == 0 && u / 2 < kPer)
-                read(cur, 1, u / 2);
+            mfma_and_read(u, 0, cur);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (NS > 2 && kb + NS - 1 < nkb)
@@ -366,64 +425,233 @@ __global__ void __launch_bounds__(256, 1) int8_mm_tile_kernel(MmArgs p, int32_t 
         const uint32_t lanes = sending(kb + NS);
 #pragma unroll
         for (int u = 0; u < kMfmas; ++u) {
-            const int i = u / TN, j = u % TN;
-            mfma_in_place(acc[i][j], B[1][j], A[1][i]);
-            if (u < kPer)
-                issue(kb + NS, dst, u, lanes);
             // (behind the last block this reads a stage that nothing uses)
-            if (u >= kPer && u - kPer < 2 * kPer && (u - kPer) % 2 == 0)
-                read(nxt, 0, (u - kPer) / 2);
+            mfma_and_read(u, 1, nxt);
+            if (u % kSendEvery == 0 && u / kSendEvery < kPer)
+                issue(kb + NS, dst, u / kSendEvery, lanes);
             __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-    if (nkb * kBlockK < p.k) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int k0 = nkb * kBlockK + 64 * s + 16 * g;
-            v4i_t b[TN];
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-                b[j] = load_frag_end(p.b + (int64_t)min(n0 + wn * 16 * TN + 16 * j + c, p.n - 1) * p.b_s, k0, p.k);
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const v4i_t a =
-                    load_frag_end(p.a + (int64_t)min(m0 + wm * 16 * TM + 16 * i + c, p.m - 1) * p.a_s, k0, p.k);
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-                    mfma_in_place<true>(acc[i][j], b[j], a);
-            }
         }
     }
     mfma_done();
 
-    // ---- scales, bias, store ----
-    const int nb = n0 + wn * 16 * TN + 4 * g;
+    const int nb = n0 + wn * 16 * TN, mb = m0 + wm * 16 * TM;
+    if constexpr (SPLIT) {
+        const int64_t pitch = part_pitch(p.n);
+        int32_t* to = part + (int64_t)blockIdx.y * p.m * pitch;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int m = m0 + wm * 16 * TM + 16 * i + c;
-        if (m >= p.m)
-            continue;
-        const float sa = p.sa[m * p.sa_s];
+        for (int i = 0; i < TM; ++i) {
+            const int m = mb + 16 * i + c;
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int n = nb + 16 * j;
-            float v[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int nq = min(n + q, p.n - 1);
-                v[q] = (float)acc[i][j][q] * sa * p.sb[nq * p.sb_s] + bias_at(p, nq);
+            for (int j = 0; j < TN; ++j) {
+                const int n = nb + 16 * j + 4 * g;
+                if (m < p.m && n < p.n)
+                    *reinterpret_cast<v4i_t*>(to + m * pitch + n) = acc[i][j];
             }
-            if (n < p.n)
-                store4<OUT>(p, m, n, v);
         }
+    } else {
+        // ---- scales, bias, store ----
+        // 16 tokens at a time through a corner of the stages of the wave's own (no
+        // DMA is in flight, no wave reads a stage for use any more), so that a
+        // store instruction writes whole runs of a row.  Rows 16 bytes apart
+        // from a multiple of 256 keep the writes free of bank conflicts.
+        constexpr int kVec = 16 / sizeof(Elem), kRowLanes = 16 * TN / kVec;
+        constexpr int kRowsPer = kRowLanes <= 4 ? 16 : kRowLanes <= 8 ? 8 : kRowLanes <= 16 ? 4 : 2;
+        static_assert(kRowLanes <= 32 && kWaves * kCornerRows * kRowBytes <= NS * kStage, "epilogue shape");
+        using Put = std::conditional_t<OUT == kOutF32, float4, uint2>;
+        uint8_t* const corner = &st[0][0] + wave * kCornerRows * kRowBytes;
+        const float* const sas = scales + wm * 16 * TM + c;
+        const float* const sbs = scales + kSa + wn * 16 * TN + 4 * g;
+        const int my_row = lane / kRowLanes, my_col = lane % kRowLanes * kVec;
+        const int rows = p.m - mb - my_row, cols = p.n - nb - my_col;  // still in range from this lane's on
+        Elem* to = reinterpret_cast<Elem*>(p.out) + (int64_t)(mb + my_row) * p.o_s + nb + my_col;
+        auto finish = [&](auto with_bias) __attribute__((always_inline)) {
+            float bias[TN][4];
+            if constexpr (decltype(with_bias)::value) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        bias[j][q] = bias_at(p, min(nb + 16 * j + 4 * g + q, p.n - 1));
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const float sa = sas[16 * i];
+                Put put[TN];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    const float4 sb = *reinterpret_cast<const float4*>(sbs + 16 * j);
+                    float v[4] = {(float)acc[i][j][0] * sa * sb.x, (float)acc[i][j][1] * sa * sb.y,
+                                  (float)acc[i][j][2] * sa * sb.z, (float)acc[i][j][3] * sa * sb.w};
+                    if constexpr (decltype(with_bias)::value) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            v[q] += bias[j][q];
+                    }
+                    if constexpr (OUT == kOutF32)
+                        put[j] = make_float4(v[0], v[1], v[2], v[3]);
+                    else
+                        put[j] = make_uint2(pack_out<OUT>(v[0], v[1]), pack_out<OUT>(v[2], v[3]));
+                }
+#pragma unroll
+                for (int h = 0; h < 16; h += kCornerRows) {
+                    if (kCornerRows == 16 || (c & 8) == h) {
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+                            *reinterpret_cast<Put*>(corner + c % kCornerRows * kRowBytes +
+                                                    (16 * j + 4 * g) * sizeof(Elem)) = put[j];
+                    }
+                    asm volatile("" ::: "memory");
+#pragma unroll
+                    for (int r = 0; r < kCornerRows; r += kRowsPer) {
+                        if (my_row < kRowsPer && 16 * i + h + r < rows) {
+                            const uint8_t* from = corner + (r + my_row) * kRowBytes + my_col * sizeof(Elem);
+                            if (cols >= kVec) {
+                                *reinterpret_cast<u32x4_a2*>(to) = *reinterpret_cast<const u32x4_t*>(from);
+                            } else {
+#pragma unroll 1
+                                for (int e = 0; e < cols; ++e)
+                                    to[e] = reinterpret_cast<const Elem*>(from)[e];
+                            }
+                        }
+                        to += kRowsPer * p.o_s;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    asm volatile("" ::: "memory");
+                }
+            }
+        };
+        if (p.bias)
+            finish(std::true_type{});
+        else
+            finish(std::false_type{});
     }
 }
 
-template <int TM, int TN, int NS, int OUT>
+// out = the sum of the partials, scaled: four channels of a token per thread.
+template <int OUT>
+__global__ void __launch_bounds__(256) int8_mm_sum_kernel(MmArgs p, const int32_t* part, int32_t splits) {
+    const int64_t pitch = part_pitch(p.n), fours = pitch / 4, slot = p.m * pitch;
+    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < p.m * fours; u += (int64_t)gridDim.x * 256) {
+        const int64_t m = u / fours;
+        const int n = (int)(u - m * fours) * 4;
+        const v4i_t* from = reinterpret_cast<const v4i_t*>(part + 4 * u);
+        v4i_t sum = from[0];
+        for (int z = 1; z < splits; ++z)
+            sum += from[z * (slot / 4)];
+        const float sa = p.sa[m * p.sa_s];
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int nq = min(n + q, p.n - 1);
+            v[q] = (float)sum[q] * sa * p.sb[nq * p.sb_s] + bias_at(p, nq);
+        }
+        store4<OUT>(p, m, n, v);
+    }
+}
+
+// ---- rows that the tiles cannot take as they are ----
+// Rows whose start or stride is no multiple of 16 bytes, or whose K is none of
+// 128, are copied to rows of a whole number of K blocks, zeros behind K (which
+// add nothing to a sum): 16 bytes per thread, a's rows, then b's.
+struct PackArgs {
+    const int8_t* from[2];
+    int64_t from_s[2];
+    int8_t* to[2];
+    int64_t rows[2];
+    int32_t k, pitch;  // pitch: K rounded up to 128
+};
+
+__global__ void __launch_bounds__(256) int8_mm_pack_kernel(PackArgs p) {
+    const int per_row = p.pitch / 16, which = blockIdx.y;
+    const int64_t total = p.rows[which] * per_row;
+    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
+        const int64_t row = u / per_row;
+        const int k = (int)(u - row * per_row) * 16;
+        *reinterpret_cast<v4i_t*>(p.to[which] + row * p.pitch + k) =
+            load_frag_end(p.from[which] + row * p.from_s[which], k, p.k);
+    }
+}
+
+// ---- schedules ----
+
+// The tiles, by what a K block costs a CU that works on one of them (measured
+// at K 7168 with a tile for nearly every CU, us: 64 x 64 21.2, 128 x 64 28.8,
+// 128 x 128 36.9, 256 x 128 52.2, 256 x 256 94 in all, about 3 of them before
+// and behind the K loop).  Below 256 x 256, which the matrix units bound (and at
+// full size the power limit), the loads of the operands' rows do: 52-56 GB/s
+// into a CU, however many blocks are in flight (NS 3, 4 and 5 alike).
+struct TileKind {
+    int bm, bn;
+    float us_per_block;
+};
+constexpr TileKind kTiles[] = {{64, 64, 0.31f}, {128, 64, 0.43f}, {128, 128, 0.60f}, {256, 128, 0.85f}, {256, 256, 1.5f}};
+constexpr int kTileKinds = 5;
+constexpr float kTileFixedUs = 3.f;
+
+struct Plan {
+    bool rows;  // straight from memory
+    int tile, splits;
+    int64_t a_bytes, b_bytes, part_bytes;  // workspace: packed a, packed b, partials
+    int64_t bytes() const { return a_bytes + b_bytes + part_bytes; }
+};
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Rows straight from memory while one pass of 16-row workgroups takes all
+// tokens, or the workgroups fit the CUs at once (24 x 2048 x 7168: 9.3 us, 10.2
+// in split tiles; 32 x 7168 x 7168: 19.8 and 16.0).  Else the tile that takes
+// the least time, counted as whole turns of the CUs; where even the smallest
+// tiles leave more than half the CUs idle they are split along K, at least eight
+// blocks each (128 x 2048 x 7168: 15.1 us, in four parts 12.2).
+Plan plan_mm(int64_t m, int64_t n, int64_t k, bool a_direct, bool b_direct) {
+    Plan plan{true, 0, 1, 0, 0, 0};
+    const int64_t cus = cu_count(), nkb = (k + kBlockK - 1) / kBlockK;
+    if (k == 0 || m <= 16 || (m + 15) / 16 * ((n + 15) / 16) <= cus)
+        return plan;
+    plan.rows = false;
+    float least = 0.f;
+    for (int i = 0; i < kTileKinds; ++i) {
+        const int64_t tiles = (m + kTiles[i].bm - 1) / kTiles[i].bm * ((n + kTiles[i].bn - 1) / kTiles[i].bn);
+        const float us = (float)((tiles + cus - 1) / cus) * (kTileFixedUs + (float)nkb * kTiles[i].us_per_block);
+        if (i == 0 || us < least) {
+            least = us;
+            plan.tile = i;
+        }
+    }
+    if (plan.tile == 0) {
+        const int64_t tiles = (m + 63) / 64 * ((n + 63) / 64);
+        plan.splits = (int)std::max<int64_t>(1, std::min(cus / tiles, nkb / 8));
+        if (plan.splits > 1)
+            plan.part_bytes = up(plan.splits * m * part_pitch(n) * 4, 256);
+    }
+    if (!a_direct)
+        plan.a_bytes = up(m * up(k, kBlockK), 256);
+    if (!b_direct)
+        plan.b_bytes = up(n * up(k, kBlockK), 256);
+    return plan;
+}
+
+// Whether the tiles' DMAs can read rows as they are (32-bit offsets over the 256 rows of a tile).
+bool direct_rows(const int8_t* p, int64_t stride, int64_t k) {
+    return aligned(p, 16) && stride % 16 == 0 && stride >= 0 && stride < (1 << 23) && k % kBlockK == 0;
+}
+
+template <int WM, int WN, int TM, int TN, int NS, int OUT>
 void launch_tiles(const MmArgs& p, hipStream_t st) {
-    const int32_t mtiles = (p.m + 32 * TM - 1) / (32 * TM), ntiles = (p.n + 32 * TN - 1) / (32 * TN);
-    hipLaunchKernelGGL((int8_mm_tile_kernel<TM, TN, NS, OUT>), dim3((unsigned)(mtiles * ntiles)), dim3(256), 0, st, p,
-                       mtiles, ntiles);
+    constexpr int kBM = 16 * TM * WM, kBN = 16 * TN * WN;
+    const int32_t mtiles = (p.m + kBM - 1) / kBM, ntiles = (p.n + kBN - 1) / kBN;
+    hipLaunchKernelGGL((int8_mm_tile_kernel<WM, WN, TM, TN, NS, OUT, false>), dim3((unsigned)(mtiles * ntiles)),
+                       dim3(64 * WM * WN), 0, st, p, mtiles, ntiles, (int32_t*)nullptr);
+}
+
+template <int OUT>
+void launch_split_tiles(const MmArgs& p, int splits, int32_t* part, hipStream_t st) {
+    const int32_t mtiles = (p.m + 63) / 64, ntiles = (p.n + 63) / 64;
+    hipLaunchKernelGGL((int8_mm_tile_kernel<2, 2, 2, 2, 4, kOutF32, true>), dim3((unsigned)(mtiles * ntiles), splits),
+                       dim3(256), 0, st, p, mtiles, ntiles, part);
+    const int64_t blocks = (p.m * (part_pitch(p.n) / 4) + 255) / 256;
+    hipLaunchKernelGGL(int8_mm_sum_kernel<OUT>, dim3((unsigned)std::min<int64_t>(blocks, 65536)), dim3(256), 0, st, p,
+                       (const int32_t*)part, (int32_t)splits);
 }
 
 template <int MT, int NW, int KS, int OUT>
@@ -433,26 +661,81 @@ void launch_rows(const MmArgs& p, hipStream_t st) {
 }
 
 template <int OUT>
-int launch_mm(const MmArgs& p, hipStream_t st) {
-    const bool al = aligned(p.a, 16) && aligned(p.b, 16) && p.a_s % 16 == 0 && p.b_s % 16 == 0 &&
-                    p.a_s < (1 << 23) && p.b_s < (1 << 23);
-    if (p.m <= 16)
-        launch_rows<1, 2, 8, OUT>(p, st);
-    else if (al && p.k > 0 && p.m > 64)
-        launch_tiles<8, 8, 2, OUT>(p, st);
-    else
-        launch_rows<2, 2, 8, OUT>(p, st);
+int launch_mm(MmArgs p, void* workspace, int64_t workspace_bytes, hipStream_t st) {
+    const bool a_direct = direct_rows(p.a, p.a_s, p.k), b_direct = direct_rows(p.b, p.b_s, p.k);
+    const Plan plan = plan_mm(p.m, p.n, p.k, a_direct, b_direct);
+    const bool room = plan.bytes() == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= plan.bytes());
+    if (plan.rows || !room) {
+        if (p.m > 32)
+            launch_rows<2, 2, 8, OUT>(p, st);
+        else if (p.k >= 16 * kBlockK)
+            launch_rows<1, 1, 8, OUT>(p, st);
+        else
+            launch_rows<1, 1, 4, OUT>(p, st);
+        return launch_status();
+    }
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (!a_direct || !b_direct) {
+        const int32_t pitch = (int32_t)up(p.k, kBlockK);
+        const PackArgs pack{{p.a, p.b},
+                            {p.a_s, p.b_s},
+                            {(int8_t*)ws, (int8_t*)ws + plan.a_bytes},
+                            {a_direct ? 0 : p.m, b_direct ? 0 : p.n},
+                            p.k,
+                            pitch};
+        const int64_t most = std::max(pack.rows[0], pack.rows[1]) * (pitch / 16);
+        hipLaunchKernelGGL(int8_mm_pack_kernel, dim3((unsigned)std::min<int64_t>((most + 255) / 256, 1 << 20), 2),
+                           dim3(256), 0, st, pack);
+        if (!a_direct) {
+            p.a = pack.to[0];
+            p.a_s = pitch;
+        }
+        if (!b_direct) {
+            p.b = pack.to[1];
+            p.b_s = pitch;
+        }
+        p.k = pitch;
+    }
+    if (plan.splits > 1) {
+        launch_split_tiles<OUT>(p, plan.splits, reinterpret_cast<int32_t*>(ws + plan.a_bytes + plan.b_bytes), st);
+        return launch_status();
+    }
+    switch (plan.tile) {
+    case 0:
+        launch_tiles<2, 2, 2, 2, 4, OUT>(p, st);
+        break;
+    case 1:
+        launch_tiles<4, 2, 2, 2, 3, OUT>(p, st);
+        break;
+    case 2:
+        launch_tiles<2, 4, 4, 2, 3, OUT>(p, st);
+        break;
+    case 3:
+        launch_tiles<4, 2, 4, 4, 3, OUT>(p, st);
+        break;
+    default:
+        launch_tiles<2, 4, 8, 4, 2, OUT>(p, st);
+        break;
+    }
     return launch_status();
 }
 
 }  // namespace
 }  // namespace fgv
 
+extern "C" int64_t fgv_int8_scaled_mm_workspace_bytes(const int8_t* a, int64_t a_stride, const int8_t* b,
+                                                      int64_t b_stride, int64_t m, int64_t n, int64_t k) {
+    using namespace fgv;
+    if (m <= 0 || n <= 0 || k <= 0 || k > kMaxK || m > kMaxM || n > kMaxN)
+        return 0;
+    return plan_mm(m, n, k, direct_rows(a, a_stride, k), direct_rows(b, b_stride, k)).bytes();
+}
+
 extern "C" int fgv_int8_scaled_mm(const int8_t* a, int64_t a_stride, const int8_t* b, int64_t b_stride,
                                   const float* scale_a, int64_t scale_a_stride, const float* scale_b,
                                   int64_t scale_b_stride, const void* bias, int32_t bias_dtype, void* out,
                                   int64_t out_stride, int64_t m, int64_t n, int64_t k, int32_t out_dtype,
-                                  void* stream) {
+                                  void* workspace, int64_t workspace_bytes, void* stream) {
     using namespace fgv;
     if (m < 0 || n < 0 || k < 0)
         return fail(FGV_E_BAD_SHAPE, "negative size");
@@ -460,8 +743,8 @@ extern "C" int fgv_int8_scaled_mm(const int8_t* a, int64_t a_stride, const int8_
         return fail(FGV_E_BAD_SHAPE, "out_dtype and bias_dtype must be 0 (bf16), 1 (fp16) or 2 (fp32)");
     if (k > kMaxK)
         return fail(FGV_E_TOO_LARGE, "k above 131071: the int32 sum could overflow");
-    if (m > 0x7fffff00LL || n > 0x7fffff00LL || m > (1LL << 20))
-        return fail(FGV_E_TOO_LARGE, "m at most 2^20, n below 2^31");
+    if (m > kMaxM || n > kMaxN)
+        return fail(FGV_E_TOO_LARGE, "m at most 2^20, n at most 2^24");
     if (m == 0 || n == 0)
         return FGV_OK;
     if (!out || !scale_a || !scale_b || (k > 0 && (!a || !b)))
@@ -474,10 +757,10 @@ extern "C" int fgv_int8_scaled_mm(const int8_t* a, int64_t a_stride, const int8_
     const hipStream_t st = static_cast<hipStream_t>(stream);
     switch (out_dtype) {
     case kOutBf16:
-        return launch_mm<kOutBf16>(p, st);
+        return launch_mm<kOutBf16>(p, workspace, workspace_bytes, st);
     case kOutF16:
-        return launch_mm<kOutF16>(p, st);
+        return launch_mm<kOutF16>(p, workspace, workspace_bytes, st);
     default:
-        return launch_mm<kOutF32>(p, st);
+        return launch_mm<kOutF32>(p, workspace, workspace_bytes, st);
     }
 }

@@ -559,10 +559,15 @@ int int8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale_a,
     const at::Tensor out = out_in ? *out_in : at::empty({m, n}, a.options().dtype(out_dtype));
     *result = out;
     const c10::DeviceGuard guard(dev);
+    // from torch's caching allocator, in the order of the current stream
+    const int64_t ws_bytes = fgv_int8_scaled_mm_workspace_bytes(a.data_ptr<int8_t>(), a.stride(0),
+                                                                b.data_ptr<int8_t>(), b.stride(0), m, n, k);
+    const at::Tensor ws = ws_bytes > 0 ? at::empty({ws_bytes}, a.options().dtype(at::kByte)) : at::Tensor();
     return fgv_int8_scaled_mm(a.data_ptr<int8_t>(), a.stride(0), b.data_ptr<int8_t>(), b.stride(0),
                               scale_a.data_ptr<float>(), sa, scale_b.data_ptr<float>(), sb,
                               bias ? bias->data_ptr() : nullptr, bias ? out_code(bias->scalar_type()) : 0,
-                              out.data_ptr(), out.stride(0), m, n, k, out_code(out_dtype), current_stream(a));
+                              out.data_ptr(), out.stride(0), m, n, k, out_code(out_dtype),
+                              ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, current_stream(a));
 }
 
 // ---- dispatcher ops: the same functions, failures raised as RuntimeError ----

@@ -326,8 +326,11 @@ def lib():
         _P, _I64, _P, _I64,  # a, stride, b, stride (bytes)
         _P, _I64, _P, _I64,  # scale_a, stride, scale_b, stride
         _P, ctypes.c_int32, _P, _I64,  # bias, bias_dtype, out, stride
-        _I64, _I64, _I64, ctypes.c_int32, _P,  # m, n, k, out_dtype, stream
+        _I64, _I64, _I64, ctypes.c_int32,  # m, n, k, out_dtype
+        _P, _I64, _P,  # workspace, workspace_bytes, stream
     ]
+    L.fgv_int8_scaled_mm_workspace_bytes.restype = ctypes.c_int64
+    L.fgv_int8_scaled_mm_workspace_bytes.argtypes = [_P, _I64, _P, _I64, _I64, _I64, _I64]
     _lib = L
     return _lib
 
@@ -373,4 +376,5 @@ EXPORTED_SYMBOLS = (
     "fgv_add_rms_norm_quant",
     "fgv_silu_mul_quant",
     "fgv_int8_scaled_mm",
+    "fgv_int8_scaled_mm_workspace_bytes",
 )

@@ -101,7 +101,7 @@ def int8_scaled_mm(
     """``out[m, n] = scale_a[m] * scale_b[n] * sum_k a[m, k] * b[n, k] + bias[n]``.
 
     Args:
-        a: [M, K] int8, contiguous rows; K at most 131071, M at most 2^20.
+        a: [M, K] int8, contiguous rows; K at most 131071, M at most 2^20, N at most 2^24.
         b: [N, K] int8, contiguous rows (the weight, a channel a row).
         scale_a: float32 [M], [M, 1] or one scale.
         scale_b: float32 [N], [N, 1], [1, N] or one scale.

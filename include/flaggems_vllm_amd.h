@@ -691,17 +691,26 @@ int fgv_silu_mul_quant(const void* x, int64_t x_stride, void* codes, int64_t cod
  * with the exact integer sum, the rest in binary32 in the order
  * (sum * scale_a) * scale_b + bias, rounded once to out.
  *   a [m, k], b [n, k] int8, unit column stride, rows a_stride / b_stride
- *   bytes apart, no alignment needed (16-byte aligned rows take the fast paths);
- *   scale_a[m * scale_a_stride], scale_b[n * scale_b_stride] float32 (stride
- *   0: one scale for all); bias [n] or NULL, in bias_dtype; out [m, n], unit
- *   column stride.  out_dtype and bias_dtype: 0 bf16, 1 fp16, 2 fp32.
- * k at most 131071 (the sum is an int32), m at most 2^20; k = 0 writes the
- * bias, or zeros.
+ *   bytes apart, no alignment needed; scale_a[m * scale_a_stride],
+ *   scale_b[n * scale_b_stride] float32 (stride 0: one scale for all); bias [n]
+ *   or NULL, in bias_dtype; out [m, n], unit column stride.  out_dtype and
+ *   bias_dtype: 0 bf16, 1 fp16, 2 fp32.
+ * k at most 131071 (the sum is an int32), m at most 2^20, n at most 2^24; k = 0
+ * writes the bias, or zeros.
+ *
+ * workspace: 16-byte aligned device memory of workspace_bytes, at least what
+ * fgv_int8_scaled_mm_workspace_bytes says for these operands (0 for many): copies
+ * of rows that are no multiple of 16 bytes apart (or k none of 128), and the
+ * partial sums where few tiles are split along k.  Without it the product is
+ * formed straight from memory, with the same bits, slower.  Calls that share a
+ * workspace must be ordered on one stream.
  */
 int fgv_int8_scaled_mm(const int8_t* a, int64_t a_stride, const int8_t* b, int64_t b_stride, const float* scale_a,
                        int64_t scale_a_stride, const float* scale_b, int64_t scale_b_stride, const void* bias,
                        int32_t bias_dtype, void* out, int64_t out_stride, int64_t m, int64_t n, int64_t k,
-                       int32_t out_dtype, void* stream);
+                       int32_t out_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t fgv_int8_scaled_mm_workspace_bytes(const int8_t* a, int64_t a_stride, const int8_t* b, int64_t b_stride,
+                                           int64_t m, int64_t n, int64_t k);
 
 #ifdef __cplusplus
 }

@@ -111,6 +111,86 @@ def test_gpu_sizes(m, n, k):
     run(m, n, k, seed=m + n)
 
 
+# sizes with ragged edges that take, on 256 CUs, split 64 x 64 tiles, 64 x 64, 128 x 64, 128 x 128, 256 x 128 and
+# 256 x 256 tiles
+TILE_SIZES = [(300, 300), (500, 1030), (1000, 1030), (1000, 2050), (2000, 3000), (4000, 4090)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", TILE_SIZES)
+@pytest.mark.parametrize("k", [128, 256, 384, 640, 1111, 2064, 5120])
+def test_gpu_every_tile(m, n, k):
+    """From fewer K blocks than a ring has stages to many; a K that is no multiple of 128, and rows that start at
+    any byte."""
+    _say(f"int8 mm tiles {m} x {n} x {k}")
+    run(m, n, k, F16 if k == 384 else BF16, F32 if k in (384, 1111) else None, seed=k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", TILE_SIZES)
+def test_gpu_every_tile_float32(m, n):
+    _say(f"int8 mm tiles {m} x {n} float32")
+    run(m, n, 1024, F32, F32 if m in (500, 4000) else None, seed=m)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", TILE_SIZES)
+def test_gpu_every_tile_writes_its_rows_only(m, n):
+    """out as a view into a wider buffer: what lies around it stays."""
+    _say(f"int8 mm tiles {m} x {n} into a wider buffer")
+    a, b, sa, sb = _codes(m, 256, 1), _codes(n, 256, 2), _scales(m, 3), _scales(n, 4)
+    buf = torch.full((m + 2, n + 21), 3.0, dtype=BF16, device=DEV)
+    got = fv.int8_scaled_mm(a.to(DEV), b.to(DEV), sa.to(DEV), sb.to(DEV), out=buf[1:m + 1, 13:13 + n])
+    torch.cuda.synchronize()
+    check(got, a, b, sa, sb, None, BF16)
+    buf[1:m + 1, 13:13 + n] = 3.0
+    assert bool((buf == 3.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(300, 300, 5120), (1000, 1030, 1111), (300, 700, 384), (2000, 3000, 256)])
+def test_gpu_without_workspace(m, n, k):
+    """The C ABI without a workspace, or with one too small: the same bits straight from memory."""
+    from flaggems_vllm import _native
+
+    _say(f"int8 mm without workspace {m} x {n} x {k}")
+    L = _native.lib()
+    a, b = _codes(m, k, 1).to(DEV), _codes(n, k, 2).to(DEV)
+    sa, sb = _scales(m, 3).to(DEV), _scales(n, 4).to(DEV)
+    ref = fv.int8_scaled_mm(a, b, sa, sb)
+    need = L.fgv_int8_scaled_mm_workspace_bytes(a.data_ptr(), k, b.data_ptr(), k, m, n, k)
+    assert (need > 0) == ((m, n, k) in ((300, 300, 5120), (1000, 1030, 1111)))
+    small = torch.full((256,), 7, dtype=torch.uint8, device=DEV)
+    for ws, size in ((None, 0), (small.data_ptr(), min(256, need - 1) if need else 256)):
+        out = torch.empty(m, n, dtype=BF16, device=DEV)
+        rc = L.fgv_int8_scaled_mm(a.data_ptr(), k, b.data_ptr(), k, sa.data_ptr(), 1, sb.data_ptr(), 1, None, 0,
+                                  out.data_ptr(), n, m, n, k, 0, ws, size, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref) and bool((small == 7).all())
+
+
+@pytest.mark.gpu
+def test_gpu_workspace_is_enough():
+    """Guard bytes behind a workspace of exactly the size asked for stay as they were."""
+    from flaggems_vllm import _native
+
+    _say("int8 mm workspace guard")
+    L = _native.lib()
+    for m, n, k in ((300, 300, 5120), (301, 333, 3001), (1000, 1030, 1111)):
+        a, b = _codes(m, k, 1).to(DEV), _codes(n, k, 2).to(DEV)
+        sa, sb = _scales(m, 3).to(DEV), _scales(n, 4).to(DEV)
+        need = L.fgv_int8_scaled_mm_workspace_bytes(a.data_ptr(), k, b.data_ptr(), k, m, n, k)
+        ws = torch.full((need + 4096,), 7, dtype=torch.uint8, device=DEV)
+        out = torch.empty(m, n, dtype=BF16, device=DEV)
+        rc = L.fgv_int8_scaled_mm(a.data_ptr(), k, b.data_ptr(), k, sa.data_ptr(), 1, sb.data_ptr(), 1, None, 0,
+                                  out.data_ptr(), n, m, n, k, 0, ws.data_ptr(), need,
+                                  torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and need > 0
+        check(out, a.cpu(), b.cpu(), sa.cpu(), sb.cpu(), None, BF16)
+        assert bool((ws[need:] == 7).all())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 33, 300])
 def test_gpu_largest_sum(m):
@@ -272,7 +352,7 @@ def test_refuses(bad, match):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(m=-1), -2), (dict(n=-1), -2), (dict(k=-1), -2), (dict(od=3), -2), (dict(bd=-1), -2),
-    (dict(k=131072), -5), (dict(m=(1 << 20) + 1), -5), (dict(n=1 << 31), -5),
+    (dict(k=131072), -5), (dict(m=(1 << 20) + 1), -5), (dict(n=(1 << 24) + 1), -5),
     (dict(a=None), -1), (dict(b=None), -1), (dict(sa=None), -1), (dict(sb=None), -1), (dict(out=None), -1),
     (dict(sa=18), -3), (dict(out=17), -3), (dict(od=2, out=18), -3), (dict(bias=17), -3),
     (dict(m=0, a=None), 0), (dict(n=0, out=None), 0),
@@ -283,5 +363,5 @@ def test_c_abi_rejects(kw, code):
     p = dict(a=16, b=16, sa=16, sb=16, bias=16, bd=0, out=16, m=4, n=8, k=64, od=0)
     p.update(kw)
     rc = _native.lib().fgv_int8_scaled_mm(p["a"], 64, p["b"], 64, p["sa"], 1, p["sb"], 1, p["bias"], p["bd"],
-                                          p["out"], 8, p["m"], p["n"], p["k"], p["od"], None)
+                                          p["out"], 8, p["m"], p["n"], p["k"], p["od"], None, 0, None)
     assert rc == code
