@@ -9,17 +9,17 @@
 //
 // The codes are those of this definition in 64 bits, every one.  In the norm r
 // cancels, so a code is the rounded quotient q h w / max |h w| and needs no
-// sum.  The fast path works on v = h w (exact in binary32 for 16-bit weights)
-// or v = y within a relative 2^-20 (float32 weights 2^-24, the activation
-// 2^-21): t = v * (q / a) in binary32 is off by less than 2^-19.4 relative, so
-// a code can be wrong only where t lies that close to the border between two
-// codes.  Those elements, one in a few thousand, are computed again in binary64
-// (with a correctly rounded division) and their bytes overwritten.  The largest
-// magnitude is settled the same way: every element within 2^-18 of the
-// binary32 maximum is computed again in binary64.  Where the binary32 values
-// leave the range in which these bounds hold (a row of zeros, of values below
-// 2^-60 or above 2^120, gates below -60 under a huge up value, NaN, infinities),
-// all elements under the scale go that way.
+// sum.  The fast path works on v = h w (exact in binary32 for 16-bit weights,
+// rounded once for float32 ones) or v = y within a relative 2^-21: t = v * (q / a)
+// in binary32 is off by less than 2^-20.4 relative, so a code can be wrong only
+// where t lies that close to the border between two codes.  Those elements, one
+// in some thousand, are computed again in binary64 (with a correctly rounded
+// division) and their bytes overwritten.  The largest magnitude is settled the
+// same way: of float32 weights by the products' rounding errors, which an FMA
+// gives exactly, of the activation by computing every element within 2^-19 of
+// the binary32 maximum again.  Where the binary32 values leave the range in which
+// these bounds hold (a row of zeros, of values below 2^-60 or above 2^120, up
+// values above 2^20, NaN, infinities), all elements under the scale go that way.
 //
 // Bound by memory: 7 bytes per element with a residual (x, residual, hidden,
 // code), 3 without, 5 for the activation.  A row is read once and held in
@@ -121,17 +121,19 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int e0, int cols, uint
 
 // ---- the value that is quantised ----
 
-// silu(g) u in binary32, within a relative 2^-21: the exponent g log2(e) is
-// split into an integer and a fraction known to 2^-26, so that v_exp_f32's
-// argument keeps its low bits (one rounding of g log2(e) alone would cost
-// 2^-17 at g = -88).  The exponent stops at g = +-128, where the sigmoid is 1
-// or below binary32's range.
+// silu(g) u in binary32, within a relative 2^-21 (units of 2^-24: v_exp_f32 and
+// v_rcp_f32 2 each, the exponent's fraction 1/3, 1 + e and two products 1 each).
+// The exponent g log2(e) is split into an integer and a fraction known to 2^-25,
+// so that v_exp_f32's argument keeps its low bits (one rounding of g log2(e)
+// alone would cost 2^-17 at g = -88).  The exponent stops at g = +-86, where the
+// sigmoid is 1 or below 2^-124.
 __device__ __forceinline__ float silu_mul32(float g, float u) {
     constexpr float kLog2e = 0x1.715476p0f, kLog2eLo = 0x1.4ae0cp-26f;  // log2(e) = their sum to 2^-49
-    const float x = __builtin_amdgcn_fmed3f(-g, -128.f, 128.f);
-    const float n = rintf(x * kLog2e);
+    constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the rounded value's
+    const float x = __builtin_amdgcn_fmed3f(-g, -86.f, 86.f);
+    const float s = fmaf(x, kLog2e, kMagic), n = s - kMagic;
     const float f = fmaf(x, kLog2eLo, fmaf(x, kLog2e, -n));
-    const float e = __builtin_ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
+    const float e = __uint_as_float(__float_as_uint(__builtin_amdgcn_exp2f(f)) + (__float_as_uint(s) << 23));
     return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
@@ -206,35 +208,83 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
     return max64(v, (uint64_t)__shfl_xor((unsigned long long)v, 32));
 }
 
+// The larger of m, |a| and |b|; NaN if any is.
+__device__ __forceinline__ float max3_abs(float m, float a, float b) {
+    return __builtin_elementwise_maximum(m, __builtin_elementwise_maximum(fabsf(a), fabsf(b)));
+}
+
 // binary32 magnitudes between these (as bits) keep the fast path's bounds
 constexpr uint32_t kLeast = (127 - 60) << 23, kMost = (127 + 120) << 23;
-constexpr float kNearMost = 1.0f - 0x1p-18f;  // nearer to the maximum than this: settled in binary64
-// distance from the next code at which a code counts as beside a border: int8
-// 0.5 - 2^-12 of a step (127 * 2^-19.4 < 2^-12); e4m3fn 0.5 - 2^-14 of a step,
-// at most 16 steps to a value (16 * 2^-19.4 < 2^-15)
-constexpr float kBorderI8 = 0.5f - 0x1p-12f, kBorderFp8 = 0.5f - 0x1p-14f;
+constexpr float kNearMost = 1.0f - 0x1p-19f;  // nearer to the maximum than this: settled in binary64
+constexpr float kWideUp = 0x1p20f;  // up values above could bring a product back from below binary32's range
+// Distance from the nearest code at which an element counts as beside a border.
+// int8: 0.5 - 2^-13 of a step (127 * 2^-20.4 < 2^-13); e4m3fn: half a step times
+// 1 - 2^-14 (the step is at least 2^-4 of the value: 16 * 2^-20.4 < 2^-15).
+constexpr float kBorderI8 = 0.5f - 0x1p-13f, kBorderFp8 = 0x1p-4f * (1.0f - 0x1p-14f);
 
-// One row per LANES threads (64: four rows to a workgroup; else one).
+// Eight weights from e0 on (zeros behind cols).
+template <bool F16, bool WF32>
+__device__ __forceinline__ void load_weights(const void* weights, int e0, int cols, float w[8]) {
+    if constexpr (WF32) {
+        const float* wp = reinterpret_cast<const float*>(weights) + e0;
+        if (e0 + 8 <= cols) {
+            const f32x4_a4 lo = *reinterpret_cast<const f32x4_a4*>(wp);
+            const f32x4_a4 hi = *reinterpret_cast<const f32x4_a4*>(wp + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = lo[i];
+                w[4 + i] = hi[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                w[i] = e0 + i < cols ? wp[i] : 0.f;
+        }
+    } else {
+        const uint16_t* wp = reinterpret_cast<const uint16_t*>(weights);
+        u32x4_t v = {0, 0, 0, 0};
+        if (e0 + 8 <= cols)
+            v = *reinterpret_cast<const u32x4_a2*>(wp + e0);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (e0 + i < cols)
+                    v[i >> 1] |= (uint32_t)wp[e0 + i] << (16 * (i & 1));
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            w[i] = i & 1 ? hi_of<F16>(v[i >> 1]) : lo_of<F16>(v[i >> 1]);
+    }
+}
+
+// One row per LANES threads (64: four rows to a workgroup; else one).  With
+// `chunks` > 1 a row is shared by that many workgroups, which need nothing of
+// each other (e4m3fn activations).
 template <int OP, bool F16, bool WF32, bool FP8, int LANES, int P>
-__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) act_quant_kernel(QuantArgs a) {
+__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) act_quant_kernel(QuantArgs a, int32_t chunks) {
     constexpr int kBlock = LANES < 256 ? 256 : LANES, kWaves = LANES / 64;
-    constexpr bool kRowScale = !FP8;                       // one scale per row, else per 16 threads and piece
-    constexpr bool kExact32 = OP == kNorm && !WF32;        // v is exact
+    constexpr bool kRowScale = !FP8;              // one scale per row, else per 16 threads and piece
+    constexpr bool kExact32 = OP == kNorm && !WF32;  // v is exact
+    constexpr bool kWithLost = OP == kNorm && WF32;  // v's rounding error is kept
     __shared__ double sum_of[kWaves];
     __shared__ uint32_t max_of[kWaves];
     __shared__ unsigned long long best_of;
 
-    const int64_t row = (int64_t)blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
+    int64_t row = (int64_t)blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
+    int t = threadIdx.x % LANES;
+    if (OP == kSilu && FP8) {
+        row = blockIdx.x / (uint32_t)chunks;
+        t += (int)(blockIdx.x % (uint32_t)chunks) * LANES * P;
+    }
     if (row >= a.rows)
         return;  // (only where waves are rows: no barrier below)
-    const int t = threadIdx.x % LANES, cols = a.cols;
+    const int cols = a.cols;
     const uint16_t* xrow = a.x + row * a.x_stride;
     uint8_t* crow = a.codes + row * a.c_stride;
 
     // ---- one pass over the row: v, the sum of squares, the largest magnitude ----
-    float v[P][8];
+    float v[P][8], lost[kWithLost ? P : 1][8];
     double ss = 0.0;
-    uint32_t mx[P];
+    float most32[P];
     {
         u32x4_t p0[P], p1[P];
 #pragma unroll
@@ -249,22 +299,23 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) act_quant_kernel(Qu
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const int e0 = 8 * (t + LANES * j);
-            mx[j] = 0;
+            float most = 0.f;
             if constexpr (OP == kSilu) {
-                float least = 0.f, widest = 0.f;
+                float widest = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float g = i & 1 ? hi_of<F16>(p0[j][i >> 1]) : lo_of<F16>(p0[j][i >> 1]);
-                    const float u = i & 1 ? hi_of<F16>(p1[j][i >> 1]) : lo_of<F16>(p1[j][i >> 1]);
-                    v[j][i] = silu_mul32(g, u);
-                    mx[j] = max(mx[j], __float_as_uint(fabsf(v[j][i])));
-                    least = fminf(least, g);
-                    widest = fmaxf(widest, fabsf(u));
+                for (int i = 0; i < 8; i += 2) {
+                    const float u0 = lo_of<F16>(p1[j][i >> 1]), u1 = hi_of<F16>(p1[j][i >> 1]);
+                    v[j][i] = silu_mul32(lo_of<F16>(p0[j][i >> 1]), u0);
+                    v[j][i + 1] = silu_mul32(hi_of<F16>(p0[j][i >> 1]), u1);
+                    most = max3_abs(most, v[j][i], v[j][i + 1]);
+                    if constexpr (!F16)  // (fp16 ends at 65504)
+                        widest = max3_abs(widest, u0, u1);
                 }
-                // below, exp(-g) may pass binary32's range under an up value that brings the product back
-                if (least < -60.f && widest > 0x1p20f)
-                    mx[j] = 0x7fffffffu;
+                if (!F16 && !(widest <= kWideUp))
+                    most = __builtin_nanf("");
             } else {
+                float w[8];
+                load_weights<F16, WF32>(a.w, e0, cols, w);
                 if (a.residual) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
@@ -272,101 +323,90 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) act_quant_kernel(Qu
                                               hi_of<F16>(p0[j][q]) + hi_of<F16>(p1[j][q]));
                     store_piece(a.hidden + row * a.h_stride, e0, cols, p0[j]);
                 }
-                float w[8];
-                if constexpr (WF32) {
-                    const float* wp = reinterpret_cast<const float*>(a.w) + e0;
-                    if (e0 + 8 <= cols) {
-                        const f32x4_a4 lo = *reinterpret_cast<const f32x4_a4*>(wp);
-                        const f32x4_a4 hi = *reinterpret_cast<const f32x4_a4*>(wp + 4);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            w[i] = lo[i];
-                            w[4 + i] = hi[i];
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            w[i] = e0 + i < cols ? wp[i] : 0.f;
-                    }
-                } else {
-                    u32x4_t wp = {0, 0, 0, 0};
-                    const uint16_t* w16 = reinterpret_cast<const uint16_t*>(a.w);
-                    if (e0 + 8 <= cols)
-                        wp = *reinterpret_cast<const u32x4_a2*>(w16 + e0);
-                    else
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (e0 + i < cols)
-                                wp[i >> 1] |= (uint32_t)w16[e0 + i] << (16 * (i & 1));
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        w[i] = i & 1 ? hi_of<F16>(wp[i >> 1]) : lo_of<F16>(wp[i >> 1]);
-                }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float h = i & 1 ? hi_of<F16>(p0[j][i >> 1]) : lo_of<F16>(p0[j][i >> 1]);
                     ss = fma((double)h, (double)h, ss);  // (the square is exact)
                     v[j][i] = h * w[i];
-                    mx[j] = max(mx[j], __float_as_uint(fabsf(v[j][i])));
+                    if constexpr (kWithLost)
+                        lost[j][i] = fmaf(h, w[i], -v[j][i]);
+                    if (i & 1)
+                        most = max3_abs(most, v[j][i - 1], v[j][i]);
                 }
             }
+            most32[j] = most;
         }
     }
 
     // ---- the row's sum, and its largest magnitude where it has one scale ----
+    uint32_t mx = 0;  // (bits: a NaN is above all)
     if constexpr (OP == kNorm || kRowScale) {
-        uint32_t m = mx[0];
 #pragma unroll
-        for (int j = 1; j < P; ++j)
-            m = max(m, mx[j]);
+        for (int j = 0; j < P; ++j)
+            mx = max(mx, __float_as_uint(most32[j]) & 0x7fffffffu);
         if constexpr (OP == kNorm)
             ss = wave_sum(ss);
         if constexpr (kRowScale)
-            m = wave_max(m);
+            mx = wave_max(mx);
         if constexpr (kWaves > 1) {
             if ((threadIdx.x & 63) == 0) {
                 sum_of[threadIdx.x >> 6] = ss;
-                max_of[threadIdx.x >> 6] = m;
+                max_of[threadIdx.x >> 6] = mx;
             }
             if (threadIdx.x == 0)
                 best_of = 0;
             __syncthreads();
             ss = sum_of[0];
-            m = max_of[0];
+            mx = max_of[0];
 #pragma unroll
             for (int i = 1; i < kWaves; ++i) {
                 ss += sum_of[i];
-                m = max(m, max_of[i]);
+                mx = max(mx, max_of[i]);
             }
         }
-        if constexpr (kRowScale)
-            mx[0] = m;
     }
-    double r = 1.0;
-    if constexpr (OP == kNorm) {
-        r = 1.0 / sqrt(ss / cols + a.eps);
-        if (!(ss < HUGE_VAL))
-            r = __builtin_nan("");  // a NaN or an infinity in the row
-    }
+    // the factor of the scales: the norm's r (NaN for a row that holds a NaN or an infinity) over q
+    auto factor = [&](double q) __attribute__((always_inline)) {
+        if constexpr (OP == kNorm)
+            return ss < HUGE_VAL ? rsqrt(ss / cols + a.eps) * (1.0 / q) : __builtin_nan("");
+        else
+            return 1.0 / q;
+    };
 
     if constexpr (kRowScale) {
         // ---- int8: one scale per row ----
-        const bool odd = !(mx[0] >= kLeast && mx[0] <= kMost);  // (the same in all threads of the row)
-        double most = __uint_as_float(mx[0]);
+        const bool odd = !(mx >= kLeast && mx <= kMost);  // (the same in all threads of the row)
+        const float top = __uint_as_float(mx);
+        double most = top;
         if (!kExact32 || odd) {
-            const float from = odd ? 0.f : __uint_as_float(mx[0]) * kNearMost;
-            uint64_t mask = 0, best = 0;
+            uint64_t best = 0;
+            if (kWithLost && !odd) {
+                // |h w| = top + what its rounding lost, of the elements that reach top
+                float more = -top;
 #pragma unroll
-            for (int j = 0; j < P; ++j)
+                for (int j = 0; j < P; ++j)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (8 * (t + LANES * j) + i < cols && (odd || fabsf(v[j][i]) >= from))
-                        mask |= 1ull << (8 * j + i);
-            while (mask) {
-                const int at = __builtin_ctzll(mask);
-                mask &= mask - 1;
-                const double y = fabs(value64<OP, F16, WF32>(a, row, 8 * (t + LANES * (at >> 3)) + (at & 7)));
-                best = max64(best, __builtin_bit_cast(uint64_t, y));  // (a NaN is above all)
+                    for (int i = 0; i < 8; ++i)
+                        if (fabsf(v[j][i]) == top)
+                            more = fmaxf(more, copysignf(1.f, v[j][i]) * lost[j][i]);
+                best = __builtin_bit_cast(uint64_t, (double)top + (double)more);  // (not negative)
+            } else {
+                const float from = odd ? -1.f : top * kNearMost;
+                uint64_t mask = 0;
+#pragma unroll
+                for (int j = 0; j < P; ++j)
+                    if (odd || most32[j] >= from) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (8 * (t + LANES * j) + i < cols && (odd || fabsf(v[j][i]) >= from))
+                                mask |= 1ull << (8 * j + i);
+                    }
+                while (mask) {
+                    const int at = __builtin_ctzll(mask);
+                    mask &= mask - 1;
+                    const double y = fabs(value64<OP, F16, WF32>(a, row, 8 * (t + LANES * (at >> 3)) + (at & 7)));
+                    best = max64(best, __builtin_bit_cast(uint64_t, y));  // (a NaN is above all)
+                }
             }
             best = wave_max64(best);
             if constexpr (kWaves > 1) {
@@ -377,33 +417,33 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) act_quant_kernel(Qu
             }
             most = __builtin_bit_cast(double, best);
         }
-        const bool finite = most < HUGE_VAL;
-        if (t == 0)
-            a.scales[row * a.s_stride] = finite ? (float)(most * r / 127.0) : __builtin_nanf("");
-        const float inv = (float)(127.0 / most);
+        const float inv = 127.f * __builtin_amdgcn_rcpf((float)most);
         uint64_t near = 0;
 #pragma unroll
         for (int j = 0; j < P; ++j) {
+            constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low byte is the rounded value's
             const int e0 = 8 * (t + LANES * j);
             uint32_t m[8];
-            uint32_t mask = 0;
+            float off[8], worst = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low byte is the rounded value's
-                const float q = v[j][i] * inv, s = q + kMagic;
+                const float s = fmaf(v[j][i], inv, kMagic);
                 m[i] = __float_as_uint(s);
-                mask |= fabsf(q - (s - kMagic)) > kBorderI8 ? 1u << i : 0u;
+                off[i] = fmaf(v[j][i], inv, -(s - kMagic));
+                if (i & 1)
+                    worst = max3_abs(worst, off[i - 1], off[i]);
             }
             const uint32_t lo = __builtin_amdgcn_perm(__builtin_amdgcn_perm(m[3], m[2], 0x0c0c0400u),
                                                       __builtin_amdgcn_perm(m[1], m[0], 0x0c0c0400u), 0x05040100u);
             const uint32_t hi = __builtin_amdgcn_perm(__builtin_amdgcn_perm(m[7], m[6], 0x0c0c0400u),
                                                       __builtin_amdgcn_perm(m[5], m[4], 0x0c0c0400u), 0x05040100u);
             store_codes(crow, e0, cols, lo, hi);
-            if (odd) {
-                const int left = cols - e0;
-                mask = left >= 8 ? 0xffu : left > 0 ? (1u << left) - 1 : 0u;
+            if (odd || worst > kBorderI8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (e0 + i < cols && (odd || fabsf(off[i]) > kBorderI8))
+                        near |= 1ull << (8 * j + i);
             }
-            near |= (uint64_t)mask << (8 * j);
         }
         while (near) {
             const int at = __builtin_ctzll(near);
@@ -411,52 +451,78 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) act_quant_kernel(Qu
             const int e = 8 * (t + LANES * (at >> 3)) + (at & 7);
             crow[e] = code64_i8(value64<OP, F16, WF32>(a, row, e), most);
         }
+        if (t == 0)
+            a.scales[row * a.s_stride] = most < HUGE_VAL ? (float)(most * factor(127.0)) : __builtin_nanf("");
     } else {
         // ---- e4m3fn: one scale per 16 threads and piece (cols a multiple of 128: a group is whole or absent) ----
+        const double each = factor(448.0);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const int e0 = 8 * (t + LANES * j);
             if (e0 >= cols)
                 continue;
-            const uint32_t m = row16_max(mx[j]);
+            const uint32_t m = row16_max(__float_as_uint(most32[j]) & 0x7fffffffu);
             const bool odd = !(m >= kLeast && m <= kMost);  // (the same in the 16 threads)
-            double most = __uint_as_float(m);
+            const float top = __uint_as_float(m);
+            double most = top;
             if (!kExact32 || odd) {
-                const float from = __uint_as_float(m) * kNearMost;
-                uint32_t mask = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    mask |= odd || fabsf(v[j][i]) >= from ? 1u << i : 0u;
                 uint64_t best = 0;
-                while (mask) {
-                    const int at = __builtin_ctz(mask);
-                    mask &= mask - 1;
-                    best = max64(best, __builtin_bit_cast(uint64_t, fabs(value64<OP, F16, WF32>(a, row, e0 + at))));
+                if (kWithLost && !odd) {
+                    float more = -top;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (fabsf(v[j][i]) == top)
+                            more = fmaxf(more, copysignf(1.f, v[j][i]) * lost[kWithLost ? j : 0][i]);
+                    best = __builtin_bit_cast(uint64_t, (double)top + (double)more);
+                } else {
+                    const float from = odd ? -1.f : top * kNearMost;
+                    uint32_t mask = 0;
+                    if (odd || most32[j] >= from) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            mask |= odd || fabsf(v[j][i]) >= from ? 1u << i : 0u;
+                    }
+                    while (mask) {
+                        const int at = __builtin_ctz(mask);
+                        mask &= mask - 1;
+                        best = max64(best,
+                                     __builtin_bit_cast(uint64_t, fabs(value64<OP, F16, WF32>(a, row, e0 + at))));
+                    }
                 }
                 most = __builtin_bit_cast(double, row16_max64(best));
             }
-            const bool finite = most < HUGE_VAL;
-            if ((t & 15) == 0)
-                a.scales[row * a.s_stride + e0 / kGroup] = finite ? (float)(most * r / 448.0) : __builtin_nanf("");
-            const float inv = (float)(448.0 / most);
-            uint32_t near = 0;
-            float q[8];
+            const float inv = 448.f * __builtin_amdgcn_rcpf((float)most);
+            float q[8], over[8], worst = -1.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 8; ++i)
                 q[i] = v[j][i] * inv;
-                // in steps of e4m3fn at this magnitude: 8 to a binade, 2^-9 below 2^-6
-                const int e = max(__builtin_amdgcn_frexp_expf(q[i]), -5);
-                const float k = __builtin_ldexpf(q[i], 4 - e);
-                near |= fabsf(k - rintf(k)) > kBorderFp8 ? 1u << i : 0u;
+            const uint32_t lo = pack_fp8x4(q[0], q[1], q[2], q[3]), hi = pack_fp8x4(q[4], q[5], q[6], q[7]);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const auto r = i & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(i < 4 ? lo : hi, true)
+                                     : __builtin_amdgcn_cvt_pk_f32_fp8(i < 4 ? lo : hi, false);
+#pragma unroll
+                for (int k = i; k < i + 2; ++k) {
+                    // half a step of e4m3fn at this magnitude: 2^-4 of its power of two, 2^-10 below 2^-6
+                    const float binade = fmaxf(__uint_as_float(__float_as_uint(q[k]) & 0x7f800000u), 0x1p-6f);
+                    over[k] = fmaf(binade, -kBorderFp8, fabsf(q[k] - r[k - i]));
+                }
+                worst = __builtin_elementwise_maximum(worst, __builtin_elementwise_maximum(over[i], over[i + 1]));
             }
-            store_codes(crow, e0, cols, pack_fp8x4(q[0], q[1], q[2], q[3]), pack_fp8x4(q[4], q[5], q[6], q[7]));
-            if (odd)
-                near = 0xffu;
-            while (near) {
-                const int at = __builtin_ctz(near);
-                near &= near - 1;
-                crow[e0 + at] = code64_fp8(value64<OP, F16, WF32>(a, row, e0 + at), most);
+            store_codes(crow, e0, cols, lo, hi);
+            if (odd || worst > 0.f) {
+                uint32_t near = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    near |= odd || over[i] > 0.f ? 1u << i : 0u;
+                while (near) {
+                    const int at = __builtin_ctz(near);
+                    near &= near - 1;
+                    crow[e0 + at] = code64_fp8(value64<OP, F16, WF32>(a, row, e0 + at), most);
+                }
             }
+            if ((t & 15) == 0)
+                a.scales[row * a.s_stride + e0 / kGroup] = most < HUGE_VAL ? (float)(most * each) : __builtin_nanf("");
         }
     }
 }
@@ -465,29 +531,45 @@ template <int OP, bool F16, bool WF32, bool FP8, int LANES, int P>
 void launch(const QuantArgs& a, hipStream_t st) {
     constexpr int kRows = LANES < 256 ? 256 / LANES : 1;
     hipLaunchKernelGGL((act_quant_kernel<OP, F16, WF32, FP8, LANES, P>), dim3((unsigned)((a.rows + kRows - 1) / kRows)),
-                       dim3(kRows * LANES), 0, st, a);
+                       dim3(kRows * LANES), 0, st, a, 1);
 }
 
 template <int OP, bool F16, bool WF32, bool FP8>
 int launch_cols(const QuantArgs& a, hipStream_t st) {
     const int pieces = (a.cols + 7) / 8;
-    if (pieces <= 64)
-        launch<OP, F16, WF32, FP8, 64, 1>(a, st);
-    else if (pieces <= 128)
-        launch<OP, F16, WF32, FP8, 64, 2>(a, st);
-    else if (pieces <= 256)
-        launch<OP, F16, WF32, FP8, 64, 4>(a, st);
-    else if (pieces <= 512)
-        launch<OP, F16, WF32, FP8, 256, 2>(a, st);
-    else if (pieces <= 1024)
-        launch<OP, F16, WF32, FP8, 256, 4>(a, st);
-    else if (pieces <= 2048)
-        launch<OP, F16, WF32, FP8, 512, 4>(a, st);
-    else if (pieces <= 4096)
-        launch<OP, F16, WF32, FP8, 1024, 4>(a, st);
-    else
-        launch<OP, F16, WF32, FP8, 1024, 8>(a, st);
-    return launch_status();
+    if constexpr (OP == kSilu && FP8) {
+        // no row has anything in common: a piece per thread, as many workgroups as it takes
+        const int chunks = (pieces + 255) / 256;
+        if (a.rows > 0x7fffffffLL / chunks)
+            return fail(FGV_E_TOO_LARGE, "too many rows of this width");
+        hipLaunchKernelGGL((act_quant_kernel<kSilu, F16, WF32, true, 256, 1>), dim3((unsigned)(a.rows * chunks)),
+                           dim3(256), 0, st, a, chunks);
+        return launch_status();
+    } else {
+        // few rows: a piece per thread as far as a workgroup reaches, the shortest way through a row
+        const bool few = a.rows <= 2 * cu_count();
+        if (pieces <= 64)
+            launch<OP, F16, WF32, FP8, 64, 1>(a, st);
+        else if (few && pieces <= 256)
+            launch<OP, F16, WF32, FP8, 256, 1>(a, st);
+        else if (few && pieces <= 1024)
+            launch<OP, F16, WF32, FP8, 1024, 1>(a, st);
+        else if (pieces <= 128)
+            launch<OP, F16, WF32, FP8, 64, 2>(a, st);
+        else if (pieces <= 256)
+            launch<OP, F16, WF32, FP8, 256, 1>(a, st);
+        else if (pieces <= 512)
+            launch<OP, F16, WF32, FP8, 256, 2>(a, st);
+        else if (pieces <= 1024)
+            launch<OP, F16, WF32, FP8, 256, 4>(a, st);
+        else if (pieces <= 2048)
+            launch<OP, F16, WF32, FP8, 1024, 2>(a, st);
+        else if (pieces <= 4096)
+            launch<OP, F16, WF32, FP8, 1024, 4>(a, st);
+        else
+            launch<OP, F16, WF32, FP8, 1024, 8>(a, st);
+        return launch_status();
+    }
 }
 
 int check_common(const QuantArgs& a, int x_dtype, int code_dtype) {
