@@ -260,8 +260,8 @@ __device__ __forceinline__ void load_weights(const void* weights, int e0, int co
 // `chunks` > 1 a row is shared by that many workgroups, which need nothing of
 // each other (e4m3fn activations).
 template <int OP, bool F16, bool WF32, bool FP8, int LANES, int P>
-__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) act_quant_kernel(QuantArgs a, int32_t chunks) {
-    constexpr int kBlock = LANES < 256 ? 256 : LANES, kWaves = LANES / 64;
+__global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(QuantArgs a, int32_t chunks) {
+    constexpr int kBlock = LANES == 64 ? 256 : LANES, kWaves = LANES / 64;
     constexpr bool kRowScale = !FP8;              // one scale per row, else per 16 threads and piece
     constexpr bool kExact32 = OP == kNorm && !WF32;  // v is exact
     constexpr bool kWithLost = OP == kNorm && WF32;  // v's rounding error is kept
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) act_quant_kernel(Qu
 
 template <int OP, bool F16, bool WF32, bool FP8, int LANES, int P>
 void launch(const QuantArgs& a, hipStream_t st) {
-    constexpr int kRows = LANES < 256 ? 256 / LANES : 1;
+    constexpr int kRows = LANES == 64 ? 4 : 1;
     hipLaunchKernelGGL((act_quant_kernel<OP, F16, WF32, FP8, LANES, P>), dim3((unsigned)((a.rows + kRows - 1) / kRows)),
                        dim3(kRows * LANES), 0, st, a, 1);
 }
@@ -546,24 +546,36 @@ int launch_cols(const QuantArgs& a, hipStream_t st) {
                            dim3(256), 0, st, a, chunks);
         return launch_status();
     } else {
-        // few rows: a piece per thread as far as a workgroup reaches, the shortest way through a row
+        // As few idle lanes as may be, and 256 threads to a workgroup while there
+        // are rows enough: 8192 rows of 4096, 7168, 16384 columns: 256 x 2 46.1
+        // us (512 x 1 50.6), 256 x 4 75.0 (512 x 2 77.4, 1024 x 1 85.8), of the
+        // activation 256 x 8 121 (512 x 4 149); with two rows to a CU or less the
+        // shortest way through a row counts: one row of 7168 1024 x 1 3.7 (256 x 4
+        // 5.7), 512 rows 9.1 (10.3), but 1024 rows 15.3 (15.2); up to eight rows
+        // to a CU of 4096 512 x 1: 2047 rows 14.9 (256 x 2 16.0).
         const bool few = a.rows <= 2 * cu_count();
         if (pieces <= 64)
             launch<OP, F16, WF32, FP8, 64, 1>(a, st);
-        else if (few && pieces <= 256)
-            launch<OP, F16, WF32, FP8, 256, 1>(a, st);
-        else if (few && pieces <= 1024)
-            launch<OP, F16, WF32, FP8, 1024, 1>(a, st);
         else if (pieces <= 128)
-            launch<OP, F16, WF32, FP8, 64, 2>(a, st);
+            launch<OP, F16, WF32, FP8, 128, 1>(a, st);
         else if (pieces <= 256)
             launch<OP, F16, WF32, FP8, 256, 1>(a, st);
+        else if (pieces <= 512 && a.rows <= 8 * cu_count())
+            launch<OP, F16, WF32, FP8, 512, 1>(a, st);
         else if (pieces <= 512)
             launch<OP, F16, WF32, FP8, 256, 2>(a, st);
+        else if (pieces <= 1024 && few)
+            launch<OP, F16, WF32, FP8, 1024, 1>(a, st);
+        else if (pieces <= 768)
+            launch<OP, F16, WF32, FP8, 256, 3>(a, st);
         else if (pieces <= 1024)
             launch<OP, F16, WF32, FP8, 256, 4>(a, st);
-        else if (pieces <= 2048)
+        else if (pieces <= 2048 && few)
             launch<OP, F16, WF32, FP8, 1024, 2>(a, st);
+        else if (pieces <= 1536)
+            launch<OP, F16, WF32, FP8, 512, 3>(a, st);
+        else if (pieces <= 2048)
+            launch<OP, F16, WF32, FP8, OP == kSilu ? 256 : 512, OP == kSilu ? 8 : 4>(a, st);
         else if (pieces <= 4096)
             launch<OP, F16, WF32, FP8, 1024, 4>(a, st);
         else
