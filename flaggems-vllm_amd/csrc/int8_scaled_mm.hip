@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(256) int8_mm_sum_kernel(MmArgs p, const int32_
 // ---- rows that the tiles cannot take as they are ----
 // Rows whose start or stride is no multiple of 16 bytes, or whose K is none of
 // 128, are copied to rows of a whole number of K blocks, zeros behind K (which
-// add nothing to a sum): 16 bytes per thread, a's rows, then b's.
+// add nothing to a sum): a row per wave, a's rows, then b's.
 struct PackArgs {
     const int8_t* from[2];
     int64_t from_s[2];
@@ -562,13 +562,26 @@ struct PackArgs {
 };
 
 __global__ void __launch_bounds__(256) int8_mm_pack_kernel(PackArgs p) {
-    const int per_row = p.pitch / 16, which = blockIdx.y;
-    const int64_t total = p.rows[which] * per_row;
-    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
-        const int64_t row = u / per_row;
-        const int k = (int)(u - row * per_row) * 16;
-        *reinterpret_cast<v4i_t*>(p.to[which] + row * p.pitch + k) =
-            load_frag_end(p.from[which] + row * p.from_s[which], k, p.k);
+    int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;  // a wave takes a row
+    const int which = row < p.rows[0] ? 0 : 1;
+    row -= which * p.rows[0];
+    if (row >= p.rows[which])
+        return;
+    const int8_t* from = p.from[which] + row * p.from_s[which];
+    int8_t* to = p.to[which] + row * p.pitch;
+    for (int k0 = 16 * (threadIdx.x % 64); k0 < p.pitch; k0 += 4096) {
+        v4i_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // all four in flight
+            v[i] = k0 + 1024 * i + 16 <= p.k ? load_frag(from, k0 + 1024 * i) : v4i_t{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = k0 + 1024 * i;
+            if (k < p.k && k + 16 > p.k)
+                v[i] = load_frag_end(from, k, p.k);
+            if (k < p.pitch)
+                *reinterpret_cast<v4i_t*>(to + k) = v[i];
+        }
     }
 }
 
@@ -576,16 +589,20 @@ __global__ void __launch_bounds__(256) int8_mm_pack_kernel(PackArgs p) {
 
 // The tiles, by what a K block costs a CU that works on one of them (measured
 // at K 7168 with a tile for nearly every CU, us: 64 x 64 21.2, 128 x 64 28.8,
-// 128 x 128 36.9, 256 x 128 52.2, 256 x 256 94 in all, about 3 of them before
-// and behind the K loop).  Below 256 x 256, which the matrix units bound (and at
+// 128 x 128 36.9, 256 x 128 52.2, 192 x 256 79, 256 x 256 94 in all, about 3 of
+// them before and behind the K loop; 128 x 192 25.1 at K 4096).  Sizes between
+// the powers of two are there for the last turn: 6144 x 6144 x 6144 takes 193 us
+// in tiles of 256 x 192, 211 in 256 x 256; 1024 x 4224 x 4096 25 in 128 x 192, 35
+// in 128 x 128.  Below 256 x 192, which the matrix units bound (and at
 // full size the power limit), the loads of the operands' rows do: 52-56 GB/s
 // into a CU, however many blocks are in flight (NS 3, 4 and 5 alike).
 struct TileKind {
     int bm, bn;
     float us_per_block;
 };
-constexpr TileKind kTiles[] = {{64, 64, 0.31f}, {128, 64, 0.43f}, {128, 128, 0.60f}, {256, 128, 0.85f}, {256, 256, 1.5f}};
-constexpr int kTileKinds = 5;
+constexpr TileKind kTiles[] = {{64, 64, 0.31f},   {128, 64, 0.43f},  {128, 128, 0.60f}, {128, 192, 0.69f},
+                               {192, 128, 0.69f}, {256, 128, 0.85f}, {192, 256, 1.38f}, {256, 192, 1.38f}, {256, 256, 1.5f}};
+constexpr int kTileKinds = 9;
 constexpr float kTileFixedUs = 3.f;
 
 struct Plan {
@@ -666,8 +683,12 @@ int launch_mm(MmArgs p, void* workspace, int64_t workspace_bytes, hipStream_t st
     const Plan plan = plan_mm(p.m, p.n, p.k, a_direct, b_direct);
     const bool room = plan.bytes() == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= plan.bytes());
     if (plan.rows || !room) {
+        // two column tiles to a workgroup halve the reads of a's rows, where enough workgroups are left (16 x 7168 x
+        // 7168 17.7 -> 13.9 us; one row of 16384 x 16384 loses)
         if (p.m > 32)
             launch_rows<2, 2, 8, OUT>(p, st);
+        else if (p.m > 2 && p.n >= 16 * cu_count())
+            launch_rows<1, 2, 8, OUT>(p, st);
         else if (p.k >= 16 * kBlockK)
             launch_rows<1, 1, 8, OUT>(p, st);
         else
@@ -683,9 +704,8 @@ int launch_mm(MmArgs p, void* workspace, int64_t workspace_bytes, hipStream_t st
                             {a_direct ? 0 : p.m, b_direct ? 0 : p.n},
                             p.k,
                             pitch};
-        const int64_t most = std::max(pack.rows[0], pack.rows[1]) * (pitch / 16);
-        hipLaunchKernelGGL(int8_mm_pack_kernel, dim3((unsigned)std::min<int64_t>((most + 255) / 256, 1 << 20), 2),
-                           dim3(256), 0, st, pack);
+        hipLaunchKernelGGL(int8_mm_pack_kernel, dim3((unsigned)((pack.rows[0] + pack.rows[1] + 3) / 4)), dim3(256), 0, st,
+                           pack);
         if (!a_direct) {
             p.a = pack.to[0];
             p.a_s = pitch;
@@ -711,7 +731,19 @@ int launch_mm(MmArgs p, void* workspace, int64_t workspace_bytes, hipStream_t st
         launch_tiles<2, 4, 4, 2, 3, OUT>(p, st);
         break;
     case 3:
+        launch_tiles<2, 4, 4, 3, 3, OUT>(p, st);
+        break;
+    case 4:
+        launch_tiles<4, 2, 3, 4, 3, OUT>(p, st);
+        break;
+    case 5:
         launch_tiles<4, 2, 4, 4, 3, OUT>(p, st);
+        break;
+    case 6:
+        launch_tiles<2, 4, 6, 4, 2, OUT>(p, st);
+        break;
+    case 7:
+        launch_tiles<4, 2, 4, 6, 2, OUT>(p, st);
         break;
     default:
         launch_tiles<2, 4, 8, 4, 2, OUT>(p, st);
