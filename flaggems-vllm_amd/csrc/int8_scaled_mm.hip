@@ -108,13 +108,24 @@ __device__ __forceinline__ void store4(const MmArgs& p, int64_t m, int n, const 
 __device__ __forceinline__ v4i_t load_frag(const int8_t* row, int k) {
     return *reinterpret_cast<const v4i_a1*>(row + k);
 }
-// ... of the last, short block: bytes from K on as 0
+// ... of the last, short block: bytes from `end` on as 0.  The chunk that the row
+// ends in is cut out of the row's last 16 bytes (a row of fewer byte by byte).
 __device__ __forceinline__ v4i_t load_frag_end(const int8_t* row, int k, int end) {
     if (k + 16 <= end)
         return load_frag(row, k);
     v4i_t v = {0, 0, 0, 0};
+    if (k >= end)
+        return v;
+    if (end >= 16) {
+        const v4i_t w = load_frag(row, end - 16);
+        const int past = 8 * (k + 16 - end);  // bits to drop, 8 .. 120
+        uint64_t lo = (uint32_t)w[0] | ((uint64_t)(uint32_t)w[1] << 32), hi = (uint32_t)w[2] | ((uint64_t)(uint32_t)w[3] << 32);
+        lo = past < 64 ? (lo >> past) | (hi << (64 - past)) : hi >> (past - 64);
+        hi = past < 64 ? hi >> past : 0;
+        return v4i_t{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+    }
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int i = 0; i < 15; ++i)
         if (k + i < end)
             v[i >> 2] |= (int)((uint32_t)(uint8_t)row[k + i] << (8 * (i & 3)));
     return v;
