@@ -324,7 +324,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) int8_mm_tile_kernel(MmArgs p,
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int c = lane & 15, g = lane >> 4, wm = wave / WN, wn = wave % WN;
-    // the workgroup's K blocks: all, or the part blockIdx.y of them (K is a multiple of 128 here)
+    // the workgroup's K blocks: all, or the part blockIdx.y of them; at least one (K is a multiple of 128 here,
+    // and no 0)
     const int all = p.k / kBlockK;
     const int kb_lo = SPLIT ? (int)((int64_t)all * blockIdx.y / gridDim.y) : 0;
     const int nkb = SPLIT ? (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y) - kb_lo : all;
@@ -409,16 +410,14 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) int8_mm_tile_kernel(MmArgs p,
 #pragma unroll
         for (int j = 0; j < TN; ++j)
             acc[i][j] = v4i_t{0, 0, 0, 0};
-    if (nkb > 0) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
-            read_b(st[0], 0, j);
+    for (int j = 0; j < TN; ++j)
+        read_b(st[0], 0, j);
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
-            read_a(st[0], 0, i);
-    }
-    int at = 0;
-    for (int kb = 0; kb < nkb; ++kb) {
+    for (int i = 0; i < TM; ++i)
+        read_a(st[0], 0, i);
+    int at = 0, kb = 0;
+    do {  // (there is a block: no way around the loop on which the accumulators would have to be moved)
         const uint8_t* cur = st[at];
         at = at + 1 < NS ? at + 1 : 0;
         const uint8_t* nxt = st[at];
@@ -442,8 +441,13 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) int8_mm_tile_kernel(MmArgs p,
                 issue(kb + NS, dst, u / kSendEvery, lanes);
             __builtin_amdgcn_sched_barrier(0);
         }
-    }
+    } while (++kb < nkb);
     mfma_done();
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            asm volatile("" : "+a"(acc[i][j]));  // (no read of it moves in front of the wait)
 
     const int nb = n0 + wn * 16 * TN, mb = m0 + wm * 16 * TM;
     if constexpr (SPLIT) {
