@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "flaggems_vllm_amd.h"
 
 namespace fgv {
@@ -21,12 +23,19 @@ inline int launch_status() {
     return e == hipSuccess ? FGV_OK : static_cast<int>(e);
 }
 
-// CUs of the current device (256 on MI355X).
+// CUs of the current device (256 on MI355X), asked once per device.
 inline int cu_count() {
+    static std::atomic<int> known[64];
     int dev = 0, cus = 0;
-    if (hipGetDevice(&dev) != hipSuccess ||
-        hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
-        cus = 256;
+    if (hipGetDevice(&dev) != hipSuccess)
+        return 256;
+    const bool kept = dev >= 0 && dev < 64;
+    if (kept && (cus = known[dev].load(std::memory_order_relaxed)) > 0)
+        return cus;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
+        return 256;
+    if (kept)
+        known[dev].store(cus, std::memory_order_relaxed);
     return cus;
 }
 

@@ -290,9 +290,18 @@ __device__ __forceinline__ void mfma_done() { asm volatile("s_nop 15\n\ts_nop 7"
 constexpr int kXcds = 8;
 
 // Tile of workgroup `at`: workgroups go to the XCDs in turn, and each XCD, with
-// an L2 of its own, takes a run of tiles in which kGroupM tiles along m share
-// their b rows and neighbouring n share the a rows.
-constexpr int kGroupM = 4;
+// an L2 of its own, takes a run of tiles in which group_m tiles along m share
+// their b rows and neighbouring n share the a rows: so many that the 32 tiles its
+// CUs work on together read as few different rows as may be, g bm = 32 / g bn.
+// (256 x 256 tiles, us, g = 2, 4, 6, 8, 16: 8192 x 7168 x 7168 341, 346, 332, 344,
+// 355; 8192^3 413, 407, 395, 407, 419.)
+constexpr int group_m(int bm, int bn) {
+    int g = 1;
+    while ((2 * g + 1) * (2 * g + 1) * bm <= 4 * 32 * bn)
+        ++g;
+    return g;
+}
+template <int kGroupM>
 __device__ __forceinline__ void tile_of(int at, int mtiles, int ntiles, int& mt, int& nt) {
     const int total = mtiles * ntiles, xcd = at % kXcds, each = total / kXcds, more = total % kXcds;
     const int t = xcd * each + min(xcd, more) + at / kXcds;
@@ -331,7 +340,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) int8_mm_tile_kernel(MmArgs p,
     const int nkb = SPLIT ? (int)((int64_t)all * (blockIdx.y + 1) / gridDim.y) - kb_lo : all;
 
     int mt, nt;
-    tile_of(blockIdx.x, mtiles, ntiles, mt, nt);
+    tile_of<group_m(kBM, kBN)>(blockIdx.x, mtiles, ntiles, mt, nt);
     const int m0 = mt * kBM, n0 = nt * kBN;
 
     // This lane's DMA sources, relative to the tile's first row: instruction j of
