@@ -18,8 +18,8 @@
 // same way: of float32 weights by the products' rounding errors, which an FMA
 // gives exactly, of the activation by computing every element within 2^-19 of
 // the binary32 maximum again.  Where the binary32 values leave the range in which
-// these bounds hold (a row of zeros, of values below 2^-60 or above 2^120, up
-// values above 2^20, NaN, infinities), all elements under the scale go that way.
+// these bounds hold (a row of zeros, of values below 2^-60 or above 2^120,
+// gates or up values above 2^20, NaN, infinities), all elements under the scale go that way.
 //
 // Bound by memory: 7 bytes per element with a residual (x, residual, hidden,
 // code), 3 without, 5 for the activation.  A row is read once and held in
@@ -126,7 +126,10 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int e0, int cols, uint
 // The exponent g log2(e) is split into an integer and a fraction known to 2^-25,
 // so that v_exp_f32's argument keeps its low bits (one rounding of g log2(e)
 // alone would cost 2^-17 at g = -88).  The exponent stops at g = +-86, where the
-// sigmoid is 1 or below 2^-124.
+// sigmoid is 1 or below 2^-124: further out on the negative side the product is
+// too large, by no more than |g u| 2^-124.  With both factors within kWide that is
+// 2^-84, under 2^-15 of a code's unit where the largest magnitude is kLeast or more
+// (448 * 2^-84 / 2^-60), so the code is 0 as it should be.
 __device__ __forceinline__ float silu_mul32(float g, float u) {
     constexpr float kLog2e = 0x1.715476p0f, kLog2eLo = 0x1.4ae0cp-26f;  // log2(e) = their sum to 2^-49
     constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the rounded value's
@@ -216,7 +219,9 @@ __device__ __forceinline__ float max3_abs(float m, float a, float b) {
 // binary32 magnitudes between these (as bits) keep the fast path's bounds
 constexpr uint32_t kLeast = (127 - 60) << 23, kMost = (127 + 120) << 23;
 constexpr float kNearMost = 1.0f - 0x1p-19f;  // nearer to the maximum than this: settled in binary64
-constexpr float kWideUp = 0x1p20f;  // up values above could bring a product back from below binary32's range
+// Gates and up values above this go the 64-bit way: an up value could bring a product
+// back from below binary32's range, a gate outweigh the least sigmoid.
+constexpr float kWide = 0x1p20f;
 // Distance from the nearest code at which an element counts as beside a border.
 // int8: 0.5 - 2^-13 of a step (127 * 2^-20.4 < 2^-13); e4m3fn: half a step times
 // 1 - 2^-14 (the step is at least 2^-4 of the value: 16 * 2^-20.4 < 2^-15).
@@ -304,14 +309,17 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
                 float widest = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
+                    const float g0 = lo_of<F16>(p0[j][i >> 1]), g1 = hi_of<F16>(p0[j][i >> 1]);
                     const float u0 = lo_of<F16>(p1[j][i >> 1]), u1 = hi_of<F16>(p1[j][i >> 1]);
-                    v[j][i] = silu_mul32(lo_of<F16>(p0[j][i >> 1]), u0);
-                    v[j][i + 1] = silu_mul32(hi_of<F16>(p0[j][i >> 1]), u1);
+                    v[j][i] = silu_mul32(g0, u0);
+                    v[j][i + 1] = silu_mul32(g1, u1);
                     most = max3_abs(most, v[j][i], v[j][i + 1]);
-                    if constexpr (!F16)  // (fp16 ends at 65504)
+                    if constexpr (!F16) {  // (fp16 ends at 65504, and its infinities reach the product)
                         widest = max3_abs(widest, u0, u1);
+                        widest = max3_abs(widest, g0, g1);
+                    }
                 }
-                if (!F16 && !(widest <= kWideUp))
+                if (!F16 && !(widest <= kWide))
                     most = __builtin_nanf("");
             } else {
                 float w[8];

@@ -348,6 +348,25 @@ def test_gpu_silu_extremes(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [I8, F8])
+@pytest.mark.parametrize("gate", [-60.0, -85.0, -87.0, -104.0, -2.0 ** 20, -2.0 ** 30, -1e20, -1e38, -3e38])
+def test_gpu_silu_far_negative_gates(dtype, gate):
+    """Gates of which nothing is left, one or many to a row, beside ordinary values, under small and large up
+    values: their products are 0, however far out they lie, and the largest magnitude is the others'."""
+    _say(f"silu far negative gates {gate} {dtype}")
+    cols = 256
+    x = _gate_up(6, cols, BF16, 38)
+    g, u = x[:, :cols], x[:, cols:]
+    g[0, 17] = gate
+    g[1, ::2] = gate
+    g[2] = gate                       # nothing else in the row
+    g[3, 5], u[3, 5] = gate, 1e6
+    g[4, 5], u[4, 5] = gate, 3e38
+    g[5, 1::2], u[5, 0::2] = gate, 1e-12
+    check_silu(x, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [I8, F8])
 def test_gpu_silu_strided(dtype):
     """Rows out of a wider buffer, at an odd offset."""
     _say(f"silu strided {dtype}")
