@@ -535,11 +535,31 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
     }
 }
 
+// A launch has fewer than 2^32 threads: more rows than that go in several.
+constexpr int64_t kLaunchThreads = 1LL << 31;
+QuantArgs rows_from(QuantArgs a, int64_t first, int64_t rows) {
+    a.x += first * a.x_stride;
+    if (a.residual) {
+        a.residual += first * a.r_stride;
+        a.hidden += first * a.h_stride;
+    }
+    a.codes += first * a.c_stride;
+    a.scales += first * a.s_stride;
+    a.rows = rows;
+    return a;
+}
+
+// `chunks` workgroups to a row, or kRows rows to a workgroup.
 template <int OP, bool F16, bool WF32, bool FP8, int LANES, int P>
-void launch(const QuantArgs& a, hipStream_t st) {
+void launch(const QuantArgs& a, hipStream_t st, int chunks = 1) {
     constexpr int kRows = LANES == 64 ? 4 : 1;
-    hipLaunchKernelGGL((act_quant_kernel<OP, F16, WF32, FP8, LANES, P>), dim3((unsigned)((a.rows + kRows - 1) / kRows)),
-                       dim3(kRows * LANES), 0, st, a, 1);
+    const int64_t most = kLaunchThreads / (LANES * chunks);
+    for (int64_t r = 0; r < a.rows; r += most) {
+        const QuantArgs s = rows_from(a, r, a.rows - r < most ? a.rows - r : most);
+        hipLaunchKernelGGL((act_quant_kernel<OP, F16, WF32, FP8, LANES, P>),
+                           dim3((unsigned)((s.rows + kRows - 1) / kRows * chunks)), dim3(kRows * LANES), 0, st, s,
+                           chunks);
+    }
 }
 
 template <int OP, bool F16, bool WF32, bool FP8>
@@ -547,11 +567,7 @@ int launch_cols(const QuantArgs& a, hipStream_t st) {
     const int pieces = (a.cols + 7) / 8;
     if constexpr (OP == kSilu && FP8) {
         // no row has anything in common: a piece per thread, as many workgroups as it takes
-        const int chunks = (pieces + 255) / 256;
-        if (a.rows > 0x7fffffffLL / chunks)
-            return fail(FGV_E_TOO_LARGE, "too many rows of this width");
-        hipLaunchKernelGGL((act_quant_kernel<kSilu, F16, WF32, true, 256, 1>), dim3((unsigned)(a.rows * chunks)),
-                           dim3(256), 0, st, a, chunks);
+        launch<kSilu, F16, WF32, true, 256, 1>(a, st, (pieces + 255) / 256);
         return launch_status();
     } else {
         // As few idle lanes as may be, and 256 threads to a workgroup while there

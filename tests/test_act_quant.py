@@ -390,6 +390,76 @@ def test_gpu_silu_every_bf16_gate():
 
 # ----------------------------------------------------------- both, elsewhere ----
 
+def _free_gib():
+    return torch.cuda.mem_get_info()[0] / 2 ** 30
+
+
+@pytest.mark.gpu
+def test_gpu_norm_more_rows_than_a_launch():
+    """2^25 + 9 rows of 8 columns, 64 threads to a row: 2^31 threads and more, so the call takes two launches."""
+    _say("norm 2^25 + 9 rows")
+    rows = 2 ** 25 + 9
+    g = torch.Generator(DEV).manual_seed(40)
+    x = torch.randn(rows, 8, generator=g, device=DEV, dtype=BF16)
+    res = torch.randn(rows, 8, generator=g, device=DEV, dtype=BF16)
+    w = _weight(8, BF16, 41).to(DEV)
+    codes, scales, h = fv.fused_add_rms_norm_quant(x, res, w, EPS)
+    for lo in (0, 2 ** 25 - 40, rows - 50):
+        ref = norm64(x[lo:lo + 50].cpu(), res[lo:lo + 50].cpu(), w.cpu(), I8)
+        check_codes(codes[lo:lo + 50], ref[0])
+        check_scales(scales[lo:lo + 50], ref[1])
+        assert torch.equal(h[lo:lo + 50].cpu(), ref[2])
+    for lo in range(0, rows, 2 ** 23):
+        hi = min(rows, lo + 2 ** 23)
+        c, s, hh = fv.fused_add_rms_norm_quant(x[lo:hi], res[lo:hi], w, EPS)
+        assert torch.equal(c, codes[lo:hi]) and torch.equal(s, scales[lo:hi]) and torch.equal(hh, h[lo:hi])
+
+
+@pytest.mark.gpu
+def test_gpu_silu_more_rows_than_a_launch():
+    """2^23 + 9 rows of one 128-column group, 256 threads to a row: two launches, and offsets past 2^32 bytes."""
+    _say("silu 2^23 + 9 rows")
+    if _free_gib() < 16:
+        pytest.skip("needs 16 GiB of device memory")
+    rows = 2 ** 23 + 9
+    x = torch.randn(rows, 256, generator=torch.Generator(DEV).manual_seed(42), device=DEV, dtype=BF16)
+    codes, scales = fv.fused_silu_mul_quant(x, F8)
+    for lo in (0, 2 ** 23 - 40, rows - 50):
+        ref = silu64(x[lo:lo + 50].cpu(), F8)
+        check_codes(codes[lo:lo + 50], ref[0], ref[2])
+        check_scales(scales[lo:lo + 50], ref[1])
+    for lo in range(0, rows, 2 ** 21):
+        hi = min(rows, lo + 2 ** 21)
+        c, s = fv.fused_silu_mul_quant(x[lo:hi], F8)
+        assert torch.equal(c.view(torch.uint8), codes[lo:hi].view(torch.uint8)) and torch.equal(s, scales[lo:hi])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [I8, F8])
+def test_gpu_offsets_past_32_bits(dtype):
+    """33000 rows of 65536 columns: more than 2^31 elements, 2^32 bytes, in each tensor."""
+    _say(f"norm and silu offsets past 32 bits {dtype}")
+    if _free_gib() < 40:
+        pytest.skip("needs 40 GiB of device memory")
+    rows, cols = 33000, 65536
+    x = torch.randn(rows, cols, generator=torch.Generator(DEV).manual_seed(43), device=DEV, dtype=BF16)
+    res = x.flip(0)
+    w = _weight(cols, BF16, 44).to(DEV)
+    codes, scales, h = fv.fused_add_rms_norm_quant(x, res, w, EPS, dtype)
+    for lo in (0, 32766, rows - 2):
+        ref = norm64(x[lo:lo + 2].cpu(), res[lo:lo + 2].cpu(), w.cpu(), dtype)
+        check_codes(codes[lo:lo + 2], ref[0])
+        check_scales(scales[lo:lo + 2], ref[1])
+        assert torch.equal(h[lo:lo + 2].cpu(), ref[2])
+    del res, h, codes, scales
+    both = torch.cat([x, x.flip(0)], 1)
+    codes, scales = fv.fused_silu_mul_quant(both, dtype)
+    for lo in (0, 32766, rows - 2):
+        ref = silu64(both[lo:lo + 2].cpu(), dtype)
+        check_codes(codes[lo:lo + 2], ref[0], ref[2])
+        check_scales(scales[lo:lo + 2], ref[1])
+
+
 @pytest.mark.gpu
 def test_gpu_no_rows():
     _say("no rows")

@@ -149,6 +149,40 @@ def test_gpu_every_tile_writes_its_rows_only(m, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(40000, 60000, 128),      # the output: 2^31 elements and more
+                                   (2 ** 20, 72, 4224),      # a: past 2^32 bytes, straight and (next) packed
+                                   (2 ** 20, 72, 4223),
+                                   (5, 2 ** 21, 2176),       # b: the same, rows from memory
+                                   (300, 2 ** 21, 2176),     # b: in tiles, straight and packed
+                                   (300, 2 ** 21, 2175)])
+def test_gpu_offsets_past_32_bits(m, n, k):
+    """The first and last rows and channels, and those each side of the middle."""
+    _say(f"int8 mm {m} x {n} x {k}")
+    if torch.cuda.mem_get_info()[0] < 24 * 2 ** 30:
+        pytest.skip("needs 24 GiB of device memory")
+    g = torch.Generator(DEV).manual_seed(m + n)
+    a = torch.empty(m, k, dtype=torch.int8, device=DEV).random_(-128, 128, generator=g)
+    b = torch.empty(n, k, dtype=torch.int8, device=DEV).random_(-128, 128, generator=g)
+    sa, sb = _scales(m, 3), _scales(n, 4)
+    out = fv.int8_scaled_mm(a, b, sa.to(DEV), sb.to(DEV))
+    pick = [torch.unique(torch.cat([torch.arange(min(40, x)), torch.arange(max(0, x // 2 - 20), min(x, x // 2 + 20)),
+                                    torch.arange(max(0, x - 40), x)])) for x in (m, n)]
+    rows, cols = pick[0].to(DEV), pick[1].to(DEV)
+    check(out[rows][:, cols], a[rows], b[cols], sa[pick[0]], sb[pick[1]], None, BF16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [20, 300, 1500])
+def test_gpu_broadcast_rows(m):
+    """One row of a for every token and one of b for every channel, as expanded views, under one scale each."""
+    _say(f"int8 mm broadcast rows {m}")
+    a, b = _codes(1, 640, 1), _codes(1, 640, 2)
+    sa, sb = torch.tensor([0.01]), torch.tensor([0.02])
+    out = fv.int8_scaled_mm(a.to(DEV).expand(m, 640), b.to(DEV).expand(600, 640), sa.to(DEV), sb.to(DEV))
+    check(out, a.expand(m, 640), b.expand(600, 640), sa, sb, None, BF16)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", [(300, 300, 5120), (1000, 1030, 1111), (300, 700, 384), (2000, 3000, 256)])
 def test_gpu_without_workspace(m, n, k):
     """The C ABI without a workspace, or with one too small: the same bits straight from memory."""
