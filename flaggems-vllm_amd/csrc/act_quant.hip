@@ -140,20 +140,28 @@ __device__ __forceinline__ float silu_mul32(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
+__device__ __forceinline__ double silu_mul64(double g, double u) { return g / (1.0 + exp(-g)) * u; }
+
 // Element e of the row in binary64.  h is read back from hidden where there
 // is a residual (this thread wrote it).
 template <int OP, bool F16, bool WF32>
 __device__ __forceinline__ double value64(const QuantArgs& a, int64_t row, int e) {
     if constexpr (OP == kSilu) {
         const uint16_t* x = a.x + row * a.x_stride;
-        const double g = elem<F16>(x[e]), u = elem<F16>(x[a.cols + e]);
-        return g / (1.0 + exp(-g)) * u;
+        return silu_mul64(elem<F16>(x[e]), elem<F16>(x[a.cols + e]));
     } else {
         const double h = elem<F16>(a.residual ? a.hidden[row * a.h_stride + e] : a.x[row * a.x_stride + e]);
         const double w = WF32 ? reinterpret_cast<const float*>(a.w)[e]
                               : elem<F16>(reinterpret_cast<const uint16_t*>(a.w)[e]);
         return h * w;
     }
+}
+
+// Element i of a piece, where reading it again would cost another memory latency.
+template <bool F16>
+__device__ __forceinline__ float elem_of(u32x4_t p, int i) {
+    const uint32_t w = i & 4 ? (i & 2 ? p[3] : p[2]) : (i & 2 ? p[1] : p[0]);
+    return i & 1 ? hi_of<F16>(w) : lo_of<F16>(w);
 }
 
 // The int8 code of v under the largest magnitude `most` (0 for a row of zeros
@@ -261,13 +269,24 @@ __device__ __forceinline__ void load_weights(const void* weights, int e0, int co
     }
 }
 
-// One row per LANES threads (64: four rows to a workgroup; else one).  With
-// `chunks` > 1 a row is shared by that many workgroups, which need nothing of
-// each other (e4m3fn activations).
+// One row per LANES threads (64: four rows to a workgroup; else one).  The
+// e4m3fn activation, whose groups of 128 columns need nothing of each other,
+// gives a wave 512 columns of a row and a second grid dimension the rest of it.
+// It is bound by the vector instructions (some 370 for a wave's 512 elements,
+// among them one evaluation in 64 bits that settles the groups' maxima), so the
+// elements for that come out of registers, not out of memory again: 8192 rows of
+// 16384 columns 159 us (256 threads to 2048 columns, a division for the row and
+// loads again 168), 65536 rows of 512 44 (60), 256 rows of 2048 4.0 (4.5), but
+// 2048 rows of 8192 25.0 (24.1).  Sixteen elements per thread, half the 64-bit
+// evaluations, took 170.
 template <int OP, bool F16, bool WF32, bool FP8, int LANES, int P>
-__global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(QuantArgs a, int32_t chunks) {
+__global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(QuantArgs a) {
     constexpr int kBlock = LANES == 64 ? 256 : LANES, kWaves = LANES / 64;
     constexpr bool kRowScale = !FP8;              // one scale per row, else per 16 threads and piece
+    constexpr bool kAlone = OP == kSilu && FP8;  // a wave by itself
+    // The piece stays in registers for its 64-bit evaluations (int8, 4096 rows of 2048 columns: 13.6 us, read again
+    // 14.3; but with four rows to a workgroup, 65536 of 512, the selection costs more than the wait: 43.7 and 41.1).
+    constexpr bool kKeep = OP == kSilu && P == 1 && (FP8 || LANES > 64);
     constexpr bool kExact32 = OP == kNorm && !WF32;  // v is exact
     constexpr bool kWithLost = OP == kNorm && WF32;  // v's rounding error is kept
     __shared__ double sum_of[kWaves];
@@ -276,9 +295,10 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
 
     int64_t row = (int64_t)blockIdx.x * (kBlock / LANES) + threadIdx.x / LANES;
     int t = threadIdx.x % LANES;
-    if (OP == kSilu && FP8) {
-        row = blockIdx.x / (uint32_t)chunks;
-        t += (int)(blockIdx.x % (uint32_t)chunks) * LANES * P;
+    if constexpr (kAlone) {
+        static_assert(LANES == 64 && P == 1);
+        row = (int64_t)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+        t += (int)blockIdx.x * 64;
     }
     if (row >= a.rows)
         return;  // (only where waves are rows: no barrier below)
@@ -290,6 +310,7 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
     float v[P][8], lost[kWithLost ? P : 1][8];
     double ss = 0.0;
     float most32[P];
+    u32x4_t kept0 = {}, kept1 = {};
     {
         u32x4_t p0[P], p1[P];
 #pragma unroll
@@ -300,6 +321,10 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
                 p1[j] = load_piece(xrow + cols, e0, cols);
             else if (a.residual)
                 p1[j] = load_piece(a.residual + row * a.r_stride, e0, cols);
+        }
+        if constexpr (kKeep) {
+            kept0 = p0[0];
+            kept1 = p1[0];
         }
 #pragma unroll
         for (int j = 0; j < P; ++j) {
@@ -373,6 +398,12 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
             }
         }
     }
+    auto value_at = [&](int j, int i) __attribute__((always_inline)) {  // element i of piece j in 64 bits
+        if constexpr (kKeep)
+            return silu_mul64(elem_of<F16>(kept0, i), elem_of<F16>(kept1, i));
+        else
+            return value64<OP, F16, WF32>(a, row, 8 * (t + LANES * j) + i);
+    };
     // the factor of the scales: the norm's r (NaN for a row that holds a NaN or an infinity) over q
     auto factor = [&](double q) __attribute__((always_inline)) {
         if constexpr (OP == kNorm)
@@ -412,7 +443,7 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
                 while (mask) {
                     const int at = __builtin_ctzll(mask);
                     mask &= mask - 1;
-                    const double y = fabs(value64<OP, F16, WF32>(a, row, 8 * (t + LANES * (at >> 3)) + (at & 7)));
+                    const double y = fabs(value_at(at >> 3, at & 7));
                     best = max64(best, __builtin_bit_cast(uint64_t, y));  // (a NaN is above all)
                 }
             }
@@ -457,7 +488,7 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
             const int at = __builtin_ctzll(near);
             near &= near - 1;
             const int e = 8 * (t + LANES * (at >> 3)) + (at & 7);
-            crow[e] = code64_i8(value64<OP, F16, WF32>(a, row, e), most);
+            crow[e] = code64_i8(value_at(at >> 3, at & 7), most);
         }
         if (t == 0)
             a.scales[row * a.s_stride] = most < HUGE_VAL ? (float)(most * factor(127.0)) : __builtin_nanf("");
@@ -493,8 +524,7 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
                     while (mask) {
                         const int at = __builtin_ctz(mask);
                         mask &= mask - 1;
-                        best = max64(best,
-                                     __builtin_bit_cast(uint64_t, fabs(value64<OP, F16, WF32>(a, row, e0 + at))));
+                        best = max64(best, __builtin_bit_cast(uint64_t, fabs(value_at(j, at))));
                     }
                 }
                 most = __builtin_bit_cast(double, row16_max64(best));
@@ -526,7 +556,7 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
                 while (near) {
                     const int at = __builtin_ctz(near);
                     near &= near - 1;
-                    crow[e0 + at] = code64_fp8(value64<OP, F16, WF32>(a, row, e0 + at), most);
+                    crow[e0 + at] = code64_fp8(value_at(j, at), most);
                 }
             }
             if ((t & 15) == 0)
@@ -535,7 +565,7 @@ __global__ void __launch_bounds__(LANES == 64 ? 256 : LANES) act_quant_kernel(Qu
     }
 }
 
-// A launch has fewer than 2^32 threads: more rows than that go in several.
+// A launch has fewer than 2^32 threads and 2^16 workgroups in its second dimension: more rows go in several.
 constexpr int64_t kLaunchThreads = 1LL << 31;
 QuantArgs rows_from(QuantArgs a, int64_t first, int64_t rows) {
     a.x += first * a.x_stride;
@@ -549,16 +579,17 @@ QuantArgs rows_from(QuantArgs a, int64_t first, int64_t rows) {
     return a;
 }
 
-// `chunks` workgroups to a row, or kRows rows to a workgroup.
 template <int OP, bool F16, bool WF32, bool FP8, int LANES, int P>
-void launch(const QuantArgs& a, hipStream_t st, int chunks = 1) {
+void launch(const QuantArgs& a, hipStream_t st) {
     constexpr int kRows = LANES == 64 ? 4 : 1;
-    const int64_t most = kLaunchThreads / (LANES * chunks);
+    constexpr bool kAlone = OP == kSilu && FP8;
+    const int64_t most = kAlone ? 65535 * kRows : kLaunchThreads / LANES;
     for (int64_t r = 0; r < a.rows; r += most) {
         const QuantArgs s = rows_from(a, r, a.rows - r < most ? a.rows - r : most);
+        const unsigned groups = (unsigned)((s.rows + kRows - 1) / kRows);
         hipLaunchKernelGGL((act_quant_kernel<OP, F16, WF32, FP8, LANES, P>),
-                           dim3((unsigned)((s.rows + kRows - 1) / kRows * chunks)), dim3(kRows * LANES), 0, st, s,
-                           chunks);
+                           kAlone ? dim3((unsigned)(a.cols + 511) / 512, groups) : dim3(groups), dim3(kRows * LANES),
+                           0, st, s);
     }
 }
 
@@ -566,8 +597,7 @@ template <int OP, bool F16, bool WF32, bool FP8>
 int launch_cols(const QuantArgs& a, hipStream_t st) {
     const int pieces = (a.cols + 7) / 8;
     if constexpr (OP == kSilu && FP8) {
-        // no row has anything in common: a piece per thread, as many workgroups as it takes
-        launch<kSilu, F16, WF32, true, 256, 1>(a, st, (pieces + 255) / 256);
+        launch<kSilu, F16, WF32, true, 64, 1>(a, st);
         return launch_status();
     } else {
         // As few idle lanes as may be, and 256 threads to a workgroup while there
