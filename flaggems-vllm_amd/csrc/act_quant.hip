@@ -666,8 +666,8 @@ extern "C" int fgv_add_rms_norm_quant(const void* x, int64_t x_stride, const voi
                       scales, scales_stride, rows, (int32_t)cols, eps};
     if (const int rc = check_common(a, x_dtype, code_dtype))
         return rc;
-    if (!(eps > 0.0))
-        return fail(FGV_E_BAD_SHAPE, "eps must be positive");
+    if (!(eps > 0.0 && eps < HUGE_VAL))
+        return fail(FGV_E_BAD_SHAPE, "eps must be positive and finite");
     if (rows == 0)
         return FGV_OK;
     if (!x || !weight || !codes || !scales || (residual && !hidden))

@@ -24,6 +24,8 @@
 // call the Python wrappers.
 // Launches go on torch's current HIP stream of the tensors' device; nothing
 // synchronises and nothing is read back from the device.
+#include <cmath>
+
 #include <torch/extension.h>
 #include <torch/library.h>
 
@@ -466,7 +468,7 @@ int add_rms_norm_quant(const at::Tensor& x, const std::optional<at::Tensor>& res
                "weight must be [size] and contiguous");
     FGV_ASSERT(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat,
                "weight must have x's type or float32");
-    FGV_ASSERT(eps > 0.0, "eps must be positive");
+    FGV_ASSERT(eps > 0.0 && std::isfinite(eps), "eps must be positive and finite");
     FGV_ASSERT(residual || !hidden_out, "hidden_out needs a residual");
     FGV_ASSERT(weight.device() == x.device(), "all tensors must be on x's device");
     if (residual) {

@@ -51,7 +51,7 @@ def fused_add_rms_norm_quant(
         x: [T, size] bfloat16 or float16, contiguous rows of any row stride.
         residual: like x, or None (then h is x).
         weight: [size], of x's type or float32.
-        eps: added to the mean of h^2, positive.
+        eps: added to the mean of h^2, positive and finite.
         dtype: torch.int8 (a scale per token) or torch.float8_e4m3fn (a scale
             per 128 columns; size a multiple of 128).  size is at most 65536.
         hidden_out: where h is written (x or residual itself, or a tensor apart

@@ -668,7 +668,8 @@ int fgv_fp8_einsum_bhr_hdr_ws(const uint8_t* x, int64_t x_stride_b, int64_t x_st
  *       neither read nor written when residual is NULL.
  *   weight  [cols] of x's type, or float32 (weight_is_fp32).
  *   codes   [rows, cols] bytes; scales [rows, 1 or cols / 128] float32.
- * cols from 1 to 65536, a multiple of 128 for e4m3fn; rows below 2^31; eps > 0.
+ * cols from 1 to 65536, a multiple of 128 for e4m3fn; rows below 2^31; eps > 0 and
+ * finite.
  * Rows need no alignment beyond their elements'.
  */
 int fgv_add_rms_norm_quant(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,

@@ -519,6 +519,7 @@ _SHARED = torch.zeros(4, 600, dtype=BF16)
     (dict(weight=torch.zeros(256, dtype=F16)), "x's type or float32"),
     (dict(eps=0.0), "eps must be positive"),
     (dict(eps=float("nan")), "eps must be positive"),
+    (dict(eps=float("inf")), "eps must be positive"),
     (dict(dtype=torch.uint8), "dtype must be"),
     (dict(dtype=torch.float8_e5m2), "dtype must be"),
     (dict(x=torch.zeros(4, 200, dtype=BF16), residual=None, weight=torch.zeros(200, dtype=BF16), dtype=F8),
@@ -571,7 +572,7 @@ def test_weights_that_train_elsewhere_pass_without_grad_mode():
 
 @pytest.mark.parametrize("kw,code", [
     (dict(rows=-1), -2), (dict(cols=0), -2), (dict(cols=65537), -5), (dict(rows=1 << 31), -5),
-    (dict(cols=200, code=1), -2), (dict(eps=0.0), -2), (dict(kind=2), -2), (dict(code=2), -2),
+    (dict(cols=200, code=1), -2), (dict(eps=0.0), -2), (dict(eps=float("inf")), -2), (dict(kind=2), -2), (dict(code=2), -2),
     (dict(x=None), -1), (dict(codes=None), -1), (dict(scales=None), -1), (dict(w=None), -1),
     (dict(hidden=None), -1), (dict(x=17), -3), (dict(scales=18), -3), (dict(w=18, w32=1), -3), (dict(rows=0, x=None), 0),
 ])
