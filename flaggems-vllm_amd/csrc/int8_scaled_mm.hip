@@ -49,13 +49,27 @@ __device__ __forceinline__ v4i_t mfma_i8(v4i_t a, v4i_t b, v4i_t c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ float bias_at(const MmArgs& p, int n) {
-    if (!p.bias)
-        return 0.f;
-    if (p.bias_type == kOutF32)
-        return reinterpret_cast<const float*>(p.bias)[n];
-    const uint16_t v = reinterpret_cast<const uint16_t*>(p.bias)[n];
-    return p.bias_type == kOutF16 ? (float)__builtin_bit_cast(_Float16, v) : __uint_as_float((uint32_t)v << 16);
+// The bias of four channels from n on (the last one's past the end), 0 without one.  One choice of type for
+// all four, so that their loads are under way together.
+__device__ __forceinline__ void bias4(const MmArgs& p, int n, float v[4]) {
+    if (!p.bias) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            v[q] = 0.f;
+    } else if (p.bias_type == kOutF32) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            v[q] = reinterpret_cast<const float*>(p.bias)[min(n + q, p.n - 1)];
+    } else {
+        uint16_t raw[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            raw[q] = reinterpret_cast<const uint16_t*>(p.bias)[min(n + q, p.n - 1)];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            v[q] = p.bias_type == kOutF16 ? (float)__builtin_bit_cast(_Float16, raw[q])
+                                          : __uint_as_float((uint32_t)raw[q] << 16);
+    }
 }
 
 // Two outputs in one word.
@@ -134,7 +148,10 @@ __device__ __forceinline__ v4i_t load_frag_end(const int8_t* row, int k, int end
 template <int MT, int NW, int KS, int OUT>
 __global__ void __launch_bounds__(64 * KS) int8_mm_rows_kernel(MmArgs p) {
     __shared__ v4i_t part[KS - 1][MT * NW][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    // K blocks whose loads go together: two where a wave has two column tiles (16 x 7168 x 7168 14.5 us, one 15.4);
+    // with one, more in flight slows the stream of b down (1 x 7168 x 7168 11.0 us, two 11.5, four 11.8)
+    constexpr int kBatch = MT * NW == 1 ? 1 : 2;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * 16 * NW, m0 = blockIdx.y * 16 * MT;
     // rows past the end read the last one: they only feed outputs that are not stored
@@ -153,28 +170,56 @@ __global__ void __launch_bounds__(64 * KS) int8_mm_rows_kernel(MmArgs p) {
 #pragma unroll
         for (int j = 0; j < NW; ++j)
             acc[i][j] = v4i_t{0, 0, 0, 0};
-    const int nkb = p.k / kBlockK;
-    for (int kb = w; kb < nkb; kb += KS) {
-        const int k0 = kb * kBlockK + 16 * g;
-        v4i_t A[MT][2], B[NW][2];
+    // scales and bias, for wave 0 at the end: on their way before the K blocks, so that nothing waits for them
+    float sa[MT], sb[NW][4], bias[NW][4];
+    if (w == 0) {
 #pragma unroll
-        for (int j = 0; j < NW; ++j) {
-            B[j][0] = load_frag(brow[j], k0);
-            B[j][1] = load_frag(brow[j], k0 + 64);
-        }
+        for (int i = 0; i < MT; ++i)
+            sa[i] = p.sa[min(m0 + 16 * i + c, p.m - 1) * p.sa_s];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            A[i][0] = load_frag(arow[i], k0);
-            A[i][1] = load_frag(arow[i], k0 + 64);
-        }
+        for (int j = 0; j < NW; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int q = 0; q < 4; ++q)
+                sb[j][q] = p.sb[min(n0 + 16 * j + 4 * g + q, p.n - 1) * p.sb_s];
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NW; ++j)
-                    acc[i][j] = mfma_i8(B[j][h], A[i][h], acc[i][j]);
+        for (int j = 0; j < NW; ++j)
+            bias4(p, n0 + 16 * j + 4 * g, bias[j]);
     }
+
+    const int nkb = p.k / kBlockK;
+    int kb = w;
+    auto blocks = [&](auto count) __attribute__((always_inline)) {
+        constexpr int kCount = decltype(count)::value;
+        v4i_t A[kCount][MT][2], B[kCount][NW][2];
+#pragma unroll
+        for (int u = 0; u < kCount; ++u) {
+            const int k0 = (kb + KS * u) * kBlockK + 16 * g;
+#pragma unroll
+            for (int j = 0; j < NW; ++j) {
+                B[u][j][0] = load_frag(brow[j], k0);
+                B[u][j][1] = load_frag(brow[j], k0 + 64);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                A[u][i][0] = load_frag(arow[i], k0);
+                A[u][i][1] = load_frag(arow[i], k0 + 64);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kCount; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NW; ++j)
+                        acc[i][j] = mfma_i8(B[u][j][h], A[u][i][h], acc[i][j]);
+        kb += KS * kCount;
+    };
+    while (kb + KS * (kBatch - 1) < nkb)
+        blocks(std::integral_constant<int, kBatch>{});
+    if (kBatch > 1 && kb < nkb)
+        blocks(std::integral_constant<int, 1>{});
     if (nkb * kBlockK < p.k && w == nkb % KS) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -216,16 +261,13 @@ __global__ void __launch_bounds__(64 * KS) int8_mm_rows_kernel(MmArgs p) {
         const int m = m0 + 16 * i + c;
         if (m >= p.m)
             continue;
-        const float sa = p.sa[m * p.sa_s];
 #pragma unroll
         for (int j = 0; j < NW; ++j) {
             const int n = n0 + 16 * j + 4 * g;
             float v[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int nq = min(n + q, p.n - 1);
-                v[q] = (float)acc[i][j][q] * sa * p.sb[nq * p.sb_s] + bias_at(p, nq);
-            }
+            for (int q = 0; q < 4; ++q)
+                v[q] = (float)acc[i][j][q] * sa[i] * sb[j][q] + bias[j][q];
             store4<OUT>(p, m, n, v);
         }
     }
@@ -493,9 +535,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 1) int8_mm_tile_kernel(MmArgs p,
             if constexpr (decltype(with_bias)::value) {
 #pragma unroll
                 for (int j = 0; j < TN; ++j)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        bias[j][q] = bias_at(p, min(nb + 16 * j + 4 * g + q, p.n - 1));
+                    bias4(p, nb + 16 * j + 4 * g, bias[j]);
             }
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
@@ -558,17 +598,19 @@ __global__ void __launch_bounds__(256) int8_mm_sum_kernel(MmArgs p, const int32_
     for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < p.m * fours; u += (int64_t)gridDim.x * 256) {
         const int64_t m = u / fours;
         const int n = (int)(u - m * fours) * 4;
+        const float sa = p.sa[m * p.sa_s];
+        float sb[4], bias[4], v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            sb[q] = p.sb[min(n + q, p.n - 1) * p.sb_s];
+        bias4(p, n, bias);
         const v4i_t* from = reinterpret_cast<const v4i_t*>(part + 4 * u);
         v4i_t sum = from[0];
         for (int z = 1; z < splits; ++z)
             sum += from[z * (slot / 4)];
-        const float sa = p.sa[m * p.sa_s];
-        float v[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int nq = min(n + q, p.n - 1);
-            v[q] = (float)sum[q] * sa * p.sb[nq * p.sb_s] + bias_at(p, nq);
-        }
+        for (int q = 0; q < 4; ++q)
+            v[q] = (float)sum[q] * sa * sb[q] + bias[q];
         store4<OUT>(p, m, n, v);
     }
 }
