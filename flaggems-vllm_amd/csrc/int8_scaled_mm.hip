@@ -23,6 +23,7 @@ typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef v4i_t v4i_a1 __attribute__((aligned(1)));
+typedef v4i_t v4i_a4 __attribute__((aligned(4)));
 
 enum OutType { kOutBf16 = 0, kOutF16 = 1, kOutF32 = 2 };
 constexpr int kBlockK = 128;
@@ -122,6 +123,19 @@ __device__ __forceinline__ void store4(const MmArgs& p, int64_t m, int n, const 
 __device__ __forceinline__ v4i_t load_frag(const int8_t* row, int k) {
     return *reinterpret_cast<const v4i_a1*>(row + k);
 }
+// 32 bytes from row + k of a row that starts at any byte, out of whole words
+// (loads across words keep the address path busy: 8 x 4096 x 4111 15.7 us, so
+// 8.4): `words` is the row rounded down to a word, `past` the bytes that dropped.
+// No word is read that holds none of the 32 bytes.
+__device__ __forceinline__ void load_frags_by_words(const int8_t* words, uint32_t past, int k, v4i_t& lo, v4i_t& hi) {
+    const v4i_t w0 = *reinterpret_cast<const v4i_a4*>(words + k), w1 = *reinterpret_cast<const v4i_a4*>(words + k + 16);
+    const int w2 = *reinterpret_cast<const int*>(words + k + (past ? 32 : 28));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        lo[i] = (int)__builtin_amdgcn_alignbyte((uint32_t)(i < 3 ? w0[i + 1] : w1[0]), (uint32_t)w0[i], past);
+        hi[i] = (int)__builtin_amdgcn_alignbyte((uint32_t)(i < 3 ? w1[i + 1] : w2), (uint32_t)w1[i], past);
+    }
+}
 // ... of the last, short block: bytes from `end` on as 0.  The chunk that the row
 // ends in is cut out of the row's last 16 bytes (a row of fewer byte by byte).
 __device__ __forceinline__ v4i_t load_frag_end(const int8_t* row, int k, int end) {
@@ -145,7 +159,7 @@ __device__ __forceinline__ v4i_t load_frag_end(const int8_t* row, int k, int end
     return v;
 }
 
-template <int MT, int NW, int KS, int OUT>
+template <int MT, int NW, int KS, int OUT, bool SHIFT>
 __global__ void __launch_bounds__(64 * KS) int8_mm_rows_kernel(MmArgs p) {
     __shared__ v4i_t part[KS - 1][MT * NW][64];
     // K blocks whose loads go together: two where a wave has two column tiles (16 x 7168 x 7168 14.5 us, one 15.4);
@@ -193,17 +207,23 @@ __global__ void __launch_bounds__(64 * KS) int8_mm_rows_kernel(MmArgs p) {
         v4i_t A[kCount][MT][2], B[kCount][NW][2];
 #pragma unroll
         for (int u = 0; u < kCount; ++u) {
-            const int k0 = (kb + KS * u) * kBlockK + 16 * g;
+            const int k0 = (kb + KS * u) * kBlockK;
+            // (which 16 bytes of the block a lane group takes does not matter, as long as a's and b's agree)
+            auto load = [&](const int8_t* row, v4i_t to[2]) __attribute__((always_inline)) {
+                if constexpr (SHIFT) {
+                    const uint32_t past = (uint32_t)reinterpret_cast<uintptr_t>(row) & 3;
+                    load_frags_by_words(row - past, past, k0 + 32 * g, to[0], to[1]);
+                } else {
+                    to[0] = load_frag(row, k0 + 16 * g);
+                    to[1] = load_frag(row, k0 + 16 * g + 64);
+                }
+            };
 #pragma unroll
-            for (int j = 0; j < NW; ++j) {
-                B[u][j][0] = load_frag(brow[j], k0);
-                B[u][j][1] = load_frag(brow[j], k0 + 64);
-            }
+            for (int j = 0; j < NW; ++j)
+                load(brow[j], B[u][j]);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                A[u][i][0] = load_frag(arow[i], k0);
-                A[u][i][1] = load_frag(arow[i], k0 + 64);
-            }
+            for (int i = 0; i < MT; ++i)
+                load(arow[i], A[u][i]);
         }
 #pragma unroll
         for (int u = 0; u < kCount; ++u)
@@ -682,7 +702,10 @@ int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // Rows straight from memory while one pass of 16-row workgroups takes all
 // tokens, or the workgroups fit the CUs at once (24 x 2048 x 7168: 9.3 us, 10.2
-// in split tiles; 32 x 7168 x 7168: 19.8 and 16.0).  Else the tile that takes
+// in split tiles; 32 x 7168 x 7168: 19.8 and 16.0).  Where tiles would need the
+// rows packed first also while workgroups of 32 x 32 fit the CUs at once and fill
+// half of them (64 x 4096 x 4111: 11.7 us, packed 20.4; 64 x 7168 x 7001: 45.9
+// and 34.8; 64 x 1031 x 8001, 66 workgroups, 21.3 and 17.8).  Else the tile that takes
 // the least time, counted as whole turns of the CUs; where even the smallest
 // tiles leave more than half the CUs idle they are split along K, at least eight
 // blocks each (128 x 2048 x 7168: 15.1 us, in four parts 12.2).
@@ -690,6 +713,9 @@ Plan plan_mm(int64_t m, int64_t n, int64_t k, bool a_direct, bool b_direct) {
     Plan plan{true, 0, 1, 0, 0, 0};
     const int64_t cus = cu_count(), nkb = (k + kBlockK - 1) / kBlockK;
     if (k == 0 || m <= 16 || (m + 15) / 16 * ((n + 15) / 16) <= cus)
+        return plan;
+    const int64_t squares = (m + 31) / 32 * ((n + 31) / 32);
+    if (!(a_direct && b_direct) && squares <= cus && 2 * squares >= cus)
         return plan;
     plan.rows = false;
     float least = 0.f;
@@ -740,7 +766,11 @@ void launch_split_tiles(const MmArgs& p, int splits, int32_t* part, hipStream_t 
 template <int MT, int NW, int KS, int OUT>
 void launch_rows(const MmArgs& p, hipStream_t st) {
     const dim3 grid((unsigned)((p.n + 16 * NW - 1) / (16 * NW)), (unsigned)((p.m + 16 * MT - 1) / (16 * MT)));
-    hipLaunchKernelGGL((int8_mm_rows_kernel<MT, NW, KS, OUT>), grid, dim3(64 * KS), 0, st, p);
+    const bool words = aligned(p.a, 4) && aligned(p.b, 4) && p.a_s % 4 == 0 && p.b_s % 4 == 0;
+    if (words)
+        hipLaunchKernelGGL((int8_mm_rows_kernel<MT, NW, KS, OUT, false>), grid, dim3(64 * KS), 0, st, p);
+    else
+        hipLaunchKernelGGL((int8_mm_rows_kernel<MT, NW, KS, OUT, true>), grid, dim3(64 * KS), 0, st, p);
 }
 
 template <int OUT>
@@ -749,11 +779,13 @@ int launch_mm(MmArgs p, void* workspace, int64_t workspace_bytes, hipStream_t st
     const Plan plan = plan_mm(p.m, p.n, p.k, a_direct, b_direct);
     const bool room = plan.bytes() == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= plan.bytes());
     if (plan.rows || !room) {
-        // two column tiles to a workgroup halve the reads of a's rows, where enough workgroups are left (16 x 7168 x
-        // 7168 17.7 -> 13.9 us; one row of 16384 x 16384 loses)
-        if (p.m > 32)
+        // two column tiles to a workgroup halve the reads of a's rows, where there are more workgroups than CUs (16 x
+        // 7168 x 7168 16.5 us, one 18.7; 16 x 4096 x 4096 8.0 and 6.2; one row of 16384 x 16384 loses); two row tiles
+        // with them those of b's (32 x 7168 x 7001 28.7, one 35.9; 32 x 4096 x 4111 11.7 and 10.6)
+        const bool wide = p.n > 16 * cu_count();
+        if (p.m > 32 || (p.m > 16 && wide))
             launch_rows<2, 2, 8, OUT>(p, st);
-        else if (p.m > 2 && p.n >= 16 * cu_count())
+        else if (p.m > 2 && wide)
             launch_rows<1, 2, 8, OUT>(p, st);
         else if (p.k >= 16 * kBlockK)
             launch_rows<1, 1, 8, OUT>(p, st);

@@ -172,6 +172,24 @@ def test_gpu_offsets_past_32_bits(m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(1, 70), (3, 4100), (9, 4096), (20, 4111), (31, 130), (40, 4000), (64, 4096), (100, 2000)])
+@pytest.mark.parametrize("k", [127, 129, 383, 1023, 2049, 4111])
+@pytest.mark.parametrize("a_at,b_at", [(0, 0), (1, 2), (3, 1), (2, 3)])
+def test_gpu_few_rows_at_any_byte(m, n, k, a_at, b_at):
+    """Rows that start at any byte of a word, a's and b's apart: what lies before and behind each row in its words
+    must not count.  The neighbours' bytes are the largest there are."""
+    _say(f"int8 mm few rows {m} x {n} x {k} at {a_at}, {b_at}")
+    def placed(codes, at, pad):
+        buf = torch.full((codes.shape[0] * (k + pad) + 16,), 127, dtype=torch.int8, device=DEV)
+        view = buf.as_strided((codes.shape[0], k), (k + pad, 1), at)
+        view.copy_(codes)
+        return view
+    a, b, sa, sb = _codes(m, k, 1), _codes(n, k, 2), _scales(m, 3), _scales(n, 4)
+    out = fv.int8_scaled_mm(placed(a, a_at, 2 - k % 2), placed(b, b_at, 1), sa.to(DEV), sb.to(DEV))
+    check(out, a, b, sa, sb, None, BF16)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [20, 300, 1500])
 def test_gpu_broadcast_rows(m):
     """One row of a for every token and one of b for every channel, as expanded views, under one scale each."""
