@@ -388,6 +388,66 @@ def test_gpu_silu_every_bf16_gate():
     check_silu(torch.cat([gates, torch.ones_like(gates)], 1), F8)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("dtype,cols", [(I8, 9), (I8, 300), (I8, 1000), (I8, 3001), (I8, 9000), (I8, 20000),
+                                        (F8, 128), (F8, 640), (F8, 4224), (F8, 20480)])
+def test_gpu_silu_extremes_at_widths(dtype, cols, kind):
+    """What leaves the binary32 path, in the first, a middle and the last element of rows of every thread layout."""
+    _say(f"silu extremes {dtype} {cols} {kind}")
+    big = torch.finfo(kind).max
+    specials = [(0.0, big), (-big, 1.0), (-big, big), (big, big), (torch.inf, 1.0), (-torch.inf, 1.0), (torch.nan, 0.0),
+                (1.0, torch.inf), (0.0, torch.inf), (-100.0, torch.inf), (1.0, torch.nan), (-20.0, big), (30.0, 1e-5)]
+    places = [0, cols // 2, cols - 1]
+    x = _gate_up(3 * len(specials) + 1, cols, kind, 45)
+    for i, (g, u) in enumerate(specials):
+        for j, at in enumerate(places):
+            x[3 * i + j, at], x[3 * i + j, cols + at] = g, u
+    x[-1] *= 1e-7
+    check_silu(x, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cols", [(I8, 9), (I8, 300), (I8, 1000), (I8, 3001), (I8, 9000), (I8, 20000), (I8, 40000),
+                                        (F8, 128), (F8, 640), (F8, 4224), (F8, 20480)])
+def test_gpu_norm_extremes_at_widths(dtype, cols):
+    """The same of the norm, by the row (infinities, NaN, products past binary32) and by the weight."""
+    _say(f"norm extremes {dtype} {cols}")
+    x, res = _x(14, cols, BF16, 46), _x(14, cols, BF16, 47)
+    for i, at in enumerate((0, cols // 2, cols - 1)):
+        x[i, at] = torch.inf
+        x[3 + i, at] = torch.nan
+        x[6 + i, at] = 3e38
+        x[9 + i] = 0
+        x[9 + i, at] = 1e-38
+    x[12], res[12] = 0, 0
+    w = _weight(cols, F32, 48)
+    check_norm(x, None, w, dtype)
+    check_norm(x, res, w, dtype)
+    for value in (torch.inf, torch.nan, 3e38, 1e-40, -2.0):
+        w = _weight(cols, F32, 48)
+        w[cols // 2] = value
+        check_norm(x, res, w, dtype)
+    check_norm(x, res, torch.zeros(cols, dtype=BF16), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [I8, F8])
+def test_gpu_inference_mode(dtype):
+    """The outputs of calls under inference mode are those of calls outside it."""
+    _say(f"inference mode {dtype}")
+    x = _x(5, 512, BF16, 49).to(DEV)
+    w = _weight(256, BF16, 50).to(DEV)
+    ref = fv.fused_silu_mul_quant(x, dtype), fv.fused_add_rms_norm_quant(x[:, :256], x[:, 256:], w, EPS, dtype)
+    with torch.inference_mode():
+        got = fv.fused_silu_mul_quant(x, dtype), fv.fused_add_rms_norm_quant(x[:, :256], x[:, 256:], w, EPS, dtype)
+        if dtype == I8:
+            mm = fv.int8_scaled_mm(got[0][0], got[1][0], got[0][1], got[1][1])
+            assert torch.equal(mm, fv.int8_scaled_mm(ref[0][0], ref[1][0], ref[0][1], ref[1][1]))
+    for a, b in zip(ref[0] + ref[1], got[0] + got[1]):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 # ----------------------------------------------------------- both, elsewhere ----
 
 def _free_gib():
