@@ -116,7 +116,7 @@ __device__ __forceinline__ void store4(const MmArgs& p, int64_t m, int n, const 
     }
 }
 
-// ---- few rows: fragments straight from memory ----
+// ---- few rows, or few tiles: fragments straight from memory ----
 // Tokens m0 .. m0 + 16 MT, channels n0 .. n0 + 16 NW of a workgroup; its KS
 // waves take the 128-byte K blocks in turn and add their sums up in LDS.
 
@@ -700,22 +700,32 @@ struct Plan {
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Rows straight from memory while one pass of 16-row workgroups takes all
-// tokens, or the workgroups fit the CUs at once (24 x 2048 x 7168: 9.3 us, 10.2
-// in split tiles; 32 x 7168 x 7168: 19.8 and 16.0).  Where tiles would need the
-// rows packed first also while workgroups of 32 x 32 fit the CUs at once and fill
-// half of them (64 x 4096 x 4111: 11.7 us, packed 20.4; 64 x 7168 x 7001: 45.9
-// and 34.8; 64 x 1031 x 8001, 66 workgroups, 21.3 and 17.8).  Else the tile that takes
-// the least time, counted as whole turns of the CUs; where even the smallest
-// tiles leave more than half the CUs idle they are split along K, at least eight
-// blocks each (128 x 2048 x 7168: 15.1 us, in four parts 12.2).
+// Workgroups of mt x nt tiles of 16 x 16.
+int64_t row_groups(int64_t m, int64_t n, int mt, int nt) {
+    return (m + 16 * mt - 1) / (16 * mt) * ((n + 16 * nt - 1) / (16 * nt));
+}
+
+// Rows straight from memory while
+// - one pass of 16-row workgroups takes all tokens, or
+// - workgroups of 16 x 16 have a CU each (256 x 256 x 7168 8.6 us, in split tiles 12), or
+// - workgroups of 16 x 32 have, and the sum is not long enough for split tiles to catch up (us, and in tiles: 24 x
+//   4096 x 4096 8.1, 9.4; 128 x 1024 x 1024 3.5, 4.6; 300 x 300 x 5120 9.3, 9.3; 48 x 2048 x 7168 11.7, 10.8), or tiles
+//   would need the rows packed first (100 x 600 x 1000 4.3, 7.1), or
+// - tiles would need that and workgroups of 32 x 32 have a CU each and fill half of them (64 x 4096 x 4111 11.7, 20.4;
+//   but 64 x 7168 x 7001 45.9, 34.8, and 64 x 1031 x 8001, 66 workgroups, 21.3, 17.8).
+// Else the tile that takes the least time, counted as whole turns of the CUs; where even the smallest tiles leave more
+// than half the CUs idle they are split along K, at least eight blocks each (128 x 2048 x 7168: 15.1 us, in four parts
+// 11.3).
 Plan plan_mm(int64_t m, int64_t n, int64_t k, bool a_direct, bool b_direct) {
     Plan plan{true, 0, 1, 0, 0, 0};
     const int64_t cus = cu_count(), nkb = (k + kBlockK - 1) / kBlockK;
-    if (k == 0 || m <= 16 || (m + 15) / 16 * ((n + 15) / 16) <= cus)
+    const bool direct = a_direct && b_direct;
+    if (k == 0 || m <= 16 || row_groups(m, n, 1, 1) <= cus)
         return plan;
-    const int64_t squares = (m + 31) / 32 * ((n + 31) / 32);
-    if (!(a_direct && b_direct) && squares <= cus && 2 * squares >= cus)
+    if (row_groups(m, n, 1, 2) <= cus && (nkb < 40 || !direct))
+        return plan;
+    const int64_t squares = row_groups(m, n, 2, 2);
+    if (!direct && squares <= cus && 2 * squares >= cus)
         return plan;
     plan.rows = false;
     float least = 0.f;
@@ -779,13 +789,14 @@ int launch_mm(MmArgs p, void* workspace, int64_t workspace_bytes, hipStream_t st
     const Plan plan = plan_mm(p.m, p.n, p.k, a_direct, b_direct);
     const bool room = plan.bytes() == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= plan.bytes());
     if (plan.rows || !room) {
-        // two column tiles to a workgroup halve the reads of a's rows, where there are more workgroups than CUs (16 x
-        // 7168 x 7168 16.5 us, one 18.7; 16 x 4096 x 4096 8.0 and 6.2; one row of 16384 x 16384 loses); two row tiles
-        // with them those of b's (32 x 7168 x 7001 28.7, one 35.9; 32 x 4096 x 4111 11.7 and 10.6)
-        const bool wide = p.n > 16 * cu_count();
-        if (p.m > 32 || (p.m > 16 && wide))
+        // One tile of 16 x 16 to a workgroup while each has a CU of its own (256 x 256 x 7168 8.6 us, 2 x 2 of them to a
+        // workgroup 15.2; 64 x 1024 x 4096 6.0 and 9.9); beyond, two along n halve the reads of a's rows (16 x 7168 x
+        // 7168 16.5, one 18.7; one row of 16384 x 16384 loses), and where those have no CU each, two along m with them
+        // those of b's (32 x 7168 x 7001 28.7, one 35.9).
+        const bool alone = row_groups(p.m, p.n, 1, 1) <= cu_count();
+        if (p.m > 16 && row_groups(p.m, p.n, 1, 2) > cu_count())
             launch_rows<2, 2, 8, OUT>(p, st);
-        else if (p.m > 2 && wide)
+        else if (p.m > 2 && !alone)
             launch_rows<1, 2, 8, OUT>(p, st);
         else if (p.k >= 16 * kBlockK)
             launch_rows<1, 1, 8, OUT>(p, st);

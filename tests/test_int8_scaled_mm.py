@@ -200,6 +200,67 @@ def test_gpu_broadcast_rows(m):
     check(out, a.expand(m, 640), b.expand(600, 640), sa, sb, None, BF16)
 
 
+# sizes that split 64 x 64 tiles along K on 256 CUs, 3 to 7 times at the longest
+SPLIT_SIZES = [(330, 600), (450, 333), (257, 1000), (48, 2048), (100, 601)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", SPLIT_SIZES)
+@pytest.mark.parametrize("k,out_dtype,bias_dtype", [(2048, BF16, None), (2064, F16, F32), (3001, F32, F32), (5120, BF16, BF16),
+                                                    (7168, F16, F16), (7168, F32, None)])
+def test_gpu_split_sums(m, n, k, out_dtype, bias_dtype):
+    """Whole and cut K blocks, packed rows, every output; twice, into a view of a wider buffer the second time."""
+    _say(f"int8 mm split {m} x {n} x {k} {out_dtype} bias {bias_dtype}")
+    run(m, n, k, out_dtype, bias_dtype, seed=k)
+    a, b, sa, sb = _codes(m, k, 1), _codes(n, k, 2), _scales(m, 3), _scales(n, 4)
+    buf = torch.full((m + 2, n + 5), 3.0, dtype=out_dtype, device=DEV)
+    got = fv.int8_scaled_mm(a.to(DEV), b.to(DEV), sa.to(DEV), sb.to(DEV), None, out_dtype, out=buf[1:m + 1, 3:3 + n])
+    torch.cuda.synchronize()
+    check(got, a, b, sa, sb, None, out_dtype)
+    buf[1:m + 1, 3:3 + n] = 3.0
+    assert bool((buf == 3.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(400, 600, 4096), (500, 700, 4111)])
+def test_gpu_workspaces_apart(m, n, k):
+    """Calls with workspaces: in flight at once on two streams, and in two graphs of one pool, replayed in turn
+    with eager calls between."""
+    from flaggems_vllm import _native
+
+    _say(f"int8 mm workspaces {m} x {n} x {k}")
+    data = [(_codes(m, k, s).to(DEV), _codes(n, k, s + 1).to(DEV)) for s in (61, 71)]
+    sa, sb = _scales(m, 3).to(DEV), _scales(n, 4).to(DEV)
+    assert _native.lib().fgv_int8_scaled_mm_workspace_bytes(data[0][0].data_ptr(), k, data[0][1].data_ptr(), k, m, n,
+                                                            k) > 0
+    expect = [fv.int8_scaled_mm(a, b, sa, sb) for a, b in data]
+    torch.cuda.synchronize()
+    for out, (a, b) in zip(expect, data):
+        check(out, a.cpu(), b.cpu(), sa.cpu(), sb.cpu(), None, BF16)
+    streams, outs = [torch.cuda.Stream() for _ in data], [[], []]
+    for _ in range(4):
+        for i, (a, b) in enumerate(data):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(fv.int8_scaled_mm(a, b, sa, sb))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, e) for got, e in zip(outs, expect) for out in got)
+    graphs, outs, pool = [], [], None
+    for a, b in data:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(fv.int8_scaled_mm(a, b, sa, sb))
+        pool = g.pool()
+        graphs.append(g)
+    for order in ((0, 1), (1, 0), (0, 0, 1)):
+        for i in order:
+            outs[i].zero_()
+            fv.int8_scaled_mm(*data[1 - i], sa, sb)
+            torch.cuda.synchronize()
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], expect[i]), (order, i)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", [(300, 300, 5120), (1000, 1030, 1111), (300, 700, 384), (2000, 3000, 256)])
 def test_gpu_without_workspace(m, n, k):
@@ -230,7 +291,7 @@ def test_gpu_workspace_is_enough():
 
     _say("int8 mm workspace guard")
     L = _native.lib()
-    for m, n, k in ((300, 300, 5120), (301, 333, 3001), (1000, 1030, 1111)):
+    for m, n, k in ((300, 300, 5120), (401, 733, 3001), (1000, 1030, 1111)):
         a, b = _codes(m, k, 1).to(DEV), _codes(n, k, 2).to(DEV)
         sa, sb = _scales(m, 3).to(DEV), _scales(n, 4).to(DEV)
         need = L.fgv_int8_scaled_mm_workspace_bytes(a.data_ptr(), k, b.data_ptr(), k, m, n, k)
