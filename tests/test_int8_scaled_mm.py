@@ -111,8 +111,8 @@ def test_gpu_sizes(m, n, k):
     run(m, n, k, seed=m + n)
 
 
-# sizes with ragged edges that take, on 256 CUs, split 64 x 64 tiles, 64 x 64, 128 x 64, 128 x 128, 128 x 192,
-# 192 x 128, 256 x 128, 192 x 256, 256 x 192 and 256 x 256 tiles
+# sizes with ragged edges that take, on 256 CUs, workgroups straight from memory (split 64 x 64 tiles at the longest
+# sum), 64 x 64, 128 x 64, 128 x 128, 128 x 192, 192 x 128, 256 x 128, 192 x 256, 256 x 192 and 256 x 256 tiles
 TILE_SIZES = [(300, 300), (500, 1030), (1000, 1030), (1000, 2050), (1021, 4099), (1500, 4090), (2000, 3900),
               (3000, 4090), (4090, 3000), (4000, 4090)]
 
