@@ -50,13 +50,13 @@ __device__ __forceinline__ v4i_t mfma_i8(v4i_t a, v4i_t b, v4i_t c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-// The bias of four channels from n on (the last one's past the end), 0 without one.  One choice of type for
-// all four, so that their loads are under way together.
+// The bias of four channels from n on (the last one's past the end); without one -0, which leaves every sum as it
+// is, also the sign of a zero.  One choice of type for all four, so that their loads are under way together.
 __device__ __forceinline__ void bias4(const MmArgs& p, int n, float v[4]) {
     if (!p.bias) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            v[q] = 0.f;
+            v[q] = -0.f;
     } else if (p.bias_type == kOutF32) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)

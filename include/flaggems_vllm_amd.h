@@ -690,14 +690,15 @@ int fgv_silu_mul_quant(const void* x, int64_t x_stride, void* codes, int64_t cod
  * Product of int8 codes with a scale per token and per channel:
  *   out[m, n] = scale_a[m] * scale_b[n] * sum_k a[m, k] * b[n, k] + bias[n]
  * with the exact integer sum, the rest in binary32 in the order
- * (sum * scale_a) * scale_b + bias, rounded once to out.
+ * (sum * scale_a) * scale_b + bias, rounded once to out (without a bias a sum
+ * of zero has the sign of scale_a * scale_b).
  *   a [m, k], b [n, k] int8, unit column stride, rows a_stride / b_stride
  *   bytes apart, no alignment needed; scale_a[m * scale_a_stride],
  *   scale_b[n * scale_b_stride] float32 (stride 0: one scale for all); bias [n]
  *   or NULL, in bias_dtype; out [m, n], unit column stride.  out_dtype and
  *   bias_dtype: 0 bf16, 1 fp16, 2 fp32.
- * k at most 131071 (the sum is an int32), m at most 2^20, n at most 2^24; k = 0
- * writes the bias, or zeros.
+ * k at most 131071 (the sum is an int32), m at most 2^20, n at most 2^24; at k = 0
+ * every sum is 0.
  *
  * workspace: 16-byte aligned device memory of workspace_bytes, at least what
  * fgv_int8_scaled_mm_workspace_bytes says for these operands (0 for many): copies

@@ -376,6 +376,35 @@ def test_gpu_scales_that_are_not_finite(m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,n,k", [(3, 70, 256), (40, 130, 384), (300, 300, 5120), (500, 1030, 384), (1000, 1030, 1111)])
+def test_gpu_sign_of_zero(m, n, k, out_dtype):
+    """Sums of zero under scales of either sign, without a bias: (0 * scale_a) * scale_b has the scales' sign, in
+    every schedule and with or without a workspace; a bias of zero makes it +0."""
+    from flaggems_vllm import _native
+
+    _say(f"int8 mm sign of zero {m} x {n} x {k} {out_dtype}")
+    L = _native.lib()
+    a, b = torch.zeros(m, k, dtype=torch.int8, device=DEV), _codes(n, k, 2).to(DEV)
+    sa, sb = _scales(m, 3), _scales(n, 4)
+    sa[::3] *= -1
+    sb[::2] *= -1
+    negative = torch.signbit(sa)[:, None] ^ torch.signbit(sb)[None]
+    sa, sb = sa.to(DEV), sb.to(DEV)
+    out = fv.int8_scaled_mm(a, b, sa, sb, None, out_dtype)
+    bare = torch.empty_like(out)
+    rc = L.fgv_int8_scaled_mm(a.data_ptr(), k, b.data_ptr(), k, sa.data_ptr(), 1, sb.data_ptr(), 1, None, 0,
+                              bare.data_ptr(), n, m, n, k, (BF16, F16, F32).index(out_dtype), None, 0,
+                              torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    biased = fv.int8_scaled_mm(a, b, sa, sb, torch.zeros(n, device=DEV), out_dtype)
+    for got in (out, bare, biased):
+        assert not bool(got.any())
+    assert torch.equal(torch.signbit(out).cpu(), negative) and torch.equal(torch.signbit(bare).cpu(), negative)
+    assert not bool(torch.signbit(biased).any())
+
+
+@pytest.mark.gpu
 def test_gpu_empty():
     _say("int8 mm empty")
     e = torch.empty(0, 64, dtype=torch.int8, device=DEV)
