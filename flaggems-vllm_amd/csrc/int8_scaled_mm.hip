@@ -700,6 +700,16 @@ struct Plan {
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
+// Where an operand's rows lie.
+struct Rows {
+    const int8_t* p;
+    int64_t stride;
+    // every row starts at a multiple of 16 bytes
+    bool chunks() const { return aligned(p, 16) && stride % 16 == 0; }
+    // the tiles' DMAs can read the rows as they are (32-bit offsets over the 256 rows of a tile)
+    bool direct(int64_t k) const { return chunks() && stride >= 0 && stride < (1 << 23) && k % kBlockK == 0; }
+};
+
 // Workgroups of mt x nt tiles of 16 x 16.
 int64_t row_groups(int64_t m, int64_t n, int mt, int nt) {
     return (m + 16 * mt - 1) / (16 * mt) * ((n + 16 * nt - 1) / (16 * nt));
@@ -710,13 +720,19 @@ int64_t row_groups(int64_t m, int64_t n, int mt, int nt) {
 // - workgroups of 16 x 16 have a CU each (256 x 256 x 7168 8.6 us, in split tiles 12), or
 // - workgroups of 16 x 32 have, and the sum is not long enough for split tiles to catch up (us, and in tiles: 24 x
 //   4096 x 4096 8.1, 9.4; 128 x 1024 x 1024 3.5, 4.6; 300 x 300 x 5120 9.3, 9.3; 48 x 2048 x 7168 11.7, 10.8), or tiles
-//   would need the rows packed first (100 x 600 x 1000 4.3, 7.1), or
-// - tiles would need that and workgroups of 32 x 32 have a CU each and fill half of them (64 x 4096 x 4111 11.7, 20.4;
-//   but 64 x 7168 x 7001 45.9, 34.8, and 64 x 1031 x 8001, 66 workgroups, 21.3, 17.8).
+//   would need the rows packed first (100 x 600 x 1000 4.8, 7.6; 64 x 1031 x 8001 17.4, 17.7; but 100 x 600 x 8001
+//   17.6, 15.9), or
+// - tiles would need that and workgroups of 32 x 32 have a CU each (64 x 4096 x 4111 11.6, 21.9), or
+// - tiles would need b packed, two reads of it and a write, and one row of workgroups of 32 x 32 reads it once, however
+//   many there are: with rows that are 16-byte aligned (17 x 16384 x 2880 10.9, 27.2; 32 x 28672 x 7008 69, 108; 32 x
+//   8224 x 16016 72.9, 72.7), at any byte while the sum is short (32 x 16384 x 2879 18.7, 26.8; but 32 x 8224 x 6001
+//   32.8, 29.7).  Beyond 32 tokens it depends (us, and packed: 64 x 8224 x 2880 14.9, 21.7; 64 x 8224 x 16016 90, 73;
+//   64 x 7168 x 7001 38.7, 31.8); those are packed.
 // Else the tile that takes the least time, counted as whole turns of the CUs; where even the smallest tiles leave more
 // than half the CUs idle they are split along K, at least eight blocks each (128 x 2048 x 7168: 15.1 us, in four parts
 // 11.3).
-Plan plan_mm(int64_t m, int64_t n, int64_t k, bool a_direct, bool b_direct) {
+Plan plan_mm(int64_t m, int64_t n, int64_t k, const Rows& a, const Rows& b) {
+    const bool a_direct = a.direct(k), b_direct = b.direct(k);
     Plan plan{true, 0, 1, 0, 0, 0};
     const int64_t cus = cu_count(), nkb = (k + kBlockK - 1) / kBlockK;
     const bool direct = a_direct && b_direct;
@@ -724,8 +740,9 @@ Plan plan_mm(int64_t m, int64_t n, int64_t k, bool a_direct, bool b_direct) {
         return plan;
     if (row_groups(m, n, 1, 2) <= cus && (nkb < 40 || !direct))
         return plan;
-    const int64_t squares = row_groups(m, n, 2, 2);
-    if (!direct && squares <= cus && 2 * squares >= cus)
+    if (!direct && row_groups(m, n, 2, 2) <= cus)
+        return plan;
+    if (!b_direct && m <= 32 && (nkb <= 32 || (a.chunks() && b.chunks())))
         return plan;
     plan.rows = false;
     float least = 0.f;
@@ -748,11 +765,6 @@ Plan plan_mm(int64_t m, int64_t n, int64_t k, bool a_direct, bool b_direct) {
     if (!b_direct)
         plan.b_bytes = up(n * up(k, kBlockK), 256);
     return plan;
-}
-
-// Whether the tiles' DMAs can read rows as they are (32-bit offsets over the 256 rows of a tile).
-bool direct_rows(const int8_t* p, int64_t stride, int64_t k) {
-    return aligned(p, 16) && stride % 16 == 0 && stride >= 0 && stride < (1 << 23) && k % kBlockK == 0;
 }
 
 template <int WM, int WN, int TM, int TN, int NS, int OUT>
@@ -785,8 +797,9 @@ void launch_rows(const MmArgs& p, hipStream_t st) {
 
 template <int OUT>
 int launch_mm(MmArgs p, void* workspace, int64_t workspace_bytes, hipStream_t st) {
-    const bool a_direct = direct_rows(p.a, p.a_s, p.k), b_direct = direct_rows(p.b, p.b_s, p.k);
-    const Plan plan = plan_mm(p.m, p.n, p.k, a_direct, b_direct);
+    const Rows a{p.a, p.a_s}, b{p.b, p.b_s};
+    const bool a_direct = a.direct(p.k), b_direct = b.direct(p.k);
+    const Plan plan = plan_mm(p.m, p.n, p.k, a, b);
     const bool room = plan.bytes() == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= plan.bytes());
     if (plan.rows || !room) {
         // One tile of 16 x 16 to a workgroup while each has a CU of its own (256 x 256 x 7168 8.6 us, 2 x 2 of them to a
@@ -869,7 +882,7 @@ extern "C" int64_t fgv_int8_scaled_mm_workspace_bytes(const int8_t* a, int64_t a
     using namespace fgv;
     if (m <= 0 || n <= 0 || k <= 0 || k > kMaxK || m > kMaxM || n > kMaxN)
         return 0;
-    return plan_mm(m, n, k, direct_rows(a, a_stride, k), direct_rows(b, b_stride, k)).bytes();
+    return plan_mm(m, n, k, Rows{a, a_stride}, Rows{b, b_stride}).bytes();
 }
 
 extern "C" int fgv_int8_scaled_mm(const int8_t* a, int64_t a_stride, const int8_t* b, int64_t b_stride,

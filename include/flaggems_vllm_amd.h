@@ -704,8 +704,8 @@ int fgv_silu_mul_quant(const void* x, int64_t x_stride, void* codes, int64_t cod
  * fgv_int8_scaled_mm_workspace_bytes says for these operands (0 for many): copies
  * of rows that are no multiple of 16 bytes apart (or k none of 128), and the
  * partial sums where few tiles are split along k.  Without it the product is
- * formed straight from memory, with the same bits, slower.  Calls that share a
- * workspace must be ordered on one stream.
+ * formed straight from memory, with the same bits, for most sizes slower.  Calls
+ * that share a workspace must be ordered on one stream.
  */
 int fgv_int8_scaled_mm(const int8_t* a, int64_t a_stride, const int8_t* b, int64_t b_stride, const float* scale_a,
                        int64_t scale_a_stride, const float* scale_b, int64_t scale_b_stride, const void* bias,

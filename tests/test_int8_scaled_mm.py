@@ -404,6 +404,32 @@ def test_gpu_sign_of_zero(m, n, k, out_dtype):
     assert not bool(torch.signbit(biased).any())
 
 
+# (tokens, channels, sum, bytes behind each row) that tiles could only take packed
+FEW_ROWS_OF_WIDE_WEIGHTS = [(17, 16384, 2880, 0), (24, 16384, 2880, 0), (32, 10240, 2368, 0), (24, 8704, 7008, 16),
+                            (32, 9000, 5136, 48), (24, 16384, 2879, 0), (32, 8224, 1375, 2)]
+
+
+@pytest.mark.parametrize("m,n,k,pad", FEW_ROWS_OF_WIDE_WEIGHTS)
+def test_few_rows_do_not_copy_the_weights(m, n, k, pad):
+    """Up to 32 tokens read b once; a call that packs it first reads it twice and writes it."""
+    from flaggems_vllm import _native
+
+    assert _native.lib().fgv_int8_scaled_mm_workspace_bytes(16, k + pad, 16, k + pad, m, n, k) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,pad", FEW_ROWS_OF_WIDE_WEIGHTS)
+def test_gpu_few_rows_of_wide_weights(m, n, k, pad):
+    _say(f"int8 mm few rows {m} x {n} x {k} pad {pad}")
+    a, b, sa, sb = _codes(m, k, 1), _codes(n, k, 2), _scales(m, 3), _scales(n, 4)
+    wide = [torch.full((x.shape[0], k + pad), 127, dtype=torch.int8, device=DEV) for x in (a, b)]
+    for w, x in zip(wide, (a, b)):
+        w[:, :k] = x.to(DEV)
+    out = fv.int8_scaled_mm(wide[0][:, :k], wide[1][:, :k], sa.to(DEV), sb.to(DEV))
+    torch.cuda.synchronize()
+    check(out, a, b, sa, sb, None, BF16)
+
+
 @pytest.mark.gpu
 def test_gpu_empty():
     _say("int8 mm empty")
