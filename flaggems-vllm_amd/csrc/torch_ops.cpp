@@ -31,6 +31,7 @@
 
 #include <c10/core/DeviceGuard.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPStream.h>
 
 #include <optional>
@@ -394,7 +395,12 @@ int slot_mapping(int64_t num_tokens, int64_t max_num_tokens, const at::Tensor& q
 
 // ---- the 8-bit linear ops: norm or activation to codes and scales, int8 product ----
 
-bool takes_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// Whether autograd expects a derivative of t: backward, or the tangent of a
+// forward-mode dual tensor (which is carried on without grad mode, too).
+bool takes_grad(const at::Tensor& t) {
+    return (at::GradMode::is_enabled() && t.requires_grad()) ||
+           (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined());
+}
 
 bool unit_rows(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1; }
 
@@ -462,7 +468,7 @@ int add_rms_norm_quant(const at::Tensor& x, const std::optional<at::Tensor>& res
                        double eps, bool int8, const std::optional<at::Tensor>& hidden_out, NormQuantOut* out) {
     FGV_ASSERT(x.dim() == 2, "x must be 2D [num_tokens, size]");
     FGV_ASSERT(!takes_grad(x) && !takes_grad(weight) && !(residual && takes_grad(*residual)),
-               "inference only: no input may require a gradient");
+               "inference only: no input may require a gradient or carry a tangent");
     const int64_t rows = x.size(0), cols = x.size(1);
     FGV_ASSERT(weight.dim() == 1 && weight.size(0) == cols && weight.is_contiguous(),
                "weight must be [size] and contiguous");
@@ -481,7 +487,7 @@ int add_rms_norm_quant(const at::Tensor& x, const std::optional<at::Tensor>& res
         const at::Tensor& h = *hidden_out;
         FGV_ASSERT(h.sizes() == x.sizes() && h.scalar_type() == x.scalar_type() && h.device() == x.device(),
                    "hidden_out must have x's shape, type and device");
-        FGV_ASSERT(!takes_grad(h), "inference only: no output may require a gradient");
+        FGV_ASSERT(!takes_grad(h), "inference only: no output may require a gradient or carry a tangent");
         FGV_ASSERT(unit_rows(h) && (rows <= 1 || h.stride(0) >= cols),
                    "hidden_out's rows must be contiguous and apart");
         FGV_ASSERT(rows_apart_or_same(h, x) && rows_apart_or_same(h, *residual) && !spans_meet(h, weight),
@@ -504,7 +510,7 @@ int add_rms_norm_quant(const at::Tensor& x, const std::optional<at::Tensor>& res
 
 int silu_mul_quant(const at::Tensor& x, bool int8, TensorPair* out) {
     FGV_ASSERT(x.dim() == 2 && x.size(1) % 2 == 0, "x must be 2D [num_tokens, 2 * size], gate beside up");
-    FGV_ASSERT(!takes_grad(x), "inference only: no input may require a gradient");
+    FGV_ASSERT(!takes_grad(x), "inference only: no input may require a gradient or carry a tangent");
     const int64_t cols = x.size(1) / 2;
     at::Tensor codes, scales;
     if (const int rc = quant_outputs(x, cols, int8, &codes, &scales))
@@ -544,7 +550,7 @@ int int8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale_a,
     FGV_ASSERT(sb >= 0, "scale_b must be float32: [N], [N, 1], [1, N] or one scale");
     FGV_ASSERT(out_code(out_dtype) >= 0, "out_dtype must be bfloat16, float16 or float32");
     FGV_ASSERT(!takes_grad(scale_a) && !takes_grad(scale_b) && !(bias && takes_grad(*bias)),
-               "inference only: no input may require a gradient");
+               "inference only: no input may require a gradient or carry a tangent");
     const c10::Device dev = a.device();
     FGV_ASSERT(b.device() == dev && scale_a.device() == dev && scale_b.device() == dev &&
                    (!bias || bias->device() == dev) && (!out_in || out_in->device() == dev),
@@ -558,7 +564,7 @@ int int8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale_a,
         const at::Tensor& o = *out_in;
         FGV_ASSERT(o.dim() == 2 && o.size(0) == m && o.size(1) == n && o.scalar_type() == out_dtype,
                    "out must be [M, N] of out_dtype");
-        FGV_ASSERT(!takes_grad(o), "inference only: no output may require a gradient");
+        FGV_ASSERT(!takes_grad(o), "inference only: no output may require a gradient or carry a tangent");
         FGV_ASSERT(unit_rows(o) && (m <= 1 || o.stride(0) >= n), "out's rows must be contiguous and apart");
         FGV_ASSERT(!spans_meet(o, a) && !spans_meet(o, b) && !spans_meet(o, scale_a) && !spans_meet(o, scale_b) &&
                        !(bias && spans_meet(o, *bias)),

@@ -259,3 +259,55 @@ def test_gpu_torch_ops_match_the_functions():
     assert torch.equal(f, out)
     torch.library.opcheck(_op("int8_scaled_mm"), (a8, b8, sa, sb, bias, BF16), **check)
     torch.library.opcheck(_op("int8_scaled_mm_out"), (a8, b8, sa, sb, bias, out), **check)
+
+
+# ----------------------------------------------------------- forward-mode duals ----
+
+def _dual_calls(dev):
+    """Calls in which one tensor carries a tangent, made within a dual level: {what: call}."""
+    from torch.autograd.forward_ad import make_dual
+
+    x, w = _randn(4, 256, seed=60).to(dev), (_randn(256, seed=61, scale=0.1) + 1).to(dev)
+    a, b = torch.ones(4, 64, dtype=I8, device=dev), torch.ones(8, 64, dtype=I8, device=dev)
+    sa, sb, bias = torch.ones(4, device=dev), torch.ones(8, device=dev), torch.zeros(8, device=dev)
+    out = torch.zeros(4, 8, dtype=BF16, device=dev)
+    dual = lambda t: make_dual(t, torch.ones_like(t))  # noqa: E731
+    norm, mm = fv.fused_add_rms_norm_quant, fv.int8_scaled_mm
+    return {"x": lambda: norm(dual(x), None, w, EPS), "residual": lambda: norm(x, dual(x), w, EPS),
+            "weight": lambda: norm(x, x, dual(w), EPS, F8), "hidden_out": lambda: norm(x, x, w, EPS, hidden_out=dual(x)),
+            "gate_up": lambda: fv.fused_silu_mul_quant(dual(x)), "scale_a": lambda: mm(a, b, dual(sa), sb),
+            "scale_b": lambda: mm(a, b, sa, dual(sb)), "bias": lambda: mm(a, b, sa, sb, dual(bias)),
+            "out": lambda: mm(a, b, sa, sb, out=dual(out))}
+
+
+DUALS = ["x", "residual", "weight", "hidden_out", "gate_up", "scale_a", "scale_b", "bias", "out"]
+
+
+@pytest.mark.parametrize("what", DUALS)
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_refuses_tangents(what, grad_mode):
+    """A tangent would be dropped without a word; no_grad does not switch tangents off."""
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        with pytest.raises(AssertionError, match="inference only.*tangent"):
+            _dual_calls("cpu")[what]()
+
+
+def test_duals_pass_under_inference_mode():
+    """Where no derivative is recorded at all the value is taken: the call gets as far as asking for a GPU."""
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(torch.zeros(4, 256), torch.ones(4, 256)).to(BF16)
+        with torch.inference_mode(), pytest.raises(AssertionError, match="GPU"):
+            fv.fused_silu_mul_quant(dual)
+
+
+@pytest.mark.gpu
+def test_gpu_refuses_tangents():
+    """On the GPU too, and through torch.ops."""
+    _say("tangents refused")
+    with torch.autograd.forward_ad.dual_level():
+        for what, call in _dual_calls(DEV).items():
+            with pytest.raises(AssertionError, match="tangent"):
+                call()
+        x = torch.autograd.forward_ad.make_dual(_randn(4, 256, seed=62).to(DEV), _randn(4, 256, seed=63).to(DEV))
+        with pytest.raises((AssertionError, RuntimeError, NotImplementedError)):
+            _op("fused_silu_mul_quant")(x)
