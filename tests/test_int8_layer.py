@@ -311,3 +311,43 @@ def test_gpu_refuses_tangents():
         x = torch.autograd.forward_ad.make_dual(_randn(4, 256, seed=62).to(DEV), _randn(4, 256, seed=63).to(DEV))
         with pytest.raises((AssertionError, RuntimeError, NotImplementedError)):
             _op("fused_silu_mul_quant")(x)
+
+
+# ------------------------------------------------------- lazily negated views ----
+
+def _negated_calls(dev):
+    """Calls in which one tensor is a view whose values in memory have the other sign: {what: call}."""
+    x, w = _randn(4, 256, seed=64).to(dev), (_randn(256, seed=65, scale=0.1) + 1).to(dev)
+    a, b = torch.ones(4, 64, dtype=I8, device=dev), torch.ones(8, 64, dtype=I8, device=dev)
+    sa, sb, bias = torch.ones(4, device=dev), torch.ones(8, device=dev), torch.zeros(8, device=dev)
+    out = torch.zeros(4, 8, dtype=BF16, device=dev)
+    neg, norm, mm = torch._neg_view, fv.fused_add_rms_norm_quant, fv.int8_scaled_mm
+    imag = torch.complex(torch.zeros(8, device=dev), torch.ones(8, device=dev)).conj().imag
+    assert imag.is_neg() and imag[:4].is_neg()
+    return {"x": lambda: norm(neg(x), None, w, EPS), "residual": lambda: norm(x, neg(x), w, EPS),
+            "weight": lambda: norm(x, x, neg(w), EPS, F8), "hidden_out": lambda: norm(x, x, w, EPS, hidden_out=neg(x)),
+            "gate_up": lambda: fv.fused_silu_mul_quant(neg(x)), "a": lambda: mm(neg(a), b, sa, sb),
+            "b": lambda: mm(a, neg(b), sa, sb), "scale_a": lambda: mm(a, b, imag[:4], sb),
+            "scale_b": lambda: mm(a, b, sa, imag), "bias": lambda: mm(a, b, sa, sb, neg(bias)),
+            "out": lambda: mm(a, b, sa, sb, out=neg(out))}
+
+
+@pytest.mark.parametrize("what", ["x", "residual", "weight", "hidden_out", "gate_up", "a", "b", "scale_a", "scale_b",
+                                  "bias", "out"])
+def test_refuses_lazily_negated_views(what):
+    with pytest.raises(AssertionError, match="lazily negated"):
+        _negated_calls("cpu")[what]()
+
+
+@pytest.mark.gpu
+def test_gpu_negated_views():
+    """Refused by the functions; torch.ops gives the kernel the negated values."""
+    _say("lazily negated views")
+    for call in _negated_calls(DEV).values():
+        with pytest.raises(AssertionError, match="lazily negated"):
+            call()
+    a, b = torch.ones(4, 64, dtype=I8, device=DEV), torch.ones(8, 64, dtype=I8, device=DEV)
+    imag = torch.complex(torch.zeros(8, device=DEV), torch.ones(8, device=DEV)).conj().imag
+    out = _op("int8_scaled_mm")(a, b, torch.ones(4, device=DEV), imag)
+    assert bool((out == -64).all())
+    assert torch.equal(out, fv.int8_scaled_mm(a, b, torch.ones(4, device=DEV), imag.resolve_neg()))
