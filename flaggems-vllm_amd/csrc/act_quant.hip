@@ -638,11 +638,16 @@ int launch_cols(const QuantArgs& a, hipStream_t st) {
     }
 }
 
-int check_common(const QuantArgs& a, int x_dtype, int code_dtype) {
-    if (a.rows < 0 || a.cols <= 0)
+// (before cols goes into 32 bits)
+int check_size(int64_t rows, int64_t cols) {
+    if (rows < 0 || cols <= 0)
         return fail(FGV_E_BAD_SHAPE, "rows must not be negative and cols positive");
-    if (a.rows > 0x7fffffffLL || a.cols > kMaxCols)
+    if (rows > 0x7fffffffLL || cols > kMaxCols)
         return fail(FGV_E_TOO_LARGE, "at most 2^31 - 1 rows of 65536 columns");
+    return FGV_OK;
+}
+
+int check_types(const QuantArgs& a, int x_dtype, int code_dtype) {
     if ((x_dtype != 0 && x_dtype != 1) || (code_dtype != 0 && code_dtype != 1))
         return fail(FGV_E_BAD_SHAPE, "x_dtype must be 0 (bf16) or 1 (fp16), code_dtype 0 (int8) or 1 (e4m3fn)");
     if (code_dtype == 1 && a.cols % kGroup)
@@ -659,12 +664,12 @@ extern "C" int fgv_add_rms_norm_quant(const void* x, int64_t x_stride, const voi
                                       int64_t rows, int64_t cols, double eps, int32_t x_dtype, int32_t code_dtype,
                                       void* stream) {
     using namespace fgv;
-    if (cols > kMaxCols)
-        return fail(FGV_E_TOO_LARGE, "at most 2^31 - 1 rows of 65536 columns");
+    if (const int rc = check_size(rows, cols))
+        return rc;
     const QuantArgs a{static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(residual), residual_stride,
                       weight, static_cast<uint16_t*>(hidden), hidden_stride, static_cast<uint8_t*>(codes), codes_stride,
                       scales, scales_stride, rows, (int32_t)cols, eps};
-    if (const int rc = check_common(a, x_dtype, code_dtype))
+    if (const int rc = check_types(a, x_dtype, code_dtype))
         return rc;
     if (!(eps > 0.0 && eps < HUGE_VAL))
         return fail(FGV_E_BAD_SHAPE, "eps must be positive and finite");
@@ -693,11 +698,11 @@ extern "C" int fgv_silu_mul_quant(const void* x, int64_t x_stride, void* codes, 
                                   int64_t scales_stride, int64_t rows, int64_t cols, int32_t x_dtype,
                                   int32_t code_dtype, void* stream) {
     using namespace fgv;
-    if (cols > kMaxCols)
-        return fail(FGV_E_TOO_LARGE, "at most 2^31 - 1 rows of 65536 columns");
+    if (const int rc = check_size(rows, cols))
+        return rc;
     const QuantArgs a{static_cast<const uint16_t*>(x), x_stride, nullptr, 0, nullptr, nullptr, 0,
                       static_cast<uint8_t*>(codes), codes_stride, scales, scales_stride, rows, (int32_t)cols, 0.0};
-    if (const int rc = check_common(a, x_dtype, code_dtype))
+    if (const int rc = check_types(a, x_dtype, code_dtype))
         return rc;
     if (rows == 0)
         return FGV_OK;

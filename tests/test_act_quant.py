@@ -659,3 +659,13 @@ def test_silu_c_abi_rejects(kw, code):
     rc = _native.lib().fgv_silu_mul_quant(a["x"], 512, a["codes"], 256, a["scales"], 1, a["rows"], a["cols"],
                                           a["kind"], a["code"], None)
     assert rc == code
+
+
+@pytest.mark.parametrize("cols", [-1, 5 - (1 << 32), 256 - (1 << 40), -(1 << 63)])
+def test_c_abi_rejects_negative_widths_of_any_size(cols):
+    """Also those whose low 32 bits are a width that exists (no rows, so that nothing could be launched)."""
+    from flaggems_vllm import _native
+
+    L = _native.lib()
+    assert L.fgv_add_rms_norm_quant(16, 256, 16, 256, 16, 0, 16, 256, 16, 256, 16, 1, 0, cols, 1e-6, 0, 0, None) == -2
+    assert L.fgv_silu_mul_quant(16, 512, 16, 256, 16, 1, 0, cols, 0, 0, None) == -2
