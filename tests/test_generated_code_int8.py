@@ -115,3 +115,98 @@ def test_every_block_is_waited_for(kernels):
                 assert re.match(r"s_waitcnt\b.*lgkmcnt\(0\)", plain[i - 1]), (name, plain[i - 3:i + 1])
         first = next(i for i, x in enumerate(code) if x.startswith("v_mfma"))
         assert any(re.match(r"s_waitcnt\b.*vmcnt", x) for x in code[first:settled(code)]), name
+
+
+# ------------------------------------------------------- the ring's hand-over ----
+
+def shape(name):
+    """WM, WN, TM, TN, NS of a tile kernel, and the DMAs that a wave sends for a K block."""
+    wm, wn, tm, tn, ns = (int(x) for x in re.search(r"tile_kernelI" + r"Li(\d+)E" * 5, name).groups())
+    return ns, (2 * tm * wm + 2 * tn * wn) // (wm * wn)
+
+
+def waits_at_barriers(code):
+    """{barrier: the counts of the last vector memory wait on every way to it}; None for a way with an LDS DMA behind
+    its last wait, or without one.  Ways are followed forwards, with the flags that the compiler sets to 0 or -1 in
+    scalar registers and tests through vcc (which choose between two waits), so that no way is taken that is none."""
+    labels = {x[:-1]: i for i, x in enumerate(code) if x.endswith(":")}
+    found, seen, todo = {}, set(), [(0, None, frozenset(), None)]
+    while todo:
+        i, wait, flags, vcc = todo.pop()
+        while i < len(code) and (i, wait, flags, vcc) not in seen:
+            seen.add((i, wait, flags, vcc))
+            x = code[i]
+            ops = operands(x)
+            i += 1
+            if x.endswith(":"):
+                continue
+            m = re.match(r"s_waitcnt\b.*vmcnt\((\d+)\)", x)
+            if m:
+                wait = int(m.group(1))
+            elif x.startswith("global_load_lds"):
+                wait = None
+            elif x.startswith("s_barrier"):
+                found.setdefault(i - 1, set()).add(wait)
+            elif x.startswith("s_endpgm"):
+                break
+            elif x.startswith("s_branch"):
+                i = labels[ops[0]]
+            elif x.startswith("s_cbranch"):
+                taken = None
+                if x.startswith(("s_cbranch_vccnz", "s_cbranch_vccz")) and vcc is not None:
+                    taken = vcc == x.startswith("s_cbranch_vccnz")
+                if taken is None:
+                    todo.append((labels[ops[0]], wait, flags, vcc))
+                elif taken:
+                    i = labels[ops[0]]
+            elif ops:
+                if ops[0] == "vcc" or x.startswith("v_cmp"):
+                    vcc = None
+                    if x.startswith("s_andn2_b64 vcc, exec, "):  # all lanes run: exec is not 0
+                        vcc = {"0": True, "-1": False}.get(dict(flags).get(ops[2]))
+                flags = frozenset(f for f in flags if not registers(f[0]) & registers(ops[0]))
+                if x.startswith("s_mov_b64 s[") and ops[1] in ("0", "-1"):
+                    flags |= {(ops[0], ops[1])}
+    return found
+
+
+def check_hand_over(name, code):
+    """The first barrier lets blocks 1 to NS - 1 be under way, the loop's blocks kb + 2 to kb + NS - 1; where no more
+    are sent both wait for all.  Counts above these would hand over a stage that has not landed."""
+    ns, per = shape(name)
+    sends = sum(x.startswith("global_load_lds_dwordx4") for x in code)
+    assert sends == (ns + 1) * per, (name, sends)
+    barriers = [i for i, x in enumerate(code) if x.startswith("s_barrier")]
+    assert len(barriers) == 2, name
+    first = next(i for i, x in enumerate(code) if x.startswith("global_load_lds_dwordx4"))
+    behind = [sum(x.startswith("global_load_lds_dwordx4") for x in code[first:b]) for b in barriers]
+    assert behind == [ns * per, ns * per], (name, behind)  # no DMA of the loop stands between the two
+    waits = waits_at_barriers(code)
+    for b, most in zip(barriers, ((ns - 1) * per, (ns - 2) * per)):
+        counts = waits[b]
+        assert None not in counts and 0 in counts and max(counts) <= most, (name, counts, most)
+
+
+def test_every_stage_has_landed_at_its_barrier(kernels):
+    for name, code in kernels.items():
+        check_hand_over(name, code)
+
+
+def test_a_late_or_short_wait_is_seen(kernels):
+    """The check above, on code with one mistake in it: a wait gone, a count one block too large, a DMA between the
+    wait and its barrier."""
+    for name, code in kernels.items():
+        per = shape(name)[1]
+        sends = [i for i, x in enumerate(code) if x.startswith("global_load_lds_dwordx4")]
+        bad = []
+        for i in range(sends[0], settled(code)):
+            m = re.match(r"s_waitcnt\b.*vmcnt\((\d+)\)", code[i])
+            if m:
+                bad.append(code[:i] + code[i + 1:])
+                bad.append(code[:i] + [f"s_waitcnt vmcnt({int(m.group(1)) + per})"] + code[i + 1:])
+            elif code[i].startswith("s_barrier"):
+                bad.append(code[:i] + [code[sends[-1]]] + code[i:])
+        assert len(bad) >= 8, name
+        for wrong in bad:
+            with pytest.raises(AssertionError):
+                check_hand_over(name, wrong)
