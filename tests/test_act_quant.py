@@ -495,6 +495,29 @@ def test_gpu_silu_more_rows_than_a_launch():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,first,cols", [
+    (F8, 65535 * 4, 128),   # a wave to a row, four rows to a workgroup, 65535 workgroups along the rows
+    (I8, 2 ** 25, 8),       # 64 threads to a row, 2^31 threads
+])
+def test_gpu_silu_rows_of_a_second_launch(dtype, first, cols):
+    """A few rows more than the first launch takes: those each side of its end, and all of them against calls that
+    take one launch."""
+    _say(f"silu rows past a launch {dtype}")
+    rows = first + 9
+    x = torch.randn(rows, 2 * cols, generator=torch.Generator(DEV).manual_seed(52), device=DEV, dtype=BF16)
+    codes, scales = fv.fused_silu_mul_quant(x, dtype)
+    for lo in (0, first - 40, rows - 50):
+        ref = silu64(x[lo:lo + 50].cpu(), dtype)
+        check_codes(codes[lo:lo + 50], ref[0], ref[2])
+        check_scales(scales[lo:lo + 50], ref[1])
+    step = first // 4 + 1
+    for lo in range(0, rows, step):
+        c, s = fv.fused_silu_mul_quant(x[lo:lo + step], dtype)
+        assert torch.equal(c.view(torch.uint8), codes[lo:lo + step].view(torch.uint8))
+        assert torch.equal(s, scales[lo:lo + step])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [I8, F8])
 def test_gpu_offsets_past_32_bits(dtype):
     """33000 rows of 65536 columns: more than 2^31 elements, 2^32 bytes, in each tensor."""
