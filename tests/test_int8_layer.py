@@ -204,6 +204,49 @@ def test_gpu_two_graphs_of_one_pool():
             assert torch.equal(outs[i], expect[i]), (order, i)
 
 
+def _workspace_bytes(m, n, k):
+    from flaggems_vllm import _native
+
+    return _native.lib().fgv_int8_scaled_mm_workspace_bytes(256, k, 256, k, m, n, k)
+
+
+# block sizes whose two products take a workspace at the token counts of the next test: packed rows (a sum of 1031) and
+# sums cut along K (of 2048 and 4096)
+WORKSPACE_BLOCKS = [(1031, 2048, 300), (600, 4096, 400)]
+
+
+@pytest.mark.parametrize("size,inner,tokens", WORKSPACE_BLOCKS)
+def test_blocks_that_need_workspaces(size, inner, tokens):
+    """What the next test, and the blocks of 1031 channels and 300 tokens above, rest on."""
+    assert _workspace_bytes(tokens, 2 * inner, size) > 0 and _workspace_bytes(tokens, size, inner) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size,inner,tokens", WORKSPACE_BLOCKS)
+def test_gpu_two_graphs_share_their_workspaces_memory(size, inner, tokens):
+    """Two captured blocks in one memory pool, so that what one graph freed is the other's too, and eager blocks in
+    between: each replay gives what the block gave alone."""
+    _say(f"int8 blocks in two graphs of one pool, {size} {inner} {tokens}")
+    blocks = [Block(size, inner, 70 + i).to(DEV) for i in range(2)]
+    ins = [(_randn(tokens, size, seed=80 + i).to(DEV), _randn(tokens, size, seed=90 + i).to(DEV)) for i in range(2)]
+    expect = [block.run(*data)[3] for block, data in zip(blocks, ins)]
+    torch.cuda.synchronize()
+    graphs, outs, pool = [], [], None
+    for block, data in zip(blocks, ins):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(block.run(*data)[3])
+        pool = g.pool()
+        graphs.append(g)
+    for order in ((0, 1), (1, 0), (1, 1, 0), (0, 0, 1)):
+        for i in order:
+            outs[i].zero_()
+            assert torch.equal(blocks[1 - i].run(*ins[1 - i])[3], expect[1 - i])
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], expect[i]), (order, i)
+
+
 # ---------------------------------------------------------------- torch.ops ----
 
 def _op(name):

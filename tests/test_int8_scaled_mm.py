@@ -475,6 +475,32 @@ def test_gpu_two_streams():
         assert all(torch.equal(got[0], g) for g in got[1:])
 
 
+# sums cut along K, packed rows, packed rows of few tokens, and both at once
+WORKSPACE_SIZES = [(400, 600, 4096), (500, 700, 1111), (40, 8224, 2880), (257, 1000, 3001)]
+
+
+@pytest.mark.parametrize("m,n,k", WORKSPACE_SIZES + [(200, 1536, 2048), (500, 700, 4111)])
+def test_sizes_that_need_a_workspace(m, n, k):
+    """Those of the next test, and of the calls in flight together above."""
+    from flaggems_vllm import _native
+
+    assert _native.lib().fgv_int8_scaled_mm_workspace_bytes(256, k, 256, k, m, n, k) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", WORKSPACE_SIZES)
+def test_gpu_calls_in_a_row_with_workspaces(m, n, k):
+    """Calls on other data, one after the other without a pause, whose workspaces take each other's memory."""
+    _say(f"int8 mm workspaces in a row {m} x {n} x {k}")
+    pairs = [(_codes(m, k, s).to(DEV), _codes(n, k, s + 1).to(DEV)) for s in (1, 11, 21)]
+    sa, sb = _scales(m, 3).to(DEV), _scales(n, 4).to(DEV)
+    runs = [[fv.int8_scaled_mm(a, b, sa, sb) for a, b in pairs] for _ in range(3)]
+    torch.cuda.synchronize()
+    for out, (a, b) in zip(runs[0], pairs):
+        check(out, a.cpu(), b.cpu(), sa.cpu(), sb.cpu(), None, BF16)
+    assert all(torch.equal(x, y) for again in runs[1:] for x, y in zip(again, runs[0]))
+
+
 # ----------------------------------------------------------------- refusals ----
 
 def _args(**over):
