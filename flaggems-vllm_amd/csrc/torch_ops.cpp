@@ -398,8 +398,8 @@ int slot_mapping(int64_t num_tokens, int64_t max_num_tokens, const at::Tensor& q
 // Whether autograd expects a derivative of t: backward, or the tangent of a
 // forward-mode dual tensor (which is carried on without grad mode, too).
 bool takes_grad(const at::Tensor& t) {
-    return (at::GradMode::is_enabled() && t.requires_grad()) ||
-           (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined());
+    return (t.requires_grad() && at::GradMode::is_enabled()) ||
+           (t._fw_grad(/*level=*/0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode());
 }
 
 // Whether what lies in t's memory are its values (a lazily negated view, such as
