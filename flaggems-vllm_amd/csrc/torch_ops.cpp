@@ -402,10 +402,27 @@ bool takes_grad(const at::Tensor& t) {
            (t._fw_grad(/*level=*/0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode());
 }
 
-// Whether what lies in t's memory are its values (a lazily negated view, such as
-// the imaginary part of a conjugate, has them with the other sign).
-bool as_stored(const at::Tensor& t) { return !t.is_neg(); }
-constexpr char kNegated[] = "no tensor may be a lazily negated view (resolve_neg() gives its values)";
+// Why t's values are not what a kernel would read at its address, or null.  A
+// lazily negated view (the imaginary part of a conjugate) has them with the other
+// sign; fake tensors and tensors whose storage was freed have no memory, and a
+// view into them has an address that is neither null nor valid.
+const char* not_readable(const at::Tensor& t) {
+    if (t.is_neg())
+        return "no tensor may be a lazily negated view (resolve_neg() gives its values)";
+    const at::Storage& s = t.unsafeGetTensorImpl()->unsafe_storage();
+    if (t.numel() > 0 && (!s || s.unsafeGetStorageImpl()->data_ptr().get() == nullptr))
+        return "every tensor must have memory (no fake tensors, no freed storage)";
+    return nullptr;
+}
+const char* not_readable(const std::optional<at::Tensor>& t) { return t ? not_readable(*t) : nullptr; }
+
+// The first reason among several tensors.
+template <class... Tensors>
+const char* any_not_readable(const Tensors&... tensors) {
+    const char* why = nullptr;
+    ((why = why ? why : not_readable(tensors)), ...);
+    return why;
+}
 
 bool unit_rows(const at::Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1; }
 
@@ -481,9 +498,8 @@ int add_rms_norm_quant(const at::Tensor& x, const std::optional<at::Tensor>& res
                "weight must have x's type or float32");
     FGV_ASSERT(eps > 0.0 && std::isfinite(eps), "eps must be positive and finite");
     FGV_ASSERT(residual || !hidden_out, "hidden_out needs a residual");
-    FGV_ASSERT(as_stored(x) && as_stored(weight) && (!residual || as_stored(*residual)) &&
-                   (!hidden_out || as_stored(*hidden_out)),
-               kNegated);
+    if (const char* why = any_not_readable(x, residual, weight, hidden_out))
+        return assert_failed(why);
     FGV_ASSERT(weight.device() == x.device(), "all tensors must be on x's device");
     if (residual) {
         FGV_ASSERT(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(),
@@ -518,7 +534,8 @@ int add_rms_norm_quant(const at::Tensor& x, const std::optional<at::Tensor>& res
 
 int silu_mul_quant(const at::Tensor& x, bool int8, TensorPair* out) {
     FGV_ASSERT(x.dim() == 2 && x.size(1) % 2 == 0, "x must be 2D [num_tokens, 2 * size], gate beside up");
-    FGV_ASSERT(as_stored(x), kNegated);
+    if (const char* why = not_readable(x))
+        return assert_failed(why);
     FGV_ASSERT(!takes_grad(x), "inference only: no input may require a gradient or carry a tangent");
     const int64_t cols = x.size(1) / 2;
     at::Tensor codes, scales;
@@ -553,9 +570,8 @@ int int8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale_a,
     FGV_ASSERT(a.scalar_type() == at::kChar && b.scalar_type() == at::kChar, "a and b must be int8");
     const int64_t m = a.size(0), n = b.size(0), k = a.size(1);
     FGV_ASSERT(unit_rows(a) && unit_rows(b), "a's and b's rows must be contiguous");
-    FGV_ASSERT(as_stored(a) && as_stored(b) && as_stored(scale_a) && as_stored(scale_b) &&
-                   (!bias || as_stored(*bias)) && (!out_in || as_stored(*out_in)),
-               kNegated);
+    if (const char* why = any_not_readable(a, b, scale_a, scale_b, bias, out_in))
+        return assert_failed(why);
     const int64_t sa = scale_stride(scale_a, m), sb = scale_stride(scale_b, n);
     FGV_ASSERT(sa >= 0 && (scale_a.numel() == 1 || scale_a.dim() == 1 || scale_a.size(0) == m),
                "scale_a must be float32: [M], [M, 1] or one scale");

@@ -394,3 +394,49 @@ def test_gpu_negated_views():
     out = _op("int8_scaled_mm")(a, b, torch.ones(4, device=DEV), imag)
     assert bool((out == -64).all())
     assert torch.equal(out, fv.int8_scaled_mm(a, b, torch.ones(4, device=DEV), imag.resolve_neg()))
+
+
+# ------------------------------------------------------- tensors without memory ----
+
+def _calls_without_memory():
+    """Calls in which one tensor has no memory and its view an offset into it (an address of some hundred bytes, which
+    is not null): {what: call}.  The others lie on the CPU, so that nothing could be launched."""
+    def bare(t):
+        base = torch.empty(t.numel() + 256, dtype=t.dtype)
+        view = base[256:].view(t.shape)
+        base.untyped_storage().resize_(0)
+        return view
+
+    x, w = _randn(4, 256, seed=66), _randn(256, seed=67)
+    a, b = torch.ones(4, 64, dtype=I8), torch.ones(8, 64, dtype=I8)
+    sa, sb, bias, out = torch.ones(4), torch.ones(8), torch.zeros(8), torch.zeros(4, 8, dtype=BF16)
+    norm, mm = fv.fused_add_rms_norm_quant, fv.int8_scaled_mm
+    return {"x": lambda: norm(bare(x), None, w, EPS), "residual": lambda: norm(x, bare(x), w, EPS),
+            "weight": lambda: norm(x, x, bare(w), EPS, F8), "hidden_out": lambda: norm(x, x, w, EPS, hidden_out=bare(x)),
+            "gate_up": lambda: fv.fused_silu_mul_quant(bare(x)), "a": lambda: mm(bare(a), b, sa, sb),
+            "b": lambda: mm(a, bare(b), sa, sb), "scale_a": lambda: mm(a, b, bare(sa), sb),
+            "scale_b": lambda: mm(a, b, sa, bare(sb)), "bias": lambda: mm(a, b, sa, sb, bare(bias)),
+            "out": lambda: mm(a, b, sa, sb, out=bare(out))}
+
+
+@pytest.mark.parametrize("what", ["x", "residual", "weight", "hidden_out", "gate_up", "a", "b", "scale_a", "scale_b",
+                                  "bias", "out"])
+def test_refuses_tensors_whose_memory_is_gone(what):
+    """Such as a parameter whose storage a sharding wrapper has freed."""
+    with pytest.raises(AssertionError, match="memory"):
+        _calls_without_memory()[what]()
+
+
+def test_refuses_fake_tensors():
+    """The functions (unlike torch.ops) run kernels whatever mode is on: fake tensors, which say that they are on
+    the GPU, are refused before anything is allocated or launched."""
+    from torch._subclasses import FakeTensorMode
+
+    with FakeTensorMode():
+        x = torch.empty(5, 512, dtype=BF16, device="cuda")[1:]
+        a = torch.empty(5, 64, dtype=I8, device="cuda")[1:]
+        s = torch.empty(5, device="cuda")[1:]
+        for call in (lambda: fv.fused_silu_mul_quant(x), lambda: fv.fused_add_rms_norm_quant(x, x, x[0], EPS),
+                     lambda: fv.int8_scaled_mm(a, a, s, s)):
+            with pytest.raises((AssertionError, RuntimeError), match="memory"):
+                call()
