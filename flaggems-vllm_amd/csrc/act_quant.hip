@@ -11,7 +11,8 @@
 // cancels, so a code is the rounded quotient q h w / max |h w| and needs no
 // sum.  The fast path works on v = h w (exact in binary32 for 16-bit weights,
 // rounded once for float32 ones) or v = y within a relative 2^-21: t = v * (q / a)
-// in binary32 is off by less than 2^-20.4 relative, so a code can be wrong only
+// in binary32 is off by less than 2^-20.2 relative (in units of 2^-24: 8 of v, 4 of
+// q / a, 1 of the product), so a code can be wrong only
 // where t lies that close to the border between two codes.  Those elements, one
 // in some thousand, are computed again in binary64 (with a correctly rounded
 // division) and their bytes overwritten.  The largest magnitude is settled the
@@ -231,8 +232,8 @@ constexpr float kNearMost = 1.0f - 0x1p-19f;  // nearer to the maximum than this
 // back from below binary32's range, a gate outweigh the least sigmoid.
 constexpr float kWide = 0x1p20f;
 // Distance from the nearest code at which an element counts as beside a border.
-// int8: 0.5 - 2^-13 of a step (127 * 2^-20.4 < 2^-13); e4m3fn: half a step times
-// 1 - 2^-14 (the step is at least 2^-4 of the value: 16 * 2^-20.4 < 2^-15).
+// int8: 0.5 - 2^-13 of a step (127 * 2^-20.2 < 2^-13); e4m3fn: half a step times
+// 1 - 2^-14 (the step is at least 2^-4 of the value: 16 * 2^-20.2 < 2^-15).
 constexpr float kBorderI8 = 0.5f - 0x1p-13f, kBorderFp8 = 0x1p-4f * (1.0f - 0x1p-14f);
 
 // Eight weights from e0 on (zeros behind cols).

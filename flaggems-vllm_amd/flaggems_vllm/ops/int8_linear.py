@@ -21,7 +21,9 @@ A layer with int8 weights runs::
 The argument checks, output allocation and launch run in C++
 (``torch_ops.cpp``) through the C ABI ``fgv_add_rms_norm_quant``,
 ``fgv_silu_mul_quant`` and ``fgv_int8_scaled_mm``, on torch's current stream of
-the tensors' device; a failed check raises AssertionError.  Inference only.
+the tensors' device; a failed check raises AssertionError.  Inference only: a
+tensor that requires a gradient (in grad mode) or carries a forward-mode tangent
+is refused, and so are lazily negated views and tensors without memory.
 """
 from typing import Optional, Tuple
 
