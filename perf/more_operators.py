@@ -1,0 +1,458 @@
+"""Serving from a paged key/value cache held in 4 bits, as cases to time.
+
+An engine's step calls three operators one after the other: request lengths
+become block tables, positions and cache slots (``tables``); the step's keys
+and values are quantised into the paged cache (``insert``); the queries attend
+over it (``attn``), one token per request or many.
+
+The cache is MXFP4: of each head's row every 32 values share a power of two
+(one UE8M0 byte) and are E2M1 codes, two to a byte, the even one low.  A block
+of the cache holds, for each head, the keys' codes of all its tokens, the
+values' codes, the keys' scale bytes and the values' scale bytes:
+uint8 [blocks, kv heads, block size, D + D / 16].
+
+``listed`` gives the cases, ``draw`` more of the same ranges, ``prepare`` what
+an engine holds before the call, ``run`` one call - through the package's
+public functions where ``own`` is true, in elementary torch operations where
+it is not - and ``exact`` the same outputs in 64 bits.
+"""
+import math
+import os
+import random
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+DEV = "cuda"
+BLOCK = 32  # values under one scale byte
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+PAD = -1
+
+
+# ------------------------------------------------------------------- cases ----
+
+def listed():
+    return [
+        # a decode step of 200 requests, some of which enter a new block: a launch's latency
+        {"name": "tables_decode_200", "op": "tables", "reqs": 200, "context": 4000, "query": 1, "width": 512,
+         "page": 16, "pad": 56},
+        # a mixed step: most requests decode, some bring chunks of up to 2000 tokens
+        {"name": "tables_mixed_333", "op": "tables", "reqs": 333, "context": 9000, "query": 2000, "width": 700,
+         "page": 16, "pad": 77},
+        # a decode step's keys and values of 24 requests
+        {"name": "insert_decode_24", "op": "insert", "tokens": 24, "kv_heads": 8, "dim": 128, "page": 16,
+         "type": "bf16"},
+        # a full prefill chunk's, heads of a wider row (a fused projection's output), odd token count
+        {"name": "insert_prefill_8191", "op": "insert", "tokens": 8191, "kv_heads": 8, "dim": 128, "page": 64,
+         "type": "fp16"},
+        # one short conversation: latency
+        {"name": "attn_decode_1", "op": "attn", "reqs": 1, "context": 517, "query": 1, "ragged": False, "heads": 32,
+         "kv_heads": 8, "dim": 128, "page": 16, "type": "bf16", "window": 0, "sink": False},
+        # a serving batch of very different lengths
+        {"name": "attn_decode_64", "op": "attn", "reqs": 64, "context": 8191, "query": 1, "ragged": True, "heads": 32,
+         "kv_heads": 8, "dim": 128, "page": 16, "type": "bf16", "window": 0, "sink": False},
+        # one long document: few rows, a long axis
+        {"name": "attn_decode_long", "op": "attn", "reqs": 1, "context": 131071, "query": 1, "ragged": False,
+         "heads": 64, "kv_heads": 8, "dim": 128, "page": 64, "type": "bf16", "window": 0, "sink": False},
+        # one key/value head for 16 query heads of 256
+        {"name": "attn_decode_wide", "op": "attn", "reqs": 24, "context": 20000, "query": 1, "ragged": True,
+         "heads": 16, "kv_heads": 1, "dim": 256, "page": 32, "type": "fp16", "window": 0, "sink": False},
+        # a sliding window with sinks, heads of 64
+        {"name": "attn_window_128", "op": "attn", "reqs": 128, "context": 6000, "query": 1, "ragged": True,
+         "heads": 64, "kv_heads": 8, "dim": 64, "page": 16, "type": "bf16", "window": 1000, "sink": True},
+        # verification of 5 drafted tokens each, seven query heads to a group
+        {"name": "attn_verify_16", "op": "attn", "reqs": 16, "context": 3001, "query": 5, "ragged": True, "heads": 28,
+         "kv_heads": 4, "dim": 128, "page": 16, "type": "fp16", "window": 0, "sink": False},
+        # a prefill chunk onto a long context: bound by the matrix instructions
+        {"name": "attn_chunk_2048", "op": "attn", "reqs": 1, "context": 14336, "query": 2048, "ragged": False,
+         "heads": 32, "kv_heads": 8, "dim": 128, "page": 16, "type": "bf16", "window": 0, "sink": False},
+        # several prompts from their first token, of different lengths, in a window
+        {"name": "attn_prompts_6", "op": "attn", "reqs": 6, "context": 0, "query": 1777, "ragged": True, "heads": 24,
+         "kv_heads": 4, "dim": 128, "page": 48, "type": "fp16", "window": 700, "sink": True},
+    ]
+
+
+def _size(rng, lo, hi):
+    """A whole number in [lo, hi], spread over its logarithm."""
+    return max(lo, min(hi, round(math.exp(rng.uniform(math.log(lo), math.log(hi))))))
+
+
+def _drawn(rng):
+    op = rng.choice(("tables", "insert", "attn", "attn", "attn", "attn"))
+    page = rng.choice((16, 16, 32, 48, 64, 128))
+    kind = rng.choice(("bf16", "fp16"))
+    dim, kv_heads = rng.choice((64, 128, 128, 256)), rng.choice((1, 2, 4, 8))
+    if op == "tables":
+        context = _size(rng, 16, 16384)
+        query = rng.choice((1, 1, _size(rng, 2, 2000)))
+        return {"op": op, "reqs": _size(rng, 1, 512), "context": context, "query": query,
+                "width": (context + query) // page + rng.randrange(1, 40), "page": page, "pad": rng.randrange(100)}
+    if op == "insert":
+        return {"op": op, "tokens": _size(rng, 1, 8192), "kv_heads": kv_heads, "dim": dim, "page": page, "type": kind}
+    kind_of = rng.choice(("decode", "decode", "verify", "chunk"))
+    context = _size(rng, 16, 131072)
+    query = 1 if kind_of == "decode" else rng.randrange(2, 9) if kind_of == "verify" else _size(rng, 9, 2048)
+    return {"op": op, "reqs": _size(rng, 1, 256), "context": context, "query": query, "ragged": rng.random() < 0.7,
+            "heads": kv_heads * rng.choice((1, 2, 3, 4, 5, 7, 8, 8, 12, 16)), "kv_heads": kv_heads, "dim": dim,
+            "page": page, "type": kind, "window": rng.choice((0, 0, 0, _size(rng, 16, 4096))),
+            "sink": rng.random() < 0.3}
+
+
+def _cost(case):
+    w = work(case)
+    return max(w["bytes"] / 5e12, w["flops"] / 1e15)
+
+
+def _padded(case):
+    """Bytes of float32 that the plain form needs for scores and for the gathered cache, requests padded to the longest."""
+    total = case["context"] + case["query"]
+    return 4 * case["reqs"] * total * (case["query"] * case["heads"] + 2 * case["kv_heads"] * case["dim"])
+
+
+def draw(rng):
+    most = {op: max(_cost(c) for c in listed() if c["op"] == op) for op in ("tables", "insert", "attn")}
+    while True:
+        case = _drawn(rng)
+        if case["op"] == "attn" and (case["heads"] > 64 or _padded(case) > 6e9):
+            continue
+        if _cost(case) <= most[case["op"]]:
+            return case
+
+
+def _lengths(case):
+    """Context and query length of each request: the case's own, or spread below them."""
+    n, context, query = case["reqs"], case["context"], case["query"]
+    if not case.get("ragged", True):
+        return [context] * n, [query] * n
+    rng = random.Random("%d %d %d" % (n, context, query))
+    # about a third as long as the longest, the first one the longest; a request of no query token among the tables
+    ctx = [context] + [int(context * rng.random() ** 2) for _ in range(n - 1)]
+    if case["op"] == "tables":
+        q = [query] + [1 if rng.random() < 0.9 else rng.randrange(0, query + 1) for _ in range(n - 1)]
+    else:
+        q = [query] + [query if query < 9 else rng.randrange(1, query + 1) for _ in range(n - 1)]
+    return ctx, q
+
+
+def _visible(ctx, query, window):
+    """Keys that each of a request's query tokens sees, added up; and how many different ones there are."""
+    if not window:
+        return query * ctx + query * (query + 1) // 2, ctx + query
+    each = sum(min(window, ctx + i + 1) for i in range(query))
+    return each, min(ctx + query, window + query - 1)
+
+
+def work(case):
+    if case["op"] == "insert":
+        row = case["kv_heads"] * case["dim"]
+        return {"bytes": case["tokens"] * (4 * row + row + row // 16 + 8), "flops": 6 * case["tokens"] * row}
+    ctx, query = _lengths(case)
+    tokens, page = sum(query), case["page"]
+    if case["op"] == "tables":
+        blocks = sum((c + q + page - 1) // page - (c + page - 1) // page for c, q in zip(ctx, query))
+        touched = sum((c + q + page - 1) // page - c // page for c, q in zip(ctx, query))
+        return {"bytes": 8 * case["reqs"] + 16 * (tokens + case["pad"]) + 4 * touched + 8 * blocks + 8 * case["reqs"],
+                "flops": 4 * tokens + 4 * case["reqs"]}
+    pairs = keys = 0
+    for c, q in zip(ctx, query):
+        p, k = _visible(c, q, case["window"])
+        pairs, keys = pairs + p, keys + k
+    row = case["kv_heads"] * case["dim"]
+    return {"bytes": keys * (row + row // 16) + tokens * case["heads"] * (4 * case["dim"] + 4),
+            "flops": 4 * pairs * case["heads"] * case["dim"]}
+
+
+# ------------------------------------------------------------------ inputs ----
+
+def _codes(x):
+    """E2M1 codes (0..15) and scale bytes of the 32-bit rows x: [..., D] -> [..., D], [..., D / 32]."""
+    blocks = x.unflatten(-1, (-1, BLOCK))
+    most = blocks.abs().amax(dim=-1)
+    m, e = torch.frexp(most)  # most = m 2^e, m in [1/2, 1): ceil(log2(most / 6)) is e - 3, one more above 3/4
+    k = torch.where(most > 0, e - 3 + (m > 0.75).int(), -126).clamp(-126, 125)
+    y = torch.ldexp(blocks.double(), -k.unsqueeze(-1))
+    a = y.abs()
+    code = torch.zeros_like(a, dtype=torch.uint8)
+    # a value on the border between two codes goes to the even one
+    for n, (border, up) in enumerate(((0.25, False), (0.75, True), (1.25, False), (1.75, True), (2.5, False),
+                                      (3.5, True), (5.0, False))):
+        code += (a >= border) if up else (a > border)
+    return (code + 8 * torch.signbit(y).to(torch.uint8)).flatten(-2), (k + 127).to(torch.uint8)
+
+
+def _empty_cache(blocks, kv_heads, page, dim):
+    return torch.empty(blocks, kv_heads, page, dim + dim // 16, dtype=torch.uint8, device=DEV)
+
+
+def _parts(cache):
+    """Views of a cache's four parts: codes of k and v [blocks, heads, page, D / 2], scales of k and v [..., D / 32]."""
+    n, h, page, width = cache.shape
+    dim = width * 16 // 17
+    flat, half, few = cache.view(n, h, page * width), page * dim // 2, page * dim // BLOCK
+    return [flat[:, :, a:b].unflatten(2, (page, -1)) for a, b in
+            ((0, half), (half, 2 * half), (2 * half, 2 * half + few), (2 * half + few, 2 * (half + few)))]
+
+
+def _rows(g, n, heads, dim, kind, wider=0):
+    """Keys or values: normal, each head at its own size, a few channels many times larger; out of rows `wider` values longer."""
+    x = torch.randn(n, heads * dim + wider, generator=g, device=DEV)
+    x[:, :heads * dim] *= torch.exp2(torch.randn(heads, generator=g, device=DEV)).repeat_interleave(dim)
+    x[:, torch.randint(0, heads * dim, (max(1, heads * dim // 100),), generator=g, device=DEV)] *= 5
+    return x.to(TYPES[kind])[:, :heads * dim].unflatten(1, (heads, dim))
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    s = {"case": case}
+    page = case["page"]
+    if case["op"] == "insert":
+        n, h, d = case["tokens"], case["kv_heads"], case["dim"]
+        s["k"], s["v"] = (_rows(g, n, h, d, case["type"], 2 * h * d) for _ in range(2))
+        blocks = max(4, 2 * n // page)
+        s["cache"] = torch.zeros_like(_empty_cache(blocks, h, page, d))
+        s["slots"] = torch.randperm(blocks * page, generator=g, device=DEV)[:n]
+        s["slots"][n // 2:n // 2 + n // 50] = PAD  # tokens of a padded batch
+        return s
+    ctx, query = _lengths(case)
+    if case["op"] == "tables":
+        # another seed moves every length and every block
+        ctx = [c + seed % 97 if c > 200 else c for c in ctx]
+        ctx = [min(c, case["width"] * page - q) for c, q in zip(ctx, query)]
+    reqs, total = case["reqs"], max(c + q for c, q in zip(ctx, query))
+    width = case.get("width") or (total + page - 1) // page
+    used = [(c + q + page - 1) // page for c, q in zip(ctx, query)]
+    s["context_lens"] = torch.tensor(ctx, dtype=torch.int32, device=DEV)
+    s["query_lens"] = torch.tensor(query, dtype=torch.int32, device=DEV)
+    blocks = sum(used) + 8
+    ids = torch.randperm(blocks, generator=g, device=DEV).to(torch.int32)
+    if case["op"] == "tables":
+        held = torch.tensor([(c + page - 1) // page for c in ctx], device=DEV)
+        inside = torch.arange(width, device=DEV) < held[:, None]
+        s["block_table"] = torch.full((reqs, width), -1, dtype=torch.int32, device=DEV)
+        s["block_table"][inside] = ids[:int(held.sum())]
+        s["free_blocks"] = ids[int(held.sum()):].contiguous()
+        s["num_free"] = torch.tensor([s["free_blocks"].numel()], dtype=torch.int32, device=DEV)
+        s["max_tokens"] = sum(query) + case["pad"]
+        return s
+    h, d = case["kv_heads"], case["dim"]
+    s["q"] = _rows(g, sum(query), case["heads"], d, case["type"])
+    s["cache"] = _empty_cache(blocks, h, page, d)
+    step = max(1, (1 << 27) // (page * h * d))
+    for first in range(0, blocks, step):  # a part of the cache at a time
+        n = min(step, blocks - first)
+        kc, vc, ks, vs = _parts(s["cache"][first:first + n])
+        for codes, scales in ((kc, ks), (vc, vs)):
+            rows = _rows(g, n * page, h, d, case["type"]).float().unflatten(0, (n, page)).transpose(1, 2)
+            c, e = _codes(rows)
+            codes.copy_(c[..., 0::2] + 16 * c[..., 1::2])
+            scales.copy_(e)
+    inside = torch.arange(width, device=DEV) < torch.tensor(used, device=DEV)[:, None]
+    s["block_table"] = torch.zeros(reqs, width, dtype=torch.int32, device=DEV)
+    s["block_table"][inside] = ids[:sum(used)]
+    s["seq_lens"] = s["context_lens"] + s["query_lens"]
+    s["query_start_loc"] = torch.nn.functional.pad(torch.cumsum(s["query_lens"], 0), (1, 0)).to(torch.int32)
+    s["max_query"], s["max_seq"] = max(query), total
+    s["scale"] = d ** -0.5 / 4
+    s["sink"] = torch.randn(case["heads"], generator=g, device=DEV) * 2 if case["sink"] else None
+    return s
+
+
+# -------------------------------------------------------------- plain forms ----
+
+def _plain_tables(s):
+    page, table, most = s["case"]["page"], s["block_table"], s["max_tokens"]
+    ctx, query = s["context_lens"].long(), s["query_lens"].long()
+    width = table.shape[1]
+    held, all_ = ((n + page - 1).div(page, rounding_mode="floor").clamp(max=width) for n in (ctx, ctx + query))
+    new = all_ - held
+    before = torch.cumsum(new, 0) - new
+    column = torch.arange(width, device=table.device)
+    fresh = (column >= held[:, None]) & (column < all_[:, None])
+    nth = s["num_free"].long() - 1 - (before[:, None] + column - held[:, None])
+    ids = torch.where(nth >= 0, s["free_blocks"][nth.clamp(0, s["free_blocks"].numel() - 1)], -1)
+    table.copy_(torch.where(fresh, ids, table))
+    start = torch.nn.functional.pad(torch.cumsum(query, 0), (1, 0))
+    token = torch.arange(most, device=table.device)
+    req = torch.searchsorted(start[1:].contiguous(), token, right=True).clamp(max=len(query) - 1)
+    inside = token < start[-1]
+    pos = torch.where(inside, ctx[req] + token - start[req], 0)
+    block = table[req, (pos // page).clamp(max=width - 1)].long()
+    slot = torch.where(inside & (pos // page < width) & (block >= 0), block * page + pos % page, PAD)
+    return {"query_start_loc": start.to(torch.int32), "seq_lens": (ctx + query).to(torch.int32), "positions": pos,
+            "slot_mapping": slot, "num_free": s["num_free"].clamp(min=0) - new.sum().to(torch.int32),
+            "block_table": table}
+
+
+def _plain_insert(s):
+    page, kept = s["case"]["page"], s["slots"] >= 0
+    block, at = s["slots"][kept] // page, s["slots"][kept] % page
+    kc, vc, ks, vs = _parts(s["cache"])
+    for rows, codes, scales in ((s["k"], kc, ks), (s["v"], vc, vs)):
+        c, e = _codes(rows[kept].float())
+        codes[block, :, at] = c[..., 0::2] + 16 * c[..., 1::2]
+        scales[block, :, at] = e
+    return s["cache"]
+
+
+def _values(codes, scales):
+    """The 32-bit values of packed codes [..., D / 2] under scale bytes [..., D / 32]."""
+    table = torch.tensor(E2M1 + tuple(-v for v in E2M1), device=codes.device)
+    x = table[torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).long()]
+    return (x.unflatten(-1, (-1, BLOCK)) * torch.exp2(scales.float() - 127).unsqueeze(-1)).flatten(-2)
+
+
+def _plain_attn(s):
+    case, q, most = s["case"], s["q"], s["max_query"]
+    heads, kv_heads = case["heads"], case["kv_heads"]
+    reqs, ctx, query = case["reqs"], s["context_lens"].long(), s["query_lens"].long()
+    # every request's cache, in order, padded to the longest: [reqs, kv heads, keys, D]
+    def gathered(codes, scales):
+        x = _values(codes[s["block_table"]], scales[s["block_table"]])
+        return x.transpose(1, 2).flatten(2, 3)
+    kc, vc, ks, vs = _parts(s["cache"])
+    k, v = gathered(kc, ks), gathered(vc, vs)
+    keys = k.shape[2]
+    # every request's queries, padded to the longest: [reqs, kv heads, tokens * group, D]
+    nth = torch.arange(most, device=q.device)
+    inside = nth < query[:, None]
+    padded = torch.zeros(reqs, most, heads, q.shape[2], device=q.device)
+    padded[inside] = q.float()
+    rows = padded.view(reqs, most, kv_heads, -1, q.shape[2]).transpose(1, 2).flatten(2, 3)
+    scores = (rows @ k.transpose(2, 3) * s["scale"]).view(reqs, kv_heads, most, -1, keys)
+    pos, key = ctx[:, None] + nth, torch.arange(keys, device=q.device)
+    hidden = key > pos[:, :, None]
+    if case["window"]:
+        hidden = hidden | (key <= pos[:, :, None] - case["window"])
+    scores = scores.masked_fill(hidden[:, None, :, None], -torch.inf)
+    top = scores.amax(dim=-1, keepdim=True)
+    p = torch.exp(scores - top)
+    total = p.sum(dim=-1, keepdim=True)
+    out = p.flatten(2, 3) @ v / total.flatten(2, 3)
+    lse = (top + torch.log(total)).squeeze(-1).transpose(1, 2).flatten(2)[inside]
+    out = out.view(reqs, kv_heads, most, -1, q.shape[2]).transpose(1, 2).flatten(2, 3)[inside]
+    if s["sink"] is not None:
+        out = out / (1 + torch.exp(s["sink"] - lse)).unsqueeze(-1)
+    return {"out": out.to(q.dtype), "lse": lse}
+
+
+# ----------------------------------------------------------- this package ----
+
+def _package():
+    if "flaggems_vllm" not in sys.modules:
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                                        "flaggems-vllm_amd"))
+    import flaggems_vllm
+
+    return flaggems_vllm
+
+
+def _own(s):
+    fv, case = _package(), s["case"]
+    if case["op"] == "tables":
+        start, lens, positions, slots, free = fv.build_block_tables(
+            s["context_lens"], s["query_lens"], s["block_table"], s["free_blocks"], s["num_free"], case["page"],
+            s["max_tokens"])
+        return {"query_start_loc": start, "seq_lens": lens, "positions": positions, "slot_mapping": slots,
+                "num_free": free, "block_table": s["block_table"]}
+    if case["op"] == "insert":
+        fv.mxfp4_kv_quant_and_cache(s["k"], s["v"], s["cache"], s["slots"])
+        return s["cache"]
+    out, lse = fv.mxfp4_paged_attention(
+        s["q"], s["cache"], s["block_table"], s["seq_lens"], s["scale"], query_start_loc=s["query_start_loc"],
+        max_query_len=s["max_query"], max_seq_len=s["max_seq"], window_size=case["window"] or None,
+        attn_sink=s["sink"])
+    return {"out": out, "lse": lse}
+
+
+def run(state):
+    if own:
+        return _own(state)
+    op = state["case"]["op"]
+    return _plain_tables(state) if op == "tables" else _plain_insert(state) if op == "insert" else _plain_attn(state)
+
+
+# --------------------------------------------------------------- in 64 bits ----
+
+def _exact_tables(s):
+    page, most = s["case"]["page"], s["max_tokens"]
+    ctx, query = s["context_lens"].tolist(), s["query_lens"].tolist()
+    table, stack = s["block_table"].cpu().numpy().copy(), s["free_blocks"].tolist()[:int(s["num_free"])]
+    start, positions, slots = [0], np.zeros(most, np.int64), np.full(most, PAD, np.int64)
+    for b, (c, q) in enumerate(zip(ctx, query)):
+        for column in range(-(-c // page), min(-(-(c + q) // page), table.shape[1])):
+            table[b, column] = stack.pop()
+        for i in range(q):
+            p = c + i
+            positions[start[-1] + i], slots[start[-1] + i] = p, int(table[b, p // page]) * page + p % page
+        start.append(start[-1] + q)
+    answers = {"query_start_loc": np.array(start, np.int32), "seq_lens": np.array(ctx, np.int32) + np.array(query, np.int32),
+               "positions": positions, "slot_mapping": slots, "num_free": np.array([len(stack)], np.int32), "block_table": table}
+    return {name: torch.from_numpy(np.ascontiguousarray(x)).to(DEV) for name, x in answers.items()}
+
+
+def _exact_insert(s):
+    case, cache = s["case"], s["cache"].clone()
+    page, d = case["page"], case["dim"]
+    flat = cache.view(cache.shape[0], case["kv_heads"], -1)
+    kept = (s["slots"] >= 0).nonzero().flatten()
+    block, at = s["slots"][kept].div(page, rounding_mode="floor"), s["slots"][kept].remainder(page)
+    values = torch.tensor(E2M1, dtype=torch.float64, device=DEV)
+    for which, rows in enumerate((s["k"], s["v"])):
+        x = rows[kept].double().reshape(len(kept), case["kv_heads"], d // BLOCK, BLOCK)
+        most = x.abs().max(dim=-1, keepdim=True).values
+        e = torch.ceil(torch.log2(most / 6)).clamp(-126, 125)
+        y = x / 2.0 ** e
+        off = (y.abs().unsqueeze(-1) - values).abs() + 1e-9 * (torch.arange(8, device=DEV) % 2)  # ties: the even code
+        code = off.argmin(dim=-1) + 8 * (y < 0).long()
+        packed = (code[..., 0::2] + 16 * code[..., 1::2]).reshape(len(kept), case["kv_heads"], d // 2).to(torch.uint8)
+        head = torch.arange(case["kv_heads"], device=DEV)[None, :, None]
+        byte = which * page * d // 2 + (at * (d // 2))[:, None, None] + torch.arange(d // 2, device=DEV)
+        flat[block[:, None, None], head, byte] = packed
+        byte = page * d + which * page * d // BLOCK + (at * (d // BLOCK))[:, None, None] + torch.arange(d // BLOCK, device=DEV)
+        flat[block[:, None, None], head, byte] = (e.squeeze(-1) + 127).to(torch.uint8)
+    return cache
+
+
+def _exact_attn(s):
+    case, q = s["case"], s["q"].double()
+    d, page, group = case["dim"], case["page"], case["heads"] // case["kv_heads"]
+    values = torch.tensor(E2M1, dtype=torch.float64, device=DEV)
+    out, lse = torch.zeros_like(q), torch.zeros(q.shape[:2], dtype=torch.float64, device=DEV)
+    start = s["query_start_loc"].tolist()
+    for b, n in enumerate(s["seq_lens"].tolist()):
+        blocks = s["block_table"][b, :-(-n // page)].long()
+        pos = torch.arange(n - (start[b + 1] - start[b]), n, device=DEV)[:, None]
+        key = torch.arange(n, device=DEV)
+        seen = key <= pos
+        if case["window"]:
+            seen &= key > pos - case["window"]
+        for h in range(case["kv_heads"]):
+            bytes_ = s["cache"][blocks, h].reshape(len(blocks), -1)
+            kv = []
+            for which in (0, 1):
+                codes = bytes_[:, which * page * d // 2:(which + 1) * page * d // 2].reshape(-1, d // 2).long()
+                at = page * d + which * page * d // BLOCK
+                e = bytes_[:, at:at + page * d // BLOCK].reshape(-1, d // BLOCK).double()
+                x = torch.empty(len(codes), d, dtype=torch.float64, device=DEV)
+                for half in (0, 1):
+                    c = codes >> (4 * half)
+                    x[:, half::2] = values[c & 7] * (1 - 2 * ((c >> 3) & 1)).double()
+                kv.append((x * (2.0 ** (e - 127)).repeat_interleave(BLOCK, dim=1))[:n])
+            for i in range(group):
+                head = h * group + i
+                z = torch.mm(q[start[b]:start[b + 1], head], kv[0].t().contiguous()) * s["scale"]
+                z = torch.where(seen, z, -torch.inf)
+                l = torch.logsumexp(z, dim=1)
+                lse[start[b]:start[b + 1], head] = l
+                below = l if s["sink"] is None else torch.logaddexp(l, s["sink"][head].double())
+                out[start[b]:start[b + 1], head] = torch.mm(torch.exp(z - below[:, None]), kv[1])
+    return {"out": out, "lse": lse}
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    return {"tables": _exact_tables, "insert": _exact_insert, "attn": _exact_attn}[case["op"]](s)
