@@ -174,7 +174,8 @@ def _codes(x):
     most = blocks.abs().amax(dim=-1)
     m, e = torch.frexp(most)  # most = m 2^e, m in [1/2, 1): ceil(log2(most / 6)) is e - 3, one more above 3/4
     k = torch.where(most > 0, e - 3 + (m > 0.75).int(), -126).clamp(-126, 125)
-    y = torch.ldexp(blocks.double(), -k.unsqueeze(-1))
+    # 2^-k by its bits
+    y = blocks.double() * ((1023 - k.long()) << 52).view(torch.float64).unsqueeze(-1)
     a = y.abs()
     code = torch.zeros_like(a, dtype=torch.uint8)
     # a value on the border between two codes goes to the even one
@@ -302,7 +303,8 @@ def _values(codes, scales):
     """The 32-bit values of packed codes [..., D / 2] under scale bytes [..., D / 32]."""
     table = torch.tensor(E2M1 + tuple(-v for v in E2M1), device=codes.device)
     x = table[torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).long()]
-    return (x.unflatten(-1, (-1, BLOCK)) * torch.exp2(scales.float() - 127).unsqueeze(-1)).flatten(-2)
+    power = (scales.int() << 23).view(torch.float32)  # 2^(byte - 127) by its bits
+    return (x.unflatten(-1, (-1, BLOCK)) * power.unsqueeze(-1)).flatten(-2)
 
 
 def _plain_attn(s):
@@ -404,8 +406,10 @@ def _exact_insert(s):
     for which, rows in enumerate((s["k"], s["v"])):
         x = rows[kept].double().reshape(len(kept), case["kv_heads"], d // BLOCK, BLOCK)
         most = x.abs().max(dim=-1, keepdim=True).values
-        e = torch.ceil(torch.log2(most / 6)).clamp(-126, 125)
-        y = x / 2.0 ** e
+        # the least power of two that is not below most / 6, looked up
+        powers = torch.tensor([2.0 ** i for i in range(-126, 126)], dtype=torch.float64, device=DEV)
+        at_power = torch.searchsorted(powers, most / 6).clamp(max=251)
+        e, y = at_power - 126, x / powers[at_power]
         off = (y.abs().unsqueeze(-1) - values).abs() + 1e-9 * (torch.arange(8, device=DEV) % 2)  # ties: the even code
         code = off.argmin(dim=-1) + 8 * (y < 0).long()
         packed = (code[..., 0::2] + 16 * code[..., 1::2]).reshape(len(kept), case["kv_heads"], d // 2).to(torch.uint8)
@@ -436,12 +440,13 @@ def _exact_attn(s):
             for which in (0, 1):
                 codes = bytes_[:, which * page * d // 2:(which + 1) * page * d // 2].reshape(-1, d // 2).long()
                 at = page * d + which * page * d // BLOCK
-                e = bytes_[:, at:at + page * d // BLOCK].reshape(-1, d // BLOCK).double()
+                e = bytes_[:, at:at + page * d // BLOCK].reshape(-1, d // BLOCK).long()
                 x = torch.empty(len(codes), d, dtype=torch.float64, device=DEV)
                 for half in (0, 1):
                     c = codes >> (4 * half)
                     x[:, half::2] = values[c & 7] * (1 - 2 * ((c >> 3) & 1)).double()
-                kv.append((x * (2.0 ** (e - 127)).repeat_interleave(BLOCK, dim=1))[:n])
+                powers = torch.tensor([2.0 ** (i - 127) for i in range(256)], dtype=torch.float64, device=DEV)
+                kv.append((x * powers[e].repeat_interleave(BLOCK, dim=1))[:n])
             for i in range(group):
                 head = h * group + i
                 z = torch.mm(q[start[b]:start[b + 1], head], kv[0].t().contiguous()) * s["scale"]
