@@ -1,0 +1,724 @@
+// gfx950 kernels for attention over the paged MXFP4 key/value cache
+// (layout: mxfp4_cache.h).
+//
+// Query token i of request b (query_start_loc[b] <= i < query_start_loc[b+1],
+// or i = b with one token each) stands at position
+//   pos = seq_lens[b] - (tokens of b) + (i - query_start_loc[b])
+// and sees the keys j with pos - window < j <= pos.  Query head h reads the
+// key/value head h / G, G = Hq / Hkv:
+//   s_j = scale * q . k_j,  lse = ln sum_j exp(s_j),
+//   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sink_h)).
+// A token that sees nothing gets out 0 and lse +inf.
+//
+// The rows of a tile are (token, head of the group) pairs of one key/value
+// head, so that a key is read once for all of them.  Everything runs
+// transposed, S^T = K q^T and O^T = V^T P^T: a lane then holds one query row,
+// whose maximum and sum are a scalar in it, and S^T's accumulator layout is the
+// second operand's of PV without a move between lanes.
+//
+// QK: the matrix instruction reads the cache's own format.  K's codes go from
+// memory into the A registers of v_mfma_scale_f32_16x16x128_f8f6f4, the UE8M0
+// bytes are its scales, and nothing is dequantised.  The query is the B
+// operand in e4m3, exactly: divided by a power of two per row that puts the
+// row's maximum into [128, 256), its 8 (bf16) or 11 (fp16) bits split into 2
+// or 3 e4m3 pieces of 4, each under a scale 2^-4 smaller.  What values far
+// below their row's maximum lose is under 2^-20 of that maximum.  Register
+// images (measured; the tests pin them through the results): lane (r, g) =
+// (l % 16, l / 16) holds of A k = 32g..32g+31 of key r, of B k = 16g..16g+15
+// and 64+16g..64+16g+15 of row r; scales apply to k = 32g..32g+31; D holds
+// keys 4g..4g+3 of row r.
+//
+// PV: v_cvt_scalef32_pk_bf16_fp4 gives V in bf16 exactly (codes have two
+// bits), token by token; LDS turns it, written by tokens and read by
+// ds_read_b64_tr_b16.  P goes in as bf16, in fp16 calls as two bf16 pieces
+// (16 bits).  A value block under byte 255 (NaN) makes the outputs of those
+// rows NaN that see it.
+#include <math.h>
+
+#include "fgv_device.h"
+#include "fgv_host.h"
+#include "mxfp4_cache.h"
+
+namespace fgv {
+namespace {
+
+typedef int v8i_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+
+constexpr int kAttThreads = 256;
+constexpr int kAttWaves = kAttThreads / 64;
+constexpr int kTileKeys = 64;  // keys a wave takes at a time: four 16-key subtiles
+constexpr int kRows = 16;      // query rows of a workgroup
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// The running maximum is raised only when a score exceeds it by more than this
+// (base 2), so that most tiles rescale nothing: P stays below 2^8.
+constexpr float kRaise = 8.0f;
+
+struct AttArgs {
+    const void* q;
+    int64_t q_st, q_sh;
+    const uint8_t* cache;
+    int64_t block_stride, num_blocks;
+    const int32_t* block_table;
+    int64_t bt_stride;
+    const int32_t* seq_lens;
+    const int32_t* query_start_loc;  // or null: one token per request
+    const float* sink;               // or null
+    void* out;
+    int64_t o_st, o_sh;
+    float* lse;
+    int64_t lse_st;
+    float scale_f;    // softmax scale * log2(e) = scale_f * 2^scale_e, |scale_f| in [1, 2)
+    int32_t scale_e;
+    int32_t num_reqs, num_tokens, kv_heads, group, page, table_keys, window;
+    int32_t q_wide, o_wide;
+};
+
+// A request's query tokens [first, first + count) and lengths.
+struct Request {
+    int32_t first, count, len;
+};
+
+__device__ __forceinline__ Request request_of(const AttArgs& a, int32_t b) {
+    Request r;
+    if (a.query_start_loc) {
+        const int32_t lo = min(max(a.query_start_loc[b], 0), a.num_tokens);
+        const int32_t hi = min(max(a.query_start_loc[b + 1], 0), a.num_tokens);
+        r.first = lo;
+        r.count = max(hi - lo, 0);
+    } else {
+        r.first = b;
+        r.count = 1;
+    }
+    r.len = max(a.seq_lens[b], 0);
+    return r;
+}
+
+// One workgroup's work: the row tile `tile` of request b.
+struct Item {
+    Request req;
+    int32_t b, tile;
+};
+
+// The row tile number `index`, counted over the requests in order; false
+// behind the last.
+__device__ __forceinline__ bool find_item(const AttArgs& a, int32_t index, Item& item) {
+    __shared__ int32_t part[kAttWaves];
+    __shared__ int32_t found[2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x == 0)
+        found[0] = -1;
+    int32_t before = 0;
+    for (int32_t base = 0; base < a.num_reqs; base += kAttThreads) {
+        const int32_t b = base + (int32_t)threadIdx.x;
+        int32_t tiles = 0;
+        if (b < a.num_reqs) {
+            const Request r = request_of(a, b);
+            tiles = (int32_t)(((int64_t)r.count * a.group + kRows - 1) / kRows);
+        }
+        int32_t s = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int32_t o = __shfl_up(s, d);
+            if (lane >= d)
+                s += o;
+        }
+        if (lane == 63)
+            part[wave] = s;
+        __syncthreads();
+        int32_t at = before + s - tiles;
+#pragma unroll
+        for (int w = 0; w < kAttWaves; ++w) {
+            at += w < wave ? part[w] : 0;
+            before += part[w];
+        }
+        if (index >= at && index < at + tiles) {
+            found[0] = b;
+            found[1] = index - at;
+        }
+        __syncthreads();
+        if (before > index)
+            break;
+    }
+    __syncthreads();
+    item.b = __builtin_amdgcn_readfirstlane(found[0]);
+    if (item.b < 0)
+        return false;
+    item.tile = __builtin_amdgcn_readfirstlane(found[1]);
+    item.req = request_of(a, item.b);
+    return true;
+}
+
+// How the dims of a head meet the matrix instruction's k of 128: kChunks
+// instructions' worth of codes, 16 bytes of them a lane each; kSteps
+// instructions for one 16 x 16 tile of scores with `kPieces` pieces of the query.
+template <int D, int kPieces>
+struct Shape {
+    static constexpr int kChunks = D < 128 ? 1 : D / 128;
+    // at D = 64 two pieces share an instruction, the keys' codes standing there twice
+    static constexpr int kSteps = D < 128 ? (kPieces + 1) / 2 : kChunks * kPieces;
+    static constexpr int kVPitch = 2 * D + 32;  // bytes between tokens of the turned V: the reads' banks differ
+    static constexpr int kVBytes = 32 * kVPitch;
+    static constexpr int kOPitch = 4 * D + 16;
+    static_assert(kRows * kOPitch <= kVBytes, "a wave's O fits its V buffer");
+};
+
+// The query rows as the instruction's B operand.
+template <int D, int kPieces>
+struct Query {
+    v8i_t q[Shape<D, kPieces>::kSteps];
+    int scale[Shape<D, kPieces>::kSteps];
+};
+
+// N consecutive 16-bit values as floats.
+template <bool kHalf, int N>
+__device__ __forceinline__ void load_values(const void* base, int64_t at, bool wide, bool valid, float* x) {
+    const uint16_t* s = static_cast<const uint16_t*>(base) + at;
+    uint32_t w[N / 2];
+    if (!valid) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+            w[i] = 0;
+    } else if (wide) {
+#pragma unroll
+        for (int i = 0; i < N / 8; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(s + 8 * i);
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+            w[i] = (uint32_t)s[2 * i] | (uint32_t)s[2 * i + 1] << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        if constexpr (kHalf) {
+            x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] & 0xffffu));
+            x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
+        } else {
+            x[2 * i] = bf16_lo(w[i]);
+            x[2 * i + 1] = bf16_hi(w[i]);
+        }
+    }
+}
+
+// Four floats of magnitude below 448 to e4m3 codes; x keeps 16 times what they leave.
+__device__ __forceinline__ uint32_t take_piece(float* x) {
+    const uint32_t w = pack_fp8x4(x[0], x[1], x[2], x[3]);
+    x[0] = (x[0] - __builtin_amdgcn_cvt_f32_fp8((int)w, 0)) * 16.0f;
+    x[1] = (x[1] - __builtin_amdgcn_cvt_f32_fp8((int)w, 1)) * 16.0f;
+    x[2] = (x[2] - __builtin_amdgcn_cvt_f32_fp8((int)w, 2)) * 16.0f;
+    x[3] = (x[3] - __builtin_amdgcn_cvt_f32_fp8((int)w, 3)) * 16.0f;
+    return w;
+}
+
+// Row r of lane (r, g) at element `at` of q.
+template <int D, int kPieces, bool kHalf>
+__device__ __forceinline__ void load_query(const AttArgs& a, int64_t at, bool valid, int g, Query<D, kPieces>& out) {
+    constexpr int kRuns = D / 64;  // runs of 16 dims per lane
+    float x[kRuns][16];
+    uint32_t most = 0;
+#pragma unroll
+    for (int c = 0; c < kRuns; ++c) {
+        load_values<kHalf, 16>(a.q, at + 64 * c + 16 * g, a.q_wide, valid, x[c]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            most = max(most, __float_as_uint(x[c][i]) & 0x7fffffffu);
+    }
+    // over the row's four lanes
+    most = max(most, (uint32_t)__shfl_xor((int)most, 16));
+    most = max(most, (uint32_t)__shfl_xor((int)most, 32));
+    const bool bad = most >= 0x7f800000u;
+    // q 2^scale_e = x 2^e with the row's maximum in [128, 256): the softmax scale's power of two goes in here, so that
+    // scores leave binary32's range only where scaled ones would.  -118 leaves room for the pieces' smaller scales.
+    const int e = min(max((int)(most >> 23) - 127 - 7 + a.scale_e, -118), 127);
+    const float down = __uint_as_float((uint32_t)min(max(127 - e + a.scale_e, 1), 254) << 23);
+#pragma unroll
+    for (int c = 0; c < kRuns; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            x[c][i] = bad ? 0.f : x[c][i] * down;
+    const int byte = e + 127;
+    if constexpr (D == 64) {
+#pragma unroll
+        for (int s = 0; s < Shape<D, kPieces>::kSteps; ++s) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    out.q[s][4 * half + i] = 2 * s + half < kPieces ? (int)take_piece(&x[0][4 * i]) : 0;
+            out.scale[s] = bad ? 255 : byte - 4 * (2 * s + (g >> 1));
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+            for (int c = 0; c < Shape<D, kPieces>::kChunks; ++c) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        out.q[p * Shape<D, kPieces>::kChunks + c][4 * half + i] = (int)take_piece(&x[2 * c + half][4 * i]);
+                out.scale[p * Shape<D, kPieces>::kChunks + c] = bad ? 255 : byte - 4 * p;
+            }
+    }
+}
+
+// A wave's 64 keys as they stand in the cache: lane (r, g) has dims 32g..32g+31
+// of each chunk of token 16t + r.
+template <int kChunks>
+struct RawTile {
+    uint4 k[4][kChunks], v[4][kChunks];
+    uint32_t ks[4][kChunks], vs[4][kChunks];
+};
+
+// Where a wave's next 16 tiles lie: lane 4i + t has subtile t of the i-th of
+// them, the head's block at `base` and the first of its tokens at `place`
+// (negative: no block).  Tiles of a wave are `stride` keys apart.
+struct Places {
+    int64_t base;
+    int32_t place;
+};
+
+__device__ __forceinline__ Places find_places(const AttArgs& a, int32_t b, int32_t h, int32_t token_bytes, int32_t key0,
+                                              int32_t stride, int32_t end, int lane) {
+    const int64_t key = (int64_t)key0 + (int64_t)(lane >> 2) * stride + 16 * (lane & 3);
+    Places p = {0, -1};
+    if (key < end) {
+        const int32_t column = (int32_t)key / a.page;
+        const int32_t id = a.block_table[(int64_t)b * a.bt_stride + column];
+        if (id >= 0 && id < a.num_blocks) {
+            p.base = (int64_t)id * a.block_stride + (int64_t)h * a.page * token_bytes;
+            p.place = (int32_t)key - column * a.page;
+        }
+    }
+    return p;
+}
+
+template <int D>
+__device__ __forceinline__ void load_tile(const AttArgs& a, const Places& p, int tile, int lane,
+                                          RawTile<D < 128 ? 1 : D / 128>& raw, int32_t (&place)[4]) {
+    constexpr int kChunks = D < 128 ? 1 : D / 128;
+    const int r = lane & 15, g = D < 128 ? (lane >> 4) & 1 : lane >> 4;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int from = (tile & 15) * 4 + t;
+        const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)p.base, from);
+        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)p.base >> 32), from);
+        place[t] = __builtin_amdgcn_readlane(p.place, from);
+        // a subtile without a block reads the cache's first one, whose values nobody sees
+        const int32_t first = max(place[t], 0);
+        const uint8_t* head = a.cache + (int64_t)((uint64_t)hi << 32 | lo);
+        const uint8_t* kc = head + (int64_t)first * (D / 2);
+        const uint8_t* vc = kc + mx_part(1, a.page, D);
+        const uint8_t* ks = head + mx_part(2, a.page, D) + (int64_t)first * (D / kMxBlock);
+        const uint8_t* vs = ks + (int64_t)a.page * (D / kMxBlock);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            raw.k[t][c] = *reinterpret_cast<const uint4*>(kc + (uint32_t)(r * (D / 2) + 64 * c + 16 * g));
+            raw.ks[t][c] = ks[(uint32_t)(r * (D / kMxBlock) + 4 * c + g)];
+            raw.v[t][c] = *reinterpret_cast<const uint4*>(vc + (uint32_t)(r * (D / 2) + 64 * c + 16 * g));
+            raw.vs[t][c] = vs[(uint32_t)(r * (D / kMxBlock) + 4 * c + g)];
+        }
+    }
+}
+
+// 8 codes times 2^(byte - 127) in bf16, exact below byte 253; byte 255 gives NaN.
+__device__ __forceinline__ uint4 values_of(uint32_t codes, float scale) {
+    return make_uint4(
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3)));
+}
+
+__device__ __forceinline__ uint2 read_turned(const uint8_t* at) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (lds_short4_t*)(__attribute__((address_space(3))) uint8_t*)at));
+}
+
+__device__ __forceinline__ v8i_t key_operand(uint4 k) {
+    const v8i_t v = {(int)k.x, (int)k.y, (int)k.z, (int)k.w, 0, 0, 0, 0};
+    return v;
+}
+
+// What a lane knows of its row: the keys (lo, pos] are seen.
+struct Seen {
+    int32_t lo, pos;
+    __device__ bool operator()(int32_t key) const { return key > lo && key <= pos; }
+};
+
+// Attends the 64 keys from key0 on for the wave's 16 rows.  kMask: some of
+// them are hidden from some of the rows.
+template <int D, int kPieces, bool kMask>
+__device__ __forceinline__ void attend(const RawTile<Shape<D, kPieces>::kChunks>& raw, const int32_t (&place)[4],
+                                       int32_t key0, int32_t any_lo, int32_t any_pos, Seen seen, float scale_f,
+                                       const Query<D, kPieces>& query, uint8_t* turned, int lane, f32x4_t (&acc)[D / 16],
+                                       float& m_run, float& l_run) {
+    using S = Shape<D, kPieces>;
+    const int r = lane & 15, g = lane >> 4;
+    f32x4_t s[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < S::kSteps; ++i) {
+            const int c = i % S::kChunks;
+            s[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(key_operand(raw.k[t][c]), query.q[i], s[t], 4, 0, 0,
+                                                                    (int)raw.ks[t][c], 0, query.scale[i]);
+        }
+    }
+    float p[16];
+    float most = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v = s[t][i] * scale_f;
+            if constexpr (kMask)
+                v = place[t] >= 0 && seen(key0 + 16 * t + 4 * g + i) ? v : -INFINITY;
+            p[4 * t + i] = v;
+            most = fmaxf(most, v);
+        }
+    most = group4_max(most);
+    if (__any(most > m_run + kRaise)) {
+        const float m_new = fmaxf(m_run, most);
+        const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+        l_run *= alpha;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+            acc[d] *= alpha;
+        m_run = m_new;
+    }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(p[i] - m_use);
+        sum += p[i];
+    }
+    l_run += sum;  // this lane's keys; the row's four lanes are added up at the end
+
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int t = 2 * half + u;
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c) {
+                uint32_t byte = raw.vs[t][c];
+                if constexpr (kMask) {
+                    // a token that no row sees may hold anything; a NaN that some rows see is dealt with below
+                    const int32_t key = key0 + 16 * t + r;
+                    if (byte == 255u || place[t] < 0 || key <= any_lo || key > any_pos)
+                        byte = 0;
+                }
+                const float scale = __uint_as_float(byte << 23);
+                if (D >= 128 || g < 2) {
+                    uint4* to = reinterpret_cast<uint4*>(turned + (16 * u + r) * S::kVPitch + 256 * c + 64 * g);
+                    to[0] = values_of(raw.v[t][c].x, scale);
+                    to[1] = values_of(raw.v[t][c].y, scale);
+                    to[2] = values_of(raw.v[t][c].z, scale);
+                    to[3] = values_of(raw.v[t][c].w, scale);
+                }
+            }
+        }
+        asm volatile("" ::: "memory");
+        // k = 8g + i of this product is key 4g + i, or 16 + 4g + i - 4
+        const float* ph = p + 8 * half;
+        const uint4 hi = make_uint4(pack_bf16x2(ph[0], ph[1]), pack_bf16x2(ph[2], ph[3]), pack_bf16x2(ph[4], ph[5]),
+                                    pack_bf16x2(ph[6], ph[7]));
+        uint4 lo = make_uint4(0, 0, 0, 0);
+        if constexpr (kPieces == 3)
+            lo = make_uint4(pack_bf16x2(ph[0] - bf16_lo(hi.x), ph[1] - bf16_hi(hi.x)),
+                            pack_bf16x2(ph[2] - bf16_lo(hi.y), ph[3] - bf16_hi(hi.y)),
+                            pack_bf16x2(ph[4] - bf16_lo(hi.z), ph[5] - bf16_hi(hi.z)),
+                            pack_bf16x2(ph[6] - bf16_lo(hi.w), ph[7] - bf16_hi(hi.w)));
+        // lane j of group g reads 4 dims of row 4g + j / 4 and gets dim j of rows 4g..4g+3
+        const uint8_t* from = turned + (4 * g + (r >> 2)) * S::kVPitch + 8 * (r & 3);
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+            const uint2 x = read_turned(from + 32 * d), y = read_turned(from + 16 * S::kVPitch + 32 * d);
+            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, make_uint4(x.x, x.y, y.x, y.y));
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, hi), acc[d], 0, 0, 0);
+            if constexpr (kPieces == 3)
+                acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, lo), acc[d], 0, 0, 0);
+        }
+    }
+
+    if constexpr (kMask) {
+        // value blocks that are NaN, for the rows that see them (rare: the loop is entered by a vote)
+        bool nan = false;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+                nan |= raw.vs[t][c] == 255u;
+        if (__any(nan)) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int c = 0; c < S::kChunks; ++c)
+#pragma unroll
+                    for (int b = 0; b < (D < 128 ? 2 : 4); ++b) {
+                        bool hit = false;
+                        for (int token = 0; token < 16; ++token)
+                            hit |= __builtin_amdgcn_readlane(raw.vs[t][c], 16 * b + token) == 255u && place[t] >= 0 &&
+                                   seen(key0 + 16 * t + token);
+                        const float add = hit ? NAN : 0.f;
+                        acc[8 * c + 2 * b] += add;
+                        acc[8 * c + 2 * b + 1] += add;
+                    }
+        }
+    }
+}
+
+// A 16-row tile over all of its keys: four waves take 64 keys each in turn,
+// and their sums meet in LDS.
+template <int D, int kPieces>
+__global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a) {
+    using S = Shape<D, kPieces>;
+    constexpr bool kHalf = kPieces == 3;
+    __shared__ __align__(16) uint8_t turned[kAttWaves][S::kVBytes];
+    __shared__ float wave_m[kAttWaves][kRows], wave_l[kAttWaves][kRows];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int h = (int)blockIdx.x % a.kv_heads;
+    Item item;
+    if (!find_item(a, (int32_t)(blockIdx.x / a.kv_heads), item))
+        return;
+    const Request req = item.req;
+    const int r = lane & 15, g = lane >> 4;
+    const int32_t rows = req.count * a.group;  // fits: count * group rows are rows of q
+    const int32_t row = item.tile * kRows + r;
+    const bool valid = row < rows;
+    const int32_t token = (valid ? row : 0) / a.group;
+    const int32_t head = h * a.group + (valid ? row - token * a.group : 0);
+
+    const int32_t pos0 = req.len - req.count;
+    const int32_t last_row = min(item.tile * kRows + kRows, rows) - 1;
+    const int32_t first_pos = pos0 + item.tile * kRows / a.group, last_pos = pos0 + last_row / a.group;
+    Seen seen;
+    seen.pos = valid ? pos0 + token : -1;
+    seen.lo = a.window > 0 ? seen.pos - a.window : -1;
+    const int32_t any_lo = a.window > 0 ? first_pos - a.window : -1;
+    const int32_t end = min(last_pos + 1, a.table_keys);
+    const int32_t begin = max(any_lo + 1, 0) & ~(kTileKeys - 1);
+
+    Query<D, kPieces> query;
+    load_query<D, kPieces, kHalf>(a, (req.first + token) * a.q_st + head * a.q_sh, valid, g, query);
+    f32x4_t acc[D / 16];
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+        acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.f;
+
+    constexpr int kStride = kAttWaves * kTileKeys;
+    const int32_t key0 = begin + wave * kTileKeys;
+    const int32_t tiles = end > key0 ? (end - key0 + kStride - 1) / kStride : 0;
+    Places places;
+    for (int32_t i = 0; i < tiles; ++i) {
+        const int32_t key = key0 + i * kStride;
+        if ((i & 15) == 0)
+            places = find_places(a, item.b, h, mx_token_bytes(D), key, kStride, end, lane);
+        RawTile<S::kChunks> raw;
+        int32_t place[4];
+        load_tile<D>(a, places, i, lane, raw, place);
+        const bool all = key + kTileKeys - 1 <= min(first_pos, end - 1) && (a.window == 0 || key > last_pos - a.window) &&
+                         place[0] >= 0 && place[1] >= 0 && place[2] >= 0 && place[3] >= 0;
+        if (all)
+            attend<D, kPieces, false>(raw, place, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane,
+                                      acc, m_run, l_run);
+        else
+            attend<D, kPieces, true>(raw, place, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane,
+                                     acc, m_run, l_run);
+    }
+    l_run = group4_sum(l_run);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+        *reinterpret_cast<f32x4_t*>(turned[wave] + r * S::kOPitch + 64 * d + 16 * g) = acc[d];
+    if (g == 0) {
+        wave_m[wave][r] = m_run;
+        wave_l[wave][r] = l_run;
+    }
+    __syncthreads();
+
+    // 16 threads per row, D / 16 dims each
+    constexpr int kDims = D / 16;
+    const int orow = threadIdx.x >> 4, part = threadIdx.x & 15;
+    const int32_t mine = item.tile * kRows + orow;
+    if (mine >= rows)
+        return;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kAttWaves; ++w)
+        m = fmaxf(m, wave_m[w][orow]);
+    const float m_use = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[kDims];
+#pragma unroll
+    for (int i = 0; i < kDims; ++i)
+        o[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kAttWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(wave_m[w][orow] - m_use);
+        l += f * wave_l[w][orow];
+        const float* from = reinterpret_cast<const float*>(turned[w] + orow * S::kOPitch) + part * kDims;
+#pragma unroll
+        for (int i = 0; i < kDims; i += 4) {
+            const f32x4_t v = *reinterpret_cast<const f32x4_t*>(from + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                o[i + j] += f * v[j];
+        }
+    }
+    const int32_t otoken = mine / a.group, ohead = h * a.group + mine - otoken * a.group;
+    const int64_t t = req.first + otoken;
+    const bool none = m == -INFINITY && l == 0.f;
+    float below = l;
+    if (a.sink)
+        below += __builtin_amdgcn_exp2f(a.sink[ohead] * kLog2e - m_use);
+    const float inv = none ? 0.f : 1.0f / below;
+    uint16_t* to = static_cast<uint16_t*>(a.out) + t * a.o_st + ohead * a.o_sh + part * kDims;
+    uint32_t w[kDims / 2];
+#pragma unroll
+    for (int i = 0; i < kDims / 2; ++i) {
+        const float x = o[2 * i] * inv, y = o[2 * i + 1] * inv;
+        if constexpr (kHalf) {
+            w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x) |
+                   (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)y) << 16;
+        } else {
+            w[i] = pack_bf16x2(x, y);
+        }
+    }
+    if (a.o_wide) {
+#pragma unroll
+        for (int i = 0; i < kDims / 2; i += 2)
+            *reinterpret_cast<uint2*>(to + 2 * i) = make_uint2(w[i], w[i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kDims / 2; ++i) {
+            to[2 * i] = (uint16_t)w[i];
+            to[2 * i + 1] = (uint16_t)(w[i] >> 16);
+        }
+    }
+    if (part == 0)
+        a.lse[t * a.lse_st + ohead] = none ? INFINITY : kLn2 * (m_use + __builtin_amdgcn_logf(l));
+}
+
+template <int D>
+void launch_attend(bool half, unsigned grid, hipStream_t st, const AttArgs& a) {
+    if (half)
+        hipLaunchKernelGGL((mxfp4_attend_kernel<D, 3>), dim3(grid), dim3(kAttThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL((mxfp4_attend_kernel<D, 2>), dim3(grid), dim3(kAttThreads), 0, st, a);
+}
+
+}  // namespace
+}  // namespace fgv
+
+extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, int32_t dtype,
+                                         int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                                         const uint8_t* kv_cache, int64_t cache_block_stride, int64_t num_blocks,
+                                         int64_t block_size, const int32_t* block_table, int64_t block_table_stride,
+                                         int64_t max_blocks_per_req, const int32_t* seq_lens,
+                                         const int32_t* query_start_loc, int64_t num_reqs, int64_t max_query_len,
+                                         int64_t max_seq_len, double softmax_scale, int64_t window_size,
+                                         const float* attn_sink, void* out, int64_t out_stride_token,
+                                         int64_t out_stride_head, float* lse, int64_t lse_stride_token, void* workspace,
+                                         int64_t workspace_bytes, void* stream) {
+    using namespace fgv;
+    (void)max_query_len;
+    (void)max_seq_len;
+    (void)workspace;
+    (void)workspace_bytes;
+    if (num_tokens < 0 || num_heads < 0 || num_kv_heads < 0 || num_blocks < 0 || num_reqs < 0 || max_blocks_per_req < 0 ||
+        max_query_len < 0 || max_seq_len < 0 || window_size < 0)
+        return fail(FGV_E_BAD_SHAPE, "negative size");
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return fail(FGV_E_BAD_SHAPE, "head_dim must be 64, 128 or 256");
+    if (dtype != 0 && dtype != 1)
+        return fail(FGV_E_BAD_SHAPE, "dtype must be 0 (bf16) or 1 (fp16)");
+    if (block_size <= 0 || block_size % 16 != 0)
+        return fail(FGV_E_BAD_SHAPE, "block_size must be a positive multiple of 16");
+    if (num_tokens == 0 || num_heads == 0 || num_reqs == 0)
+        return FGV_OK;
+    if (num_kv_heads == 0 || num_heads % num_kv_heads != 0)
+        return fail(FGV_E_BAD_SHAPE, "num_heads must be a multiple of num_kv_heads");
+    if (!query_start_loc && num_tokens != num_reqs)
+        return fail(FGV_E_BAD_SHAPE, "without query_start_loc there is one token per request");
+    if (!(softmax_scale >= -1e30 && softmax_scale <= 1e30))
+        return fail(FGV_E_BAD_SHAPE, "softmax_scale must be finite");
+    if (num_heads > 65536 || block_size > 4096 || num_reqs > 0x3fffffffLL || num_blocks > 0x7fffffffLL ||
+        num_tokens * num_heads > 0x3fffffffLL || max_blocks_per_req > (0x3fffffffLL / block_size))
+        return fail(FGV_E_TOO_LARGE, "at most 65536 heads, 4096 tokens per block, 2^30 - 1 query rows and table keys");
+    if (!q || !out || !lse || !seq_lens || (max_blocks_per_req > 0 && !block_table) || (num_blocks > 0 && !kv_cache))
+        return fail(FGV_E_NULL_POINTER, "null pointer argument");
+    if (num_blocks > 0 && (cache_block_stride < num_kv_heads * block_size * mx_token_bytes((int)head_dim) ||
+                           cache_block_stride % 16 != 0))
+        return fail(FGV_E_BAD_STRIDE, "cache_block_stride must hold a block and be a multiple of 16");
+    if (!aligned(kv_cache, 16) || !aligned(q, 2) || !aligned(out, 2) || !aligned(lse, 4))
+        return fail(FGV_E_MISALIGNED, "kv_cache must be 16-byte aligned, q, out and lse by element");
+    AttArgs a;
+    a.q = q;
+    a.q_st = q_stride_token;
+    a.q_sh = q_stride_head;
+    a.cache = kv_cache;
+    a.block_stride = cache_block_stride;
+    a.num_blocks = num_blocks;
+    a.block_table = block_table;
+    a.bt_stride = block_table_stride;
+    a.seq_lens = seq_lens;
+    a.query_start_loc = query_start_loc;
+    a.sink = attn_sink;
+    a.out = out;
+    a.o_st = out_stride_token;
+    a.o_sh = out_stride_head;
+    a.lse = lse;
+    a.lse_st = lse_stride_token;
+    const double scale_log2 = softmax_scale * 1.4426950408889634;
+    int e = 0;
+    frexp(scale_log2, &e);
+    a.scale_e = scale_log2 == 0.0 ? 0 : e - 1 < -100 ? -100 : e - 1;
+    a.scale_f = (float)ldexp(scale_log2, -a.scale_e);
+    a.num_reqs = (int32_t)num_reqs;
+    a.num_tokens = (int32_t)num_tokens;
+    a.kv_heads = (int32_t)num_kv_heads;
+    a.group = (int32_t)(num_heads / num_kv_heads);
+    a.page = (int32_t)block_size;
+    // without a block nothing is seen
+    a.table_keys = num_blocks > 0 ? (int32_t)(max_blocks_per_req * block_size) : 0;
+    a.window = (int32_t)(window_size < 0x3fffffffLL ? window_size : 0);
+    a.q_wide = aligned(q, 16) && ((q_stride_token | q_stride_head) & 7) == 0;
+    a.o_wide = aligned(out, 8) && ((out_stride_token | out_stride_head) & 3) == 0;
+    // no request has more tiles than its rows' share, rounded up
+    const int64_t tiles = num_tokens * a.group / kRows + num_reqs;
+    if (tiles * num_kv_heads > 0x7fffffffLL)
+        return fail(FGV_E_TOO_LARGE, "too many row tiles");
+    const unsigned grid = (unsigned)(tiles * num_kv_heads);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    switch (head_dim) {
+        case 64: launch_attend<64>(dtype == 1, grid, st, a); break;
+        case 128: launch_attend<128>(dtype == 1, grid, st, a); break;
+        default: launch_attend<256>(dtype == 1, grid, st, a); break;
+    }
+    return launch_status();
+}
+
+extern "C" int64_t fgv_mxfp4_paged_attention_workspace_bytes(int64_t num_tokens, int64_t num_heads,
+                                                             int64_t num_kv_heads, int64_t head_dim, int64_t num_reqs,
+                                                             int64_t max_query_len, int64_t max_seq_len) {
+    (void)num_tokens;
+    (void)num_heads;
+    (void)num_kv_heads;
+    (void)head_dim;
+    (void)num_reqs;
+    (void)max_query_len;
+    (void)max_seq_len;
+    return 0;
+}

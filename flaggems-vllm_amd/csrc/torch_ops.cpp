@@ -7,7 +7,9 @@
 // dequantize_and_gather_k_cache, fused_indexer_q_rope_quant,
 // compute_slot_mapping_parallel, indexer_k_quant_and_cache) and the 8-bit
 // linear ops around the layer (fused_add_rms_norm_quant,
-// fused_silu_mul_quant, int8_scaled_mm), which have no counterpart there.
+// fused_silu_mul_quant, int8_scaled_mm) and the ops of the 4-bit paged cache
+// (build_block_tables, mxfp4_kv_quant_and_cache, mxfp4_paged_attention), which
+// have no counterpart there.
 //
 // The argument checks, the output allocation and the launch run here in C++,
 // so an eager call costs a few microseconds of host time instead of the
@@ -613,6 +615,167 @@ int int8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& scale_a,
                               ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, current_stream(a));
 }
 
+// ---- serving from the 4-bit paged cache: block tables, insert, attention ----
+
+bool is_i32_vector(const at::Tensor& t, int64_t n) {
+    return t.dim() == 1 && t.size(0) == n && t.scalar_type() == at::kInt && (n <= 1 || t.stride(0) == 1);
+}
+
+using TablesOut = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+int build_block_tables(const at::Tensor& context_lens, const at::Tensor& query_lens, const at::Tensor& block_table,
+                       const at::Tensor& free_blocks, const at::Tensor& num_free, int64_t block_size,
+                       int64_t max_num_tokens, int64_t pad_id, TablesOut* out) {
+    FGV_ASSERT(context_lens.dim() == 1, "context_lens must be 1-D");
+    const int64_t reqs = context_lens.size(0);
+    FGV_ASSERT(is_i32_vector(context_lens, reqs) && is_i32_vector(query_lens, reqs),
+               "context_lens and query_lens must be contiguous int32 [num_reqs]");
+    FGV_ASSERT(block_table.dim() == 2 && block_table.size(0) == reqs && block_table.scalar_type() == at::kInt,
+               "block_table must be int32 [num_reqs, max blocks]");
+    FGV_ASSERT(unit_rows(block_table) && (reqs <= 1 || block_table.stride(0) >= block_table.size(1)),
+               "block_table's rows must be contiguous and apart");
+    FGV_ASSERT(free_blocks.dim() == 1 && is_i32_vector(free_blocks, free_blocks.size(0)),
+               "free_blocks must be contiguous 1-D int32");
+    FGV_ASSERT(num_free.numel() == 1 && num_free.scalar_type() == at::kInt, "num_free must be one int32");
+    FGV_ASSERT(block_size > 0, "block_size must be positive");
+    FGV_ASSERT(max_num_tokens >= 0, "max_num_tokens must not be negative");
+    if (const char* why = any_not_readable(context_lens, query_lens, block_table, free_blocks, num_free))
+        return assert_failed(why);
+    FGV_ASSERT(!spans_meet(block_table, context_lens) && !spans_meet(block_table, query_lens) &&
+                   !spans_meet(block_table, free_blocks) && !spans_meet(block_table, num_free),
+               "block_table must not overlap an input");
+    const c10::Device dev = block_table.device();
+    FGV_ASSERT(dev.is_cuda(), "flaggems_vllm runs on the GPU (HIP) only");
+    FGV_ASSERT(context_lens.device() == dev && query_lens.device() == dev && free_blocks.device() == dev &&
+                   num_free.device() == dev,
+               "all tensors must be on block_table's device");
+    const c10::DeviceGuard guard(dev);
+    const at::Tensor qsl = new_on(dev, {reqs + 1}, at::kInt), lens = new_on(dev, {reqs}, at::kInt);
+    const at::Tensor positions = new_on(dev, {max_num_tokens}, at::kLong);
+    const at::Tensor slots = new_on(dev, {max_num_tokens}, at::kLong), left = new_on(dev, {1}, at::kInt);
+    *out = TablesOut(qsl, lens, positions, slots, left);
+    return fgv_build_block_tables(i32_ptr(context_lens), i32_ptr(query_lens), reqs, i32_ptr(block_table),
+                                  block_table.stride(0), block_table.size(1), i32_ptr(free_blocks), free_blocks.size(0),
+                                  i32_ptr(num_free), block_size, max_num_tokens, pad_id, i32_ptr(qsl), i32_ptr(lens),
+                                  positions.data_ptr<int64_t>(), slots.data_ptr<int64_t>(), i32_ptr(left),
+                                  current_stream(block_table));
+}
+
+// The head dim of an MXFP4 cache [blocks, kv heads, block size, D + D / 16]; 0: it is none.
+int64_t mx_head_dim(const at::Tensor& cache) {
+    if (cache.dim() != 4 || cache.scalar_type() != at::kByte)
+        return 0;
+    const int64_t width = cache.size(3);
+    return width == 68 ? 64 : width == 136 ? 128 : width == 272 ? 256 : 0;
+}
+
+constexpr const char* kMxCache =
+    "kv_cache must be uint8 [num_blocks, num_kv_heads, block_size, D + D / 16], D 64, 128 or 256";
+
+int mxfp4_insert(const at::Tensor& k, const at::Tensor& v, const at::Tensor& cache, const at::Tensor& slots) {
+    const int64_t dim = mx_head_dim(cache);
+    FGV_ASSERT(dim > 0, kMxCache);
+    FGV_ASSERT(blocks_contiguous(cache), "each kv_cache block must be contiguous bytes");
+    FGV_ASSERT(cache.size(2) > 0 && cache.size(2) % 16 == 0 && cache.size(2) <= 4096,
+               "block_size must be a multiple of 16 of at most 4096");
+    FGV_ASSERT(k.dim() == 3 && v.sizes() == k.sizes() && k.size(1) == cache.size(1) && k.size(2) == dim,
+               "k and v must be [num_tokens, num_kv_heads, D]");
+    FGV_ASSERT((k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kHalf) && v.scalar_type() == k.scalar_type(),
+               "k and v must both be bfloat16 or float16");
+    FGV_ASSERT(k.stride(2) == 1 && v.stride(2) == 1, "k's and v's rows must be contiguous");
+    FGV_ASSERT(slots.dim() == 1 && slots.scalar_type() == at::kLong && (slots.size(0) <= 1 || slots.stride(0) == 1),
+               "slot_mapping must be contiguous 1-D int64");
+    FGV_ASSERT(slots.size(0) <= k.size(0), "slot_mapping is longer than the number of tokens");
+    FGV_ASSERT(!takes_grad(k) && !takes_grad(v), "inference only: no input may require a gradient or carry a tangent");
+    if (const char* why = any_not_readable(k, v, cache, slots))
+        return assert_failed(why);
+    FGV_ASSERT(!spans_meet(cache, k) && !spans_meet(cache, v) && !spans_meet(cache, slots),
+               "kv_cache must not overlap an input");
+    const c10::Device dev = cache.device();
+    FGV_ASSERT(dev.is_cuda(), "flaggems_vllm runs on the GPU (HIP) only");
+    FGV_ASSERT(k.device() == dev && v.device() == dev && slots.device() == dev,
+               "all tensors must be on kv_cache's device");
+    const c10::DeviceGuard guard(dev);
+    return fgv_mxfp4_kv_quant_and_cache(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                                        k.scalar_type() == at::kHalf ? 1 : 0, slots.size(0), k.size(1), dim,
+                                        cache.data_ptr<uint8_t>(), cache.stride(0), cache.size(0), cache.size(2),
+                                        slots.data_ptr<int64_t>(), current_stream(cache));
+}
+
+int mxfp4_attention(const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_table,
+                    const at::Tensor& seq_lens, double scale, const std::optional<at::Tensor>& query_start_loc,
+                    std::optional<int64_t> max_query_len, std::optional<int64_t> max_seq_len,
+                    std::optional<int64_t> window, const std::optional<at::Tensor>& sink,
+                    const std::optional<at::Tensor>& out_in, TensorPair* result) {
+    const int64_t dim = mx_head_dim(cache);
+    FGV_ASSERT(dim > 0, kMxCache);
+    FGV_ASSERT(blocks_contiguous(cache), "each kv_cache block must be contiguous bytes");
+    const int64_t page = cache.size(2), kv_heads = cache.size(1);
+    FGV_ASSERT(page > 0 && page % 16 == 0 && page <= 4096, "block_size must be a multiple of 16 of at most 4096");
+    FGV_ASSERT(q.dim() == 3 && q.size(2) == dim, "q must be [num_tokens, num_heads, D]");
+    FGV_ASSERT(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "q must be bfloat16 or float16");
+    FGV_ASSERT(q.stride(2) == 1, "q's rows must be contiguous");
+    const int64_t tokens = q.size(0), heads = q.size(1);
+    FGV_ASSERT(kv_heads > 0 && heads % kv_heads == 0, "num_heads must be a multiple of num_kv_heads");
+    FGV_ASSERT(seq_lens.dim() == 1, "seq_lens must be 1-D");
+    const int64_t reqs = seq_lens.size(0);
+    FGV_ASSERT(is_i32_vector(seq_lens, reqs), "seq_lens must be contiguous int32 [num_reqs]");
+    FGV_ASSERT(block_table.dim() == 2 && block_table.size(0) == reqs && block_table.scalar_type() == at::kInt,
+               "block_table must be int32 [num_reqs, max blocks]");
+    FGV_ASSERT(unit_rows(block_table), "block_table's rows must be contiguous");
+    if (query_start_loc)
+        FGV_ASSERT(is_i32_vector(*query_start_loc, reqs + 1), "query_start_loc must be contiguous int32 [num_reqs + 1]");
+    else
+        FGV_ASSERT(tokens == reqs, "without query_start_loc there is one token per request");
+    FGV_ASSERT(std::isfinite(scale) && std::fabs(scale) <= 1e30, "softmax_scale must be finite");
+    FGV_ASSERT(!window || *window >= 1, "window_size must be at least 1");
+    FGV_ASSERT((!max_query_len || *max_query_len >= 0) && (!max_seq_len || *max_seq_len >= 0),
+               "max_query_len and max_seq_len must not be negative");
+    if (sink)
+        FGV_ASSERT(sink->dim() == 1 && sink->size(0) == heads && sink->scalar_type() == at::kFloat &&
+                       (heads <= 1 || sink->stride(0) == 1),
+                   "attn_sink must be contiguous float32 [num_heads]");
+    FGV_ASSERT(!takes_grad(q) && !(sink && takes_grad(*sink)),
+               "inference only: no input may require a gradient or carry a tangent");
+    if (const char* why = any_not_readable(q, cache, block_table, seq_lens, query_start_loc, sink, out_in))
+        return assert_failed(why);
+    const c10::Device dev = q.device();
+    FGV_ASSERT(cache.device() == dev && block_table.device() == dev && seq_lens.device() == dev &&
+                   (!query_start_loc || query_start_loc->device() == dev) && (!sink || sink->device() == dev) &&
+                   (!out_in || out_in->device() == dev),
+               "all tensors must be on q's device");
+    if (out_in) {
+        const at::Tensor& o = *out_in;
+        FGV_ASSERT(o.sizes() == q.sizes() && o.scalar_type() == q.scalar_type(), "out must have q's shape and type");
+        FGV_ASSERT(!takes_grad(o), "inference only: no output may require a gradient or carry a tangent");
+        FGV_ASSERT(o.stride(2) == 1 && (heads <= 1 || o.stride(1) >= dim) &&
+                       (tokens <= 1 || o.stride(0) >= (heads - 1) * o.stride(1) + dim),
+                   "out's rows must be contiguous and apart, heads within tokens");
+        FGV_ASSERT(!spans_meet(o, q) && !spans_meet(o, cache) && !spans_meet(o, block_table) &&
+                       !spans_meet(o, seq_lens) && !(query_start_loc && spans_meet(o, *query_start_loc)) &&
+                       !(sink && spans_meet(o, *sink)),
+                   "out must not overlap an input");
+    }
+    FGV_ASSERT(dev.is_cuda(), "flaggems_vllm runs on the GPU (HIP) only");
+    const c10::DeviceGuard guard(dev);
+    const at::Tensor out = out_in ? *out_in : new_on(dev, {tokens, heads, dim}, q.scalar_type());
+    const at::Tensor lse = new_on(dev, {tokens, heads}, at::kFloat);
+    *result = TensorPair(out, lse);
+    const int64_t most_q = max_query_len ? *max_query_len : query_start_loc ? tokens : 1;
+    const int64_t most_s = max_seq_len ? *max_seq_len : block_table.size(1) * page;
+    // from torch's caching allocator, in the order of the current stream
+    const int64_t ws_bytes =
+        fgv_mxfp4_paged_attention_workspace_bytes(tokens, heads, kv_heads, dim, reqs, most_q, most_s);
+    const at::Tensor ws = ws_bytes > 0 ? new_on(dev, {ws_bytes}, at::kByte) : at::Tensor();
+    return fgv_mxfp4_paged_attention(
+        q.data_ptr(), q.stride(0), q.stride(1), q.scalar_type() == at::kHalf ? 1 : 0, tokens, heads, kv_heads, dim,
+        cache.data_ptr<uint8_t>(), cache.stride(0), cache.size(0), page, i32_ptr(block_table), block_table.stride(0),
+        block_table.size(1), i32_ptr(seq_lens), query_start_loc ? i32_ptr(*query_start_loc) : nullptr, reqs, most_q,
+        most_s, scale, window ? *window : 0, sink ? sink->data_ptr<float>() : nullptr, out.data_ptr(), out.stride(0),
+        out.stride(1), lse.data_ptr<float>(), lse.stride(0), ws.defined() ? ws.data_ptr() : nullptr, ws_bytes,
+        current_stream(q));
+}
+
 // ---- dispatcher ops: the same functions, failures raised as RuntimeError ----
 
 void raise_on_status(int rc, const char* op) {
@@ -661,7 +824,8 @@ TORCH_LIBRARY_IMPL(flaggems_vllm, CUDA, m) {
 
 PYBIND11_MODULE(_fgv_torch, m) {
     m.doc() = "C++ checks and launches of fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert, "
-              "fused_inv_rope_fp8_quant, the five ops beside them and the 8-bit linear ops (status-returning; the "
+              "fused_inv_rope_fp8_quant, the five ops beside them, the 8-bit linear ops and those of the 4-bit "
+              "paged cache (status-returning; the "
               "Python wrappers map the status)";
     m.attr("ASSERT_FAILED") = kAssertFailed;
     m.def("qnorm_rope_kv_insert", &qnorm_rope_kv_insert);
@@ -712,5 +876,25 @@ PYBIND11_MODULE(_fgv_torch, m) {
         const int rc = int8_mm(a, b, scale_a, scale_b, bias, out_dtype, out_in, &out);
         return std::make_tuple(rc, out);
     });
+    m.def("build_block_tables",
+          [](const at::Tensor& context_lens, const at::Tensor& query_lens, const at::Tensor& block_table,
+             const at::Tensor& free_blocks, const at::Tensor& num_free, int64_t block_size, int64_t max_num_tokens,
+             int64_t pad_id) {
+              TablesOut out;
+              const int rc = build_block_tables(context_lens, query_lens, block_table, free_blocks, num_free,
+                                                block_size, max_num_tokens, pad_id, &out);
+              return std::make_tuple(rc, out);
+          });
+    m.def("mxfp4_insert", &mxfp4_insert);
+    m.def("mxfp4_attention",
+          [](const at::Tensor& q, const at::Tensor& cache, const at::Tensor& block_table, const at::Tensor& seq_lens,
+             double scale, const std::optional<at::Tensor>& query_start_loc, std::optional<int64_t> max_query_len,
+             std::optional<int64_t> max_seq_len, std::optional<int64_t> window, const std::optional<at::Tensor>& sink,
+             const std::optional<at::Tensor>& out_in) {
+              TensorPair out;
+              const int rc = mxfp4_attention(q, cache, block_table, seq_lens, scale, query_start_loc, max_query_len,
+                                             max_seq_len, window, sink, out_in, &out);
+              return std::make_tuple(rc, std::get<0>(out), std::get<1>(out));
+          });
     m.def("assert_message", []() { return g_assert_message; });
 }

@@ -9,8 +9,9 @@ K-cache gather, q/kv RMSNorm, the sparse indexer (q quant, key cache and
 logits and their top-k per row), the index rows sparse attention reads (global
 top-k indices, top-k plus sliding window), slot mapping, sparse MLA decode, sparse MLA prefill
 (``flash_mla_sparse_fwd``) and the block-FP8 grouped output projection (``fp8_einsum``) after the sibling op.  The 8-bit linear ops around the layer (``fused_add_rms_norm_quant``,
-``fused_silu_mul_quant``, ``int8_scaled_mm``) have no counterpart in the reference package's
-exports used here.  Every op runs hand-written HIP kernels through the C ABI declared in
+``fused_silu_mul_quant``, ``int8_scaled_mm``) and serving from a 4-bit paged cache
+(``build_block_tables``, ``mxfp4_kv_quant_and_cache``, ``mxfp4_paged_attention``) have no
+counterpart in the reference package's exports used here.  Every op runs hand-written HIP kernels through the C ABI declared in
 include/flaggems_vllm_amd.h; there is no Triton, no vendor dispatch and no
 CPU fallback.
 """
@@ -18,6 +19,7 @@ from . import ops  # noqa: F401
 from .ops import (  # noqa: F401
     SUPPORTED_FP8_DTYPE,
     FlashMLASchedMeta,
+    build_block_tables,
     combine_topk_swa_indices,
     compute_global_topk_indices_and_lens,
     compute_slot_mapping_parallel,
@@ -37,6 +39,8 @@ from .ops import (  # noqa: F401
     get_mla_metadata,
     indexer_k_quant_and_cache,
     int8_scaled_mm,
+    mxfp4_kv_quant_and_cache,
+    mxfp4_paged_attention,
     persistent_topk,
     top_k_per_row_decode,
     top_k_per_row_prefill,
@@ -53,6 +57,7 @@ ops_inv_rope_fp8_quant = fused_inv_rope_fp8_quant
 
 __all__ = [
     "FlashMLASchedMeta",
+    "build_block_tables",
     "combine_topk_swa_indices",
     "compute_global_topk_indices_and_lens",
     "compute_slot_mapping_parallel",
@@ -75,6 +80,8 @@ __all__ = [
     "ops_deepseek_v4_qnorm_rope_kv_rope_quant_insert",
     "ops_inv_rope_fp8_quant",
     "SUPPORTED_FP8_DTYPE",
+    "mxfp4_kv_quant_and_cache",
+    "mxfp4_paged_attention",
     "persistent_topk",
     "top_k_per_row_decode",
     "top_k_per_row_prefill",

@@ -331,6 +331,35 @@ def lib():
     ]
     L.fgv_int8_scaled_mm_workspace_bytes.restype = ctypes.c_int64
     L.fgv_int8_scaled_mm_workspace_bytes.argtypes = [_P, _I64, _P, _I64, _I64, _I64, _I64]
+    L.fgv_build_block_tables.restype = ctypes.c_int
+    L.fgv_build_block_tables.argtypes = [
+        _P, _P, _I64,  # context_lens, query_lens, num_reqs
+        _P, _I64, _I64,  # block_table, stride, max_blocks_per_req
+        _P, _I64, _P,  # free_blocks, size, num_free
+        _I64, _I64, _I64,  # block_size, max_num_tokens, pad_id
+        _P, _P, _P, _P, _P,  # query_start_loc, seq_lens, positions, slot_mapping, num_free_out
+        _P,  # stream
+    ]
+    L.fgv_mxfp4_kv_quant_and_cache.restype = ctypes.c_int
+    L.fgv_mxfp4_kv_quant_and_cache.argtypes = [
+        _P, _I64, _I64, _P, _I64, _I64,  # k, strides (token, head), v, strides
+        ctypes.c_int32, _I64, _I64, _I64,  # dtype, num_tokens, num_kv_heads, head_dim
+        _P, _I64, _I64, _I64,  # kv_cache, block stride, num_blocks, block_size
+        _P, _P,  # slot_mapping, stream
+    ]
+    L.fgv_mxfp4_paged_attention.restype = ctypes.c_int
+    L.fgv_mxfp4_paged_attention.argtypes = [
+        _P, _I64, _I64, ctypes.c_int32,  # q, strides (token, head), dtype
+        _I64, _I64, _I64, _I64,  # num_tokens, num_heads, num_kv_heads, head_dim
+        _P, _I64, _I64, _I64,  # kv_cache, block stride, num_blocks, block_size
+        _P, _I64, _I64,  # block_table, stride, max_blocks_per_req
+        _P, _P, _I64,  # seq_lens, query_start_loc, num_reqs
+        _I64, _I64, ctypes.c_double, _I64, _P,  # max_query_len, max_seq_len, softmax_scale, window_size, attn_sink
+        _P, _I64, _I64, _P, _I64,  # out, strides, lse, token stride
+        _P, _I64, _P,  # workspace, workspace_bytes, stream
+    ]
+    L.fgv_mxfp4_paged_attention_workspace_bytes.restype = ctypes.c_int64
+    L.fgv_mxfp4_paged_attention_workspace_bytes.argtypes = [_I64] * 7
     _lib = L
     return _lib
 
@@ -377,4 +406,8 @@ EXPORTED_SYMBOLS = (
     "fgv_silu_mul_quant",
     "fgv_int8_scaled_mm",
     "fgv_int8_scaled_mm_workspace_bytes",
+    "fgv_build_block_tables",
+    "fgv_mxfp4_kv_quant_and_cache",
+    "fgv_mxfp4_paged_attention",
+    "fgv_mxfp4_paged_attention_workspace_bytes",
 )

@@ -9,7 +9,9 @@ for the gather, ``slot_mapping`` for the slot mapping, ``kv_cache`` for the
 indexer key insert and ``k_fp8`` / ``k_fp8_scale`` for its gather, ``indices`` for the top-k per row
 (``output`` and, for rows long enough to split, ``workspace`` for ``persistent_topk``),
 ``out`` for ``fp8_einsum_out`` (the index-row ops, ``fp8_einsum``, ``flash_mla_sparse_fwd`` and the 8-bit linear ops write only what they return, but for
-``int8_scaled_mm_out``'s ``out``).  The fake (meta)
+``int8_scaled_mm_out``'s ``out``; of those of the 4-bit paged cache
+``build_block_tables`` writes ``block_table``, the insert ``kv_cache`` and
+``mxfp4_paged_attention_out`` ``out``, returning the lse).  The fake (meta)
 implementations give the output shapes and strides the real ops return.
 The main op and the sibling are C++ ops (the torch extension's
 ``torch_ops.cpp``, loaded here): the same checks and launch the Python
@@ -30,6 +32,7 @@ import torch
 
 from . import _native
 from .ops import (
+    build_block_tables,
     combine_topk_swa_indices,
     compute_global_topk_indices_and_lens,
     compute_slot_mapping_parallel,
@@ -43,6 +46,8 @@ from .ops import (
     fused_silu_mul_quant,
     indexer_k_quant_and_cache,
     int8_scaled_mm,
+    mxfp4_kv_quant_and_cache,
+    mxfp4_paged_attention,
     persistent_topk,
     top_k_per_row_decode,
     top_k_per_row_prefill,
@@ -318,6 +323,68 @@ def _(a, b, scale_a, scale_b, bias, out):
     return None
 
 
+@_op("build_block_tables", ("block_table",))
+def _build_block_tables(
+        context_lens: torch.Tensor, query_lens: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
+        num_free: torch.Tensor, block_size: int, max_num_tokens: int, pad_id: int = -1
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return build_block_tables(context_lens, query_lens, block_table, free_blocks, num_free, block_size,
+                              max_num_tokens, pad_id)
+
+
+@_build_block_tables.register_fake
+def _(context_lens, query_lens, block_table, free_blocks, num_free, block_size, max_num_tokens, pad_id=-1):
+    n = context_lens.shape[0]
+    i64 = [context_lens.new_empty((max_num_tokens,), dtype=torch.int64) for _ in range(2)]
+    return (context_lens.new_empty((n + 1,), dtype=torch.int32), context_lens.new_empty((n,), dtype=torch.int32),
+            i64[0], i64[1], context_lens.new_empty((1,), dtype=torch.int32))
+
+
+@_op("mxfp4_kv_quant_and_cache", ("kv_cache",))
+def _mxfp4_kv_quant_and_cache(k: torch.Tensor, v: torch.Tensor, kv_cache: torch.Tensor,
+                              slot_mapping: torch.Tensor) -> None:
+    mxfp4_kv_quant_and_cache(k, v, kv_cache, slot_mapping)
+
+
+@_mxfp4_kv_quant_and_cache.register_fake
+def _(k, v, kv_cache, slot_mapping):
+    return None
+
+
+@_op("mxfp4_paged_attention")
+def _mxfp4_paged_attention(
+        q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+        softmax_scale: float, query_start_loc: Optional[torch.Tensor] = None, max_query_len: Optional[int] = None,
+        max_seq_len: Optional[int] = None, window_size: Optional[int] = None,
+        attn_sink: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    return mxfp4_paged_attention(q, kv_cache, block_table, seq_lens, softmax_scale, query_start_loc=query_start_loc,
+                                 max_query_len=max_query_len, max_seq_len=max_seq_len, window_size=window_size,
+                                 attn_sink=attn_sink)
+
+
+@_mxfp4_paged_attention.register_fake
+def _(q, kv_cache, block_table, seq_lens, softmax_scale, query_start_loc=None, max_query_len=None, max_seq_len=None,
+      window_size=None, attn_sink=None):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+@_op("mxfp4_paged_attention_out", ("out",))
+def _mxfp4_paged_attention_out(
+        q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+        softmax_scale: float, out: torch.Tensor, query_start_loc: Optional[torch.Tensor] = None,
+        max_query_len: Optional[int] = None, max_seq_len: Optional[int] = None, window_size: Optional[int] = None,
+        attn_sink: Optional[torch.Tensor] = None) -> torch.Tensor:
+    return mxfp4_paged_attention(q, kv_cache, block_table, seq_lens, softmax_scale, query_start_loc=query_start_loc,
+                                 max_query_len=max_query_len, max_seq_len=max_seq_len, window_size=window_size,
+                                 attn_sink=attn_sink, out=out)[1]
+
+
+@_mxfp4_paged_attention_out.register_fake
+def _(q, kv_cache, block_table, seq_lens, softmax_scale, out, query_start_loc=None, max_query_len=None,
+      max_seq_len=None, window_size=None, attn_sink=None):
+    return q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
 REGISTERED: List[str] = [
     "fused_deepseek_v4_qnorm_rope_kv_rope_quant_insert",
     "fused_inv_rope_fp8_quant",
@@ -343,4 +410,12 @@ REGISTERED_LINEAR: List[str] = [
     "fused_silu_mul_quant",
     "int8_scaled_mm",
     "int8_scaled_mm_out",
+]
+
+# serving from a 4-bit paged cache, without a counterpart either
+REGISTERED_PAGED: List[str] = [
+    "build_block_tables",
+    "mxfp4_kv_quant_and_cache",
+    "mxfp4_paged_attention",
+    "mxfp4_paged_attention_out",
 ]

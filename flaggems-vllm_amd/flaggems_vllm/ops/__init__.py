@@ -1,5 +1,5 @@
 """DeepSeek-V4 attention pre-processing ops (reference: src/flaggems_vllm/ops/__init__.py:23-38, 55, 56, 57, 58-65, 78, 122, 142-143, 187, 229),
-and the 8-bit linear ops around the layer (``int8_linear``)."""
+the 8-bit linear ops around the layer (``int8_linear``) and serving from a 4-bit paged cache (``mxfp4_paged``)."""
 from .cp_gather_indexer_k_quant_cache import cp_gather_indexer_k_quant_cache
 from .deepseek_v4_attention_combine_topk_swa_indices import combine_topk_swa_indices
 from .deepseek_v4_attention_compute_global_topk_indices_and_lens import compute_global_topk_indices_and_lens
@@ -17,12 +17,14 @@ from .fused_indexer_q_rope_quant import fused_indexer_q_rope_quant
 from .fused_inv_rope_fp8_quant import SUPPORTED_FP8_DTYPE, fused_inv_rope_fp8_quant
 from .int8_linear import fused_add_rms_norm_quant, fused_silu_mul_quant, int8_scaled_mm
 from .indexer_k_quant_and_cache import indexer_k_quant_and_cache
+from .mxfp4_paged import build_block_tables, mxfp4_kv_quant_and_cache, mxfp4_paged_attention
 from .persistent_topk import persistent_topk
 from .slot_mapping import compute_slot_mapping_parallel
 from .top_k_per_row import top_k_per_row_decode, top_k_per_row_prefill
 
 __all__ = [
     "FlashMLASchedMeta",
+    "build_block_tables",
     "combine_topk_swa_indices",
     "compute_global_topk_indices_and_lens",
     "compute_slot_mapping_parallel",
@@ -43,6 +45,8 @@ __all__ = [
     "fused_inv_rope_fp8_quant",
     "indexer_k_quant_and_cache",
     "SUPPORTED_FP8_DTYPE",
+    "mxfp4_kv_quant_and_cache",
+    "mxfp4_paged_attention",
     "persistent_topk",
     "top_k_per_row_decode",
     "top_k_per_row_prefill",

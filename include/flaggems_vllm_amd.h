@@ -714,6 +714,94 @@ int fgv_int8_scaled_mm(const int8_t* a, int64_t a_stride, const int8_t* b, int64
 int64_t fgv_int8_scaled_mm_workspace_bytes(const int8_t* a, int64_t a_stride, const int8_t* b, int64_t b_stride,
                                            int64_t m, int64_t n, int64_t k);
 
+/*
+ * A step's request lengths turned into what the paged-cache ops read.  Request b
+ * (of num_reqs) brings query_lens[b] new tokens behind its context_lens[b] cached
+ * ones (negative lengths count as 0); tokens past max_num_tokens, counted over
+ * the requests in order, are dropped.  With page = block_size and
+ * W = max_blocks_per_req, q_b the tokens that are kept:
+ *   query_start_loc [num_reqs + 1] int32: running sum of q_b;
+ *   seq_lens [num_reqs] int32: context_lens[b] + q_b;
+ *   block_table [num_reqs, W] int32 (rows block_table_stride apart): columns
+ *       ceil(context / page) .. ceil(seq_len / page) - 1, as far as they are below
+ *       W, get blocks from the top of the stack free_blocks[0 .. num_free), in the
+ *       order of requests and columns (free_blocks[num_free - 1] first), and -1
+ *       once it is empty; other columns are left as they are;
+ *   positions [max_num_tokens] int64: context + i of token i of a request;
+ *   slot_mapping [max_num_tokens] int64: block * page + position % page, block out
+ *       of the table; pad_id where that is negative or the column is not below W;
+ *   positions and slot_mapping behind the last token: 0 and pad_id;
+ *   num_free_out [1] int32: num_free (within 0 and free_blocks_size) less the
+ *       blocks that were wanted; negative: so many were missing.
+ * One launch; outputs must not overlap inputs or one another.
+ */
+int fgv_build_block_tables(const int32_t* context_lens, const int32_t* query_lens, int64_t num_reqs,
+                           int32_t* block_table, int64_t block_table_stride, int64_t max_blocks_per_req,
+                           const int32_t* free_blocks, int64_t free_blocks_size, const int32_t* num_free,
+                           int64_t block_size, int64_t max_num_tokens, int64_t pad_id, int32_t* query_start_loc,
+                           int32_t* seq_lens, int64_t* positions, int64_t* slot_mapping, int32_t* num_free_out,
+                           void* stream);
+
+/*
+ * Keys and values quantised to MXFP4 and written into a paged cache.
+ *
+ * The cache: block b at kv_cache + b * cache_block_stride bytes (a multiple of 16);
+ * in it, for each of num_kv_heads heads, with page = block_size tokens (a multiple
+ * of 16, at most 4096) and D = head_dim (64, 128 or 256):
+ *   page x D/2 bytes key codes, page x D/2 bytes value codes (E2M1, even dim in the
+ *   low nibble), page x D/32 bytes key scales, page x D/32 bytes value scales
+ *   (UE8M0, one per 32 dims: the values are code * 2^(byte - 127)).
+ * Per 32 values x, a = max |x|: byte = 127 + clamp(ceil(log2(a / 6)), -126, 125), codes
+ * the nearest to x / 2^(byte - 127), ties to the even code, at most 6 in magnitude; a
+ * block that holds a NaN or an infinity gets byte 255 (NaN) and codes 0.
+ *
+ *   k, v  [num_tokens, num_kv_heads, D] bf16 (dtype 0) or fp16 (1), unit last
+ *         stride, any other strides (in elements).
+ *   slot_mapping  int64 [num_tokens]: token t goes to block slot / page, place
+ *         slot % page; slots < 0 and slots of blocks >= num_blocks are skipped.
+ *         Two tokens of one call must not have the same slot.
+ */
+int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t k_stride_head, const void* v,
+                                 int64_t v_stride_token, int64_t v_stride_head, int32_t dtype, int64_t num_tokens,
+                                 int64_t num_kv_heads, int64_t head_dim, uint8_t* kv_cache, int64_t cache_block_stride,
+                                 int64_t num_blocks, int64_t block_size, const int64_t* slot_mapping, void* stream);
+
+/*
+ * Causal attention of grouped heads over that cache.  Request b's query tokens are
+ * q[query_start_loc[b] .. query_start_loc[b + 1]), the last of its seq_lens[b]
+ * tokens (query_start_loc NULL: one token per request, num_tokens = num_reqs);
+ * token at position p sees the keys j, p - window_size < j <= p (window_size 0: all
+ * j <= p), j < max_blocks_per_req * block_size, whose block in block_table lies
+ * in [0, num_blocks).  Head h reads key/value head h / (num_heads / num_kv_heads):
+ *   lse = ln sum_j exp(softmax_scale q . k_j)
+ *   out = sum_j exp(softmax_scale q . k_j) v_j / (exp(lse) + exp(attn_sink[h]))
+ * (attn_sink NULL: none; it does not enter lse).  A row that sees nothing gets out 0
+ * and lse +inf.  A row that sees a key or value block of byte 255, or whose
+ * query holds a NaN or an infinity and that sees a key, gets NaN.  Rows of q
+ * outside query_start_loc's ranges are not written.
+ *
+ *   q, out  [num_tokens, num_heads, D] bf16 (dtype 0) or fp16 (1), unit last
+ *         stride; lse [num_tokens, num_heads] float32, unit last stride.
+ *   max_query_len, max_seq_len  the most query tokens and keys of a request, as
+ *         far as the caller knows; they choose how the work is cut, not what is
+ *         computed, and numbers that are too small cost time only.
+ *   workspace: 16-byte aligned device memory of workspace_bytes; without as many
+ *         as fgv_mxfp4_paged_attention_workspace_bytes says for these sizes, no
+ *         keys are split over workgroups.  Calls that share one must be ordered.
+ */
+int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, int64_t q_stride_head, int32_t dtype,
+                              int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+                              const uint8_t* kv_cache, int64_t cache_block_stride, int64_t num_blocks,
+                              int64_t block_size, const int32_t* block_table, int64_t block_table_stride,
+                              int64_t max_blocks_per_req, const int32_t* seq_lens, const int32_t* query_start_loc,
+                              int64_t num_reqs, int64_t max_query_len, int64_t max_seq_len, double softmax_scale,
+                              int64_t window_size, const float* attn_sink, void* out, int64_t out_stride_token,
+                              int64_t out_stride_head, float* lse, int64_t lse_stride_token, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+int64_t fgv_mxfp4_paged_attention_workspace_bytes(int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads,
+                                                  int64_t head_dim, int64_t num_reqs, int64_t max_query_len,
+                                                  int64_t max_seq_len);
+
 #ifdef __cplusplus
 }
 #endif
