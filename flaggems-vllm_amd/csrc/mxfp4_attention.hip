@@ -22,7 +22,7 @@
 // operand in e4m3, exactly: divided by a power of two per row that puts the
 // row's maximum into [128, 256), its 8 (bf16) or 11 (fp16) bits split into 2
 // or 3 e4m3 pieces of 4, each under a scale 2^-4 smaller.  What values far
-// below their row's maximum lose is under 2^-20 of that maximum.  Register
+// below their row's maximum lose is under 2^-16 (2^-20) of that maximum.  Register
 // images (measured; the tests pin them through the results): lane (r, g) =
 // (l % 16, l / 16) holds of A k = 32g..32g+31 of key r, of B k = 16g..16g+15
 // and 64+16g..64+16g+15 of row r; scales apply to k = 32g..32g+31; D holds
@@ -30,8 +30,8 @@
 //
 // PV: v_cvt_scalef32_pk_bf16_fp4 gives V in bf16 exactly (codes have two
 // bits), token by token; LDS turns it, written by tokens and read by
-// ds_read_b64_tr_b16.  P goes in as bf16, in fp16 calls as two bf16 pieces
-// (16 bits).  A value block under byte 255 (NaN) makes the outputs of those
+// ds_read_b64_tr_b16.  P goes in as two bf16 pieces (16 bits): one alone would
+// put its own 2^-9 beside the output's.  A value block under byte 255 (NaN) makes the outputs of those
 // rows NaN that see it.
 #include <math.h>
 
@@ -53,6 +53,9 @@ constexpr int kAttThreads = 256;
 constexpr int kAttWaves = kAttThreads / 64;
 constexpr int kTileKeys = 64;  // keys a wave takes at a time: four 16-key subtiles
 constexpr int kRows = 16;      // query rows of a workgroup
+constexpr int kChunkStep = kAttWaves * kTileKeys;  // keys are cut between workgroups in steps of a turn of the waves
+constexpr int kMostCuts = 1100;                    // of one tile: more than split_items + 1 ever is
+constexpr int kSplitTurns = 2;                     // workgroups a CU holds at a time
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // The running maximum is raised only when a score exceeds it by more than this
@@ -77,6 +80,17 @@ struct AttArgs {
     int32_t scale_e;
     int32_t num_reqs, num_tokens, kv_heads, group, page, table_keys, window;
     int32_t q_wide, o_wide;
+    // split mode (split_items > 0): about how many workgroups per head to cut the keys
+    // into, slots of partial results per head, and their places in the workspace
+    int32_t split_items, slots_per_head;
+    float* partials;
+    struct SplitTile* split_tiles;
+    int32_t* num_split_tiles;
+};
+
+// A row tile whose keys are cut: `count` slots of each head from `slot` on.
+struct SplitTile {
+    int32_t first_token, first_row, rows, slot, count;
 };
 
 // A request's query tokens [first, first + count) and lengths.
@@ -99,57 +113,132 @@ __device__ __forceinline__ Request request_of(const AttArgs& a, int32_t b) {
     return r;
 }
 
-// One workgroup's work: the row tile `tile` of request b.
+// Keys that a request's tokens see, from the first tile boundary on.
+__device__ __forceinline__ void key_range(const AttArgs& a, const Request& r, int32_t& begin, int32_t& end) {
+    end = min(r.len, a.table_keys);
+    begin = a.window > 0 ? max(r.len - r.count - a.window + 1, 0) & ~(kTileKeys - 1) : 0;
+}
+
+// One workgroup's work: row tile `tile` of request b, the keys of cut `cut` of
+// `cuts` that are `chunk` keys each.
 struct Item {
     Request req;
-    int32_t b, tile;
+    int32_t b, tile, cut, cuts, chunk;
+    int32_t slot;   // cuts > 1: the first of the tile's slots
+    int32_t order;  // and its number among the cut tiles
 };
 
-// The row tile number `index`, counted over the requests in order; false
-// behind the last.
-__device__ __forceinline__ bool find_item(const AttArgs& a, int32_t index, Item& item) {
-    __shared__ int32_t part[kAttWaves];
-    __shared__ int32_t found[2];
+// Sum of v over the lanes up to this one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
+// The item number `index`, counted over requests, tiles and cuts in order; false
+// behind the last.  Each workgroup works out the plan for itself: lengths are
+// known on the device only, and a launch to do it would cost more.  With
+// split_items > 0 the keys of all row tiles, together `total`, are cut into
+// chunks of total / split_items keys (in steps of kChunkStep), so that
+// workgroups have about the same to do whatever the lengths are; at most twice
+// as many cuts as split_items come from tiles that are cut at all.
+__device__ __forceinline__ bool find_item(const AttArgs& a, int32_t index, int32_t rows_per_tile, Item& item) {
+    __shared__ float part_keys[kAttWaves];
+    __shared__ uint32_t part[3][kAttWaves];
+    __shared__ int32_t found[6];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool split = a.split_items > 0;
     if (threadIdx.x == 0)
         found[0] = -1;
-    int32_t before = 0;
+    int32_t chunk = 0x7fffffff;
+    auto tiles_of = [&](const Request& r) {
+        return (int32_t)(((int64_t)r.count * a.group + rows_per_tile - 1) / rows_per_tile);
+    };
+    if (split) {
+        float keys = 0.f;
+        for (int32_t b = (int32_t)threadIdx.x; b < a.num_reqs; b += kAttThreads) {
+            const Request r = request_of(a, b);
+            int32_t begin, end;
+            key_range(a, r, begin, end);
+            keys += (float)tiles_of(r) * (float)max(end - begin, 0);
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1)
+            keys += __shfl_xor(keys, d);
+        if (lane == 0)
+            part_keys[wave] = keys;
+        __syncthreads();
+        keys = 0.f;
+#pragma unroll
+        for (int w = 0; w < kAttWaves; ++w)
+            keys += part_keys[w];
+        const float each = keys / (float)a.split_items;
+        chunk = each < 1e9f ? ((int32_t)each / kChunkStep + 1) * kChunkStep : 0x7fffffff;
+    }
+    uint32_t before[3] = {0, 0, 0};  // items, slots, cut tiles of the requests in front
     for (int32_t base = 0; base < a.num_reqs; base += kAttThreads) {
         const int32_t b = base + (int32_t)threadIdx.x;
-        int32_t tiles = 0;
+        uint32_t n[3] = {0, 0, 0};
+        int32_t tiles = 0, cuts = 1;
         if (b < a.num_reqs) {
             const Request r = request_of(a, b);
-            tiles = (int32_t)(((int64_t)r.count * a.group + kRows - 1) / kRows);
+            tiles = tiles_of(r);
+            if (split) {
+                int32_t begin, end;
+                key_range(a, r, begin, end);
+                cuts = max((int32_t)(((int64_t)(end - begin) + chunk - 1) / chunk), 1);
+            }
+            n[0] = (uint32_t)tiles * cuts;
+            n[1] = cuts > 1 ? n[0] : 0;
+            n[2] = cuts > 1 ? tiles : 0;
         }
-        int32_t s = tiles;
+        uint32_t at[3];
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int32_t o = __shfl_up(s, d);
-            if (lane >= d)
-                s += o;
+        for (int i = 0; i < 3; ++i) {
+            const uint32_t s = wave_scan(n[i]);
+            if (lane == 63)
+                part[i][wave] = s;
+            at[i] = before[i] + s - n[i];
         }
-        if (lane == 63)
-            part[wave] = s;
         __syncthreads();
-        int32_t at = before + s - tiles;
 #pragma unroll
-        for (int w = 0; w < kAttWaves; ++w) {
-            at += w < wave ? part[w] : 0;
-            before += part[w];
-        }
-        if (index >= at && index < at + tiles) {
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int w = 0; w < kAttWaves; ++w) {
+                at[i] += w < wave ? part[i][w] : 0;
+                before[i] += part[i][w];
+            }
+        const uint32_t mine = (uint32_t)index - at[0];
+        if ((uint32_t)index >= at[0] && mine < n[0]) {
+            const int32_t tile = (int32_t)(mine / cuts);
             found[0] = b;
-            found[1] = index - at;
+            found[1] = tile;
+            found[2] = (int32_t)mine - tile * cuts;
+            found[3] = cuts;
+            found[4] = (int32_t)at[1] + tile * cuts;
+            found[5] = (int32_t)at[2] + tile;
         }
         __syncthreads();
-        if (before > index)
+        // the first workgroup sees all requests, for the number of cut tiles
+        if (before[0] > (uint32_t)index && !(split && blockIdx.x == 0))
             break;
     }
     __syncthreads();
+    if (split && blockIdx.x == 0 && threadIdx.x == 0)
+        *a.num_split_tiles = (int32_t)before[2];
     item.b = __builtin_amdgcn_readfirstlane(found[0]);
     if (item.b < 0)
         return false;
     item.tile = __builtin_amdgcn_readfirstlane(found[1]);
+    item.cut = __builtin_amdgcn_readfirstlane(found[2]);
+    item.cuts = __builtin_amdgcn_readfirstlane(found[3]);
+    item.slot = __builtin_amdgcn_readfirstlane(found[4]);
+    item.order = __builtin_amdgcn_readfirstlane(found[5]);
+    item.chunk = chunk;
     item.req = request_of(a, item.b);
     return true;
 }
@@ -207,9 +296,21 @@ __device__ __forceinline__ void load_values(const void* base, int64_t at, bool w
     }
 }
 
-// Four floats of magnitude below 448 to e4m3 codes; x keeps 16 times what they leave.
+// Four floats of magnitude below 448 to e4m3 codes; x keeps 16 times what they
+// leave.  The first piece takes whole multiples of 1/8 only: the instruction
+// cuts a product's bits below 2^-13 of the largest one that is added with it,
+// and so those of small values, which the pieces behind then hold as well
+// (scores of normal queries, error rms: 1.3e-5 without, 4.8e-6 with it in two
+// pieces, 3.4e-7 in three; multiples of 1/4 and 1/16 lie between).
+template <bool kFirst>
 __device__ __forceinline__ uint32_t take_piece(float* x) {
-    const uint32_t w = pack_fp8x4(x[0], x[1], x[2], x[3]);
+    constexpr float kWhole = 1.5f * (float)(1 << 20);  // adding it and taking it away rounds to multiples of 1/8
+    uint32_t w;
+    if constexpr (kFirst)
+        w = pack_fp8x4((x[0] + kWhole) - kWhole, (x[1] + kWhole) - kWhole, (x[2] + kWhole) - kWhole,
+                       (x[3] + kWhole) - kWhole);
+    else
+        w = pack_fp8x4(x[0], x[1], x[2], x[3]);
     x[0] = (x[0] - __builtin_amdgcn_cvt_f32_fp8((int)w, 0)) * 16.0f;
     x[1] = (x[1] - __builtin_amdgcn_cvt_f32_fp8((int)w, 1)) * 16.0f;
     x[2] = (x[2] - __builtin_amdgcn_cvt_f32_fp8((int)w, 2)) * 16.0f;
@@ -251,7 +352,7 @@ __device__ __forceinline__ void load_query(const AttArgs& a, int64_t at, bool va
             for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    out.q[s][4 * half + i] = 2 * s + half < kPieces ? (int)take_piece(&x[0][4 * i]) : 0;
+                    out.q[s][4 * half + i] = 2 * s + half < kPieces ? (int)(s + half == 0 ? take_piece<true>(&x[0][4 * i]) : take_piece<false>(&x[0][4 * i])) : 0;
             out.scale[s] = bad ? 255 : byte - 4 * (2 * s + (g >> 1));
         }
     } else {
@@ -263,31 +364,33 @@ __device__ __forceinline__ void load_query(const AttArgs& a, int64_t at, bool va
                 for (int half = 0; half < 2; ++half)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        out.q[p * Shape<D, kPieces>::kChunks + c][4 * half + i] = (int)take_piece(&x[2 * c + half][4 * i]);
+                        out.q[p * Shape<D, kPieces>::kChunks + c][4 * half + i] = (int)(p == 0 ? take_piece<true>(&x[2 * c + half][4 * i]) : take_piece<false>(&x[2 * c + half][4 * i]));
                 out.scale[p * Shape<D, kPieces>::kChunks + c] = bad ? 255 : byte - 4 * p;
             }
     }
 }
 
-// A wave's 64 keys as they stand in the cache: lane (r, g) has dims 32g..32g+31
-// of each chunk of token 16t + r.
-template <int kChunks>
+// A wave's keys as they stand in the cache, kSub subtiles of 16: lane (r, g) has
+// dims 32g..32g+31 of each chunk of token 16t + r.
+template <int kSub, int kChunks>
 struct RawTile {
-    uint4 k[4][kChunks], v[4][kChunks];
-    uint32_t ks[4][kChunks], vs[4][kChunks];
+    uint4 k[kSub][kChunks], v[kSub][kChunks];
+    uint32_t ks[kSub][kChunks], vs[kSub][kChunks];
+    int32_t place[kSub];  // of its first token in the block, negative: there is none
 };
 
-// Where a wave's next 16 tiles lie: lane 4i + t has subtile t of the i-th of
-// them, the head's block at `base` and the first of its tokens at `place`
+// Where a wave's next 64 subtiles lie: lane kSub i + t has subtile t of the i-th
+// tile, the head's block at `base` and the first of its tokens at `place`
 // (negative: no block).  Tiles of a wave are `stride` keys apart.
 struct Places {
     int64_t base;
     int32_t place;
 };
 
+template <int kSub>
 __device__ __forceinline__ Places find_places(const AttArgs& a, int32_t b, int32_t h, int32_t token_bytes, int32_t key0,
                                               int32_t stride, int32_t end, int lane) {
-    const int64_t key = (int64_t)key0 + (int64_t)(lane >> 2) * stride + 16 * (lane & 3);
+    const int64_t key = (int64_t)key0 + (int64_t)(lane / kSub) * stride + 16 * (lane % kSub);
     Places p = {0, -1};
     if (key < end) {
         const int32_t column = (int32_t)key / a.page;
@@ -300,19 +403,19 @@ __device__ __forceinline__ Places find_places(const AttArgs& a, int32_t b, int32
     return p;
 }
 
-template <int D>
+template <int D, int kSub>
 __device__ __forceinline__ void load_tile(const AttArgs& a, const Places& p, int tile, int lane,
-                                          RawTile<D < 128 ? 1 : D / 128>& raw, int32_t (&place)[4]) {
+                                          RawTile<kSub, D < 128 ? 1 : D / 128>& raw) {
     constexpr int kChunks = D < 128 ? 1 : D / 128;
     const int r = lane & 15, g = D < 128 ? (lane >> 4) & 1 : lane >> 4;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int from = (tile & 15) * 4 + t;
+    for (int t = 0; t < kSub; ++t) {
+        const int from = tile % (64 / kSub) * kSub + t;
         const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)p.base, from);
         const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)p.base >> 32), from);
-        place[t] = __builtin_amdgcn_readlane(p.place, from);
+        raw.place[t] = __builtin_amdgcn_readlane(p.place, from);
         // a subtile without a block reads the cache's first one, whose values nobody sees
-        const int32_t first = max(place[t], 0);
+        const int32_t first = max(raw.place[t], 0);
         const uint8_t* head = a.cache + (int64_t)((uint64_t)hi << 32 | lo);
         const uint8_t* kc = head + (int64_t)first * (D / 2);
         const uint8_t* vc = kc + mx_part(1, a.page, D);
@@ -353,18 +456,18 @@ struct Seen {
     __device__ bool operator()(int32_t key) const { return key > lo && key <= pos; }
 };
 
-// Attends the 64 keys from key0 on for the wave's 16 rows.  kMask: some of
-// them are hidden from some of the rows.
-template <int D, int kPieces, bool kMask>
-__device__ __forceinline__ void attend(const RawTile<Shape<D, kPieces>::kChunks>& raw, const int32_t (&place)[4],
-                                       int32_t key0, int32_t any_lo, int32_t any_pos, Seen seen, float scale_f,
+// Attends the tile's keys, from key0 on, for the wave's 16 rows.  kMask: some
+// of them are hidden from some of the rows.
+template <int D, int kPieces, int kSub, bool kMask>
+__device__ __forceinline__ void attend(const RawTile<kSub, Shape<D, kPieces>::kChunks>& raw, int32_t key0,
+                                       int32_t any_lo, int32_t any_pos, Seen seen, float scale_f,
                                        const Query<D, kPieces>& query, uint8_t* turned, int lane, f32x4_t (&acc)[D / 16],
                                        float& m_run, float& l_run) {
     using S = Shape<D, kPieces>;
     const int r = lane & 15, g = lane >> 4;
-    f32x4_t s[4];
+    f32x4_t s[kSub];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < kSub; ++t) {
         s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < S::kSteps; ++i) {
@@ -373,15 +476,15 @@ __device__ __forceinline__ void attend(const RawTile<Shape<D, kPieces>::kChunks>
                                                                     (int)raw.ks[t][c], 0, query.scale[i]);
         }
     }
-    float p[16];
+    float p[4 * kSub];
     float most = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < kSub; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float v = s[t][i] * scale_f;
             if constexpr (kMask)
-                v = place[t] >= 0 && seen(key0 + 16 * t + 4 * g + i) ? v : -INFINITY;
+                v = raw.place[t] >= 0 && seen(key0 + 16 * t + 4 * g + i) ? v : -INFINITY;
             p[4 * t + i] = v;
             most = fmaxf(most, v);
         }
@@ -398,14 +501,14 @@ __device__ __forceinline__ void attend(const RawTile<Shape<D, kPieces>::kChunks>
     const float m_use = m_run == -INFINITY ? 0.f : m_run;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 4 * kSub; ++i) {
         p[i] = __builtin_amdgcn_exp2f(p[i] - m_use);
         sum += p[i];
     }
     l_run += sum;  // this lane's keys; the row's four lanes are added up at the end
 
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int half = 0; half < kSub / 2; ++half) {
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -416,7 +519,7 @@ __device__ __forceinline__ void attend(const RawTile<Shape<D, kPieces>::kChunks>
                 if constexpr (kMask) {
                     // a token that no row sees may hold anything; a NaN that some rows see is dealt with below
                     const int32_t key = key0 + 16 * t + r;
-                    if (byte == 255u || place[t] < 0 || key <= any_lo || key > any_pos)
+                    if (byte == 255u || raw.place[t] < 0 || key <= any_lo || key > any_pos)
                         byte = 0;
                 }
                 const float scale = __uint_as_float(byte << 23);
@@ -434,12 +537,10 @@ __device__ __forceinline__ void attend(const RawTile<Shape<D, kPieces>::kChunks>
         const float* ph = p + 8 * half;
         const uint4 hi = make_uint4(pack_bf16x2(ph[0], ph[1]), pack_bf16x2(ph[2], ph[3]), pack_bf16x2(ph[4], ph[5]),
                                     pack_bf16x2(ph[6], ph[7]));
-        uint4 lo = make_uint4(0, 0, 0, 0);
-        if constexpr (kPieces == 3)
-            lo = make_uint4(pack_bf16x2(ph[0] - bf16_lo(hi.x), ph[1] - bf16_hi(hi.x)),
-                            pack_bf16x2(ph[2] - bf16_lo(hi.y), ph[3] - bf16_hi(hi.y)),
-                            pack_bf16x2(ph[4] - bf16_lo(hi.z), ph[5] - bf16_hi(hi.z)),
-                            pack_bf16x2(ph[6] - bf16_lo(hi.w), ph[7] - bf16_hi(hi.w)));
+        const uint4 lo = make_uint4(pack_bf16x2(ph[0] - bf16_lo(hi.x), ph[1] - bf16_hi(hi.x)),
+                                    pack_bf16x2(ph[2] - bf16_lo(hi.y), ph[3] - bf16_hi(hi.y)),
+                                    pack_bf16x2(ph[4] - bf16_lo(hi.z), ph[5] - bf16_hi(hi.z)),
+                                    pack_bf16x2(ph[6] - bf16_lo(hi.w), ph[7] - bf16_hi(hi.w)));
         // lane j of group g reads 4 dims of row 4g + j / 4 and gets dim j of rows 4g..4g+3
         const uint8_t* from = turned + (4 * g + (r >> 2)) * S::kVPitch + 8 * (r & 3);
 #pragma unroll
@@ -447,8 +548,7 @@ __device__ __forceinline__ void attend(const RawTile<Shape<D, kPieces>::kChunks>
             const uint2 x = read_turned(from + 32 * d), y = read_turned(from + 16 * S::kVPitch + 32 * d);
             const bf16x8_t v = __builtin_bit_cast(bf16x8_t, make_uint4(x.x, x.y, y.x, y.y));
             acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, hi), acc[d], 0, 0, 0);
-            if constexpr (kPieces == 3)
-                acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, lo), acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, lo), acc[d], 0, 0, 0);
         }
     }
 
@@ -456,20 +556,20 @@ __device__ __forceinline__ void attend(const RawTile<Shape<D, kPieces>::kChunks>
         // value blocks that are NaN, for the rows that see them (rare: the loop is entered by a vote)
         bool nan = false;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < kSub; ++t)
 #pragma unroll
             for (int c = 0; c < S::kChunks; ++c)
                 nan |= raw.vs[t][c] == 255u;
         if (__any(nan)) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < kSub; ++t)
 #pragma unroll
                 for (int c = 0; c < S::kChunks; ++c)
 #pragma unroll
                     for (int b = 0; b < (D < 128 ? 2 : 4); ++b) {
                         bool hit = false;
                         for (int token = 0; token < 16; ++token)
-                            hit |= __builtin_amdgcn_readlane(raw.vs[t][c], 16 * b + token) == 255u && place[t] >= 0 &&
+                            hit |= __builtin_amdgcn_readlane(raw.vs[t][c], 16 * b + token) == 255u && raw.place[t] >= 0 &&
                                    seen(key0 + 16 * t + token);
                         const float add = hit ? NAN : 0.f;
                         acc[8 * c + 2 * b] += add;
@@ -479,18 +579,69 @@ __device__ __forceinline__ void attend(const RawTile<Shape<D, kPieces>::kChunks>
     }
 }
 
-// A 16-row tile over all of its keys: four waves take 64 keys each in turn,
-// and their sums meet in LDS.
+// kN consecutive outputs of a row times inv, in its type.
+template <bool kHalf, int kN>
+__device__ __forceinline__ void store_out(uint16_t* to, const float* o, float inv, bool wide) {
+    uint32_t w[kN / 2];
+#pragma unroll
+    for (int i = 0; i < kN / 2; ++i) {
+        const float x = o[2 * i] * inv, y = o[2 * i + 1] * inv;
+        if constexpr (kHalf)
+            w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x) |
+                   (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)y) << 16;
+        else
+            w[i] = pack_bf16x2(x, y);
+    }
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < kN / 2; i += 2)
+            *reinterpret_cast<uint2*>(to + 2 * i) = make_uint2(w[i], w[i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN / 2; ++i) {
+            to[2 * i] = (uint16_t)w[i];
+            to[2 * i + 1] = (uint16_t)(w[i] >> 16);
+        }
+    }
+}
+
+// What a row's sums under reference m (base 2) come to: the factor of O and the lse.
+struct RowEnd {
+    float inv, lse;
+};
+
+__device__ __forceinline__ RowEnd finish_row(const AttArgs& a, int32_t head, float m, float l) {
+    const float m_use = m == -INFINITY ? 0.f : m;
+    RowEnd e;
+    if (m == -INFINITY && l == 0.f) {  // nothing was seen
+        e.inv = 0.f;
+        e.lse = INFINITY;
+        return e;
+    }
+    float below = l;
+    if (a.sink)
+        below += __builtin_amdgcn_exp2f(a.sink[head] * kLog2e - m_use);
+    e.inv = 1.0f / below;
+    e.lse = kLn2 * (m_use + __builtin_amdgcn_logf(l));
+    return e;
+}
+
+// Floats of a slot of partial results: O of kRows rows, their references and sums.
+constexpr int slot_floats(int dim) { return kRows * (dim + 2); }
+
+// A 16-row tile over its keys, or over one cut of them: four waves take a tile
+// of keys each in turn, loaded one tile ahead, and their sums meet in LDS.
 template <int D, int kPieces>
 __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a) {
     using S = Shape<D, kPieces>;
     constexpr bool kHalf = kPieces == 3;
+    constexpr int kSub = D == 256 ? 2 : 4;  // two tiles of registers have to fit
     __shared__ __align__(16) uint8_t turned[kAttWaves][S::kVBytes];
     __shared__ float wave_m[kAttWaves][kRows], wave_l[kAttWaves][kRows];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int h = (int)blockIdx.x % a.kv_heads;
     Item item;
-    if (!find_item(a, (int32_t)(blockIdx.x / a.kv_heads), item))
+    if (!find_item(a, (int32_t)(blockIdx.x / a.kv_heads), kRows, item))
         return;
     const Request req = item.req;
     const int r = lane & 15, g = lane >> 4;
@@ -507,8 +658,22 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a)
     seen.pos = valid ? pos0 + token : -1;
     seen.lo = a.window > 0 ? seen.pos - a.window : -1;
     const int32_t any_lo = a.window > 0 ? first_pos - a.window : -1;
-    const int32_t end = min(last_pos + 1, a.table_keys);
-    const int32_t begin = max(any_lo + 1, 0) & ~(kTileKeys - 1);
+    int32_t begin, end;
+    key_range(a, req, begin, end);
+    if (item.cuts > 1) {
+        begin += item.cut * item.chunk;  // below the request's end
+        end = item.chunk < end - begin ? begin + item.chunk : end;
+    }
+    end = min(end, last_pos + 1);
+    begin = max(begin, max(any_lo + 1, 0) & ~(kTileKeys - 1));
+
+    constexpr int kKeys = 16 * kSub, kStride = kAttWaves * kKeys, kBatch = 64 / kSub;
+    const int32_t key0 = begin + wave * kKeys;
+    const int32_t tiles = end > key0 ? (end - key0 + kStride - 1) / kStride : 0;
+    Places places = find_places<kSub>(a, item.b, h, mx_token_bytes(D), key0, kStride, end, lane);
+    RawTile<kSub, S::kChunks> raw[2];
+    if (tiles > 0)
+        load_tile<D, kSub>(a, places, 0, lane, raw[0]);
 
     Query<D, kPieces> query;
     load_query<D, kPieces, kHalf>(a, (req.first + token) * a.q_st + head * a.q_sh, valid, g, query);
@@ -518,25 +683,28 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a)
         acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, l_run = 0.f;
 
-    constexpr int kStride = kAttWaves * kTileKeys;
-    const int32_t key0 = begin + wave * kTileKeys;
-    const int32_t tiles = end > key0 ? (end - key0 + kStride - 1) / kStride : 0;
-    Places places;
-    for (int32_t i = 0; i < tiles; ++i) {
+    auto step = [&](int32_t i, const RawTile<kSub, S::kChunks>& now, RawTile<kSub, S::kChunks>& next) {
+        if (i + 1 < tiles) {
+            if ((i + 1) % kBatch == 0)
+                places = find_places<kSub>(a, item.b, h, mx_token_bytes(D), key0 + (i + 1) * kStride, kStride, end, lane);
+            load_tile<D, kSub>(a, places, i + 1, lane, next);
+        }
         const int32_t key = key0 + i * kStride;
-        if ((i & 15) == 0)
-            places = find_places(a, item.b, h, mx_token_bytes(D), key, kStride, end, lane);
-        RawTile<S::kChunks> raw;
-        int32_t place[4];
-        load_tile<D>(a, places, i, lane, raw, place);
-        const bool all = key + kTileKeys - 1 <= min(first_pos, end - 1) && (a.window == 0 || key > last_pos - a.window) &&
-                         place[0] >= 0 && place[1] >= 0 && place[2] >= 0 && place[3] >= 0;
+        bool all = key + kKeys - 1 <= min(first_pos, end - 1) && (a.window == 0 || key > last_pos - a.window);
+#pragma unroll
+        for (int t = 0; t < kSub; ++t)
+            all = all && now.place[t] >= 0;
         if (all)
-            attend<D, kPieces, false>(raw, place, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane,
-                                      acc, m_run, l_run);
+            attend<D, kPieces, kSub, false>(now, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane, acc,
+                                            m_run, l_run);
         else
-            attend<D, kPieces, true>(raw, place, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane,
-                                     acc, m_run, l_run);
+            attend<D, kPieces, kSub, true>(now, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane, acc,
+                                           m_run, l_run);
+    };
+    for (int32_t i = 0; i < tiles; i += 2) {
+        step(i, raw[0], raw[1]);
+        if (i + 1 < tiles)
+            step(i + 1, raw[1], raw[0]);
     }
     l_run = group4_sum(l_run);
     asm volatile("" ::: "memory");
@@ -553,6 +721,15 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a)
     constexpr int kDims = D / 16;
     const int orow = threadIdx.x >> 4, part = threadIdx.x & 15;
     const int32_t mine = item.tile * kRows + orow;
+    if (item.cuts > 1 && item.cut == 0 && h == 0 && threadIdx.x == 0) {
+        SplitTile t;
+        t.first_token = req.first;
+        t.first_row = item.tile * kRows;
+        t.rows = rows;
+        t.slot = item.slot;
+        t.count = item.cuts;
+        a.split_tiles[item.order] = t;
+    }
     if (mine >= rows)
         return;
     float m = -INFINITY;
@@ -577,46 +754,120 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a)
                 o[i + j] += f * v[j];
         }
     }
+    if (item.cuts > 1) {
+        float* slot = a.partials + ((int64_t)h * a.slots_per_head + item.slot + item.cut) * slot_floats(D);
+#pragma unroll
+        for (int i = 0; i < kDims; i += 4)
+            *reinterpret_cast<f32x4_t*>(slot + orow * D + part * kDims + i) = f32x4_t{o[i], o[i + 1], o[i + 2], o[i + 3]};
+        if (part == 0) {
+            slot[kRows * D + orow] = m;
+            slot[kRows * D + kRows + orow] = l;
+        }
+        return;
+    }
     const int32_t otoken = mine / a.group, ohead = h * a.group + mine - otoken * a.group;
     const int64_t t = req.first + otoken;
-    const bool none = m == -INFINITY && l == 0.f;
-    float below = l;
-    if (a.sink)
-        below += __builtin_amdgcn_exp2f(a.sink[ohead] * kLog2e - m_use);
-    const float inv = none ? 0.f : 1.0f / below;
-    uint16_t* to = static_cast<uint16_t*>(a.out) + t * a.o_st + ohead * a.o_sh + part * kDims;
-    uint32_t w[kDims / 2];
-#pragma unroll
-    for (int i = 0; i < kDims / 2; ++i) {
-        const float x = o[2 * i] * inv, y = o[2 * i + 1] * inv;
-        if constexpr (kHalf) {
-            w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)x) |
-                   (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)y) << 16;
-        } else {
-            w[i] = pack_bf16x2(x, y);
-        }
-    }
-    if (a.o_wide) {
-#pragma unroll
-        for (int i = 0; i < kDims / 2; i += 2)
-            *reinterpret_cast<uint2*>(to + 2 * i) = make_uint2(w[i], w[i + 1]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kDims / 2; ++i) {
-            to[2 * i] = (uint16_t)w[i];
-            to[2 * i + 1] = (uint16_t)(w[i] >> 16);
-        }
-    }
+    const RowEnd e = finish_row(a, ohead, m, l);
+    store_out<kHalf, kDims>(static_cast<uint16_t*>(a.out) + t * a.o_st + ohead * a.o_sh + part * kDims, o, e.inv, a.o_wide);
     if (part == 0)
-        a.lse[t * a.lse_st + ohead] = none ? INFINITY : kLn2 * (m_use + __builtin_amdgcn_logf(l));
+        a.lse[t * a.lse_st + ohead] = e.lse;
+}
+
+// Joins the cuts of one row: workgroup (cut tile and head, row of the tile).
+template <int D, bool kHalf>
+__global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
+    __shared__ float factor[kMostCuts];
+    __shared__ float sums[kAttThreads * 4];
+    constexpr int kLanes = D / 4, kGroups = kAttThreads / kLanes;
+    const int32_t order = (int32_t)(blockIdx.x / a.kv_heads), h = (int32_t)(blockIdx.x % a.kv_heads);
+    if (order >= *a.num_split_tiles)
+        return;
+    const SplitTile tile = a.split_tiles[order];
+    const int32_t r = (int32_t)blockIdx.y, row = tile.first_row + r;
+    if (row >= tile.rows)
+        return;
+    const float* slots = a.partials + ((int64_t)h * a.slots_per_head + tile.slot) * slot_floats(D);
+    const int lane = threadIdx.x & 63;
+    // every wave finds the reference and the sum for itself
+    float m = -INFINITY;
+    for (int32_t i = lane; i < tile.count; i += 64)
+        m = fmaxf(m, slots[(int64_t)i * slot_floats(D) + kRows * D + r]);
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1)
+        m = fmaxf(m, __shfl_xor(m, d));
+    const float m_use = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int32_t i = lane; i < tile.count; i += 64) {
+        const float* slot = slots + (int64_t)i * slot_floats(D) + kRows * D + r;
+        const float f = __builtin_amdgcn_exp2f(slot[0] - m_use);
+        l += f * slot[kRows];
+        if (threadIdx.x < 64)
+            factor[i] = f;
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1)
+        l += __shfl_xor(l, d);
+    __syncthreads();
+    const int part = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int32_t i = group; i < tile.count; i += kGroups)
+        o += factor[i] * *reinterpret_cast<const f32x4_t*>(slots + (int64_t)i * slot_floats(D) + r * D + 4 * part);
+    *reinterpret_cast<f32x4_t*>(sums + 4 * threadIdx.x) = o;
+    __syncthreads();
+    if (group != 0)
+        return;
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i)
+        o += *reinterpret_cast<const f32x4_t*>(sums + 4 * (i * kLanes + part));
+    const int32_t token = row / a.group, head = h * a.group + row - token * a.group;
+    const int64_t t = tile.first_token + token;
+    const RowEnd e = finish_row(a, head, m, l);
+    const float out[4] = {o[0], o[1], o[2], o[3]};
+    store_out<kHalf, 4>(static_cast<uint16_t*>(a.out) + t * a.o_st + head * a.o_sh + 4 * part, out, e.inv, a.o_wide);
+    if (part == 0)
+        a.lse[t * a.lse_st + head] = e.lse;
+}
+
+// How a call is cut, from what the host knows.
+struct Cutting {
+    int32_t split_items, slots_per_head, most_tiles;  // split_items 0: not at all
+    int64_t grid_tiles;                               // row tiles at most
+    int64_t tiles_at, count_at, bytes;                // parts of the workspace
+};
+
+Cutting cutting_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t reqs, int64_t max_seq) {
+    Cutting c = {};
+    // no request has more tiles than its rows' share, rounded up
+    c.grid_tiles = tokens * (heads / kv_heads) / kRows + reqs;
+    const int64_t target = kSplitTurns * cu_count() < kMostCuts - 76 ? kSplitTurns * cu_count() : kMostCuts - 76;
+    // keys that one turn of the waves takes, or more tiles than the chip holds several times over: nothing to cut
+    if (max_seq <= kChunkStep || c.grid_tiles * kv_heads > 8 * target)
+        return c;
+    c.split_items = (int32_t)(target / kv_heads > 0 ? target / kv_heads : 1);
+    // tiles that are cut have more than a chunk of keys: at most split_items + 1 chunks and one more each
+    c.slots_per_head = 2 * c.split_items + 8;
+    c.most_tiles = (int32_t)(c.grid_tiles < c.split_items + 4 ? c.grid_tiles : c.split_items + 4);
+    c.tiles_at = kv_heads * c.slots_per_head * (int64_t)slot_floats((int)dim) * 4;
+    c.count_at = c.tiles_at + c.most_tiles * (int64_t)sizeof(SplitTile);
+    c.bytes = (c.count_at + 4 + 255) / 256 * 256;
+    return c;
+}
+
+template <int D, int kPieces>
+void launch_attend(const Cutting& cut, hipStream_t st, const AttArgs& a) {
+    const unsigned grid = (unsigned)((cut.grid_tiles + a.split_items) * a.kv_heads);
+    hipLaunchKernelGGL((mxfp4_attend_kernel<D, kPieces>), dim3(grid), dim3(kAttThreads), 0, st, a);
+    if (a.split_items > 0) {
+        const unsigned rows = a.query_start_loc || a.group >= kRows ? kRows : a.group;
+        hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3>), dim3((unsigned)(cut.most_tiles * a.kv_heads), rows),
+                           dim3(kAttThreads), 0, st, a);
+    }
 }
 
 template <int D>
-void launch_attend(bool half, unsigned grid, hipStream_t st, const AttArgs& a) {
-    if (half)
-        hipLaunchKernelGGL((mxfp4_attend_kernel<D, 3>), dim3(grid), dim3(kAttThreads), 0, st, a);
-    else
-        hipLaunchKernelGGL((mxfp4_attend_kernel<D, 2>), dim3(grid), dim3(kAttThreads), 0, st, a);
+void launch_attend(bool half, const Cutting& cut, hipStream_t st, const AttArgs& a) {
+    half ? launch_attend<D, 3>(cut, st, a) : launch_attend<D, 2>(cut, st, a);
 }
 
 }  // namespace
@@ -633,10 +884,6 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
                                          int64_t out_stride_head, float* lse, int64_t lse_stride_token, void* workspace,
                                          int64_t workspace_bytes, void* stream) {
     using namespace fgv;
-    (void)max_query_len;
-    (void)max_seq_len;
-    (void)workspace;
-    (void)workspace_bytes;
     if (num_tokens < 0 || num_heads < 0 || num_kv_heads < 0 || num_blocks < 0 || num_reqs < 0 || max_blocks_per_req < 0 ||
         max_query_len < 0 || max_seq_len < 0 || window_size < 0)
         return fail(FGV_E_BAD_SHAPE, "negative size");
@@ -696,16 +943,23 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
     a.window = (int32_t)(window_size < 0x3fffffffLL ? window_size : 0);
     a.q_wide = aligned(q, 16) && ((q_stride_token | q_stride_head) & 7) == 0;
     a.o_wide = aligned(out, 8) && ((out_stride_token | out_stride_head) & 3) == 0;
-    // no request has more tiles than its rows' share, rounded up
-    const int64_t tiles = num_tokens * a.group / kRows + num_reqs;
-    if (tiles * num_kv_heads > 0x7fffffffLL)
+    Cutting cut = cutting_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_seq_len);
+    if (workspace && workspace_bytes >= cut.bytes && !aligned(workspace, 16))
+        return fail(FGV_E_MISALIGNED, "workspace must be 16-byte aligned");
+    if (!workspace || workspace_bytes < cut.bytes)
+        cut.split_items = 0;
+    a.split_items = cut.split_items;
+    a.slots_per_head = cut.slots_per_head;
+    a.partials = static_cast<float*>(workspace);
+    a.split_tiles = reinterpret_cast<SplitTile*>(static_cast<uint8_t*>(workspace) + cut.tiles_at);
+    a.num_split_tiles = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + cut.count_at);
+    if ((cut.grid_tiles + a.split_items) * num_kv_heads > 0x7fffffffLL)
         return fail(FGV_E_TOO_LARGE, "too many row tiles");
-    const unsigned grid = (unsigned)(tiles * num_kv_heads);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     switch (head_dim) {
-        case 64: launch_attend<64>(dtype == 1, grid, st, a); break;
-        case 128: launch_attend<128>(dtype == 1, grid, st, a); break;
-        default: launch_attend<256>(dtype == 1, grid, st, a); break;
+        case 64: launch_attend<64>(dtype == 1, cut, st, a); break;
+        case 128: launch_attend<128>(dtype == 1, cut, st, a); break;
+        default: launch_attend<256>(dtype == 1, cut, st, a); break;
     }
     return launch_status();
 }
@@ -713,12 +967,10 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
 extern "C" int64_t fgv_mxfp4_paged_attention_workspace_bytes(int64_t num_tokens, int64_t num_heads,
                                                              int64_t num_kv_heads, int64_t head_dim, int64_t num_reqs,
                                                              int64_t max_query_len, int64_t max_seq_len) {
-    (void)num_tokens;
-    (void)num_heads;
-    (void)num_kv_heads;
-    (void)head_dim;
-    (void)num_reqs;
     (void)max_query_len;
-    (void)max_seq_len;
-    return 0;
+    if (num_tokens <= 0 || num_reqs <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || num_heads > 65536 ||
+        num_tokens * num_heads > 0x3fffffffLL || num_reqs > 0x3fffffffLL)
+        return 0;
+    const fgv::Cutting cut = fgv::cutting_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_seq_len);
+    return cut.split_items > 0 ? cut.bytes : 0;
 }

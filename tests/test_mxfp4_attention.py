@@ -2,8 +2,11 @@
 
 What the kernels may be off, row by row (``bounds``), counted before their first run:
 
-* the query enters as e4m3 pieces under one power of two per row: of each value less
-  than 2^-20 of the row's maximum is lost;
+* the query enters as e4m3 pieces under one power of two per row that puts its maximum into
+  [128, 256).  The first piece leaves of small values up to 1/16 (it takes multiples of 1/8) and of
+  others what 4 bits do not hold; of what it leaves of a small value, at most 1 after the factor 16,
+  the second leaves half a step of 4 bits below 1, 2^-5: 2^-9 in all, 2^-16 of the row's maximum
+  (large bf16 values are held whole).  A third piece (fp16) leaves 2^-5 of 2^-4 of that;
 * the matrix instruction adds at most 32 products at a time, each cut below
   2^(E - 13), E the largest exponent among them.  A product has 6 bits, and the codes'
   exponents span 3 binades, so only products of query values more than 6 binades
@@ -11,7 +14,7 @@ What the kernels may be off, row by row (``bounds``), counted before their first
   behind the first, 2^-4 as large at least, any may be;
 * scores are scaled and exp2 taken in 32 bits: 2^-20 (1 + |s|) together covers the
   scaling, the subtraction and two ulp of the exponential;
-* P is rounded to bf16 (2^-8), in fp16 calls to two bf16 pieces (2^-16);
+* P enters as two bf16 pieces (2^-16);
 * sums in 32 bits: a step of 2^-23 per 32 keys and per joined part;
 * P below 2^-126 of a row's largest is nothing in 32 bits (the first run showed that this had
   been left out: a dim where all keys but such ones hold zeros came out as 0 instead of 4e-39): at
@@ -135,13 +138,14 @@ def reference(q, cache, table, lens, start, scale, window=None, sink=None):
             cut = far * 2.0 ** -13 * torch.exp2(e.amax(2)) * (blocks.amax(2) > 0)
             kscale = torch.exp2(kbytes[h // group].double() - 127) * 4
             kabs = torch.where(torch.isnan(kh), 0.0, kh).abs().sum(1)
-            d = abs(scale) * (cut @ torch.where(kscale > 1e30, 0.0, kscale).t().contiguous() + 2.0 ** -20 * top * kabs)
+            d = abs(scale) * (cut @ torch.where(kscale > 1e30, 0.0, kscale).t().contiguous()
+                             + 2.0 ** (-20 if three else -16) * top * kabs)
             d = torch.where(seen, d + 2.0 ** -20 * (1 + s.abs()), 0.0).nan_to_num(0.0).amax(1)
             steps = (n / 32 + 40) * 2.0 ** -23
             weight = p @ torch.where(nan, 0.0, vh).abs() * share[:, None]
             o = o * share[:, None]
             half = torch.finfo(q.dtype).eps / 2
-            ob = weight * (2.0 ** (-16 if three else -8) + 2.5 * d + steps)[:, None] * (1 + half)
+            ob = weight * (2.0 ** -16 + 2.5 * d + steps)[:, None] * (1 + half)
             ob = ob + half * o.abs() + torch.finfo(q.dtype).smallest_normal * half
             ob = ob + 2.0 ** -125 * torch.where(nan, 0.0, vh).abs().sum(0)
             out[t0:t1, h] = torch.where(some[:, None], o, 0.0)
