@@ -51,16 +51,21 @@ typedef __attribute__((address_space(3))) short4_t lds_short4_t;
 
 constexpr int kAttThreads = 256;
 constexpr int kAttWaves = kAttThreads / 64;
-constexpr int kTileKeys = 64;  // keys a wave takes at a time: four 16-key subtiles
+constexpr int kTileKeys = 64;  // keys of every tile begin at a multiple of this
 constexpr int kRows = 16;      // query rows of a workgroup
-constexpr int kChunkStep = kAttWaves * kTileKeys;  // keys are cut between workgroups in steps of a turn of the waves
-constexpr int kMostCuts = 1100;                    // of one tile: more than split_items + 1 ever is
-constexpr int kSplitTurns = 2;                     // workgroups a CU holds at a time
+constexpr int kMostWorkers = 1024;  // per head
+constexpr int kWorkersPerCu = 2;    // workgroups that a CU holds at a time
+constexpr int kLeastUnits = 4;      // turns of the waves that a worker takes at least
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// The running maximum is raised only when a score exceeds it by more than this
-// (base 2), so that most tiles rescale nothing: P stays below 2^8.
-constexpr float kRaise = 8.0f;
+// A row's reference is raised when a score exceeds it, and then to this much
+// above the score (base 2), so that most tiles rescale nothing.  P is at most 1.
+constexpr float kAhead = 8.0f;
+
+// 16-key subtiles that a wave takes at a time: two such tiles have to fit its registers.
+__host__ __device__ constexpr int key_subtiles(int dim) { return dim == 256 ? 2 : 4; }
+// Keys of a turn of the workgroup's waves, in which keys are dealt out.
+__host__ __device__ constexpr int unit_keys(int dim) { return kAttWaves * 16 * key_subtiles(dim); }
 
 struct AttArgs {
     const void* q;
@@ -80,17 +85,16 @@ struct AttArgs {
     int32_t scale_e;
     int32_t num_reqs, num_tokens, kv_heads, group, page, table_keys, window;
     int32_t q_wide, o_wide;
-    // split mode (split_items > 0): about how many workgroups per head to cut the keys
-    // into, slots of partial results per head, and their places in the workspace
-    int32_t split_items, slots_per_head;
+    // Stream mode (workers > 0): workers per head, at least how many units of keys
+    // each takes, and the workspace's parts.
+    int32_t workers, least_units;
     float* partials;
-    struct SplitTile* split_tiles;
-    int32_t* num_split_tiles;
+    struct CutTile* cut_tiles;
 };
 
-// A row tile whose keys are cut: `count` slots of each head from `slot` on.
-struct SplitTile {
-    int32_t first_token, first_row, rows, slot, count;
+// A row tile whose keys are cut between workers: `count` of them from the first one on.
+struct CutTile {
+    int32_t first_token, first_row, rows, count;
 };
 
 // A request's query tokens [first, first + count) and lengths.
@@ -119,127 +123,123 @@ __device__ __forceinline__ void key_range(const AttArgs& a, const Request& r, in
     begin = a.window > 0 ? max(r.len - r.count - a.window + 1, 0) & ~(kTileKeys - 1) : 0;
 }
 
-// One workgroup's work: row tile `tile` of request b, the keys of cut `cut` of
-// `cuts` that are `chunk` keys each.
-struct Item {
+// A request and its tiles of kRows rows, `units` units of keys each.
+struct Tiles {
     Request req;
-    int32_t b, tile, cut, cuts, chunk;
-    int32_t slot;   // cuts > 1: the first of the tile's slots
-    int32_t order;  // and its number among the cut tiles
+    int32_t count, units;
+};
+
+__device__ __forceinline__ Tiles tiles_of(const AttArgs& a, int32_t b, int32_t rows_per_tile, int32_t unit_keys) {
+    Tiles t;
+    t.req = request_of(a, b);
+    t.count = (int32_t)(((int64_t)t.req.count * a.group + rows_per_tile - 1) / rows_per_tile);
+    t.units = 1;
+    if (a.workers > 0) {
+        int32_t begin, end;
+        key_range(a, t.req, begin, end);
+        t.units = max((end - begin + unit_keys - 1) / unit_keys, 1);
+    }
+    return t;
+}
+
+// Where a workgroup begins: unit `unit` of tile `tile` of request b; it takes
+// `take` units, through tiles and requests in order.  `each` is what workers take.
+struct Start {
+    Tiles tiles;
+    int32_t b, tile, unit;
+    int64_t take, each;
 };
 
 // Sum of v over the lanes up to this one.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x111, 0xF, 0xF, false);  // row_shr:1
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ uint64_t dpp_moved(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)v, kCtrl, kRowMask, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(v >> 32), kCtrl, kRowMask, 0xF, false);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+    v += dpp_moved<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+    v += dpp_moved<0x112, 0xF>(v);
+    v += dpp_moved<0x114, 0xF>(v);
+    v += dpp_moved<0x118, 0xF>(v);
+    v += dpp_moved<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    v += dpp_moved<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
     return v;
 }
 
-// The item number `index`, counted over requests, tiles and cuts in order; false
-// behind the last.  Each workgroup works out the plan for itself: lengths are
-// known on the device only, and a launch to do it would cost more.  With
-// split_items > 0 the keys of all row tiles, together `total`, are cut into
-// chunks of total / split_items keys (in steps of kChunkStep), so that
-// workgroups have about the same to do whatever the lengths are; at most twice
-// as many cuts as split_items come from tiles that are cut at all.
-__device__ __forceinline__ bool find_item(const AttArgs& a, int32_t index, int32_t rows_per_tile, Item& item) {
-    __shared__ float part_keys[kAttWaves];
-    __shared__ uint32_t part[3][kAttWaves];
-    __shared__ int32_t found[6];
+// The start of worker `index`; false if there is nothing for it.  Every workgroup
+// works out the plan for itself: lengths are known on the device only, and a
+// launch to do it would cost more than the scan.  In stream mode the units of
+// all tiles, one after the other, are dealt out evenly, so that workgroups have
+// the same to do whatever the lengths are; a tile that is longer than the
+// rest of its worker's share goes on with the next.  Otherwise a worker is a tile.
+__device__ __forceinline__ bool find_start(const AttArgs& a, int32_t index, int32_t rows_per_tile, int32_t unit_keys,
+                                           Start& start) {
+    __shared__ uint64_t part[kAttWaves];
+    __shared__ int32_t found[8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const bool split = a.split_items > 0;
     if (threadIdx.x == 0)
         found[0] = -1;
-    int32_t chunk = 0x7fffffff;
-    auto tiles_of = [&](const Request& r) {
-        return (int32_t)(((int64_t)r.count * a.group + rows_per_tile - 1) / rows_per_tile);
-    };
-    if (split) {
-        float keys = 0.f;
-        for (int32_t b = (int32_t)threadIdx.x; b < a.num_reqs; b += kAttThreads) {
-            const Request r = request_of(a, b);
-            int32_t begin, end;
-            key_range(a, r, begin, end);
-            keys += (float)tiles_of(r) * (float)max(end - begin, 0);
-        }
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1)
-            keys += __shfl_xor(keys, d);
-        if (lane == 0)
-            part_keys[wave] = keys;
-        __syncthreads();
-        keys = 0.f;
-#pragma unroll
-        for (int w = 0; w < kAttWaves; ++w)
-            keys += part_keys[w];
-        const float each = keys / (float)a.split_items;
-        chunk = each < 1e9f ? ((int32_t)each / kChunkStep + 1) * kChunkStep : 0x7fffffff;
-    }
-    uint32_t before[3] = {0, 0, 0};  // items, slots, cut tiles of the requests in front
-    for (int32_t base = 0; base < a.num_reqs; base += kAttThreads) {
+    Tiles mine = {};
+    uint64_t at = 0, n = 0;  // units in front of this thread's request of the turn, and its own
+    auto scan_turn = [&](int32_t base, uint64_t& before) {
         const int32_t b = base + (int32_t)threadIdx.x;
-        uint32_t n[3] = {0, 0, 0};
-        int32_t tiles = 0, cuts = 1;
+        n = 0;
         if (b < a.num_reqs) {
-            const Request r = request_of(a, b);
-            tiles = tiles_of(r);
-            if (split) {
-                int32_t begin, end;
-                key_range(a, r, begin, end);
-                cuts = max((int32_t)(((int64_t)(end - begin) + chunk - 1) / chunk), 1);
-            }
-            n[0] = (uint32_t)tiles * cuts;
-            n[1] = cuts > 1 ? n[0] : 0;
-            n[2] = cuts > 1 ? tiles : 0;
+            mine = tiles_of(a, b, rows_per_tile, unit_keys);
+            n = (uint64_t)mine.count * mine.units;
         }
-        uint32_t at[3];
+        const uint64_t s = wave_scan(n);
+        if (lane == 63)
+            part[wave] = s;
+        __syncthreads();
+        at = before + s - n;
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            const uint32_t s = wave_scan(n[i]);
-            if (lane == 63)
-                part[i][wave] = s;
-            at[i] = before[i] + s - n[i];
+        for (int w = 0; w < kAttWaves; ++w) {
+            at += w < wave ? part[w] : 0;
+            before += part[w];
         }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 3; ++i)
-#pragma unroll
-            for (int w = 0; w < kAttWaves; ++w) {
-                at[i] += w < wave ? part[i][w] : 0;
-                before[i] += part[i][w];
-            }
-        const uint32_t mine = (uint32_t)index - at[0];
-        if ((uint32_t)index >= at[0] && mine < n[0]) {
-            const int32_t tile = (int32_t)(mine / cuts);
-            found[0] = b;
+    };
+    uint64_t total = 0;
+    for (int32_t base = 0; base < a.num_reqs; base += kAttThreads)
+        scan_turn(base, total);
+    uint64_t each = 1;
+    if (a.workers > 0) {
+        each = (total + a.workers - 1) / a.workers;
+        each = each < (uint64_t)a.least_units ? a.least_units : each;
+    }
+    const uint64_t first = each * index;
+    if (first >= total)
+        return false;
+    uint64_t before = 0;
+    for (int32_t base = 0; base < a.num_reqs; base += kAttThreads) {
+        if (a.num_reqs > kAttThreads)
+            scan_turn(base, before);
+        if (first >= at && first - at < n) {
+            const uint64_t in = first - at;
+            const int32_t tile = mine.units == 1 ? (int32_t)in : (int32_t)(in / mine.units);
+            found[0] = base + (int32_t)threadIdx.x;
             found[1] = tile;
-            found[2] = (int32_t)mine - tile * cuts;
-            found[3] = cuts;
-            found[4] = (int32_t)at[1] + tile * cuts;
-            found[5] = (int32_t)at[2] + tile;
+            found[2] = (int32_t)(in - (uint64_t)tile * mine.units);
+            found[3] = mine.req.first;
+            found[4] = mine.req.count;
+            found[5] = mine.req.len;
+            found[6] = mine.count;
+            found[7] = mine.units;
         }
-        __syncthreads();
-        // the first workgroup sees all requests, for the number of cut tiles
-        if (before[0] > (uint32_t)index && !(split && blockIdx.x == 0))
-            break;
     }
     __syncthreads();
-    if (split && blockIdx.x == 0 && threadIdx.x == 0)
-        *a.num_split_tiles = (int32_t)before[2];
-    item.b = __builtin_amdgcn_readfirstlane(found[0]);
-    if (item.b < 0)
-        return false;
-    item.tile = __builtin_amdgcn_readfirstlane(found[1]);
-    item.cut = __builtin_amdgcn_readfirstlane(found[2]);
-    item.cuts = __builtin_amdgcn_readfirstlane(found[3]);
-    item.slot = __builtin_amdgcn_readfirstlane(found[4]);
-    item.order = __builtin_amdgcn_readfirstlane(found[5]);
-    item.chunk = chunk;
-    item.req = request_of(a, item.b);
+    start.b = __builtin_amdgcn_readfirstlane(found[0]);
+    start.tile = __builtin_amdgcn_readfirstlane(found[1]);
+    start.unit = __builtin_amdgcn_readfirstlane(found[2]);
+    start.tiles.req.first = __builtin_amdgcn_readfirstlane(found[3]);
+    start.tiles.req.count = __builtin_amdgcn_readfirstlane(found[4]);
+    start.tiles.req.len = __builtin_amdgcn_readfirstlane(found[5]);
+    start.tiles.count = __builtin_amdgcn_readfirstlane(found[6]);
+    start.tiles.units = __builtin_amdgcn_readfirstlane(found[7]);
+    start.each = (int64_t)each;
+    start.take = (int64_t)(total - first < each ? total - first : each);
     return true;
 }
 
@@ -489,8 +489,8 @@ __device__ __forceinline__ void attend(const RawTile<kSub, Shape<D, kPieces>::kC
             most = fmaxf(most, v);
         }
     most = group4_max(most);
-    if (__any(most > m_run + kRaise)) {
-        const float m_new = fmaxf(m_run, most);
+    if (__any(most > m_run)) {
+        const float m_new = most > m_run ? most + kAhead : m_run;
         const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
         l_run *= alpha;
 #pragma unroll
@@ -629,176 +629,201 @@ __device__ __forceinline__ RowEnd finish_row(const AttArgs& a, int32_t head, flo
 // Floats of a slot of partial results: O of kRows rows, their references and sums.
 constexpr int slot_floats(int dim) { return kRows * (dim + 2); }
 
-// A 16-row tile over its keys, or over one cut of them: four waves take a tile
-// of keys each in turn, loaded one tile ahead, and their sums meet in LDS.
+// A worker has two slots of each head: for a tile that began before it (or is all
+// cut through it), and for one that begins in it and goes on.
+__device__ __forceinline__ int64_t slot_of(const AttArgs& a, int32_t h, int32_t worker, bool begins) {
+    return 2 * ((int64_t)h * a.workers + worker) + (begins ? 1 : 0);
+}
+
+// A worker's tiles of 16 rows: four waves take a tile of keys each in turn,
+// loaded one tile ahead, and their sums meet in LDS.
 template <int D, int kPieces>
 __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a) {
     using S = Shape<D, kPieces>;
     constexpr bool kHalf = kPieces == 3;
-    constexpr int kSub = D == 256 ? 2 : 4;  // two tiles of registers have to fit
+    constexpr int kSub = key_subtiles(D);
+    constexpr int kKeys = 16 * kSub, kUnit = unit_keys(D), kBatch = 64 / kSub;
     __shared__ __align__(16) uint8_t turned[kAttWaves][S::kVBytes];
     __shared__ float wave_m[kAttWaves][kRows], wave_l[kAttWaves][kRows];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int h = (int)blockIdx.x % a.kv_heads;
-    Item item;
-    if (!find_item(a, (int32_t)(blockIdx.x / a.kv_heads), kRows, item))
-        return;
-    const Request req = item.req;
+    const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads);
     const int r = lane & 15, g = lane >> 4;
-    const int32_t rows = req.count * a.group;  // fits: count * group rows are rows of q
-    const int32_t row = item.tile * kRows + r;
-    const bool valid = row < rows;
-    const int32_t token = (valid ? row : 0) / a.group;
-    const int32_t head = h * a.group + (valid ? row - token * a.group : 0);
-
-    const int32_t pos0 = req.len - req.count;
-    const int32_t last_row = min(item.tile * kRows + kRows, rows) - 1;
-    const int32_t first_pos = pos0 + item.tile * kRows / a.group, last_pos = pos0 + last_row / a.group;
-    Seen seen;
-    seen.pos = valid ? pos0 + token : -1;
-    seen.lo = a.window > 0 ? seen.pos - a.window : -1;
-    const int32_t any_lo = a.window > 0 ? first_pos - a.window : -1;
-    int32_t begin, end;
-    key_range(a, req, begin, end);
-    if (item.cuts > 1) {
-        begin += item.cut * item.chunk;  // below the request's end
-        end = item.chunk < end - begin ? begin + item.chunk : end;
-    }
-    end = min(end, last_pos + 1);
-    begin = max(begin, max(any_lo + 1, 0) & ~(kTileKeys - 1));
-
-    constexpr int kKeys = 16 * kSub, kStride = kAttWaves * kKeys, kBatch = 64 / kSub;
-    const int32_t key0 = begin + wave * kKeys;
-    const int32_t tiles = end > key0 ? (end - key0 + kStride - 1) / kStride : 0;
-    Places places = find_places<kSub>(a, item.b, h, mx_token_bytes(D), key0, kStride, end, lane);
-    RawTile<kSub, S::kChunks> raw[2];
-    if (tiles > 0)
-        load_tile<D, kSub>(a, places, 0, lane, raw[0]);
-
-    Query<D, kPieces> query;
-    load_query<D, kPieces, kHalf>(a, (req.first + token) * a.q_st + head * a.q_sh, valid, g, query);
-    f32x4_t acc[D / 16];
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d)
-        acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float m_run = -INFINITY, l_run = 0.f;
-
-    auto step = [&](int32_t i, const RawTile<kSub, S::kChunks>& now, RawTile<kSub, S::kChunks>& next) {
-        if (i + 1 < tiles) {
-            if ((i + 1) % kBatch == 0)
-                places = find_places<kSub>(a, item.b, h, mx_token_bytes(D), key0 + (i + 1) * kStride, kStride, end, lane);
-            load_tile<D, kSub>(a, places, i + 1, lane, next);
+    const int orow = threadIdx.x >> 4, part = threadIdx.x & 15;  // of the end: 16 threads per row
+    Start w;
+    const bool busy = find_start(a, worker, kRows, kUnit, w);
+    CutTile cut = {0, 0, 0, 0};  // the tile that begins here and goes on with the next workers
+    int64_t left = busy ? w.take : 0;
+    while (left > 0) {
+        const Request req = w.tiles.req;
+        const int32_t units = (int32_t)min(left, (int64_t)(w.tiles.units - w.unit));
+        const bool whole = units == w.tiles.units;
+        const int32_t rows = req.count * a.group;  // fits: count * group rows are rows of q
+        const int32_t row = w.tile * kRows + r;
+        const bool valid = row < rows;
+        const int32_t token = (valid ? row : 0) / a.group;
+        const int32_t head = h * a.group + (valid ? row - token * a.group : 0);
+        const int32_t pos0 = req.len - req.count;
+        const int32_t last_row = min(w.tile * kRows + kRows, rows) - 1;
+        const int32_t first_pos = pos0 + w.tile * kRows / a.group, last_pos = pos0 + last_row / a.group;
+        Seen seen;
+        seen.pos = valid ? pos0 + token : -1;
+        seen.lo = a.window > 0 ? seen.pos - a.window : -1;
+        const int32_t any_lo = a.window > 0 ? first_pos - a.window : -1;
+        int32_t begin, end;
+        key_range(a, req, begin, end);
+        if (!whole) {
+            begin += w.unit * kUnit;  // below the request's end
+            end = units <= (end - begin) / kUnit ? begin + units * kUnit : end;
         }
-        const int32_t key = key0 + i * kStride;
-        bool all = key + kKeys - 1 <= min(first_pos, end - 1) && (a.window == 0 || key > last_pos - a.window);
-#pragma unroll
-        for (int t = 0; t < kSub; ++t)
-            all = all && now.place[t] >= 0;
-        if (all)
-            attend<D, kPieces, kSub, false>(now, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane, acc,
-                                            m_run, l_run);
-        else
-            attend<D, kPieces, kSub, true>(now, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane, acc,
-                                           m_run, l_run);
-    };
-    for (int32_t i = 0; i < tiles; i += 2) {
-        step(i, raw[0], raw[1]);
-        if (i + 1 < tiles)
-            step(i + 1, raw[1], raw[0]);
-    }
-    l_run = group4_sum(l_run);
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d)
-        *reinterpret_cast<f32x4_t*>(turned[wave] + r * S::kOPitch + 64 * d + 16 * g) = acc[d];
-    if (g == 0) {
-        wave_m[wave][r] = m_run;
-        wave_l[wave][r] = l_run;
-    }
-    __syncthreads();
+        end = min(end, last_pos + 1);
+        begin = max(begin, max(any_lo + 1, 0) & ~(kTileKeys - 1));
 
-    // 16 threads per row, D / 16 dims each
-    constexpr int kDims = D / 16;
-    const int orow = threadIdx.x >> 4, part = threadIdx.x & 15;
-    const int32_t mine = item.tile * kRows + orow;
-    if (item.cuts > 1 && item.cut == 0 && h == 0 && threadIdx.x == 0) {
-        SplitTile t;
-        t.first_token = req.first;
-        t.first_row = item.tile * kRows;
-        t.rows = rows;
-        t.slot = item.slot;
-        t.count = item.cuts;
-        a.split_tiles[item.order] = t;
-    }
-    if (mine >= rows)
-        return;
-    float m = -INFINITY;
+        const int32_t key0 = begin + wave * kKeys;
+        const int32_t tiles = end > key0 ? (end - key0 + kUnit - 1) / kUnit : 0;
+        Places places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0, kUnit, end, lane);
+        RawTile<kSub, S::kChunks> raw[2];
+        if (tiles > 0)
+            load_tile<D, kSub>(a, places, 0, lane, raw[0]);
+
+        Query<D, kPieces> query;
+        load_query<D, kPieces, kHalf>(a, (req.first + token) * a.q_st + head * a.q_sh, valid, g, query);
+        f32x4_t acc[D / 16];
 #pragma unroll
-    for (int w = 0; w < kAttWaves; ++w)
-        m = fmaxf(m, wave_m[w][orow]);
-    const float m_use = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[kDims];
+        for (int d = 0; d < D / 16; ++d)
+            acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        float m_run = -INFINITY, l_run = 0.f;
+
+        auto step = [&](int32_t i, const RawTile<kSub, S::kChunks>& now, RawTile<kSub, S::kChunks>& next) {
+            if (i + 1 < tiles) {
+                if ((i + 1) % kBatch == 0)
+                    places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0 + (i + 1) * kUnit, kUnit, end, lane);
+                load_tile<D, kSub>(a, places, i + 1, lane, next);
+            }
+            const int32_t key = key0 + i * kUnit;
+            bool all = key + kKeys - 1 <= min(first_pos, end - 1) && (a.window == 0 || key > last_pos - a.window);
 #pragma unroll
-    for (int i = 0; i < kDims; ++i)
-        o[i] = 0.f;
+            for (int t = 0; t < kSub; ++t)
+                all = all && now.place[t] >= 0;
+            if (all)
+                attend<D, kPieces, kSub, false>(now, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane,
+                                                acc, m_run, l_run);
+            else
+                attend<D, kPieces, kSub, true>(now, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane,
+                                               acc, m_run, l_run);
+        };
+        for (int32_t i = 0; i < tiles; i += 2) {
+            step(i, raw[0], raw[1]);
+            if (i + 1 < tiles)
+                step(i + 1, raw[1], raw[0]);
+        }
+        l_run = group4_sum(l_run);
+        asm volatile("" ::: "memory");
 #pragma unroll
-    for (int w = 0; w < kAttWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(wave_m[w][orow] - m_use);
-        l += f * wave_l[w][orow];
-        const float* from = reinterpret_cast<const float*>(turned[w] + orow * S::kOPitch) + part * kDims;
+        for (int d = 0; d < D / 16; ++d)
+            *reinterpret_cast<f32x4_t*>(turned[wave] + r * S::kOPitch + 64 * d + 16 * g) = acc[d];
+        if (g == 0) {
+            wave_m[wave][r] = m_run;
+            wave_l[wave][r] = l_run;
+        }
+        __syncthreads();
+
+        constexpr int kDims = D / 16;
+        const int32_t mine = w.tile * kRows + orow;
+        if (mine < rows) {
+            float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kDims; i += 4) {
-            const f32x4_t v = *reinterpret_cast<const f32x4_t*>(from + i);
+            for (int i = 0; i < kAttWaves; ++i)
+                m = fmaxf(m, wave_m[i][orow]);
+            const float m_use = m == -INFINITY ? 0.f : m;
+            float l = 0.f, o[kDims];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                o[i + j] += f * v[j];
+            for (int i = 0; i < kDims; ++i)
+                o[i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kAttWaves; ++i) {
+                const float f = __builtin_amdgcn_exp2f(wave_m[i][orow] - m_use);
+                l += f * wave_l[i][orow];
+                const float* from = reinterpret_cast<const float*>(turned[i] + orow * S::kOPitch) + part * kDims;
+#pragma unroll
+                for (int d = 0; d < kDims; d += 4) {
+                    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(from + d);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        o[d + j] += f * v[j];
+                }
+            }
+            if (whole) {
+                const int32_t otoken = mine / a.group, ohead = h * a.group + mine - otoken * a.group;
+                const int64_t t = req.first + otoken;
+                const RowEnd e = finish_row(a, ohead, m, l);
+                store_out<kHalf, kDims>(static_cast<uint16_t*>(a.out) + t * a.o_st + ohead * a.o_sh + part * kDims, o,
+                                        e.inv, a.o_wide);
+                if (part == 0)
+                    a.lse[t * a.lse_st + ohead] = e.lse;
+            } else {
+                // a worker's first slot holds the tile that came from the one before, its second the one that goes on
+                float* slot = a.partials + slot_of(a, h, worker, w.unit == 0) * slot_floats(D);
+#pragma unroll
+                for (int i = 0; i < kDims; i += 4)
+                    *reinterpret_cast<f32x4_t*>(slot + orow * D + part * kDims + i) =
+                        f32x4_t{o[i], o[i + 1], o[i + 2], o[i + 3]};
+                if (part == 0) {
+                    slot[kRows * D + orow] = m;
+                    slot[kRows * D + kRows + orow] = l;
+                }
+            }
+        }
+        left -= units;
+        if (!whole && w.unit == 0) {
+            cut.first_token = req.first;
+            cut.first_row = w.tile * kRows;
+            cut.rows = rows;
+            // the units behind this worker's, dealt out to the next ones
+            cut.count = 1 + (int32_t)((w.tiles.units - units + w.each - 1) / w.each);
+        }
+        if (left > 0) {
+            w.unit = 0;
+            if (++w.tile == w.tiles.count) {
+                w.tile = 0;
+                do
+                    w.tiles = tiles_of(a, ++w.b, kRows, kUnit);  // there is one: units are left
+                while (w.tiles.count == 0);
+            }
+            __syncthreads();  // the joined sums were read
         }
     }
-    if (item.cuts > 1) {
-        float* slot = a.partials + ((int64_t)h * a.slots_per_head + item.slot + item.cut) * slot_floats(D);
-#pragma unroll
-        for (int i = 0; i < kDims; i += 4)
-            *reinterpret_cast<f32x4_t*>(slot + orow * D + part * kDims + i) = f32x4_t{o[i], o[i + 1], o[i + 2], o[i + 3]};
-        if (part == 0) {
-            slot[kRows * D + orow] = m;
-            slot[kRows * D + kRows + orow] = l;
-        }
-        return;
-    }
-    const int32_t otoken = mine / a.group, ohead = h * a.group + mine - otoken * a.group;
-    const int64_t t = req.first + otoken;
-    const RowEnd e = finish_row(a, ohead, m, l);
-    store_out<kHalf, kDims>(static_cast<uint16_t*>(a.out) + t * a.o_st + ohead * a.o_sh + part * kDims, o, e.inv, a.o_wide);
-    if (part == 0)
-        a.lse[t * a.lse_st + ohead] = e.lse;
+    if (a.workers > 0 && h == 0 && threadIdx.x == 0)
+        a.cut_tiles[worker] = cut;
 }
 
-// Joins the cuts of one row: workgroup (cut tile and head, row of the tile).
+// Joins the cuts of one row: workgroup (worker in which the tile begins and head, row of the tile).
 template <int D, bool kHalf>
 __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
-    __shared__ float factor[kMostCuts];
+    __shared__ float factor[kMostWorkers];
     __shared__ float sums[kAttThreads * 4];
     constexpr int kLanes = D / 4, kGroups = kAttThreads / kLanes;
-    const int32_t order = (int32_t)(blockIdx.x / a.kv_heads), h = (int32_t)(blockIdx.x % a.kv_heads);
-    if (order >= *a.num_split_tiles)
-        return;
-    const SplitTile tile = a.split_tiles[order];
+    const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads), h = (int32_t)(blockIdx.x % a.kv_heads);
+    const CutTile tile = a.cut_tiles[worker];
     const int32_t r = (int32_t)blockIdx.y, row = tile.first_row + r;
-    if (row >= tile.rows)
+    if (tile.count == 0 || row >= tile.rows)
         return;
-    const float* slots = a.partials + ((int64_t)h * a.slots_per_head + tile.slot) * slot_floats(D);
+    // the cuts are this worker's second slot and the next ones' first
+    auto slot_at = [&](int32_t i) {
+        return a.partials + slot_of(a, h, worker + i, i == 0) * slot_floats(D);
+    };
     const int lane = threadIdx.x & 63;
     // every wave finds the reference and the sum for itself
     float m = -INFINITY;
     for (int32_t i = lane; i < tile.count; i += 64)
-        m = fmaxf(m, slots[(int64_t)i * slot_floats(D) + kRows * D + r]);
+        m = fmaxf(m, slot_at(i)[kRows * D + r]);
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1)
         m = fmaxf(m, __shfl_xor(m, d));
     const float m_use = m == -INFINITY ? 0.f : m;
     float l = 0.f;
     for (int32_t i = lane; i < tile.count; i += 64) {
-        const float* slot = slots + (int64_t)i * slot_floats(D) + kRows * D + r;
+        const float* slot = slot_at(i) + kRows * D + r;
         const float f = __builtin_amdgcn_exp2f(slot[0] - m_use);
         l += f * slot[kRows];
         if (threadIdx.x < 64)
@@ -812,7 +837,7 @@ __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int32_t i = group; i < tile.count; i += kGroups)
-        o += factor[i] * *reinterpret_cast<const f32x4_t*>(slots + (int64_t)i * slot_floats(D) + r * D + 4 * part);
+        o += factor[i] * *reinterpret_cast<const f32x4_t*>(slot_at(i) + r * D + 4 * part);
     *reinterpret_cast<f32x4_t*>(sums + 4 * threadIdx.x) = o;
     __syncthreads();
     if (group != 0)
@@ -829,45 +854,41 @@ __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
         a.lse[t * a.lse_st + head] = e.lse;
 }
 
-// How a call is cut, from what the host knows.
-struct Cutting {
-    int32_t split_items, slots_per_head, most_tiles;  // split_items 0: not at all
-    int64_t grid_tiles;                               // row tiles at most
-    int64_t tiles_at, count_at, bytes;                // parts of the workspace
+// How a call is dealt out, from what the host knows.
+struct Dealing {
+    int64_t tiles;    // row tiles at most
+    int32_t workers;  // per head; 0: a workgroup per tile
+    int64_t cut_tiles_at, bytes;  // of the workspace
 };
 
-Cutting cutting_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t reqs, int64_t max_seq) {
-    Cutting c = {};
+Dealing dealing_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t reqs, int64_t max_seq) {
+    Dealing d = {};
     // no request has more tiles than its rows' share, rounded up
-    c.grid_tiles = tokens * (heads / kv_heads) / kRows + reqs;
-    const int64_t target = kSplitTurns * cu_count() < kMostCuts - 76 ? kSplitTurns * cu_count() : kMostCuts - 76;
-    // keys that one turn of the waves takes, or more tiles than the chip holds several times over: nothing to cut
-    if (max_seq <= kChunkStep || c.grid_tiles * kv_heads > 8 * target)
-        return c;
-    c.split_items = (int32_t)(target / kv_heads > 0 ? target / kv_heads : 1);
-    // tiles that are cut have more than a chunk of keys: at most split_items + 1 chunks and one more each
-    c.slots_per_head = 2 * c.split_items + 8;
-    c.most_tiles = (int32_t)(c.grid_tiles < c.split_items + 4 ? c.grid_tiles : c.split_items + 4);
-    c.tiles_at = kv_heads * c.slots_per_head * (int64_t)slot_floats((int)dim) * 4;
-    c.count_at = c.tiles_at + c.most_tiles * (int64_t)sizeof(SplitTile);
-    c.bytes = (c.count_at + 4 + 255) / 256 * 256;
-    return c;
+    d.tiles = tokens * (heads / kv_heads) / kRows + reqs;
+    int64_t workers = kWorkersPerCu * cu_count() / kv_heads;
+    workers = workers < 1 ? 1 : workers > kMostWorkers ? kMostWorkers : workers;
+    // nothing to cut: no tile has more keys than a worker takes at least
+    if (max_seq <= kLeastUnits * unit_keys((int)dim))
+        return d;
+    d.workers = (int32_t)workers;
+    d.cut_tiles_at = 2 * workers * kv_heads * (int64_t)slot_floats((int)dim) * 4;
+    d.bytes = (d.cut_tiles_at + workers * (int64_t)sizeof(CutTile) + 255) / 256 * 256;
+    return d;
 }
 
 template <int D, int kPieces>
-void launch_attend(const Cutting& cut, hipStream_t st, const AttArgs& a) {
-    const unsigned grid = (unsigned)((cut.grid_tiles + a.split_items) * a.kv_heads);
+void launch_attend(const Dealing& d, hipStream_t st, const AttArgs& a) {
+    const unsigned grid = (unsigned)((a.workers > 0 ? a.workers : d.tiles) * a.kv_heads);
     hipLaunchKernelGGL((mxfp4_attend_kernel<D, kPieces>), dim3(grid), dim3(kAttThreads), 0, st, a);
-    if (a.split_items > 0) {
+    if (a.workers > 0) {
         const unsigned rows = a.query_start_loc || a.group >= kRows ? kRows : a.group;
-        hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3>), dim3((unsigned)(cut.most_tiles * a.kv_heads), rows),
-                           dim3(kAttThreads), 0, st, a);
+        hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3>), dim3(grid, rows), dim3(kAttThreads), 0, st, a);
     }
 }
 
 template <int D>
-void launch_attend(bool half, const Cutting& cut, hipStream_t st, const AttArgs& a) {
-    half ? launch_attend<D, 3>(cut, st, a) : launch_attend<D, 2>(cut, st, a);
+void launch_attend(bool half, const Dealing& d, hipStream_t st, const AttArgs& a) {
+    half ? launch_attend<D, 3>(d, st, a) : launch_attend<D, 2>(d, st, a);
 }
 
 }  // namespace
@@ -943,23 +964,21 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
     a.window = (int32_t)(window_size < 0x3fffffffLL ? window_size : 0);
     a.q_wide = aligned(q, 16) && ((q_stride_token | q_stride_head) & 7) == 0;
     a.o_wide = aligned(out, 8) && ((out_stride_token | out_stride_head) & 3) == 0;
-    Cutting cut = cutting_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_seq_len);
-    if (workspace && workspace_bytes >= cut.bytes && !aligned(workspace, 16))
+    const Dealing deal = dealing_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_seq_len);
+    const bool stream_mode = deal.workers > 0 && workspace && workspace_bytes >= deal.bytes;
+    if (stream_mode && !aligned(workspace, 16))
         return fail(FGV_E_MISALIGNED, "workspace must be 16-byte aligned");
-    if (!workspace || workspace_bytes < cut.bytes)
-        cut.split_items = 0;
-    a.split_items = cut.split_items;
-    a.slots_per_head = cut.slots_per_head;
-    a.partials = static_cast<float*>(workspace);
-    a.split_tiles = reinterpret_cast<SplitTile*>(static_cast<uint8_t*>(workspace) + cut.tiles_at);
-    a.num_split_tiles = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + cut.count_at);
-    if ((cut.grid_tiles + a.split_items) * num_kv_heads > 0x7fffffffLL)
+    if (!stream_mode && deal.tiles * num_kv_heads > 0x7fffffffLL)
         return fail(FGV_E_TOO_LARGE, "too many row tiles");
+    a.workers = stream_mode ? deal.workers : 0;
+    a.least_units = kLeastUnits;
+    a.partials = static_cast<float*>(workspace);
+    a.cut_tiles = reinterpret_cast<CutTile*>(static_cast<uint8_t*>(workspace) + deal.cut_tiles_at);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     switch (head_dim) {
-        case 64: launch_attend<64>(dtype == 1, cut, st, a); break;
-        case 128: launch_attend<128>(dtype == 1, cut, st, a); break;
-        default: launch_attend<256>(dtype == 1, cut, st, a); break;
+        case 64: launch_attend<64>(dtype == 1, deal, st, a); break;
+        case 128: launch_attend<128>(dtype == 1, deal, st, a); break;
+        default: launch_attend<256>(dtype == 1, deal, st, a); break;
     }
     return launch_status();
 }
@@ -971,6 +990,5 @@ extern "C" int64_t fgv_mxfp4_paged_attention_workspace_bytes(int64_t num_tokens,
     if (num_tokens <= 0 || num_reqs <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || num_heads > 65536 ||
         num_tokens * num_heads > 0x3fffffffLL || num_reqs > 0x3fffffffLL)
         return 0;
-    const fgv::Cutting cut = fgv::cutting_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_seq_len);
-    return cut.split_items > 0 ? cut.bytes : 0;
+    return fgv::dealing_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_seq_len).bytes;
 }
