@@ -46,7 +46,6 @@ typedef int v8i_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) short4_t lds_short4_t;
 
 constexpr int kAttThreads = 256;
@@ -60,7 +59,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // A row's reference is raised when a score exceeds it, and then to this much
 // above the score (base 2), so that most tiles rescale nothing.  P is at most 1.
-constexpr float kAhead = 8.0f;
+constexpr float kAhead = 4.0f;
 
 // 16-key subtiles that a wave takes at a time: two such tiles have to fit its registers.
 __host__ __device__ constexpr int key_subtiles(int dim) { return dim == 256 ? 2 : 4; }
@@ -81,8 +80,9 @@ struct AttArgs {
     int64_t o_st, o_sh;
     float* lse;
     int64_t lse_st;
-    float scale_f;    // softmax scale * log2(e) = scale_f * 2^scale_e, |scale_f| in [1, 2)
+    float scale_f;    // softmax scale * log2(e) = scale_sign * scale_f * 2^scale_e, scale_f in [1, 2), sign 1, 0 or -1
     int32_t scale_e;
+    float scale_sign;
     int32_t num_reqs, num_tokens, kv_heads, group, page, table_keys, window;
     int32_t q_wide, o_wide;
     // Stream mode (workers > 0): workers per head, at least how many units of keys
@@ -252,7 +252,7 @@ struct Shape {
     // at D = 64 two pieces share an instruction, the keys' codes standing there twice
     static constexpr int kSteps = D < 128 ? (kPieces + 1) / 2 : kChunks * kPieces;
     static constexpr int kVPitch = 2 * D + 32;  // bytes between tokens of the turned V: the reads' banks differ
-    static constexpr int kVBytes = 32 * kVPitch;
+    static constexpr int kVBytes = 16 * key_subtiles(D) * kVPitch;
     static constexpr int kOPitch = 4 * D + 16;
     static_assert(kRows * kOPitch <= kVBytes, "a wave's O fits its V buffer");
 };
@@ -338,7 +338,7 @@ __device__ __forceinline__ void load_query(const AttArgs& a, int64_t at, bool va
     // q 2^scale_e = x 2^e with the row's maximum in [128, 256): the softmax scale's power of two goes in here, so that
     // scores leave binary32's range only where scaled ones would.  -118 leaves room for the pieces' smaller scales.
     const int e = min(max((int)(most >> 23) - 127 - 7 + a.scale_e, -118), 127);
-    const float down = __uint_as_float((uint32_t)min(max(127 - e + a.scale_e, 1), 254) << 23);
+    const float down = __uint_as_float((uint32_t)min(max(127 - e + a.scale_e, 1), 254) << 23) * a.scale_sign;
 #pragma unroll
     for (int c = 0; c < kRuns; ++c)
 #pragma unroll
@@ -450,45 +450,91 @@ __device__ __forceinline__ v8i_t key_operand(uint4 k) {
     return v;
 }
 
-// What a lane knows of its row: the keys (lo, pos] are seen.
+// What a lane knows of its row: the `count` keys from `first` on are seen.
 struct Seen {
-    int32_t lo, pos;
-    __device__ bool operator()(int32_t key) const { return key > lo && key <= pos; }
+    int32_t first;
+    uint32_t count;
+    __device__ bool operator()(int32_t key) const { return (uint32_t)(key - first) < count; }
 };
+constexpr int32_t kNoKey = -0x40000000;  // seen by nobody: keys are below 2^30
 
-// Attends the tile's keys, from key0 on, for the wave's 16 rows.  kMask: some
-// of them are hidden from some of the rows.
-template <int D, int kPieces, int kSub, bool kMask>
-__device__ __forceinline__ void attend(const RawTile<kSub, Shape<D, kPieces>::kChunks>& raw, int32_t key0,
-                                       int32_t any_lo, int32_t any_pos, Seen seen, float scale_f,
-                                       const Query<D, kPieces>& query, uint8_t* turned, int lane, f32x4_t (&acc)[D / 16],
-                                       float& m_run, float& l_run) {
+// Attends the tile's keys, from key0 on, for the wave's 16 rows.  `plain`: all of
+// them are seen by all rows; otherwise some may be hidden, hold anything or be NaN.
+// (One body for both: with two, the compiler keeps two sets of sums.)
+//
+// `refill` loads the next tile into `raw` as soon as this one has left it, for
+// the matrix instruction and for LDS.
+template <int D, int kPieces, int kSub, class Refill>
+__device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>& raw, int32_t key0, bool plain,
+                                       Seen any, Seen seen, float scale_f, const Query<D, kPieces>& query,
+                                       uint8_t* turned, int lane, f32x4_t (&acc)[D / 16], float& m_run, float& l_run,
+                                       Refill refill) {
     using S = Shape<D, kPieces>;
     const int r = lane & 15, g = lane >> 4;
     f32x4_t s[kSub];
 #pragma unroll
-    for (int t = 0; t < kSub; ++t) {
+    for (int t = 0; t < kSub; ++t)
         s[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < S::kSteps; ++i) {
+    for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+        for (int t = 0; t < kSub; ++t) {
             const int c = i % S::kChunks;
             s[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(key_operand(raw.k[t][c]), query.q[i], s[t], 4, 0, 0,
                                                                     (int)raw.ks[t][c], 0, query.scale[i]);
         }
+
+    uint64_t nan[kSub][S::kChunks];  // which value blocks are NaN, bit by lane
+    int32_t key_of[kSub];            // each subtile's first key
+    bool any_nan = false;
+    if (!plain) {
+#pragma unroll
+        for (int t = 0; t < kSub; ++t) {
+            key_of[t] = raw.place[t] >= 0 ? key0 + 16 * t : kNoKey;
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c) {
+                // a token that no row sees may hold anything; a NaN that some rows see is dealt with at the end
+                const uint32_t byte = any(key_of[t] + r) ? raw.vs[t][c] : 0;
+                nan[t][c] = __ballot(byte == 255u);
+                any_nan |= nan[t][c] != 0;
+                raw.vs[t][c] = byte == 255u ? 0 : byte;
+            }
+        }
     }
-    float p[4 * kSub];
+
+    // V into LDS while the scores are on their way
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < kSub; ++t)
+#pragma unroll
+        for (int c = 0; c < S::kChunks; ++c) {
+            const float scale = __uint_as_float(raw.vs[t][c] << 23);
+            if (D >= 128 || g < 2) {
+                uint4* to = reinterpret_cast<uint4*>(turned + (16 * t + r) * S::kVPitch + 256 * c + 64 * g);
+                to[0] = values_of(raw.v[t][c].x, scale);
+                to[1] = values_of(raw.v[t][c].y, scale);
+                to[2] = values_of(raw.v[t][c].z, scale);
+                to[3] = values_of(raw.v[t][c].w, scale);
+            }
+            // (the scheduler would convert the whole tile first, into registers that there are not)
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    asm volatile("" ::: "memory");
+
+    if (!plain) {
+#pragma unroll
+        for (int t = 0; t < kSub; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s[t][i] = seen(key_of[t] + 4 * g + i) ? s[t][i] : -INFINITY;
+    }
     float most = -INFINITY;
 #pragma unroll
     for (int t = 0; t < kSub; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v = s[t][i] * scale_f;
-            if constexpr (kMask)
-                v = raw.place[t] >= 0 && seen(key0 + 16 * t + 4 * g + i) ? v : -INFINITY;
-            p[4 * t + i] = v;
-            most = fmaxf(most, v);
-        }
-    most = group4_max(most);
+        for (int i = 0; i < 4; ++i)
+            most = fmaxf(most, s[t][i]);
+    most = group4_max(most) * scale_f;
     if (__any(most > m_run)) {
         const float m_new = most > m_run ? most + kAhead : m_run;
         const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
@@ -498,41 +544,25 @@ __device__ __forceinline__ void attend(const RawTile<kSub, Shape<D, kPieces>::kC
             acc[d] *= alpha;
         m_run = m_new;
     }
+    // (here, not earlier: behind the branch above the products above have left K's registers)
+    refill();
     const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    float p[4 * kSub];
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4 * kSub; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(p[i] - m_use);
-        sum += p[i];
-    }
+    for (int t = 0; t < kSub; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            p[4 * t + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], scale_f, -m_use));
+            sum += p[4 * t + i];
+        }
     l_run += sum;  // this lane's keys; the row's four lanes are added up at the end
 
+    // lane j of group g reads 4 dims of row 4g + j / 4 and gets dim j of rows 4g..4g+3
+    const uint8_t* from = turned + (4 * g + (r >> 2)) * S::kVPitch + 8 * (r & 3);
+    constexpr int kAtOnce = 4;  // 16-dim tiles whose reads are in flight together
 #pragma unroll
     for (int half = 0; half < kSub / 2; ++half) {
-        asm volatile("" ::: "memory");
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int t = 2 * half + u;
-#pragma unroll
-            for (int c = 0; c < S::kChunks; ++c) {
-                uint32_t byte = raw.vs[t][c];
-                if constexpr (kMask) {
-                    // a token that no row sees may hold anything; a NaN that some rows see is dealt with below
-                    const int32_t key = key0 + 16 * t + r;
-                    if (byte == 255u || raw.place[t] < 0 || key <= any_lo || key > any_pos)
-                        byte = 0;
-                }
-                const float scale = __uint_as_float(byte << 23);
-                if (D >= 128 || g < 2) {
-                    uint4* to = reinterpret_cast<uint4*>(turned + (16 * u + r) * S::kVPitch + 256 * c + 64 * g);
-                    to[0] = values_of(raw.v[t][c].x, scale);
-                    to[1] = values_of(raw.v[t][c].y, scale);
-                    to[2] = values_of(raw.v[t][c].z, scale);
-                    to[3] = values_of(raw.v[t][c].w, scale);
-                }
-            }
-        }
-        asm volatile("" ::: "memory");
         // k = 8g + i of this product is key 4g + i, or 16 + 4g + i - 4
         const float* ph = p + 8 * half;
         const uint4 hi = make_uint4(pack_bf16x2(ph[0], ph[1]), pack_bf16x2(ph[2], ph[3]), pack_bf16x2(ph[4], ph[5]),
@@ -541,41 +571,41 @@ __device__ __forceinline__ void attend(const RawTile<kSub, Shape<D, kPieces>::kC
                                     pack_bf16x2(ph[2] - bf16_lo(hi.y), ph[3] - bf16_hi(hi.y)),
                                     pack_bf16x2(ph[4] - bf16_lo(hi.z), ph[5] - bf16_hi(hi.z)),
                                     pack_bf16x2(ph[6] - bf16_lo(hi.w), ph[7] - bf16_hi(hi.w)));
-        // lane j of group g reads 4 dims of row 4g + j / 4 and gets dim j of rows 4g..4g+3
-        const uint8_t* from = turned + (4 * g + (r >> 2)) * S::kVPitch + 8 * (r & 3);
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-            const uint2 x = read_turned(from + 32 * d), y = read_turned(from + 16 * S::kVPitch + 32 * d);
-            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, make_uint4(x.x, x.y, y.x, y.y));
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, hi), acc[d], 0, 0, 0);
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, lo), acc[d], 0, 0, 0);
+        for (int d0 = 0; d0 < D / 16; d0 += kAtOnce) {
+            bf16x8_t v[kAtOnce];
+#pragma unroll
+            for (int d = 0; d < kAtOnce; ++d) {
+                const uint8_t* at = from + 32 * half * S::kVPitch + 32 * (d0 + d);
+                const uint2 x = read_turned(at), y = read_turned(at + 16 * S::kVPitch);
+                v[d] = __builtin_bit_cast(bf16x8_t, make_uint4(x.x, x.y, y.x, y.y));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < kAtOnce; ++d)
+                acc[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[d], __builtin_bit_cast(bf16x8_t, hi), acc[d0 + d], 0,
+                                                                      0, 0);
+#pragma unroll
+            for (int d = 0; d < kAtOnce; ++d)
+                acc[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[d], __builtin_bit_cast(bf16x8_t, lo), acc[d0 + d], 0,
+                                                                      0, 0);
         }
     }
 
-    if constexpr (kMask) {
-        // value blocks that are NaN, for the rows that see them (rare: the loop is entered by a vote)
-        bool nan = false;
+    // value blocks that are NaN, for the rows that see them
+    if (any_nan) {
 #pragma unroll
         for (int t = 0; t < kSub; ++t)
 #pragma unroll
             for (int c = 0; c < S::kChunks; ++c)
-                nan |= raw.vs[t][c] == 255u;
-        if (__any(nan)) {
 #pragma unroll
-            for (int t = 0; t < kSub; ++t)
-#pragma unroll
-                for (int c = 0; c < S::kChunks; ++c)
-#pragma unroll
-                    for (int b = 0; b < (D < 128 ? 2 : 4); ++b) {
-                        bool hit = false;
-                        for (int token = 0; token < 16; ++token)
-                            hit |= __builtin_amdgcn_readlane(raw.vs[t][c], 16 * b + token) == 255u && raw.place[t] >= 0 &&
-                                   seen(key0 + 16 * t + token);
-                        const float add = hit ? NAN : 0.f;
-                        acc[8 * c + 2 * b] += add;
-                        acc[8 * c + 2 * b + 1] += add;
-                    }
-        }
+                for (int b = 0; b < (D < 128 ? 2 : 4); ++b) {
+                    float add = 0.f;
+                    for (uint32_t bits = (uint32_t)(nan[t][c] >> (16 * b)) & 0xffffu; bits; bits &= bits - 1)
+                        add = seen(key_of[t] + __builtin_ctz(bits)) ? NAN : add;
+                    acc[8 * c + 2 * b] += add;
+                    acc[8 * c + 2 * b + 1] += add;
+                }
     }
 }
 
@@ -645,7 +675,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a)
     constexpr int kKeys = 16 * kSub, kUnit = unit_keys(D), kBatch = 64 / kSub;
     __shared__ __align__(16) uint8_t turned[kAttWaves][S::kVBytes];
     __shared__ float wave_m[kAttWaves][kRows], wave_l[kAttWaves][kRows];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = (int)blockIdx.x % a.kv_heads;
     const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads);
     const int r = lane & 15, g = lane >> 4;
@@ -666,10 +696,12 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a)
         const int32_t pos0 = req.len - req.count;
         const int32_t last_row = min(w.tile * kRows + kRows, rows) - 1;
         const int32_t first_pos = pos0 + w.tile * kRows / a.group, last_pos = pos0 + last_row / a.group;
-        Seen seen;
-        seen.pos = valid ? pos0 + token : -1;
-        seen.lo = a.window > 0 ? seen.pos - a.window : -1;
-        const int32_t any_lo = a.window > 0 ? first_pos - a.window : -1;
+        // keys seen by a row, and by any of them
+        Seen seen, any;
+        seen.first = a.window > 0 ? pos0 + token - a.window + 1 : 0;
+        seen.count = valid ? (uint32_t)max(pos0 + token - seen.first + 1, 0) : 0;
+        any.first = a.window > 0 ? first_pos - a.window + 1 : 0;
+        any.count = (uint32_t)max(last_pos - any.first + 1, 0);
         int32_t begin, end;
         key_range(a, req, begin, end);
         if (!whole) {
@@ -677,14 +709,14 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a)
             end = units <= (end - begin) / kUnit ? begin + units * kUnit : end;
         }
         end = min(end, last_pos + 1);
-        begin = max(begin, max(any_lo + 1, 0) & ~(kTileKeys - 1));
+        begin = max(begin, max(any.first, 0) & ~(kTileKeys - 1));
 
         const int32_t key0 = begin + wave * kKeys;
         const int32_t tiles = end > key0 ? (end - key0 + kUnit - 1) / kUnit : 0;
         Places places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0, kUnit, end, lane);
-        RawTile<kSub, S::kChunks> raw[2];
+        RawTile<kSub, S::kChunks> raw;
         if (tiles > 0)
-            load_tile<D, kSub>(a, places, 0, lane, raw[0]);
+            load_tile<D, kSub>(a, places, 0, lane, raw);
 
         Query<D, kPieces> query;
         load_query<D, kPieces, kHalf>(a, (req.first + token) * a.q_st + head * a.q_sh, valid, g, query);
@@ -694,28 +726,21 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a)
             acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         float m_run = -INFINITY, l_run = 0.f;
 
-        auto step = [&](int32_t i, const RawTile<kSub, S::kChunks>& now, RawTile<kSub, S::kChunks>& next) {
-            if (i + 1 < tiles) {
-                if ((i + 1) % kBatch == 0)
-                    places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0 + (i + 1) * kUnit, kUnit, end, lane);
-                load_tile<D, kSub>(a, places, i + 1, lane, next);
-            }
+        for (int32_t i = 0; i < tiles; ++i) {
+            auto refill = [&]() {
+                if (i + 1 < tiles) {
+                    if ((i + 1) % kBatch == 0)
+                        places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0 + (i + 1) * kUnit, kUnit, end, lane);
+                    load_tile<D, kSub>(a, places, i + 1, lane, raw);
+                }
+            };
             const int32_t key = key0 + i * kUnit;
-            bool all = key + kKeys - 1 <= min(first_pos, end - 1) && (a.window == 0 || key > last_pos - a.window);
+            bool plain = (key + kKeys - 1 <= min(first_pos, end - 1)) & ((a.window == 0) | (key > last_pos - a.window));
 #pragma unroll
             for (int t = 0; t < kSub; ++t)
-                all = all && now.place[t] >= 0;
-            if (all)
-                attend<D, kPieces, kSub, false>(now, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane,
-                                                acc, m_run, l_run);
-            else
-                attend<D, kPieces, kSub, true>(now, key, any_lo, last_pos, seen, a.scale_f, query, turned[wave], lane,
-                                               acc, m_run, l_run);
-        };
-        for (int32_t i = 0; i < tiles; i += 2) {
-            step(i, raw[0], raw[1]);
-            if (i + 1 < tiles)
-                step(i + 1, raw[1], raw[0]);
+                plain = plain & (raw.place[t] >= 0);
+            attend<D, kPieces, kSub>(raw, key, plain, any, seen, a.scale_f, query, turned[wave], lane, acc, m_run, l_run,
+                                     refill);
         }
         l_run = group4_sum(l_run);
         asm volatile("" ::: "memory");
@@ -953,7 +978,8 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
     int e = 0;
     frexp(scale_log2, &e);
     a.scale_e = scale_log2 == 0.0 ? 0 : e - 1 < -100 ? -100 : e - 1;
-    a.scale_f = (float)ldexp(scale_log2, -a.scale_e);
+    a.scale_f = scale_log2 == 0.0 ? 1.0f : (float)ldexp(fabs(scale_log2), -a.scale_e);
+    a.scale_sign = scale_log2 > 0.0 ? 1.0f : scale_log2 < 0.0 ? -1.0f : 0.0f;
     a.num_reqs = (int32_t)num_reqs;
     a.num_tokens = (int32_t)num_tokens;
     a.kv_heads = (int32_t)num_kv_heads;

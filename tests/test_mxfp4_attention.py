@@ -15,11 +15,11 @@ What the kernels may be off, row by row (``bounds``), counted before their first
 * scores are scaled and exp2 taken in 32 bits: 2^-20 (1 + |s|) together covers the
   scaling, the subtraction and two ulp of the exponential;
 * P enters as two bf16 pieces (2^-16);
-* sums in 32 bits: a step of 2^-23 per 32 keys and per joined part;
 * P below 2^-126 is nothing in 32 bits (the first run showed that this had been left out: a dim
   where all keys but such ones hold zeros came out as 0 instead of 4e-39).  P is taken under a
-  reference of at most 2^8 times the row's largest, so that is 2^-118 |v| a key, as a score
+  reference of at most 2^4 times the row's largest, so that is 2^-122 |v| a key, as a score
   and again as a sum that is joined;
+* sums in 32 bits: a step of 2^-23 per 32 keys and per joined part;
 * the output is rounded once (eps / 2 of the type, or half its least subnormal).
 """
 import math
@@ -148,7 +148,7 @@ def reference(q, cache, table, lens, start, scale, window=None, sink=None):
             half = torch.finfo(q.dtype).eps / 2
             ob = weight * (2.0 ** -16 + 2.5 * d + steps)[:, None] * (1 + half)
             ob = ob + half * o.abs() + torch.finfo(q.dtype).smallest_normal * half
-            ob = ob + 2.0 ** -117 * torch.where(nan, 0.0, vh).abs().sum(0)
+            ob = ob + 2.0 ** -121 * torch.where(nan, 0.0, vh).abs().sum(0)
             out[t0:t1, h] = torch.where(some[:, None], o, 0.0)
             lse[t0:t1, h] = torch.where(some, l, torch.inf)
             obound[t0:t1, h] = ob
