@@ -53,16 +53,20 @@ constexpr int kAttWaves = kAttThreads / 64;
 constexpr int kTileKeys = 64;  // keys of every tile begin at a multiple of this
 constexpr int kRows = 16;      // query rows of a workgroup
 constexpr int kMostWorkers = 1024;  // per head
-constexpr int kWorkersPerCu = 2;    // workgroups that a CU holds at a time
-constexpr int kLeastUnits = 4;      // turns of the waves that a worker takes at least
+constexpr int kLeastUnits = 8;      // turns of the waves that a worker takes at least
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // A row's reference is raised when a score exceeds it, and then to this much
 // above the score (base 2), so that most tiles rescale nothing.  P is at most 1.
 constexpr float kAhead = 4.0f;
+// References farther from 0 are rounded by more than the one below which a score that is not
+// rounded may lie: there both are.
+constexpr float kFar = 1 << 20;
 
 // 16-key subtiles that a wave takes at a time: two such tiles have to fit its registers.
-__host__ __device__ constexpr int key_subtiles(int dim) { return dim == 256 ? 2 : 4; }
+__host__ __device__ constexpr int key_subtiles(int) { return 2; }
+// Workgroups that a CU holds at a time.
+__host__ __device__ constexpr int groups_per_cu(int dim) { return dim == 256 ? 2 : 3; }
 // Keys of a turn of the workgroup's waves, in which keys are dealt out.
 __host__ __device__ constexpr int unit_keys(int dim) { return kAttWaves * 16 * key_subtiles(dim); }
 
@@ -552,10 +556,20 @@ __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>
 #pragma unroll
     for (int t = 0; t < kSub; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            p[4 * t + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], scale_f, -m_use));
-            sum += p[4 * t + i];
-        }
+        for (int i = 0; i < 4; ++i)
+            p[4 * t + i] = __builtin_fmaf(s[t][i], scale_f, -m_use);
+    if (__any(fabsf(m_use) > kFar)) {
+#pragma unroll
+        for (int t = 0; t < kSub; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                p[4 * t + i] = s[t][i] * scale_f - m_use;
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * kSub; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(p[i]);
+        sum += p[i];
+    }
     l_run += sum;  // this lane's keys; the row's four lanes are added up at the end
 
     // lane j of group g reads 4 dims of row 4g + j / 4 and gets dim j of rows 4g..4g+3
@@ -668,7 +682,7 @@ __device__ __forceinline__ int64_t slot_of(const AttArgs& a, int32_t h, int32_t 
 // A worker's tiles of 16 rows: four waves take a tile of keys each in turn,
 // loaded one tile ahead, and their sums meet in LDS.
 template <int D, int kPieces>
-__global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_kernel(AttArgs a) {
+__global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_kernel(AttArgs a) {
     using S = Shape<D, kPieces>;
     constexpr bool kHalf = kPieces == 3;
     constexpr int kSub = key_subtiles(D);
@@ -890,7 +904,7 @@ Dealing dealing_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim,
     Dealing d = {};
     // no request has more tiles than its rows' share, rounded up
     d.tiles = tokens * (heads / kv_heads) / kRows + reqs;
-    int64_t workers = kWorkersPerCu * cu_count() / kv_heads;
+    int64_t workers = groups_per_cu((int)dim) * cu_count() / kv_heads;
     workers = workers < 1 ? 1 : workers > kMostWorkers ? kMostWorkers : workers;
     // nothing to cut: no tile has more keys than a worker takes at least
     if (max_seq <= kLeastUnits * unit_keys((int)dim))
