@@ -53,7 +53,13 @@ constexpr int kAttWaves = kAttThreads / 64;
 constexpr int kTileKeys = 64;  // keys of every tile begin at a multiple of this
 constexpr int kRows = 16;      // query rows of a workgroup
 constexpr int kMostWorkers = 1024;  // per head
-constexpr int kLeastUnits = 8;      // turns of the waves that a worker takes at least
+// Work is dealt out in units, a turn of the workgroup's waves over 128 keys, about 1 us.
+// Beginning and ending a tile (block table, query, joining the waves) costs as
+// much as this many more, so that a worker of many short tiles gets fewer units.
+constexpr int kTileCost = 4;
+constexpr int kLeastCost = kTileCost + 2;  // what a worker takes at least
+// Tiles of no more units than this are not cut: joining cuts takes a launch, 5 us.
+constexpr int kWholeUnits = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // A row's reference is raised when a score exceeds it, and then to this much
@@ -66,7 +72,7 @@ constexpr float kFar = 1 << 20;
 // 16-key subtiles that a wave takes at a time: two such tiles have to fit its registers.
 __host__ __device__ constexpr int key_subtiles(int) { return 2; }
 // Workgroups that a CU holds at a time.
-__host__ __device__ constexpr int groups_per_cu(int dim) { return dim == 256 ? 2 : 3; }
+__host__ __device__ constexpr int groups_per_cu(int dim) { return dim == 64 ? 3 : 2; }
 // Keys of a turn of the workgroup's waves, in which keys are dealt out.
 __host__ __device__ constexpr int unit_keys(int dim) { return kAttWaves * 16 * key_subtiles(dim); }
 
@@ -89,9 +95,8 @@ struct AttArgs {
     float scale_sign;
     int32_t num_reqs, num_tokens, kv_heads, group, page, table_keys, window;
     int32_t q_wide, o_wide;
-    // Stream mode (workers > 0): workers per head, at least how many units of keys
-    // each takes, and the workspace's parts.
-    int32_t workers, least_units;
+    // Stream mode (workers > 0): workers per head, and the workspace's parts.
+    int32_t workers;
     float* partials;
     struct CutTile* cut_tiles;
 };
@@ -127,10 +132,11 @@ __device__ __forceinline__ void key_range(const AttArgs& a, const Request& r, in
     begin = a.window > 0 ? max(r.len - r.count - a.window + 1, 0) & ~(kTileKeys - 1) : 0;
 }
 
-// A request and its tiles of kRows rows, `units` units of keys each.
+// A request and its tiles of rows, `units` units of keys each, dealt out as `cost`.
 struct Tiles {
     Request req;
     int32_t count, units;
+    __device__ int32_t cost(const AttArgs& a) const { return a.workers > 0 ? kTileCost + units : 1; }
 };
 
 __device__ __forceinline__ Tiles tiles_of(const AttArgs& a, int32_t b, int32_t rows_per_tile, int32_t unit_keys) {
@@ -146,54 +152,47 @@ __device__ __forceinline__ Tiles tiles_of(const AttArgs& a, int32_t b, int32_t r
     return t;
 }
 
-// Where a workgroup begins: unit `unit` of tile `tile` of request b; it takes
-// `take` units, through tiles and requests in order.  `each` is what workers take.
+// Where a workgroup begins: `at` into the cost of tile `tile` of request b; it takes
+// `take` of cost, through tiles and requests in order.  `each` is what workers take.
 struct Start {
     Tiles tiles;
-    int32_t b, tile, unit;
-    int64_t take, each;
+    int32_t b, tile, at;
+    int32_t take, each;
 };
 
 // Sum of v over the lanes up to this one.
-template <int kCtrl, int kRowMask>
-__device__ __forceinline__ uint64_t dpp_moved(uint64_t v) {
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)v, kCtrl, kRowMask, 0xF, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(v >> 32), kCtrl, kRowMask, 0xF, false);
-    return (uint64_t)hi << 32 | lo;
-}
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
-    v += dpp_moved<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
-    v += dpp_moved<0x112, 0xF>(v);
-    v += dpp_moved<0x114, 0xF>(v);
-    v += dpp_moved<0x118, 0xF>(v);
-    v += dpp_moved<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
-    v += dpp_moved<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0u, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
     return v;
 }
 
 // The start of worker `index`; false if there is nothing for it.  Every workgroup
 // works out the plan for itself: lengths are known on the device only, and a
-// launch to do it would cost more than the scan.  In stream mode the units of
-// all tiles, one after the other, are dealt out evenly, so that workgroups have
+// launch to do it would cost more than the scan.  In stream mode the cost of
+// all tiles, one after the other, is dealt out evenly, so that workgroups have
 // the same to do whatever the lengths are; a tile that is longer than the
 // rest of its worker's share goes on with the next.  Otherwise a worker is a tile.
-__device__ __forceinline__ bool find_start(const AttArgs& a, int32_t index, int32_t rows_per_tile, int32_t unit_keys,
+// (The host sees to it that the cost fits 31 bits.)
+__device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int32_t rows_per_tile, int32_t unit_keys,
                                            Start& start) {
-    __shared__ uint64_t part[kAttWaves];
+    __shared__ uint32_t part[kAttWaves];
     __shared__ int32_t found[8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0)
-        found[0] = -1;
     Tiles mine = {};
-    uint64_t at = 0, n = 0;  // units in front of this thread's request of the turn, and its own
-    auto scan_turn = [&](int32_t base, uint64_t& before) {
+    uint32_t at = 0, n = 0;  // cost in front of this thread's request of the turn, and its own
+    auto scan_turn = [&](int32_t base, uint32_t& before) {
         const int32_t b = base + (int32_t)threadIdx.x;
         n = 0;
         if (b < a.num_reqs) {
             mine = tiles_of(a, b, rows_per_tile, unit_keys);
-            n = (uint64_t)mine.count * mine.units;
+            n = (uint32_t)mine.count * mine.cost(a);
         }
-        const uint64_t s = wave_scan(n);
+        const uint32_t s = wave_scan(n);
         if (lane == 63)
             part[wave] = s;
         __syncthreads();
@@ -203,29 +202,31 @@ __device__ __forceinline__ bool find_start(const AttArgs& a, int32_t index, int3
             at += w < wave ? part[w] : 0;
             before += part[w];
         }
-        __syncthreads();
     };
-    uint64_t total = 0;
-    for (int32_t base = 0; base < a.num_reqs; base += kAttThreads)
+    uint32_t total = 0;
+    for (int32_t base = 0; base < a.num_reqs; base += kAttThreads) {
+        if (base > 0)
+            __syncthreads();  // the last turn's sums were read
         scan_turn(base, total);
-    uint64_t each = 1;
-    if (a.workers > 0) {
-        each = (total + a.workers - 1) / a.workers;
-        each = each < (uint64_t)a.least_units ? a.least_units : each;
     }
-    const uint64_t first = each * index;
+    uint32_t each = 1;
+    if (a.workers > 0)
+        each = max((total + a.workers - 1) / a.workers, (uint32_t)kLeastCost);
+    const uint64_t first = (uint64_t)each * index;
     if (first >= total)
         return false;
-    uint64_t before = 0;
+    uint32_t before = 0;
     for (int32_t base = 0; base < a.num_reqs; base += kAttThreads) {
-        if (a.num_reqs > kAttThreads)
+        if (a.num_reqs > kAttThreads) {
+            __syncthreads();
             scan_turn(base, before);
+        }
         if (first >= at && first - at < n) {
-            const uint64_t in = first - at;
-            const int32_t tile = mine.units == 1 ? (int32_t)in : (int32_t)(in / mine.units);
+            const uint32_t in = (uint32_t)first - at, cost = mine.cost(a);
+            const uint32_t tile = in / cost;
             found[0] = base + (int32_t)threadIdx.x;
-            found[1] = tile;
-            found[2] = (int32_t)(in - (uint64_t)tile * mine.units);
+            found[1] = (int32_t)tile;
+            found[2] = (int32_t)(in - tile * cost);
             found[3] = mine.req.first;
             found[4] = mine.req.count;
             found[5] = mine.req.len;
@@ -236,14 +237,14 @@ __device__ __forceinline__ bool find_start(const AttArgs& a, int32_t index, int3
     __syncthreads();
     start.b = __builtin_amdgcn_readfirstlane(found[0]);
     start.tile = __builtin_amdgcn_readfirstlane(found[1]);
-    start.unit = __builtin_amdgcn_readfirstlane(found[2]);
+    start.at = __builtin_amdgcn_readfirstlane(found[2]);
     start.tiles.req.first = __builtin_amdgcn_readfirstlane(found[3]);
     start.tiles.req.count = __builtin_amdgcn_readfirstlane(found[4]);
     start.tiles.req.len = __builtin_amdgcn_readfirstlane(found[5]);
     start.tiles.count = __builtin_amdgcn_readfirstlane(found[6]);
     start.tiles.units = __builtin_amdgcn_readfirstlane(found[7]);
-    start.each = (int64_t)each;
-    start.take = (int64_t)(total - first < each ? total - first : each);
+    start.each = (int32_t)each;
+    start.take = (int32_t)(total - first < each ? total - first : each);
     return true;
 }
 
@@ -268,11 +269,10 @@ struct Query {
     int scale[Shape<D, kPieces>::kSteps];
 };
 
-// N consecutive 16-bit values as floats.
-template <bool kHalf, int N>
-__device__ __forceinline__ void load_values(const void* base, int64_t at, bool wide, bool valid, float* x) {
+// N consecutive 16-bit values, two to a word; 0 where not valid.
+template <int N>
+__device__ __forceinline__ void load_words(const void* base, int64_t at, bool wide, bool valid, uint32_t (&w)[N / 2]) {
     const uint16_t* s = static_cast<const uint16_t*>(base) + at;
-    uint32_t w[N / 2];
     if (!valid) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i)
@@ -288,6 +288,10 @@ __device__ __forceinline__ void load_values(const void* base, int64_t at, bool w
         for (int i = 0; i < N / 2; ++i)
             w[i] = (uint32_t)s[2 * i] | (uint32_t)s[2 * i + 1] << 16;
     }
+}
+
+template <bool kHalf, int N>
+__device__ __forceinline__ void to_floats(const uint32_t (&w)[N / 2], float (&x)[N]) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
         if constexpr (kHalf) {
@@ -322,15 +326,28 @@ __device__ __forceinline__ uint32_t take_piece(float* x) {
     return w;
 }
 
-// Row r of lane (r, g) at element `at` of q.
+// A lane's part of a query row: dims 16g..16g+15 of each 64.
+template <int D>
+struct RawQuery {
+    uint32_t w[D / 64][8];
+};
+
+template <int D>
+__device__ __forceinline__ void load_query(const AttArgs& a, int64_t at, bool valid, int g, RawQuery<D>& raw) {
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+        load_words<16>(a.q, at + 64 * c + 16 * g, a.q_wide, valid, raw.w[c]);
+}
+
+// Row r of lane (r, g) as the matrix instruction's operand.
 template <int D, int kPieces, bool kHalf>
-__device__ __forceinline__ void load_query(const AttArgs& a, int64_t at, bool valid, int g, Query<D, kPieces>& out) {
+__device__ __forceinline__ void split_query(const AttArgs& a, const RawQuery<D>& raw, Query<D, kPieces>& out, int g) {
     constexpr int kRuns = D / 64;  // runs of 16 dims per lane
     float x[kRuns][16];
     uint32_t most = 0;
 #pragma unroll
     for (int c = 0; c < kRuns; ++c) {
-        load_values<kHalf, 16>(a.q, at + 64 * c + 16 * g, a.q_wide, valid, x[c]);
+        to_floats<kHalf, 16>(raw.w[c], x[c]);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             most = max(most, __float_as_uint(x[c][i]) & 0x7fffffffu);
@@ -687,20 +704,27 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
     constexpr bool kHalf = kPieces == 3;
     constexpr int kSub = key_subtiles(D);
     constexpr int kKeys = 16 * kSub, kUnit = unit_keys(D), kBatch = 64 / kSub;
+    constexpr int kDepth = D == 256 ? 1 : 2;  // tiles in registers
     __shared__ __align__(16) uint8_t turned[kAttWaves][S::kVBytes];
     __shared__ float wave_m[kAttWaves][kRows], wave_l[kAttWaves][kRows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = (int)blockIdx.x % a.kv_heads;
     const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads);
     const int r = lane & 15, g = lane >> 4;
+    const int32_t tile_cost = a.workers > 0 ? kTileCost : 0;
     const int orow = threadIdx.x >> 4, part = threadIdx.x & 15;  // of the end: 16 threads per row
     Start w;
     const bool busy = find_start(a, worker, kRows, kUnit, w);
     CutTile cut = {0, 0, 0, 0};  // the tile that begins here and goes on with the next workers
-    int64_t left = busy ? w.take : 0;
+    int32_t left = busy ? w.take : 0;
     while (left > 0) {
         const Request req = w.tiles.req;
-        const int32_t units = (int32_t)min(left, (int64_t)(w.tiles.units - w.unit));
+        // of the tile's cost kTileCost stands before its first unit
+        const int32_t cost = min(left, w.tiles.cost(a) - w.at);
+        const int32_t unit = max(w.at - tile_cost, 0);
+        const int32_t units = a.workers > 0 ? max(w.at + cost - tile_cost, 0) - unit : 1;
+        if (units == 0)
+            break;  // the tile begins with the next worker
         const bool whole = units == w.tiles.units;
         const int32_t rows = req.count * a.group;  // fits: count * group rows are rows of q
         const int32_t row = w.tile * kRows + r;
@@ -719,7 +743,7 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
         int32_t begin, end;
         key_range(a, req, begin, end);
         if (!whole) {
-            begin += w.unit * kUnit;  // below the request's end
+            begin += unit * kUnit;  // below the request's end
             end = units <= (end - begin) / kUnit ? begin + units * kUnit : end;
         }
         end = min(end, last_pos + 1);
@@ -727,34 +751,47 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
 
         const int32_t key0 = begin + wave * kKeys;
         const int32_t tiles = end > key0 ? (end - key0 + kUnit - 1) / kUnit : 0;
+        // in the order in which they are waited for: the query's values are split while the first tiles come
+        RawQuery<D> raw_query;
+        load_query<D>(a, (req.first + token) * a.q_st + head * a.q_sh, valid, g, raw_query);
         Places places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0, kUnit, end, lane);
-        RawTile<kSub, S::kChunks> raw;
-        if (tiles > 0)
-            load_tile<D, kSub>(a, places, 0, lane, raw);
+        // kDepth tiles are on their way: a tile's registers take another as soon as they are free
+        RawTile<kSub, S::kChunks> raw[kDepth];
+#pragma unroll
+        for (int i = 0; i < kDepth; ++i)
+            if (i < tiles)
+                load_tile<D, kSub>(a, places, i, lane, raw[i]);
 
         Query<D, kPieces> query;
-        load_query<D, kPieces, kHalf>(a, (req.first + token) * a.q_st + head * a.q_sh, valid, g, query);
+        split_query<D, kPieces, kHalf>(a, raw_query, query, g);
         f32x4_t acc[D / 16];
 #pragma unroll
         for (int d = 0; d < D / 16; ++d)
             acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         float m_run = -INFINITY, l_run = 0.f;
 
-        for (int32_t i = 0; i < tiles; ++i) {
+        auto step = [&](int32_t i, RawTile<kSub, S::kChunks>& now) {
             auto refill = [&]() {
-                if (i + 1 < tiles) {
-                    if ((i + 1) % kBatch == 0)
-                        places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0 + (i + 1) * kUnit, kUnit, end, lane);
-                    load_tile<D, kSub>(a, places, i + 1, lane, raw);
+                const int32_t next = i + kDepth;
+                if (next < tiles) {
+                    if (next % kBatch == 0)
+                        places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0 + next * kUnit, kUnit, end, lane);
+                    load_tile<D, kSub>(a, places, next, lane, now);
                 }
             };
             const int32_t key = key0 + i * kUnit;
             bool plain = (key + kKeys - 1 <= min(first_pos, end - 1)) & ((a.window == 0) | (key > last_pos - a.window));
 #pragma unroll
             for (int t = 0; t < kSub; ++t)
-                plain = plain & (raw.place[t] >= 0);
-            attend<D, kPieces, kSub>(raw, key, plain, any, seen, a.scale_f, query, turned[wave], lane, acc, m_run, l_run,
+                plain = plain & (now.place[t] >= 0);
+            attend<D, kPieces, kSub>(now, key, plain, any, seen, a.scale_f, query, turned[wave], lane, acc, m_run, l_run,
                                      refill);
+        };
+        for (int32_t i = 0; i < tiles; i += kDepth) {
+#pragma unroll
+            for (int u = 0; u < kDepth; ++u)
+                if (i + u < tiles)
+                    step(i + u, raw[u]);
         }
         l_run = group4_sum(l_run);
         asm volatile("" ::: "memory");
@@ -802,7 +839,7 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
                     a.lse[t * a.lse_st + ohead] = e.lse;
             } else {
                 // a worker's first slot holds the tile that came from the one before, its second the one that goes on
-                float* slot = a.partials + slot_of(a, h, worker, w.unit == 0) * slot_floats(D);
+                float* slot = a.partials + slot_of(a, h, worker, unit == 0) * slot_floats(D);
 #pragma unroll
                 for (int i = 0; i < kDims; i += 4)
                     *reinterpret_cast<f32x4_t*>(slot + orow * D + part * kDims + i) =
@@ -813,20 +850,20 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
                 }
             }
         }
-        left -= units;
-        if (!whole && w.unit == 0) {
+        left -= cost;
+        if (!whole && unit == 0) {
             cut.first_token = req.first;
             cut.first_row = w.tile * kRows;
             cut.rows = rows;
             // the units behind this worker's, dealt out to the next ones
-            cut.count = 1 + (int32_t)((w.tiles.units - units + w.each - 1) / w.each);
+            cut.count = 1 + (w.tiles.units - units + w.each - 1) / w.each;
         }
         if (left > 0) {
-            w.unit = 0;
+            w.at = 0;
             if (++w.tile == w.tiles.count) {
                 w.tile = 0;
                 do
-                    w.tiles = tiles_of(a, ++w.b, kRows, kUnit);  // there is one: units are left
+                    w.tiles = tiles_of(a, ++w.b, kRows, kUnit);  // there is one: cost is left
                 while (w.tiles.count == 0);
             }
             __syncthreads();  // the joined sums were read
@@ -836,54 +873,11 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
         a.cut_tiles[worker] = cut;
 }
 
-// Joins the cuts of one row: workgroup (worker in which the tile begins and head, row of the tile).
+// Writes a joined row: kLanes lanes from `part` 0 on hold four dims each.
 template <int D, bool kHalf>
-__global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
-    __shared__ float factor[kMostWorkers];
-    __shared__ float sums[kAttThreads * 4];
-    constexpr int kLanes = D / 4, kGroups = kAttThreads / kLanes;
-    const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads), h = (int32_t)(blockIdx.x % a.kv_heads);
-    const CutTile tile = a.cut_tiles[worker];
-    const int32_t r = (int32_t)blockIdx.y, row = tile.first_row + r;
-    if (tile.count == 0 || row >= tile.rows)
-        return;
-    // the cuts are this worker's second slot and the next ones' first
-    auto slot_at = [&](int32_t i) {
-        return a.partials + slot_of(a, h, worker + i, i == 0) * slot_floats(D);
-    };
-    const int lane = threadIdx.x & 63;
-    // every wave finds the reference and the sum for itself
-    float m = -INFINITY;
-    for (int32_t i = lane; i < tile.count; i += 64)
-        m = fmaxf(m, slot_at(i)[kRows * D + r]);
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1)
-        m = fmaxf(m, __shfl_xor(m, d));
-    const float m_use = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int32_t i = lane; i < tile.count; i += 64) {
-        const float* slot = slot_at(i) + kRows * D + r;
-        const float f = __builtin_amdgcn_exp2f(slot[0] - m_use);
-        l += f * slot[kRows];
-        if (threadIdx.x < 64)
-            factor[i] = f;
-    }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1)
-        l += __shfl_xor(l, d);
-    __syncthreads();
-    const int part = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int32_t i = group; i < tile.count; i += kGroups)
-        o += factor[i] * *reinterpret_cast<const f32x4_t*>(slot_at(i) + r * D + 4 * part);
-    *reinterpret_cast<f32x4_t*>(sums + 4 * threadIdx.x) = o;
-    __syncthreads();
-    if (group != 0)
-        return;
-#pragma unroll
-    for (int i = 1; i < kGroups; ++i)
-        o += *reinterpret_cast<const f32x4_t*>(sums + 4 * (i * kLanes + part));
+__device__ __forceinline__ void write_row(const AttArgs& a, const CutTile& tile, int32_t r, int32_t h, int part, f32x4_t o,
+                                          float m, float l) {
+    const int32_t row = tile.first_row + r;
     const int32_t token = row / a.group, head = h * a.group + row - token * a.group;
     const int64_t t = tile.first_token + token;
     const RowEnd e = finish_row(a, head, m, l);
@@ -893,21 +887,96 @@ __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
         a.lse[t * a.lse_st + head] = e.lse;
 }
 
+// Joins the cuts of the tile that begins in a worker, for one head (blockIdx.x) and the
+// rows of blockIdx.y.  kWide: a workgroup per row, its waves share out the cuts
+// (few rows, of many cuts); otherwise a wave per row.  (The grid has as many rows
+// as the host was told of; there may be more.)
+template <int D, bool kHalf, bool kWide>
+__global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
+    constexpr int kLanes = D / 4, kGroups = 64 / kLanes;  // lanes per row, cuts that a wave takes at a time
+    constexpr int kRowsAtOnce = kWide ? 1 : kAttWaves;
+    __shared__ f32x4_t sums[kWide ? kAttWaves : 1][kLanes];
+    __shared__ float factors[kAttWaves][64];
+    const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads), h = (int32_t)(blockIdx.x % a.kv_heads);
+    const CutTile tile = a.cut_tiles[worker];
+    if (tile.count == 0)
+        return;
+    const int32_t rows = min(tile.rows - tile.first_row, kRows);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int part = lane % kLanes, group = lane / kLanes;
+    // the cuts are this worker's second slot and the next ones' first
+    auto slot_at = [&](int32_t i) {
+        return a.partials + slot_of(a, h, worker + i, i == 0) * slot_floats(D);
+    };
+    for (int32_t r = (int32_t)blockIdx.y * kRowsAtOnce + (kWide ? 0 : wave); r < rows;
+         r += (int32_t)gridDim.y * kRowsAtOnce) {
+        // every wave finds the reference for itself
+        float m = -INFINITY;
+        for (int32_t i = lane; i < tile.count; i += 64)
+            m = fmaxf(m, slot_at(i)[kRows * D + r]);
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1)
+            m = fmaxf(m, __shfl_xor(m, d));
+        const float m_use = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+        for (int32_t base = 0; base < tile.count; base += 64) {
+            float f = 0.f;
+            if (base + lane < tile.count) {
+                const float* slot = slot_at(base + lane) + kRows * D + r;
+                f = __builtin_amdgcn_exp2f(slot[0] - m_use);
+                l += f * slot[kRows];
+            }
+            const int32_t n = min(tile.count - base, 64);
+            factors[wave][lane] = f;  // read by this wave alone
+#pragma unroll 8
+            for (int32_t i = kWide ? wave * kGroups + group : group; i < n; i += kWide ? kAttWaves * kGroups : kGroups)
+                o += factors[wave][i] * *reinterpret_cast<const f32x4_t*>(slot_at(base + i) + r * D + 4 * part);
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1)
+            l += __shfl_xor(l, d);
+#pragma unroll
+        for (int d = kLanes; d < 64; d <<= 1)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                o[j] += __shfl_xor(o[j], d);
+        if constexpr (kWide) {
+            if (group == 0)
+                sums[wave][part] = o;
+            __syncthreads();
+            if (wave == 0 && group == 0) {
+#pragma unroll
+                for (int i = 1; i < kAttWaves; ++i)
+                    o += sums[i][part];
+                write_row<D, kHalf>(a, tile, r, h, part, o, m, l);
+            }
+            __syncthreads();  // before the next row's sums
+        } else {
+            if (group == 0)
+                write_row<D, kHalf>(a, tile, r, h, part, o, m, l);
+        }
+    }
+}
+
 // How a call is dealt out, from what the host knows.
 struct Dealing {
     int64_t tiles;    // row tiles at most
+    int32_t rows;     // of a tile, as far as the host knows
     int32_t workers;  // per head; 0: a workgroup per tile
     int64_t cut_tiles_at, bytes;  // of the workspace
 };
 
-Dealing dealing_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t reqs, int64_t max_seq) {
+Dealing dealing_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t reqs, int64_t max_query,
+                   int64_t max_seq) {
     Dealing d = {};
+    const int64_t most_rows = (heads / kv_heads) * (max_query < 1 ? 1 : max_query < kRows ? max_query : kRows);
+    d.rows = (int32_t)(most_rows < kRows ? most_rows : kRows);
     // no request has more tiles than its rows' share, rounded up
     d.tiles = tokens * (heads / kv_heads) / kRows + reqs;
     int64_t workers = groups_per_cu((int)dim) * cu_count() / kv_heads;
     workers = workers < 1 ? 1 : workers > kMostWorkers ? kMostWorkers : workers;
-    // nothing to cut: no tile has more keys than a worker takes at least
-    if (max_seq <= kLeastUnits * unit_keys((int)dim))
+    if (max_seq <= kWholeUnits * unit_keys((int)dim))
         return d;
     d.workers = (int32_t)workers;
     d.cut_tiles_at = 2 * workers * kv_heads * (int64_t)slot_floats((int)dim) * 4;
@@ -920,8 +989,14 @@ void launch_attend(const Dealing& d, hipStream_t st, const AttArgs& a) {
     const unsigned grid = (unsigned)((a.workers > 0 ? a.workers : d.tiles) * a.kv_heads);
     hipLaunchKernelGGL((mxfp4_attend_kernel<D, kPieces>), dim3(grid), dim3(kAttThreads), 0, st, a);
     if (a.workers > 0) {
-        const unsigned rows = a.query_start_loc || a.group >= kRows ? kRows : a.group;
-        hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3>), dim3(grid, rows), dim3(kAttThreads), 0, st, a);
+        // a wave per row where that fills the chip (4 x 256 rows)
+        const int64_t cut_tiles = (d.tiles < a.workers ? d.tiles : a.workers) * a.kv_heads;
+        if (cut_tiles * d.rows >= 1024)
+            hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, false>), dim3(grid, (d.rows + 3) / 4),
+                               dim3(kAttThreads), 0, st, a);
+        else
+            hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, true>), dim3(grid, d.rows), dim3(kAttThreads), 0, st,
+                               a);
     }
 }
 
@@ -1004,14 +1079,15 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
     a.window = (int32_t)(window_size < 0x3fffffffLL ? window_size : 0);
     a.q_wide = aligned(q, 16) && ((q_stride_token | q_stride_head) & 7) == 0;
     a.o_wide = aligned(out, 8) && ((out_stride_token | out_stride_head) & 3) == 0;
-    const Dealing deal = dealing_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_seq_len);
-    const bool stream_mode = deal.workers > 0 && workspace && workspace_bytes >= deal.bytes;
+    const Dealing deal = dealing_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len);
+    // (the cost of all tiles has to fit 31 bits: with more of it there is nothing to gain either)
+    const bool stream_mode = deal.workers > 0 && workspace && workspace_bytes >= deal.bytes &&
+                             deal.tiles * (kTileCost + 1 + a.table_keys / unit_keys((int)head_dim)) <= 0x7fffffffLL;
     if (stream_mode && !aligned(workspace, 16))
         return fail(FGV_E_MISALIGNED, "workspace must be 16-byte aligned");
     if (!stream_mode && deal.tiles * num_kv_heads > 0x7fffffffLL)
         return fail(FGV_E_TOO_LARGE, "too many row tiles");
     a.workers = stream_mode ? deal.workers : 0;
-    a.least_units = kLeastUnits;
     a.partials = static_cast<float*>(workspace);
     a.cut_tiles = reinterpret_cast<CutTile*>(static_cast<uint8_t*>(workspace) + deal.cut_tiles_at);
     const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -1026,9 +1102,8 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
 extern "C" int64_t fgv_mxfp4_paged_attention_workspace_bytes(int64_t num_tokens, int64_t num_heads,
                                                              int64_t num_kv_heads, int64_t head_dim, int64_t num_reqs,
                                                              int64_t max_query_len, int64_t max_seq_len) {
-    (void)max_query_len;
     if (num_tokens <= 0 || num_reqs <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || num_heads > 65536 ||
         num_tokens * num_heads > 0x3fffffffLL || num_reqs > 0x3fffffffLL)
         return 0;
-    return fgv::dealing_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_seq_len).bytes;
+    return fgv::dealing_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len).bytes;
 }
