@@ -95,6 +95,7 @@ struct AttArgs {
     float scale_sign;
     int32_t num_reqs, num_tokens, kv_heads, group, page, table_keys, window;
     int32_t q_wide, o_wide;
+    int32_t rows_from, rows_to;  // requests of other numbers of rows are another launch's
     // Stream mode (workers > 0): workers per head, and the workspace's parts.
     int32_t workers;
     float* partials;
@@ -142,7 +143,8 @@ struct Tiles {
 __device__ __forceinline__ Tiles tiles_of(const AttArgs& a, int32_t b, int32_t rows_per_tile, int32_t unit_keys) {
     Tiles t;
     t.req = request_of(a, b);
-    t.count = (int32_t)(((int64_t)t.req.count * a.group + rows_per_tile - 1) / rows_per_tile);
+    const int32_t rows = t.req.count * a.group;  // fits: they are rows of q
+    t.count = rows >= a.rows_from && rows <= a.rows_to ? (rows + rows_per_tile - 1) / rows_per_tile : 0;
     t.units = 1;
     if (a.workers > 0) {
         int32_t begin, end;
@@ -212,9 +214,11 @@ __device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int
     uint32_t each = 1;
     if (a.workers > 0)
         each = max((total + a.workers - 1) / a.workers, (uint32_t)kLeastCost);
-    const uint64_t first = (uint64_t)each * index;
+    uint64_t first = (uint64_t)each * index;
     if (first >= total)
         return false;
+    if (a.workers == 0)
+        first = total - 1 - first;  // from the end: of a prompt's tiles the last have the most keys
     uint32_t before = 0;
     for (int32_t base = 0; base < a.num_reqs; base += kAttThreads) {
         if (a.num_reqs > kAttThreads) {
@@ -339,6 +343,25 @@ __device__ __forceinline__ void load_query(const AttArgs& a, int64_t at, bool va
         load_words<16>(a.q, at + 64 * c + 16 * g, a.q_wide, valid, raw.w[c]);
 }
 
+// How a row with largest magnitude `most` (its bits) enters: q 2^scale_e = x 2^e,
+// x = q * down with its maximum in [128, 256).  The softmax scale's power of two
+// goes in here, so that scores leave binary32's range only where scaled ones
+// would.  -118 leaves room for the pieces' smaller scales.
+struct QueryScale {
+    bool bad;  // not finite: the scale says NaN
+    int byte;
+    float down;
+};
+
+__device__ __forceinline__ QueryScale query_scale(const AttArgs& a, uint32_t most) {
+    const int e = min(max((int)(most >> 23) - 127 - 7 + a.scale_e, -118), 127);
+    QueryScale q;
+    q.bad = most >= 0x7f800000u;
+    q.byte = e + 127;
+    q.down = __uint_as_float((uint32_t)min(max(127 - e + a.scale_e, 1), 254) << 23) * a.scale_sign;
+    return q;
+}
+
 // Row r of lane (r, g) as the matrix instruction's operand.
 template <int D, int kPieces, bool kHalf>
 __device__ __forceinline__ void split_query(const AttArgs& a, const RawQuery<D>& raw, Query<D, kPieces>& out, int g) {
@@ -355,17 +378,12 @@ __device__ __forceinline__ void split_query(const AttArgs& a, const RawQuery<D>&
     // over the row's four lanes
     most = max(most, (uint32_t)__shfl_xor((int)most, 16));
     most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-    const bool bad = most >= 0x7f800000u;
-    // q 2^scale_e = x 2^e with the row's maximum in [128, 256): the softmax scale's power of two goes in here, so that
-    // scores leave binary32's range only where scaled ones would.  -118 leaves room for the pieces' smaller scales.
-    const int e = min(max((int)(most >> 23) - 127 - 7 + a.scale_e, -118), 127);
-    const float down = __uint_as_float((uint32_t)min(max(127 - e + a.scale_e, 1), 254) << 23) * a.scale_sign;
+    const QueryScale q = query_scale(a, most);
 #pragma unroll
     for (int c = 0; c < kRuns; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            x[c][i] = bad ? 0.f : x[c][i] * down;
-    const int byte = e + 127;
+            x[c][i] = q.bad ? 0.f : x[c][i] * q.down;
     if constexpr (D == 64) {
 #pragma unroll
         for (int s = 0; s < Shape<D, kPieces>::kSteps; ++s) {
@@ -373,8 +391,10 @@ __device__ __forceinline__ void split_query(const AttArgs& a, const RawQuery<D>&
             for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    out.q[s][4 * half + i] = 2 * s + half < kPieces ? (int)(s + half == 0 ? take_piece<true>(&x[0][4 * i]) : take_piece<false>(&x[0][4 * i])) : 0;
-            out.scale[s] = bad ? 255 : byte - 4 * (2 * s + (g >> 1));
+                    out.q[s][4 * half + i] = 2 * s + half >= kPieces ? 0
+                                             : (int)(s + half == 0 ? take_piece<true>(&x[0][4 * i])
+                                                                   : take_piece<false>(&x[0][4 * i]));
+            out.scale[s] = q.bad ? 255 : q.byte - 4 * (2 * s + (g >> 1));
         }
     } else {
 #pragma unroll
@@ -385,8 +405,10 @@ __device__ __forceinline__ void split_query(const AttArgs& a, const RawQuery<D>&
                 for (int half = 0; half < 2; ++half)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        out.q[p * Shape<D, kPieces>::kChunks + c][4 * half + i] = (int)(p == 0 ? take_piece<true>(&x[2 * c + half][4 * i]) : take_piece<false>(&x[2 * c + half][4 * i]));
-                out.scale[p * Shape<D, kPieces>::kChunks + c] = bad ? 255 : byte - 4 * p;
+                        out.q[p * Shape<D, kPieces>::kChunks + c][4 * half + i] =
+                            (int)(p == 0 ? take_piece<true>(&x[2 * c + half][4 * i])
+                                         : take_piece<false>(&x[2 * c + half][4 * i]));
+                out.scale[p * Shape<D, kPieces>::kChunks + c] = q.bad ? 255 : q.byte - 4 * p;
             }
     }
 }
@@ -687,8 +709,8 @@ __device__ __forceinline__ RowEnd finish_row(const AttArgs& a, int32_t head, flo
     return e;
 }
 
-// Floats of a slot of partial results: O of kRows rows, their references and sums.
-constexpr int slot_floats(int dim) { return kRows * (dim + 2); }
+// Floats of a slot of partial results: O of the tile's rows, their references and sums.
+constexpr int slot_floats(int dim, int rows) { return rows * (dim + 2); }
 
 // A worker has two slots of each head: for a tile that began before it (or is all
 // cut through it), and for one that begins in it and goes on.
@@ -839,7 +861,7 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
                     a.lse[t * a.lse_st + ohead] = e.lse;
             } else {
                 // a worker's first slot holds the tile that came from the one before, its second the one that goes on
-                float* slot = a.partials + slot_of(a, h, worker, unit == 0) * slot_floats(D);
+                float* slot = a.partials + slot_of(a, h, worker, unit == 0) * slot_floats(D, kRows);
 #pragma unroll
                 for (int i = 0; i < kDims; i += 4)
                     *reinterpret_cast<f32x4_t*>(slot + orow * D + part * kDims + i) =
@@ -873,6 +895,14 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
         a.cut_tiles[worker] = cut;
 }
 
+}  // namespace
+}  // namespace fgv
+
+#include "mxfp4_attend_wide.h"
+
+namespace fgv {
+namespace {
+
 // Writes a joined row: kLanes lanes from `part` 0 on hold four dims each.
 template <int D, bool kHalf>
 __device__ __forceinline__ void write_row(const AttArgs& a, const CutTile& tile, int32_t r, int32_t h, int part, f32x4_t o,
@@ -891,7 +921,7 @@ __device__ __forceinline__ void write_row(const AttArgs& a, const CutTile& tile,
 // rows of blockIdx.y.  kWide: a workgroup per row, its waves share out the cuts
 // (few rows, of many cuts); otherwise a wave per row.  (The grid has as many rows
 // as the host was told of; there may be more.)
-template <int D, bool kHalf, bool kWide>
+template <int D, bool kHalf, int kTileRows, bool kWide>
 __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
     constexpr int kLanes = D / 4, kGroups = 64 / kLanes;  // lanes per row, cuts that a wave takes at a time
     constexpr int kRowsAtOnce = kWide ? 1 : kAttWaves;
@@ -901,19 +931,19 @@ __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
     const CutTile tile = a.cut_tiles[worker];
     if (tile.count == 0)
         return;
-    const int32_t rows = min(tile.rows - tile.first_row, kRows);
+    const int32_t rows = min(tile.rows - tile.first_row, kTileRows);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int part = lane % kLanes, group = lane / kLanes;
     // the cuts are this worker's second slot and the next ones' first
     auto slot_at = [&](int32_t i) {
-        return a.partials + slot_of(a, h, worker + i, i == 0) * slot_floats(D);
+        return a.partials + slot_of(a, h, worker + i, i == 0) * slot_floats(D, kTileRows);
     };
     for (int32_t r = (int32_t)blockIdx.y * kRowsAtOnce + (kWide ? 0 : wave); r < rows;
          r += (int32_t)gridDim.y * kRowsAtOnce) {
         // every wave finds the reference for itself
         float m = -INFINITY;
         for (int32_t i = lane; i < tile.count; i += 64)
-            m = fmaxf(m, slot_at(i)[kRows * D + r]);
+            m = fmaxf(m, slot_at(i)[kTileRows * D + r]);
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1)
             m = fmaxf(m, __shfl_xor(m, d));
@@ -923,9 +953,9 @@ __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
         for (int32_t base = 0; base < tile.count; base += 64) {
             float f = 0.f;
             if (base + lane < tile.count) {
-                const float* slot = slot_at(base + lane) + kRows * D + r;
+                const float* slot = slot_at(base + lane) + kTileRows * D + r;
                 f = __builtin_amdgcn_exp2f(slot[0] - m_use);
-                l += f * slot[kRows];
+                l += f * slot[kTileRows];
             }
             const int32_t n = min(tile.count - base, 64);
             factors[wave][lane] = f;  // read by this wave alone
@@ -959,7 +989,7 @@ __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
     }
 }
 
-// How a call is dealt out, from what the host knows.
+// How a launch is dealt out, from what the host knows.
 struct Dealing {
     int64_t tiles;    // row tiles at most
     int32_t rows;     // of a tile, as far as the host knows
@@ -967,42 +997,84 @@ struct Dealing {
     int64_t cut_tiles_at, bytes;  // of the workspace
 };
 
-Dealing dealing_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t reqs, int64_t max_query,
-                   int64_t max_seq) {
+// One launch takes all requests, or two share them by their rows: 16-row tiles for
+// up to kFewRows, 128-row tiles (whose waves would have nothing to do) for more.
+constexpr int kFewRows = 64;
+
+struct Call {
+    int64_t tokens, heads, kv_heads, dim, reqs, max_query, max_seq;
+    bool wide() const { return max_query * (heads / kv_heads) > kFewRows; }
+    bool few() const { return !wide() || reqs > 1; }
+};
+
+Dealing dealing_of(const Call& c, bool wide) {
+    const int64_t group = c.heads / c.kv_heads, tile_rows = wide ? kWideRows : kRows;
+    const int64_t slots = (wide ? (c.dim == 256 ? 1 : 2) : groups_per_cu((int)c.dim)) * cu_count();
+    const int64_t unit = wide ? kWideKeys : unit_keys((int)c.dim);
     Dealing d = {};
-    const int64_t most_rows = (heads / kv_heads) * (max_query < 1 ? 1 : max_query < kRows ? max_query : kRows);
-    d.rows = (int32_t)(most_rows < kRows ? most_rows : kRows);
+    const int64_t rows = group * (c.max_query < 1 ? 1 : c.max_query < tile_rows ? c.max_query : tile_rows);
+    d.rows = (int32_t)(rows < tile_rows ? rows : tile_rows);
     // no request has more tiles than its rows' share, rounded up
-    d.tiles = tokens * (heads / kv_heads) / kRows + reqs;
-    int64_t workers = groups_per_cu((int)dim) * cu_count() / kv_heads;
+    d.tiles = c.tokens * group / tile_rows + c.reqs;
+    int64_t workers = slots / c.kv_heads;
     workers = workers < 1 ? 1 : workers > kMostWorkers ? kMostWorkers : workers;
-    if (max_seq <= kWholeUnits * unit_keys((int)dim))
+    // Nothing to cut; or (128-row tiles take long, and the first to end take the next) enough of them.
+    if (c.max_seq <= kWholeUnits * unit || (wide && d.tiles * c.kv_heads >= 2 * slots + c.reqs * c.kv_heads))
         return d;
     d.workers = (int32_t)workers;
-    d.cut_tiles_at = 2 * workers * kv_heads * (int64_t)slot_floats((int)dim) * 4;
+    d.cut_tiles_at = 2 * workers * c.kv_heads * (int64_t)slot_floats((int)c.dim, (int)tile_rows) * 4;
     d.bytes = (d.cut_tiles_at + workers * (int64_t)sizeof(CutTile) + 255) / 256 * 256;
     return d;
 }
 
+template <int D, int kPieces, int kTileRows>
+void launch_part(const Dealing& d, uint8_t* workspace, int64_t unit, hipStream_t st, AttArgs a) {
+    // (the cost of all tiles has to fit 31 bits: with more of it there is nothing to gain either)
+    const bool stream = workspace && d.workers > 0 && d.tiles * (kTileCost + 1 + a.table_keys / unit) <= 0x7fffffffLL;
+    a.workers = stream ? d.workers : 0;
+    a.partials = reinterpret_cast<float*>(workspace);
+    a.cut_tiles = reinterpret_cast<CutTile*>(workspace + d.cut_tiles_at);
+    const unsigned grid = (unsigned)((stream ? d.workers : d.tiles) * a.kv_heads);
+    if constexpr (kTileRows == kRows)
+        hipLaunchKernelGGL((mxfp4_attend_kernel<D, kPieces>), dim3(grid), dim3(kAttThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL((mxfp4_attend_wide_kernel<D, kPieces>), dim3(grid), dim3(kAttThreads), 0, st, a);
+    if (!stream)
+        return;
+    // a wave per row where that fills the chip (4 x 256 rows)
+    const int64_t cut_tiles = (d.tiles < a.workers ? d.tiles : a.workers) * a.kv_heads;
+    if (cut_tiles * d.rows >= 1024)
+        hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, kTileRows, false>), dim3(grid, (d.rows + 3) / 4),
+                           dim3(kAttThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, kTileRows, true>), dim3(grid, d.rows),
+                           dim3(kAttThreads), 0, st, a);
+}
+
 template <int D, int kPieces>
-void launch_attend(const Dealing& d, hipStream_t st, const AttArgs& a) {
-    const unsigned grid = (unsigned)((a.workers > 0 ? a.workers : d.tiles) * a.kv_heads);
-    hipLaunchKernelGGL((mxfp4_attend_kernel<D, kPieces>), dim3(grid), dim3(kAttThreads), 0, st, a);
-    if (a.workers > 0) {
-        // a wave per row where that fills the chip (4 x 256 rows)
-        const int64_t cut_tiles = (d.tiles < a.workers ? d.tiles : a.workers) * a.kv_heads;
-        if (cut_tiles * d.rows >= 1024)
-            hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, false>), dim3(grid, (d.rows + 3) / 4),
-                               dim3(kAttThreads), 0, st, a);
-        else
-            hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, true>), dim3(grid, d.rows), dim3(kAttThreads), 0, st,
-                               a);
+void launch_attend(const Call& c, uint8_t* workspace, hipStream_t st, AttArgs a) {
+    const bool both = c.wide() && c.few();
+    a.rows_from = 0;
+    a.rows_to = 0x7fffffff;
+    if (c.wide()) {
+        const Dealing d = dealing_of(c, true);
+        a.rows_from = both ? kFewRows + 1 : 0;
+        launch_part<D, kPieces, kWideRows>(d, workspace, kWideKeys, st, a);
+        workspace = workspace ? workspace + d.bytes : nullptr;
+        a.rows_from = 0;
+        a.rows_to = kFewRows;
     }
+    if (c.few())
+        launch_part<D, kPieces, kRows>(dealing_of(c, false), workspace, unit_keys(D), st, a);
 }
 
 template <int D>
-void launch_attend(bool half, const Dealing& d, hipStream_t st, const AttArgs& a) {
-    half ? launch_attend<D, 3>(d, st, a) : launch_attend<D, 2>(d, st, a);
+void launch_attend(bool half, const Call& c, uint8_t* workspace, hipStream_t st, const AttArgs& a) {
+    half ? launch_attend<D, 3>(c, workspace, st, a) : launch_attend<D, 2>(c, workspace, st, a);
+}
+
+int64_t workspace_of(const Call& c) {
+    return (c.wide() ? dealing_of(c, true).bytes : 0) + (c.few() ? dealing_of(c, false).bytes : 0);
 }
 
 }  // namespace
@@ -1079,22 +1151,18 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
     a.window = (int32_t)(window_size < 0x3fffffffLL ? window_size : 0);
     a.q_wide = aligned(q, 16) && ((q_stride_token | q_stride_head) & 7) == 0;
     a.o_wide = aligned(out, 8) && ((out_stride_token | out_stride_head) & 3) == 0;
-    const Dealing deal = dealing_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len);
-    // (the cost of all tiles has to fit 31 bits: with more of it there is nothing to gain either)
-    const bool stream_mode = deal.workers > 0 && workspace && workspace_bytes >= deal.bytes &&
-                             deal.tiles * (kTileCost + 1 + a.table_keys / unit_keys((int)head_dim)) <= 0x7fffffffLL;
-    if (stream_mode && !aligned(workspace, 16))
-        return fail(FGV_E_MISALIGNED, "workspace must be 16-byte aligned");
-    if (!stream_mode && deal.tiles * num_kv_heads > 0x7fffffffLL)
+    const Call call = {num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len};
+    if ((num_tokens * a.group / kRows + num_reqs) * num_kv_heads > 0x7fffffffLL)
         return fail(FGV_E_TOO_LARGE, "too many row tiles");
-    a.workers = stream_mode ? deal.workers : 0;
-    a.partials = static_cast<float*>(workspace);
-    a.cut_tiles = reinterpret_cast<CutTile*>(static_cast<uint8_t*>(workspace) + deal.cut_tiles_at);
+    const int64_t bytes = workspace_of(call);
+    uint8_t* const ws = bytes > 0 && workspace_bytes >= bytes ? static_cast<uint8_t*>(workspace) : nullptr;
+    if (ws && !aligned(ws, 16))
+        return fail(FGV_E_MISALIGNED, "workspace must be 16-byte aligned");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     switch (head_dim) {
-        case 64: launch_attend<64>(dtype == 1, deal, st, a); break;
-        case 128: launch_attend<128>(dtype == 1, deal, st, a); break;
-        default: launch_attend<256>(dtype == 1, deal, st, a); break;
+        case 64: launch_attend<64>(dtype == 1, call, ws, st, a); break;
+        case 128: launch_attend<128>(dtype == 1, call, ws, st, a); break;
+        default: launch_attend<256>(dtype == 1, call, ws, st, a); break;
     }
     return launch_status();
 }
@@ -1105,5 +1173,5 @@ extern "C" int64_t fgv_mxfp4_paged_attention_workspace_bytes(int64_t num_tokens,
     if (num_tokens <= 0 || num_reqs <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || num_heads > 65536 ||
         num_tokens * num_heads > 0x3fffffffLL || num_reqs > 0x3fffffffLL)
         return 0;
-    return fgv::dealing_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len).bytes;
+    return fgv::workspace_of({num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len});
 }

@@ -14,7 +14,10 @@ What the kernels may be off, row by row (``bounds``), counted before their first
   behind the first, 2^-4 as large at least, any may be;
 * scores are scaled and exp2 taken in 32 bits: 2^-20 (1 + |s|) together covers the
   scaling, the subtraction and two ulp of the exponential;
-* P enters as two bf16 pieces (2^-16);
+* P enters as two bf16 pieces (2^-16).  Where a request has more than 64 rows for a key head (or
+  is alone), bf16 calls have one fp16 piece of it, 2^-11, and both types lose of P times 2^7 what lies
+  below fp16's least step, half of 2^-24: under a reference of at most 2^4 times the row's largest
+  that is 2^(-25 - 7 + 4) = 2^-28 of the row's largest a key;
 * P below 2^-126 is nothing in 32 bits (the first run showed that this had been left out: a dim
   where all keys but such ones hold zeros came out as 0 instead of 4e-39).  P is taken under a
   reference of at most 2^4 times the row's largest, so that is 2^-122 |v| a key, as a score
@@ -146,7 +149,10 @@ def reference(q, cache, table, lens, start, scale, window=None, sink=None):
             weight = p @ torch.where(nan, 0.0, vh).abs() * share[:, None]
             o = o * share[:, None]
             half = torch.finfo(q.dtype).eps / 2
-            ob = weight * (2.0 ** -16 + 2.5 * d + steps)[:, None] * (1 + half)
+            many = (t1 - t0) * group > 64 or len(lens) == 1
+            ob = weight * ((2.0 ** -11 if many and not three else 2.0 ** -16) + 2.5 * d + steps)[:, None] * (1 + half)
+            if many:
+                ob = ob + 2.0 ** -28 * (p.amax(1) * share)[:, None] * torch.where(nan, 0.0, vh).abs().sum(0)
             ob = ob + half * o.abs() + torch.finfo(q.dtype).smallest_normal * half
             ob = ob + 2.0 ** -121 * torch.where(nan, 0.0, vh).abs().sum(0)
             out[t0:t1, h] = torch.where(some[:, None], o, 0.0)
@@ -362,6 +368,40 @@ def test_gpu_every_scale_byte(dtype):
         ks[live] = torch.where(ks[live] == 255, 255, b).to(torch.uint8)
         one.scale = one.scale * 2.0 ** min(max(127 - b, -90), 90)
         one.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [(BF, 64), (FP, 128), (BF, 128), (BF, 256), (FP, 256)])
+def test_gpu_value_sizes_with_many_tokens(dtype, dim):
+    """Value blocks each side of what fp16 holds, from the first key on, from a later one, and only here and there."""
+    for seed, where in enumerate([slice(0, 700), slice(640, 700), slice(300, 301), slice(100, 700, 37)]):
+        for low, high in ((109, 114), (145, 150), (0, 3), (111, 148), (1, 253)):
+            print(f"\n[case] value sizes {dtype} {dim} {where} {low} {high}", flush=True)
+            c = Case(30 + seed, [700, 90], [130, 1], dtype=dtype, dim=dim)
+            at = torch.arange(700)[where]
+            block = c.table[0, at.to(DEV) // 16].long()
+            vs = parts(c.cache)[3]
+            for h in range(2):
+                byte = torch.randint(low, high, (len(at), dim // 32), generator=c.g).to(torch.uint8)
+                vs[block, h, at.to(DEV) % 16] = byte.to(DEV)
+            c.check()
+            c.check(window=77)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lens,query,heads,kv_heads,dim", [
+    ([5000], [5000], 2, 1, 64), ([3000, 9, 2000], [2500, 9, 2000], 8, 2, 128), ([20000], [129], 4, 1, 128),
+    ([9000, 100], [33, 1], 12, 2, 256), ([300] * 40, [65] * 40, 3, 3, 64), ([40000], [7], 16, 1, 256),
+    ([20001] + [5] * 300, [200] + [1] * 300, 4, 2, 64)])
+def test_gpu_prompts(dtype, lens, query, heads, kv_heads, dim):
+    """Prompts, chunks and mixed batches, their tiles whole and cut, and the same bits every time."""
+    print(f"\n[case] prompts {dtype} {lens[:3]} {query[:3]} {heads} {kv_heads} {dim}", flush=True)
+    c = Case(21, lens, query, heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype, page=32)
+    first = c.check(max_query_len=max(query), max_seq_len=max(lens))
+    for x, y in zip(first, c.run(max_query_len=max(query), max_seq_len=max(lens))):
+        assert torch.equal(x, y)
+    c.check(500, torch.randn(heads, device=DEV), max_query_len=1000)
 
 
 @pytest.mark.gpu
