@@ -21,6 +21,7 @@
 namespace fgv {
 namespace {
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
@@ -32,13 +33,14 @@ constexpr int kWideKeys = 64;   // keys of a tile, and of a unit
 // would: P is held to 2^-32.  2^-7 * 0.5 * 2^(111 - 127) is fp16's least value,
 // and 2^-7 * 6 * 2^(147 - 127) below its largest.
 constexpr int kHalfShift = 7;
-__device__ __forceinline__ bool half_holds(uint32_t byte, uint4 codes) {
+__device__ __forceinline__ bool half_holds(uint32_t byte, u32x4_t codes) {
     const bool zeros = ((codes.x | codes.y | codes.z | codes.w) & 0x77777777u) == 0;
     return (byte - (104u + kHalfShift) <= 36u) | (zeros & (byte != 255u));
 }
 
 template <int D, int kPieces>
 struct WideShape {
+    static constexpr bool kFp16 = D <= 128;  // with both loops, more than registers hold of D = 256
     static constexpr int kChunks = D / 64;                // of 64 dims: one QK instruction per piece
     static constexpr int kVChunks = D < 128 ? 1 : D / 128;  // of 128 dims: 16 bytes of codes a lane
     static constexpr int kVPitch = D == 64 ? 192 : 2 * D + 64;  // four rows of 64 bytes meet no bank twice
@@ -49,70 +51,103 @@ struct WideShape {
 
 template <int D>
 struct WideKeyTile {
-    uint4 k[2][D / 64];
-    uint32_t ks[2][D / 64];
-    uint32_t live;  // which of the four subtiles have a block, bit by bit
+    u32x4_t k[2][D / 64];
+    uint32_t ks[2][(D + 127) / 128];  // of 4 blocks, moved by h bytes: byte 0 or 2 is this lane's
 };
 
 template <int D>
 struct WideValueTile {
-    uint4 v[D < 128 ? 1 : D / 128];
-    uint32_t vs[D < 128 ? 1 : D / 128];
+    u32x4_t v[D < 128 ? 1 : D / 128];
+    uint32_t vs[D < 128 ? 1 : D / 128];  // of 4 blocks (2 where D = 64); `look` takes this lane's
     int32_t key;  // of the first of the wave's 16 tokens, kNoKey: no block
 };
 
-// Codes and scales of the head's subtile `from` of `p`, at its first token.
+// Where the wave's next 64 subtiles lie, one a lane: the K codes and K scales of
+// their first token.  One without a block is taken from the cache's first block,
+// whose values nobody sees.
+struct WidePlaces {
+    uint64_t codes, scales;
+    uint64_t live;  // the lanes that have a block
+};
+
 template <int D>
-__device__ __forceinline__ const uint8_t* subtile_at(const AttArgs& a, const Places& p, int from, int32_t& place,
-                                                     const uint8_t*& scales) {
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)p.base, from);
-    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)p.base >> 32), from);
-    place = __builtin_amdgcn_readlane(p.place, from);
-    // one without a block reads the cache's first one, whose values nobody sees
-    const int32_t first = max(place, 0);
-    const uint8_t* head = a.cache + (int64_t)((uint64_t)hi << 32 | lo);
-    scales = head + mx_part(2, a.page, D) + (int64_t)first * (D / kMxBlock);
-    return head + (int64_t)first * (D / 2);
+__device__ __forceinline__ WidePlaces find_wide_places(const AttArgs& a, int32_t b, int32_t h, int32_t key, int32_t end,
+                                                       int lane) {
+    const Places p = find_places<4>(a, b, h, mx_token_bytes(D), key, kWideKeys, end, lane);
+    const uint64_t head = (uint64_t)a.cache + (uint64_t)p.base;
+    const uint32_t first = (uint32_t)max(p.place, 0);
+    WidePlaces w;
+    w.codes = head + first * (D / 2);
+    w.scales = head + (uint64_t)mx_part(2, a.page, D) + first * (D / kMxBlock);
+    w.live = __ballot(p.place >= 0);
+    return w;
+}
+
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * lane, (int)(uint32_t)v);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * lane, (int)(uint32_t)(v >> 32));
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t from_uniform(uint64_t v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
+    return (uint64_t)hi << 32 | lo;
+}
+
+// (told to be global memory: a flat load would count as LDS work, which barriers wait for)
+template <typename T>
+__device__ __forceinline__ const __attribute__((address_space(1))) T* global(uint64_t at) {
+    return reinterpret_cast<const __attribute__((address_space(1))) T*>(at);
 }
 
 template <int D>
-__device__ __forceinline__ void load_keys(const AttArgs& a, const Places& p, int tile, int lane, WideKeyTile<D>& out) {
-    const int r = lane & 15, h = lane >> 5;
-    const bool upper = lane & 16;
-    out.live = 0;
+__device__ __forceinline__ uint32_t scales_of(uint64_t at) {
+    return D == 64 ? *global<uint16_t>(at) : *global<uint32_t>(at);
+}
+
+// What this lane loads of a tile of K: keys l % 32 of its halves.
+struct WideKeyAt {
+    uint64_t codes[2], scales[2];
+};
+
+template <int D>
+__device__ __forceinline__ WideKeyAt find_keys(const WidePlaces& p, int tile, int lane) {
+    const int r = lane & 15, h = lane >> 5, upper = lane >> 4 & 1;
+    WideKeyAt at;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-        const uint8_t *codes[2], *scales[2];
+        const int from = (tile & 15) * 4 + 2 * t + upper;
+        at.codes[t] = from_lane(p.codes, from) + (uint32_t)(r * (D / 2) + 16 * h);
+        at.scales[t] = from_lane(p.scales, from) + (uint32_t)(r * (D / kMxBlock));
+    }
+    return at;
+}
+
+template <int D>
+__device__ __forceinline__ void load_keys(const WideKeyAt& at, WideKeyTile<D>& out) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            int32_t place;
-            codes[u] = subtile_at<D>(a, p, (tile & 15) * 4 + 2 * t + u, place, scales[u]);
-            out.live |= place >= 0 ? 1u << (2 * t + u) : 0;
-        }
-        const uint8_t* c = (upper ? codes[1] : codes[0]) + (uint32_t)(r * (D / 2) + 16 * h);
-        const uint8_t* s = (upper ? scales[1] : scales[0]) + (uint32_t)(r * (D / kMxBlock) + h);
+    for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-            out.k[t][i] = *reinterpret_cast<const uint4*>(c + 32 * i);
-            out.ks[t][i] = s[2 * i];
-        }
+        for (int i = 0; i < D / 64; ++i)
+            out.k[t][i] = *global<u32x4_t>(at.codes[t] + 32 * i);
+#pragma unroll
+        for (int i = 0; i < (D + 127) / 128; ++i)
+            out.ks[t][i] = scales_of<D>(at.scales[t] + 4 * i);
     }
 }
 
 template <int D>
-__device__ __forceinline__ void load_values(const AttArgs& a, const Places& p, int tile, int wave, int lane, int32_t key0,
+__device__ __forceinline__ void load_values(const AttArgs& a, const WidePlaces& p, int tile, int wave, int lane, int32_t key0,
                                             WideValueTile<D>& out) {
     const int r = lane & 15, g = D < 128 ? (lane >> 4) & 1 : lane >> 4;
-    int32_t place;
-    const uint8_t* scales;
-    const uint8_t* codes = subtile_at<D>(a, p, (tile & 15) * 4 + wave, place, scales);
-    out.key = place >= 0 ? key0 + 16 * wave : kNoKey;
-    codes += mx_part(1, a.page, D);
-    scales += (int64_t)a.page * (D / kMxBlock);
+    const int from = (tile & 15) * 4 + wave;
+    const uint64_t codes = from_uniform(p.codes, from) + (uint64_t)mx_part(1, a.page, D);
+    const uint64_t scales = from_uniform(p.scales, from) + (uint64_t)a.page * (D / kMxBlock);
+    out.key = p.live >> from & 1 ? key0 + 16 * wave : kNoKey;
 #pragma unroll
     for (int c = 0; c < (D < 128 ? 1 : D / 128); ++c) {
-        out.v[c] = *reinterpret_cast<const uint4*>(codes + (uint32_t)(r * (D / 2) + 64 * c + 16 * g));
-        out.vs[c] = scales[(uint32_t)(r * (D / kMxBlock) + 4 * c + g)];
+        out.v[c] = *global<u32x4_t>(codes + (uint32_t)(r * (D / 2) + 64 * c + 16 * g));
+        out.vs[c] = scales_of<D>(scales + (uint32_t)(r * (D / kMxBlock) + 4 * c));
     }
 }
 
@@ -121,7 +156,7 @@ __device__ __forceinline__ void load_values(const AttArgs& a, const Places& p, i
 // be too many for them, in LDS.
 template <int D, int kPieces>
 struct WideQuery {
-    static constexpr int kHeld = kPieces == 2 ? 2 : D == 256 ? 1 : 2;
+    static constexpr int kHeld = D == 256 ? 1 : 2;
     static constexpr int kInLds = (kPieces - kHeld) * D / 32;  // 16 bytes of each lane
     v8i_t q[D / 64 * kHeld];
     int scale;  // of the first piece
@@ -237,6 +272,9 @@ __device__ __forceinline__ f32x16_t wide_product(uint4 v, uint4 p, f32x16_t acc)
                                                        __builtin_bit_cast(bf16x8_t, p), acc, 0, 0, 0);
 }
 
+// What sched_group_barrier takes.
+constexpr int kValu = 0x2, kMfma = 0x8, kLdsRead = 0x100, kLdsWrite = 0x200;
+
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
@@ -254,14 +292,12 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
     const int h = (int)blockIdx.x % a.kv_heads;
     const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads);
     const int32_t tile_cost = a.workers > 0 ? kTileCost : 0;
-    // where this lane writes its 16-byte pieces of V, rotated so that the lanes of a write meet
-    // no bank twice, and where it reads them turned
-    const int turn = r >> 2;
-    uint32_t write_at[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        write_at[i] = (uint32_t)((16 * wave + r) * S::kVPitch + 64 * g + 16 * ((i + turn) & 3));
-    const uint32_t read_at = (uint32_t)((4 * hh + (r >> 2)) * S::kVPitch + 32 * ((lane >> 4) & 1) + 8 * (lane & 3));
+    // Where this lane writes its first 16-byte piece of V, and reads V turned: piece i of a 64-byte run
+    // lies at i ^ (row / 4 % 4), so that neither the lanes of a write nor of a read meet a bank twice.
+    static_assert(S::kVPitch % 64 == 0 && S::kVBytes % 64 == 0, "pieces are found by xor");
+    const uint32_t write_at = (uint32_t)((16 * wave + r) * S::kVPitch + 64 * (D < 128 ? g & 1 : g) + 16 * (r >> 2));
+    const uint32_t read_at = (uint32_t)((4 * hh + (r >> 2)) * S::kVPitch +
+                                        16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ hh) + 8 * (lane & 1));
 
     Start w;
     const bool busy = find_start(a, worker, kWideRows, kWideKeys, w);
@@ -304,16 +340,14 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
 
         RawWideQuery<D> raw_query;
         load_wide_query<D>(a, (req.first + token) * a.q_st + head * a.q_sh, valid, hh, raw_query);
-        Places places = find_places<4>(a, w.b, h, mx_token_bytes(D), begin, kWideKeys, end, lane);
+        WidePlaces places = find_wide_places<D>(a, w.b, h, begin, end, lane);
         WideKeyTile<D> keys;
         WideValueTile<D> now, next;
-        keys.live = 0;
         if (tiles > 0) {
-            load_keys<D>(a, places, 0, lane, keys);
+            load_keys<D>(find_keys<D>(places, 0, lane), keys);
             load_values<D>(a, places, 0, wave, lane, begin, now);
-            next = now;
-            if (tiles > 1)
-                load_values<D>(a, places, 1, wave, lane, begin + kWideKeys, next);
+            if constexpr (S::kFp16)
+                load_values<D>(a, places, min(1, tiles - 1), wave, lane, begin + kWideKeys, next);
         }
         Rows query;
         split_wide_query<D, kPieces, kHalf>(a, raw_query, query, more_query[wave], lane);
@@ -330,25 +364,62 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
             bool held = true;
 #pragma unroll
             for (int c = 0; c < S::kVChunks; ++c) {
-                t.vs[c] = any(t.key + r) ? t.vs[c] : 127;
+                t.vs[c] = any(t.key + r) ? t.vs[c] >> (8 * (D < 128 ? g & 1 : g)) & 255u : 127;
                 held = held & half_holds(t.vs[c], t.v[c]);
             }
-            const bool all = __all(held);
-            if (lane == 0)
-                held_by[buffer][wave] = all;
+            if constexpr (S::kFp16)
+                held_by[buffer][wave] = __all(held);
         };
-        auto all_held = [&](int buffer) {
-            const uint4 f = *reinterpret_cast<const uint4*>(held_by[buffer]);
-            return __builtin_amdgcn_readfirstlane(f.x & f.y & f.z & f.w) != 0;
-        };
+        uint32_t live_next = (uint32_t)places.live & 15u;  // which of the next tile's subtiles have a block
+        bool all_held = false;  // by fp16, the next tile's values
+        auto read_held = [&](int buffer) { return *reinterpret_cast<const uint4*>(held_by[buffer]); };
+        auto set_held = [&](uint4 f) { all_held = __builtin_amdgcn_readfirstlane(f.x & f.y & f.z & f.w) != 0; };
 
         auto step = [&](auto kind, int32_t i) {
             constexpr bool kFast = decltype(kind)::value;
             constexpr int kPPieces = kFast && kPieces == 2 ? 1 : 2;
             const int buffer = i & 1;
             const int32_t key = begin + i * kWideKeys;
-            // ---- this tile's V into LDS; whether the next one's can go as fp16
-            asm volatile("" ::: "memory");
+            constexpr int kAheadOf = S::kFp16 ? 2 : 1;  // tiles that V is loaded ahead
+            auto refresh = [&] {
+                if (i + kAheadOf < tiles && ((i + kAheadOf) & 15) == 0)
+                    places = find_wide_places<D>(a, w.b, h, key + kAheadOf * kWideKeys, end, lane);
+            };
+            if constexpr (!S::kFp16) {
+                look(now, buffer);
+                refresh();
+            }
+            const WideKeyAt next_keys = find_keys<D>(places, min(i + 1, tiles - 1), lane);
+            const uint32_t live = live_next;
+            live_next = (uint32_t)(places.live >> (4 * ((i + 1) & 15))) & 15u;
+            if constexpr (S::kFp16)
+                refresh();
+            // ---- scores; between the matrix instructions this tile's V into LDS
+            f32x16_t s[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    s[t][j] = 0.f;
+#pragma unroll
+            for (int q = 0; q < S::kChunks * kPieces; ++q) {
+                const int c = q % S::kChunks, piece = q / S::kChunks;
+                v8i_t rows_q;
+                if (piece >= Rows::kHeld) {
+                    const uint4* at = more_query[wave] + 128 * (q - Rows::kHeld * S::kChunks) + lane;
+                    const uint4 x = at[0], y = at[64];
+                    rows_q = v8i_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+                } else {
+                    rows_q = query.q[q];
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const v8i_t k = key_operand(__builtin_bit_cast(uint4, keys.k[t][c]));
+                    const int scales = (int)(keys.ks[t][c / 2] >> 8 * hh), q_scale = piece_scale(query.scale, piece);
+                    s[t] = c & 1 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, rows_q, s[t], 4, 0, 2, scales, 0, q_scale)
+                                 : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, rows_q, s[t], 4, 0, 0, scales, 0, q_scale);
+                }
+            }
 #pragma unroll
             for (int c = 0; c < S::kVChunks; ++c) {
                 uint32_t byte = now.vs[c];
@@ -361,59 +432,46 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
                     byte = byte == 255u ? 0 : byte;
                 }
                 const float scale = __uint_as_float(byte << 23);
-                uint4 q = now.v[c];
-                q = turn & 1 ? make_uint4(q.y, q.z, q.w, q.x) : q;
-                q = turn & 2 ? make_uint4(q.z, q.w, q.x, q.y) : q;
-                if (D >= 128 || g < 2) {
-                    uint8_t* to = turned[buffer] + 256 * c;
-                    *reinterpret_cast<uint4*>(to + write_at[0]) = wide_values<kFast>(q.x, scale);
-                    *reinterpret_cast<uint4*>(to + write_at[1]) = wide_values<kFast>(q.y, scale);
-                    *reinterpret_cast<uint4*>(to + write_at[2]) = wide_values<kFast>(q.z, scale);
-                    *reinterpret_cast<uint4*>(to + write_at[3]) = wide_values<kFast>(q.w, scale);
-                }
+                // D = 64: both halves of the wave write the same values
+                const uint32_t to = (uint32_t)(buffer * S::kVBytes) + write_at;
+                const uint32_t words[4] = {now.v[c].x, now.v[c].y, now.v[c].z, now.v[c].w};
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+                    *reinterpret_cast<uint4*>(turned[0] + (to ^ (16 * p)) + 256 * c) = wide_values<kFast>(words[p], scale);
             }
-            now = next;
-            look(now, buffer ^ 1);
-            asm volatile("" ::: "memory");
+            if constexpr (kFast)
+#pragma unroll
+            for (int q = 0; q < S::kChunks * kPieces * 2; ++q) {
+                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kValu, 12 / kPieces, 0);
+                __builtin_amdgcn_sched_group_barrier(kLdsWrite, 1, 0);
+            }
+            if constexpr (S::kFp16) {
+                now = next;
+                look(now, buffer ^ 1);
+            }
+            // ---- the next tile of K, and the one after it of V
+            load_keys<D>(next_keys, keys);
+            load_values<D>(a, places, min(i + kAheadOf, tiles - 1), wave, lane, key + kAheadOf * kWideKeys,
+                           S::kFp16 ? next : now);
+            lds_barrier();
+            uint4 held = {};
+            if constexpr (S::kFp16)
+                held = read_held(buffer ^ 1);
 
-            // ---- scores
-            const bool active = (key <= wave_last) & ((a.window == 0) | (key + kWideKeys > wave_first - a.window + 1));
-            f32x16_t s[2];
-            if (active) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        s[t][j] = 0.f;
-#pragma unroll
-                for (int q = 0; q < S::kChunks * kPieces; ++q) {
-                    const int c = q % S::kChunks, piece = q / S::kChunks;
-                    v8i_t rows_q;
-                    if (piece >= Rows::kHeld) {
-                        const uint4* at = more_query[wave] + 128 * (q - Rows::kHeld * S::kChunks) + lane;
-                        const uint4 x = at[0], y = at[64];
-                        rows_q = v8i_t{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
-                    } else {
-                        rows_q = query.q[q];
-                    }
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-                        s[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key_operand(keys.k[t][c]), rows_q, s[t], 4,
-                                                                               0, 0, (int)keys.ks[t][c], 0,
-                                                                               piece_scale(query.scale, piece));
-                }
+            {
                 const bool plain = (key + kWideKeys - 1 <= min(wave_first, end - 1)) &
-                                   ((a.window == 0) | (key > wave_last - a.window)) & (keys.live == 15u);
+                                   ((a.window == 0) | (key > wave_last - a.window)) & (live == 15u);
                 if (!plain) {
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
-                            const int32_t base = keys.live >> (2 * t + u) & 1 ? key + 32 * t + 16 * u : kNoKey;
+                            int32_t base = (live >> (2 * t + u) & 1 ? key + 32 * t + 16 * u : kNoKey) + 4 * hh;
+                            asm("" : "+v"(base));  // one register in all, not one for each key
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
-                                s[t][8 * u + j] =
-                                    seen(base + 8 * (j / 4) + 4 * hh + j % 4) ? s[t][8 * u + j] : -INFINITY;
+                                s[t][8 * u + j] = seen(base + 8 * (j / 4) + j % 4) ? s[t][8 * u + j] : -INFINITY;
                         }
                 }
                 float most = -INFINITY;
@@ -432,71 +490,76 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
                         acc[d] *= alpha;
                     m_run = m_new;
                 }
-            }
-            // ---- the next tile of K, and the one after it of V
-            if (i + 1 < tiles)
-                load_keys<D>(a, places, i + 1, lane, keys);
-            if (i + 2 < tiles) {
-                if (((i + 2) & 15) == 0)
-                    places = find_places<4>(a, w.b, h, mx_token_bytes(D), key + 2 * kWideKeys, kWideKeys, end, lane);
-                load_values<D>(a, places, i + 2, wave, lane, key + 2 * kWideKeys, next);
-            }
-            uint4 pw[kPPieces][4];  // by 16 keys: keys 4h..4h+3 and 8+4h..8+4h+3 of them
-            if (active) {
-                const float m_use = (m_run == -INFINITY ? 0.f : m_run) - (kFast ? (float)kHalfShift : 0.f);
-                const bool far = __any(fabsf(m_use) > kFar);
-                float sum = 0.f;
+                float m_use = (m_run == -INFINITY ? 0.f : m_run) - (kFast ? (float)kHalfShift : 0.f);
+                float times = a.scale_f;
+                if (__any(fabsf(m_use) > kFar)) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    float p[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        p[j] = __builtin_fmaf(s[t][j], a.scale_f, -m_use);
-                    if (far) {
+                    for (int t = 0; t < 2; ++t)
 #pragma unroll
                         for (int j = 0; j < 16; ++j)
-                            p[j] = s[t][j] * a.scale_f - m_use;
+                            s[t][j] = s[t][j] * a.scale_f - m_use;
+                    times = 1.f;
+                    m_use = 0.f;
+                }
+                // Products of the first 32 keys' values go between the second's exponentials, and those
+                // between the sums; operands are read kFetch products ahead.
+                constexpr int kOps = 2 * (D / 32), kFetch = D == 128 ? 3 : 2;
+                const uint32_t from0 = (uint32_t)(buffer * S::kVBytes) + read_at;
+                const uint32_t from1 = (from0 + 8 * S::kVPitch) ^ 32;
+                float p[32];
+                uint4 pw[2][kPPieces][2];  // by 16 keys: keys 4h..4h+3 and 8+4h..8+4h+3 of them
+                uint4 v[2 * kOps];
+                auto fetch = [&](int q) {
+                    if (q < 2 * kOps) {
+                        const uint8_t* at = turned[0] + 16 * (q / (D / 32)) * S::kVPitch + 64 * (q % (D / 32));
+                        const uint2 x = read_turned(at + from0), y = read_turned(at + from1);
+                        v[q] = make_uint4(x.x, x.y, y.x, y.y);
                     }
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        p[j] = __builtin_amdgcn_exp2f(p[j]);
-                        sum += p[j];
-                    }
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float* x = p + 8 * u;
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            hi[j] = pack_pair<kFast>(x[2 * j], x[2 * j + 1]);
-                            lo[j] = kPPieces == 2 ? pack_pair<kFast>(x[2 * j] - first_of<kFast>(hi[j]),
-                                                                     x[2 * j + 1] - second_of<kFast>(hi[j]))
-                                                  : 0;
-                        }
-                        pw[0][2 * t + u] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                };
+                auto weigh = [&](int j) {
+                    p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 16][j % 16], times, -m_use));
+                    if (j & 1) {
+                        const uint32_t hi = pack_pair<kFast>(p[j - 1], p[j]);
+                        uint32_t* to = &pw[j / 16][0][j / 8 % 2].x;
+                        to[j / 2 % 4] = hi;
                         if constexpr (kPPieces == 2)
-                            pw[1][2 * t + u] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            (&pw[j / 16][1][j / 8 % 2].x)[j / 2 % 4] =
+                                pack_pair<kFast>(p[j - 1] - first_of<kFast>(hi), p[j] - second_of<kFast>(hi));
                     }
+                };
+                auto product = [&](int q) {
+                    const int t = q / kOps, u = q / (D / 32) % 2, d = q % (D / 32);
+#pragma unroll
+                    for (int piece = 0; piece < kPPieces; ++piece)
+                        acc[d] = wide_product<kFast>(v[q], pw[t][piece][u], acc[d]);
+                };
+#pragma unroll
+                for (int q = 0; q < kFetch; ++q)
+                    fetch(q);
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    weigh(j);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int q = 0; q < kOps; ++q) {
+                    fetch(q + kFetch);
+                    product(q);
+#pragma unroll
+                    for (int j = 16 + q * 16 / kOps; j < 16 + (q + 1) * 16 / kOps; ++j)
+                        weigh(j);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                float sum = 0.f;
+#pragma unroll
+                for (int q = kOps; q < 2 * kOps; ++q) {
+                    fetch(q + kFetch);
+                    product(q);
+#pragma unroll
+                    for (int j = (q - kOps) * 32 / kOps; j < (q + 1 - kOps) * 32 / kOps; ++j)
+                        sum += p[j];
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 l_run += kFast ? sum * (1.0f / (1 << kHalfShift)) : sum;
-            }
-            lds_barrier();
-            if (active) {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const uint8_t* from = turned[buffer] + read_at + 16 * u * S::kVPitch;
-                    uint4 v[D / 32];
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d) {
-                        const uint2 x = read_turned(from + 64 * d), y = read_turned(from + 8 * S::kVPitch + 64 * d);
-                        v[d] = make_uint4(x.x, x.y, y.x, y.y);
-                    }
-#pragma unroll
-                    for (int q = 0; q < kPPieces; ++q)
-#pragma unroll
-                        for (int d = 0; d < D / 32; ++d)
-                            acc[d] = wide_product<kFast>(v[d], pw[q][u], acc[d]);
-                }
                 if constexpr (!kFast) {
                     // value blocks that are NaN, for the rows that see them
 #pragma unroll
@@ -516,24 +579,36 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
                         }
                 }
             }
+            set_held(held);
         };
 
         if (tiles > 0) {
-            look(now, 0);
-            lds_barrier();
+            if constexpr (S::kFp16) {
+                look(now, 0);
+                lds_barrier();
+                set_held(read_held(0));
+            }
             int32_t i = 0;
-            for (; i < tiles && all_held(i & 1); ++i)
-                step(Yes{}, i);
+            if constexpr (S::kFp16)
+                for (; i < tiles && all_held; ++i)
+                    step(Yes{}, i);
             for (; i < tiles; ++i)
                 step(No{}, i);
         }
 
         l_run += __shfl_xor(l_run, 32);
         lds_barrier();  // V was read
+        int lane_again = lane;
+        asm("" : "+v"(lane_again));  // what follows from it takes no registers in the loops
+        const int end_n = lane_again & 31, end_hh = lane_again >> 5;
+        const int32_t end_row = wave_row0 + end_n;
+        const bool end_valid = end_row < rows;
+        const int32_t end_token = (end_valid ? end_row : 0) / a.group;
+        const int32_t end_head = h * a.group + (end_valid ? end_row - end_token * a.group : 0);
         if (whole) {
-            const RowEnd e = finish_row(a, head, m_run, l_run);
-            if (valid && hh == 0)
-                a.lse[(req.first + token) * a.lse_st + head] = e.lse;
+            const RowEnd e = finish_row(a, end_head, m_run, l_run);
+            if (end_valid && end_hh == 0)
+                a.lse[(req.first + end_token) * a.lse_st + end_head] = e.lse;
             // through LDS, so that whole rows are written: the wave's 32 rows in its own quarter
             uint8_t* stage = &turned[0][0] + wave * 32 * S::kOPitch;
 #pragma unroll
@@ -542,14 +617,14 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
                 for (int q = 0; q < 4; ++q) {
                     const float x0 = acc[d][4 * q] * e.inv, x1 = acc[d][4 * q + 1] * e.inv;
                     const float x2 = acc[d][4 * q + 2] * e.inv, x3 = acc[d][4 * q + 3] * e.inv;
-                    *reinterpret_cast<uint2*>(stage + n * S::kOPitch + 2 * (32 * d + 8 * q + 4 * hh)) =
+                    *reinterpret_cast<uint2*>(stage + end_n * S::kOPitch + 2 * (32 * d + 8 * q + 4 * end_hh)) =
                         make_uint2(pack_pair<kHalf>(x0, x1), pack_pair<kHalf>(x2, x3));
                 }
             asm volatile("" ::: "memory");
             constexpr int kPieceLanes = D / 8;  // lanes of 16 bytes a row
 #pragma unroll 2
             for (int base = 0; base < 32; base += 64 / kPieceLanes) {
-                const int mine = base + lane / kPieceLanes, piece = lane % kPieceLanes;
+                const int mine = base + lane_again / kPieceLanes, piece = lane_again % kPieceLanes;
                 const int32_t out_row = wave_row0 + mine;
                 const uint4 x = *reinterpret_cast<const uint4*>(stage + mine * S::kOPitch + 16 * piece);
                 if (out_row < rows) {
@@ -569,18 +644,18 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
                     }
                 }
             }
-        } else if (valid) {
+        } else if (end_valid) {
             // a worker's first slot holds the tile that came from the one before, its second the one that goes on
             float* slot = a.partials + slot_of(a, h, worker, unit == 0) * slot_floats(D, kWideRows);
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<f32x4_t*>(slot + (32 * wave + n) * D + 32 * d + 8 * q + 4 * hh) =
+                    *reinterpret_cast<f32x4_t*>(slot + (32 * wave + end_n) * D + 32 * d + 8 * q + 4 * end_hh) =
                         f32x4_t{acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]};
-            if (hh == 0) {
-                slot[kWideRows * D + 32 * wave + n] = m_run;
-                slot[kWideRows * D + kWideRows + 32 * wave + n] = l_run;
+            if (end_hh == 0) {
+                slot[kWideRows * D + 32 * wave + end_n] = m_run;
+                slot[kWideRows * D + kWideRows + 32 * wave + end_n] = l_run;
             }
         }
         left -= cost;

@@ -247,8 +247,8 @@ __device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int
     start.tiles.req.len = __builtin_amdgcn_readfirstlane(found[5]);
     start.tiles.count = __builtin_amdgcn_readfirstlane(found[6]);
     start.tiles.units = __builtin_amdgcn_readfirstlane(found[7]);
-    start.each = (int32_t)each;
-    start.take = (int32_t)(total - first < each ? total - first : each);
+    start.each = __builtin_amdgcn_readfirstlane((int32_t)each);
+    start.take = __builtin_amdgcn_readfirstlane((int32_t)(total - first < each ? total - first : each));
     return true;
 }
 

@@ -15,7 +15,7 @@ What the kernels may be off, row by row (``bounds``), counted before their first
 * scores are scaled and exp2 taken in 32 bits: 2^-20 (1 + |s|) together covers the
   scaling, the subtraction and two ulp of the exponential;
 * P enters as two bf16 pieces (2^-16).  Where a request has more than 64 rows for a key head (or
-  is alone), bf16 calls have one fp16 piece of it, 2^-11, and both types lose of P times 2^7 what lies
+  is alone) and D is at most 128, bf16 calls have one fp16 piece of it, 2^-11, and both types lose of P times 2^7 what lies
   below fp16's least step, half of 2^-24: under a reference of at most 2^4 times the row's largest
   that is 2^(-25 - 7 + 4) = 2^-28 of the row's largest a key;
 * P below 2^-126 is nothing in 32 bits (the first run showed that this had been left out: a dim
@@ -149,7 +149,7 @@ def reference(q, cache, table, lens, start, scale, window=None, sink=None):
             weight = p @ torch.where(nan, 0.0, vh).abs() * share[:, None]
             o = o * share[:, None]
             half = torch.finfo(q.dtype).eps / 2
-            many = (t1 - t0) * group > 64 or len(lens) == 1
+            many = dim <= 128 and ((t1 - t0) * group > 64 or len(lens) == 1)
             ob = weight * ((2.0 ** -11 if many and not three else 2.0 ** -16) + 2.5 * d + steps)[:, None] * (1 + half)
             if many:
                 ob = ob + 2.0 ** -28 * (p.amax(1) * share)[:, None] * torch.where(nan, 0.0, vh).abs().sum(0)
