@@ -105,34 +105,37 @@ __device__ __forceinline__ uint32_t scales_of(uint64_t at) {
     return D == 64 ? *global<uint16_t>(at) : *global<uint32_t>(at);
 }
 
-// What this lane loads of a tile of K: keys l % 32 of its halves.
+// Where the subtiles lie that hold this lane's keys of a tile: l % 32 of its halves.
 struct WideKeyAt {
     uint64_t codes[2], scales[2];
 };
 
 template <int D>
 __device__ __forceinline__ WideKeyAt find_keys(const WidePlaces& p, int tile, int lane) {
-    const int r = lane & 15, h = lane >> 5, upper = lane >> 4 & 1;
+    const int upper = lane >> 4 & 1;
     WideKeyAt at;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int from = (tile & 15) * 4 + 2 * t + upper;
-        at.codes[t] = from_lane(p.codes, from) + (uint32_t)(r * (D / 2) + 16 * h);
-        at.scales[t] = from_lane(p.scales, from) + (uint32_t)(r * (D / kMxBlock));
+        at.codes[t] = from_lane(p.codes, from);
+        at.scales[t] = from_lane(p.scales, from);
     }
     return at;
 }
 
 template <int D>
-__device__ __forceinline__ void load_keys(const WideKeyAt& at, WideKeyTile<D>& out) {
+__device__ __forceinline__ void load_keys(const WideKeyAt& at, int lane, WideKeyTile<D>& out) {
+    const int r = lane & 15, h = lane >> 5;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+        const uint64_t codes = at.codes[t] + (uint32_t)(r * (D / 2) + 16 * h);
+        const uint64_t scales = at.scales[t] + (uint32_t)(r * (D / kMxBlock));
 #pragma unroll
         for (int i = 0; i < D / 64; ++i)
-            out.k[t][i] = *global<u32x4_t>(at.codes[t] + 32 * i);
+            out.k[t][i] = *global<u32x4_t>(codes + 32 * i);
 #pragma unroll
         for (int i = 0; i < (D + 127) / 128; ++i)
-            out.ks[t][i] = scales_of<D>(at.scales[t] + 4 * i);
+            out.ks[t][i] = scales_of<D>(scales + 4 * i);
     }
 }
 
@@ -272,8 +275,7 @@ __device__ __forceinline__ f32x16_t wide_product(uint4 v, uint4 p, f32x16_t acc)
                                                        __builtin_bit_cast(bf16x8_t, p), acc, 0, 0, 0);
 }
 
-// What sched_group_barrier takes.
-constexpr int kValu = 0x2, kMfma = 0x8, kLdsRead = 0x100, kLdsWrite = 0x200;
+constexpr int kLdsRead = 0x100;  // what sched_barrier lets pass
 
 struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
         WideKeyTile<D> keys;
         WideValueTile<D> now, next;
         if (tiles > 0) {
-            load_keys<D>(find_keys<D>(places, 0, lane), keys);
+            load_keys<D>(find_keys<D>(places, 0, lane), lane, keys);
             load_values<D>(a, places, 0, wave, lane, begin, now);
             if constexpr (S::kFp16)
                 load_values<D>(a, places, min(1, tiles - 1), wave, lane, begin + kWideKeys, next);
@@ -395,12 +397,26 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
             if constexpr (S::kFp16)
                 refresh();
             // ---- scores; between the matrix instructions this tile's V into LDS
+            __builtin_amdgcn_s_setprio(1);
             f32x16_t s[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
                     s[t][j] = 0.f;
+            const uint32_t to = (uint32_t)(buffer * S::kVBytes) + write_at;
+            float v_scale[S::kVChunks];
+#pragma unroll
+            for (int c = 0; c < S::kVChunks; ++c) {
+                uint32_t byte = now.vs[c];
+                if constexpr (kFast) {
+                    byte = max(byte, (uint32_t)kHalfShift) - kHalfShift;
+                } else {
+                    nan_of[buffer][wave][c] = __ballot(byte == 255u);
+                    byte = byte == 255u ? 0 : byte;
+                }
+                v_scale[c] = __uint_as_float(byte << 23);
+            }
 #pragma unroll
             for (int q = 0; q < S::kChunks * kPieces; ++q) {
                 const int c = q % S::kChunks, piece = q / S::kChunks;
@@ -418,40 +434,24 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
                     const int scales = (int)(keys.ks[t][c / 2] >> 8 * hh), q_scale = piece_scale(query.scale, piece);
                     s[t] = c & 1 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, rows_q, s[t], 4, 0, 2, scales, 0, q_scale)
                                  : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, rows_q, s[t], 4, 0, 0, scales, 0, q_scale);
+                    const int part = 2 * q + t;
+                    if (part < 4 * S::kVChunks) {
+                        // (D = 64: both halves of the wave write the same values)
+                        const uint32_t words[4] = {now.v[part / 4].x, now.v[part / 4].y, now.v[part / 4].z, now.v[part / 4].w};
+                        *reinterpret_cast<uint4*>(turned[0] + (to ^ (16 * (part % 4))) + 256 * (part / 4)) =
+                            wide_values<kFast>(words[part % 4], v_scale[part / 4]);
+                    }
+                    __builtin_amdgcn_sched_barrier(kLdsRead);
                 }
             }
-#pragma unroll
-            for (int c = 0; c < S::kVChunks; ++c) {
-                uint32_t byte = now.vs[c];
-                if constexpr (kFast) {
-                    byte = max(byte, (uint32_t)kHalfShift) - kHalfShift;
-                } else {
-                    const uint64_t nan = __ballot(byte == 255u);
-                    if (lane == 0)
-                        nan_of[buffer][wave][c] = nan;
-                    byte = byte == 255u ? 0 : byte;
-                }
-                const float scale = __uint_as_float(byte << 23);
-                // D = 64: both halves of the wave write the same values
-                const uint32_t to = (uint32_t)(buffer * S::kVBytes) + write_at;
-                const uint32_t words[4] = {now.v[c].x, now.v[c].y, now.v[c].z, now.v[c].w};
-#pragma unroll
-                for (int p = 0; p < 4; ++p)
-                    *reinterpret_cast<uint4*>(turned[0] + (to ^ (16 * p)) + 256 * c) = wide_values<kFast>(words[p], scale);
-            }
-            if constexpr (kFast)
-#pragma unroll
-            for (int q = 0; q < S::kChunks * kPieces * 2; ++q) {
-                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(kValu, 12 / kPieces, 0);
-                __builtin_amdgcn_sched_group_barrier(kLdsWrite, 1, 0);
-            }
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
             if constexpr (S::kFp16) {
                 now = next;
                 look(now, buffer ^ 1);
             }
             // ---- the next tile of K, and the one after it of V
-            load_keys<D>(next_keys, keys);
+            load_keys<D>(next_keys, lane, keys);
             load_values<D>(a, places, min(i + kAheadOf, tiles - 1), wave, lane, key + kAheadOf * kWideKeys,
                            S::kFp16 ? next : now);
             lds_barrier();
@@ -474,15 +474,15 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
                                 s[t][8 * u + j] = seen(base + 8 * (j / 4) + j % 4) ? s[t][8 * u + j] : -INFINITY;
                         }
                 }
-                float most = -INFINITY;
+                float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        most = fmaxf(most, s[t][j]);
-                most = pair_max(most) * a.scale_f;
-                if (__any(most > m_run)) {
-                    const float m_new = most > m_run ? most + kAhead : m_run;
+                for (int j = 0; j < 16; ++j) {
+                    most[j & 1] = fmaxf(most[j & 1], s[0][j]);
+                    most[2 + (j & 1)] = fmaxf(most[2 + (j & 1)], s[1][j]);
+                }
+                const float top = pair_max(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * a.scale_f;
+                if (__any(top > m_run)) {
+                    const float m_new = top > m_run ? top + kAhead : m_run;
                     const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
                     l_run *= alpha;
 #pragma unroll
