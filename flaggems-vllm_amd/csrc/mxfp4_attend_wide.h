@@ -330,14 +330,11 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
         seen.count = valid ? (uint32_t)max(pos0 + token - seen.first + 1, 0) : 0;
         any.first = a.window > 0 ? first_pos - a.window + 1 : 0;
         any.count = (uint32_t)max(last_pos - any.first + 1, 0);
-        int32_t begin, end;
-        key_range(a, req, begin, end);
+        int32_t begin = keys_begin(a, first_pos), end = min(min(req.len, a.table_keys), last_pos + 1);
         if (!whole) {
-            begin += unit * kWideKeys;  // below the request's end
-            end = units <= (end - begin) / kWideKeys ? begin + units * kWideKeys : end;
+            begin += unit * kWideKeys;
+            end = min(end, begin + units * kWideKeys);
         }
-        end = min(end, last_pos + 1);
-        begin = max(begin, max(any.first, 0) & ~(kTileKeys - 1));
         const int32_t tiles = end > begin ? (end - begin + kWideKeys - 1) / kWideKeys : 0;
 
         RawWideQuery<D> raw_query;

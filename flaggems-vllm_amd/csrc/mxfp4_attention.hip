@@ -127,10 +127,9 @@ __device__ __forceinline__ Request request_of(const AttArgs& a, int32_t b) {
     return r;
 }
 
-// Keys that a request's tokens see, from the first tile boundary on.
-__device__ __forceinline__ void key_range(const AttArgs& a, const Request& r, int32_t& begin, int32_t& end) {
-    end = min(r.len, a.table_keys);
-    begin = a.window > 0 ? max(r.len - r.count - a.window + 1, 0) & ~(kTileKeys - 1) : 0;
+// The first tile boundary in front of what a row at position `pos` sees.
+__device__ __forceinline__ int32_t keys_begin(const AttArgs& a, int32_t pos) {
+    return a.window > 0 ? max(pos - a.window + 1, 0) & ~(kTileKeys - 1) : 0;
 }
 
 // A request and its tiles of rows, `units` units of keys each, dealt out as `cost`.
@@ -147,9 +146,12 @@ __device__ __forceinline__ Tiles tiles_of(const AttArgs& a, int32_t b, int32_t r
     t.count = rows >= a.rows_from && rows <= a.rows_to ? (rows + rows_per_tile - 1) / rows_per_tile : 0;
     t.units = 1;
     if (a.workers > 0) {
-        int32_t begin, end;
-        key_range(a, t.req, begin, end);
-        t.units = max((end - begin + unit_keys - 1) / unit_keys, 1);
+        // the same for all tiles, as many as the longest can have: all keys from its first row's on, or what
+        // its rows' windows cover
+        int32_t keys = min(t.req.len, a.table_keys) - keys_begin(a, t.req.len - t.req.count);
+        if (a.window > 0)
+            keys = min(keys, a.window + (rows_per_tile + a.group - 2) / a.group + kTileKeys);
+        t.units = max((keys + unit_keys - 1) / unit_keys, 1);
     }
     return t;
 }
@@ -762,14 +764,11 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
         seen.count = valid ? (uint32_t)max(pos0 + token - seen.first + 1, 0) : 0;
         any.first = a.window > 0 ? first_pos - a.window + 1 : 0;
         any.count = (uint32_t)max(last_pos - any.first + 1, 0);
-        int32_t begin, end;
-        key_range(a, req, begin, end);
+        int32_t begin = keys_begin(a, first_pos), end = min(min(req.len, a.table_keys), last_pos + 1);
         if (!whole) {
-            begin += unit * kUnit;  // below the request's end
-            end = units <= (end - begin) / kUnit ? begin + units * kUnit : end;
+            begin += unit * kUnit;
+            end = min(end, begin + units * kUnit);
         }
-        end = min(end, last_pos + 1);
-        begin = max(begin, max(any.first, 0) & ~(kTileKeys - 1));
 
         const int32_t key0 = begin + wave * kKeys;
         const int32_t tiles = end > key0 ? (end - key0 + kUnit - 1) / kUnit : 0;
@@ -1018,8 +1017,9 @@ Dealing dealing_of(const Call& c, bool wide) {
     d.tiles = c.tokens * group / tile_rows + c.reqs;
     int64_t workers = slots / c.kv_heads;
     workers = workers < 1 ? 1 : workers > kMostWorkers ? kMostWorkers : workers;
-    // Nothing to cut; or (128-row tiles take long, and the first to end take the next) enough of them.
-    if (c.max_seq <= kWholeUnits * unit || (wide && d.tiles * c.kv_heads >= 2 * slots + c.reqs * c.kv_heads))
+    // Nothing to cut; or two 128-row tiles a workgroup and more.  Their partial results are 66 KB at D = 128: prompts
+    // of 1140 tiles on 512 workgroups took 151 us with cuts, which leave no workgroup idle, and 108 without.
+    if (c.max_seq <= kWholeUnits * unit || (wide && (d.tiles - c.reqs) * c.kv_heads >= 2 * slots))
         return d;
     d.workers = (int32_t)workers;
     d.cut_tiles_at = 2 * workers * c.kv_heads * (int64_t)slot_floats((int)c.dim, (int)tile_rows) * 4;
