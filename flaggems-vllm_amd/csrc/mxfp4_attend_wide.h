@@ -293,7 +293,6 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
     const int n = lane & 31, hh = lane >> 5, r = lane & 15, g = lane >> 4;
     const int h = (int)blockIdx.x % a.kv_heads;
     const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads);
-    const int32_t tile_cost = a.workers > 0 ? kTileCost : 0;
     // Where this lane writes its first 16-byte piece of V, and reads V turned: piece i of a 64-byte run
     // lies at i ^ (row / 4 % 4), so that neither the lanes of a write nor of a read meet a bank twice.
     static_assert(S::kVPitch % 64 == 0 && S::kVBytes % 64 == 0, "pieces are found by xor");
@@ -308,8 +307,8 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
     while (left > 0) {
         const Request req = w.tiles.req;
         const int32_t cost = min(left, w.tiles.cost(a) - w.at);
-        const int32_t unit = max(w.at - tile_cost, 0);
-        const int32_t units = a.workers > 0 ? max(w.at + cost - tile_cost, 0) - unit : 1;
+        const int32_t unit = max(w.at - a.tile_cost, 0);
+        const int32_t units = max(w.at + cost - a.tile_cost, 0) - unit;
         if (units == 0)
             break;  // the tile begins with the next worker
         const bool whole = units == w.tiles.units;

@@ -57,7 +57,7 @@ constexpr int kMostWorkers = 1024;  // per head
 // Beginning and ending a tile (block table, query, joining the waves) costs as
 // much as this many more, so that a worker of many short tiles gets fewer units.
 constexpr int kTileCost = 4;
-constexpr int kLeastCost = kTileCost + 2;  // what a worker takes at least
+constexpr int kLeastCost = kTileCost + 1;  // what a worker takes at least
 // Tiles of no more units than this are not cut: joining cuts takes a launch, 5 us.
 constexpr int kWholeUnits = 8;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -97,7 +97,7 @@ struct AttArgs {
     int32_t q_wide, o_wide;
     int32_t rows_from, rows_to;  // requests of other numbers of rows are another launch's
     // Stream mode (workers > 0): workers per head, and the workspace's parts.
-    int32_t workers;
+    int32_t workers, per_cu, tile_cost;
     float* partials;
     struct CutTile* cut_tiles;
 };
@@ -136,7 +136,7 @@ __device__ __forceinline__ int32_t keys_begin(const AttArgs& a, int32_t pos) {
 struct Tiles {
     Request req;
     int32_t count, units;
-    __device__ int32_t cost(const AttArgs& a) const { return a.workers > 0 ? kTileCost + units : 1; }
+    __device__ int32_t cost(const AttArgs& a) const { return a.tile_cost + units; }
 };
 
 __device__ __forceinline__ Tiles tiles_of(const AttArgs& a, int32_t b, int32_t rows_per_tile, int32_t unit_keys) {
@@ -214,8 +214,14 @@ __device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int
         scan_turn(base, total);
     }
     uint32_t each = 1;
-    if (a.workers > 0)
-        each = max((total + a.workers - 1) / a.workers, (uint32_t)kLeastCost);
+    if (a.workers > 0) {
+        // as many workgroups to every CU, and fewer rather than with less than kLeastCost to do (24 requests of up to
+        // 20000 keys, D = 256: 285 workgroups with 7 each 27.5 us, 333 with 6 32.5, as most CUs had one and some two)
+        uint32_t to = (uint32_t)a.workers;
+        for (int32_t k = a.per_cu - 1; k > 0; --k)
+            to = total < to * (uint32_t)kLeastCost ? (uint32_t)(a.workers * k / a.per_cu) : to;
+        each = max((total + to - 1) / to, (uint32_t)kLeastCost);
+    }
     uint64_t first = (uint64_t)each * index;
     if (first >= total)
         return false;
@@ -735,7 +741,6 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
     const int h = (int)blockIdx.x % a.kv_heads;
     const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads);
     const int r = lane & 15, g = lane >> 4;
-    const int32_t tile_cost = a.workers > 0 ? kTileCost : 0;
     const int orow = threadIdx.x >> 4, part = threadIdx.x & 15;  // of the end: 16 threads per row
     Start w;
     const bool busy = find_start(a, worker, kRows, kUnit, w);
@@ -743,10 +748,10 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
     int32_t left = busy ? w.take : 0;
     while (left > 0) {
         const Request req = w.tiles.req;
-        // of the tile's cost kTileCost stands before its first unit
+        // of the tile's cost a.tile_cost stands before its first unit
         const int32_t cost = min(left, w.tiles.cost(a) - w.at);
-        const int32_t unit = max(w.at - tile_cost, 0);
-        const int32_t units = a.workers > 0 ? max(w.at + cost - tile_cost, 0) - unit : 1;
+        const int32_t unit = max(w.at - a.tile_cost, 0);
+        const int32_t units = max(w.at + cost - a.tile_cost, 0) - unit;
         if (units == 0)
             break;  // the tile begins with the next worker
         const bool whole = units == w.tiles.units;
@@ -1006,9 +1011,11 @@ struct Call {
     bool few() const { return !wide() || reqs > 1; }
 };
 
+int per_cu(int dim, bool wide) { return wide ? (dim == 256 ? 1 : 2) : groups_per_cu(dim); }
+
 Dealing dealing_of(const Call& c, bool wide) {
     const int64_t group = c.heads / c.kv_heads, tile_rows = wide ? kWideRows : kRows;
-    const int64_t slots = (wide ? (c.dim == 256 ? 1 : 2) : groups_per_cu((int)c.dim)) * cu_count();
+    const int64_t slots = per_cu((int)c.dim, wide) * cu_count();
     const int64_t unit = wide ? kWideKeys : unit_keys((int)c.dim);
     Dealing d = {};
     const int64_t rows = group * (c.max_query < 1 ? 1 : c.max_query < tile_rows ? c.max_query : tile_rows);
@@ -1032,6 +1039,8 @@ void launch_part(const Dealing& d, uint8_t* workspace, int64_t unit, hipStream_t
     // (the cost of all tiles has to fit 31 bits: with more of it there is nothing to gain either)
     const bool stream = workspace && d.workers > 0 && d.tiles * (kTileCost + 1 + a.table_keys / unit) <= 0x7fffffffLL;
     a.workers = stream ? d.workers : 0;
+    a.tile_cost = stream ? kTileCost : 0;
+    a.per_cu = per_cu(D, kTileRows == kWideRows);
     a.partials = reinterpret_cast<float*>(workspace);
     a.cut_tiles = reinterpret_cast<CutTile*>(workspace + d.cut_tiles_at);
     const unsigned grid = (unsigned)((stream ? d.workers : d.tiles) * a.kv_heads);
