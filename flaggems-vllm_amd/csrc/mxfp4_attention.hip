@@ -164,14 +164,15 @@ struct Start {
     int32_t take, each;
 };
 
-// Sum of v over the lanes up to this one.
+// Sum of v over the lanes up to this one; sums stay at 2^32 - 1.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
-    v += __builtin_amdgcn_update_dpp(0u, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0u, v, 0x111, 0xF, 0xF, false));  // row_shr:1, 2, 4, 8
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0u, v, 0x112, 0xF, 0xF, false));
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0u, v, 0x114, 0xF, 0xF, false));
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0u, v, 0x118, 0xF, 0xF, false));
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0u, v, 0x142, 0xA, 0xF, false));  // row_bcast:15 into rows 1 and 3
+    v = add_sat(v, __builtin_amdgcn_update_dpp(0u, v, 0x143, 0xC, 0xF, false));  // row_bcast:31 into rows 2 and 3
     return v;
 }
 
@@ -181,7 +182,8 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 // all tiles, one after the other, is dealt out evenly, so that workgroups have
 // the same to do whatever the lengths are; a tile that is longer than the
 // rest of its worker's share goes on with the next.  Otherwise a worker is a tile.
-// (The host sees to it that the cost fits 31 bits.)
+// (The host sees to it that the cost fits 31 bits.  Starts that fall could make it
+// more; then nothing is computed.)
 __device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int32_t rows_per_tile, int32_t unit_keys,
                                            Start& start) {
     __shared__ uint32_t part[kAttWaves];
@@ -194,17 +196,17 @@ __device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int
         n = 0;
         if (b < a.num_reqs) {
             mine = tiles_of(a, b, rows_per_tile, unit_keys);
-            n = (uint32_t)mine.count * mine.cost(a);
+            n = __umulhi(mine.count, mine.cost(a)) ? ~0u : (uint32_t)mine.count * mine.cost(a);
         }
         const uint32_t s = wave_scan(n);
         if (lane == 63)
             part[wave] = s;
         __syncthreads();
-        at = before + s - n;
+        at = add_sat(before, s - n);
 #pragma unroll
         for (int w = 0; w < kAttWaves; ++w) {
-            at += w < wave ? part[w] : 0;
-            before += part[w];
+            at = add_sat(at, w < wave ? part[w] : 0);
+            before = add_sat(before, part[w]);
         }
     };
     uint32_t total = 0;
@@ -223,7 +225,7 @@ __device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int
         each = max((total + to - 1) / to, (uint32_t)kLeastCost);
     }
     uint64_t first = (uint64_t)each * index;
-    if (first >= total)
+    if (first >= total || total == ~0u)
         return false;
     if (a.workers == 0)
         first = total - 1 - first;  // from the end: of a prompt's tiles the last have the most keys
