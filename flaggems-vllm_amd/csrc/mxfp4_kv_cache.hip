@@ -32,9 +32,9 @@ struct InsertArgs {
     const void* v;
     int64_t k_st, k_sh, v_st, v_sh;  // elements
     uint8_t* cache;
-    int64_t block_stride, num_blocks;
+    int64_t block_stride, num_slots;  // num_slots at most 2^32
     const int64_t* slots;
-    int32_t num_tokens, kv_heads, page;
+    uint32_t num_rows, kv_heads, page;  // rows: num_tokens * kv_heads
     uint32_t blocks_per_xcd;  // 0: in the launch's order
 };
 
@@ -118,24 +118,23 @@ __global__ void __launch_bounds__(kInsThreads) mxfp4_insert_kernel(InsertArgs a)
     uint32_t wg = blockIdx.x;
     if (a.blocks_per_xcd)
         wg = (wg & 7) * a.blocks_per_xcd + (wg >> 3);
-    const int64_t idx = (int64_t)wg * kInsThreads + threadIdx.x;
-    const int piece = (int)(idx % kPieces);
-    const int64_t row = idx / kPieces;
-    const int64_t t = row / a.kv_heads;
-    if (t >= a.num_tokens)
+    const int piece = threadIdx.x % kPieces;
+    const uint32_t row = wg * (kInsThreads / kPieces) + threadIdx.x / kPieces;
+    if (row >= a.num_rows)
         return;  // whole rows of lanes: the DPP steps of the others stay inside theirs
-    const int h = (int)(row - t * a.kv_heads);
+    const uint32_t t = row / a.kv_heads, h = row - t * a.kv_heads;
     uint32_t kw[4], vw[4];
-    load8<kWide>(a.k, t * a.k_st + h * a.k_sh + 8 * piece, kw);
-    load8<kWide>(a.v, t * a.v_st + h * a.v_sh + 8 * piece, vw);
+    load8<kWide>(a.k, t * a.k_st + (int64_t)h * a.k_sh + 8 * piece, kw);
+    load8<kWide>(a.v, t * a.v_st + (int64_t)h * a.v_sh + 8 * piece, vw);
     const int64_t slot = a.slots[t];
     uint32_t kb, vb;
     const uint32_t kc = mx_codes<kHalf>(kw, kb);
     const uint32_t vc = mx_codes<kHalf>(vw, vb);
-    const int64_t block = slot / a.page;
-    if (slot < 0 || block >= a.num_blocks)
+    if (slot < 0 || slot >= a.num_slots)
         return;
-    const int64_t page = a.page, place = slot - block * page;
+    // 32 bits: the 64-bit divisions of slot and row took more instructions than all the rest
+    const uint32_t block = (uint32_t)slot / a.page;
+    const int64_t page = a.page, place = (uint32_t)slot - block * a.page;
     uint8_t* head = a.cache + block * a.block_stride + h * page * mx_token_bytes(D);
     *reinterpret_cast<uint32_t*>(head + mx_part(0, page, D) + place * (D / 2) + 4 * piece) = kc;
     *reinterpret_cast<uint32_t*>(head + mx_part(1, page, D) + place * (D / 2) + 4 * piece) = vc;
@@ -178,8 +177,10 @@ extern "C" int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_toke
     if (num_kv_heads > 65536 || block_size > 4096)
         return fail(FGV_E_TOO_LARGE, "at most 65536 heads and 4096 tokens per block");
     const int64_t threads_per_token = num_kv_heads * (head_dim / 8);
-    if (num_tokens > 0x7fffffffLL * kInsThreads / threads_per_token || num_tokens > 0x7fffffffLL)
-        return fail(FGV_E_TOO_LARGE, "num_tokens * num_kv_heads is too large");
+    if (num_tokens > 0x7fffffffLL / num_kv_heads)
+        return fail(FGV_E_TOO_LARGE, "num_tokens * num_kv_heads must be below 2^31");
+    if (num_blocks > 0x100000000LL / block_size)
+        return fail(FGV_E_TOO_LARGE, "the cache may hold at most 2^32 tokens");
     if (!k || !v || !kv_cache || !slot_mapping)
         return fail(FGV_E_NULL_POINTER, "null pointer argument");
     if (cache_block_stride < num_kv_heads * block_size * mx_token_bytes((int)head_dim) || cache_block_stride % 16 != 0)
@@ -195,14 +196,14 @@ extern "C" int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_toke
     a.v_sh = v_stride_head;
     a.cache = kv_cache;
     a.block_stride = cache_block_stride;
-    a.num_blocks = num_blocks;
+    a.num_slots = num_blocks * block_size;
     a.slots = slot_mapping;
-    a.num_tokens = (int32_t)num_tokens;
-    a.kv_heads = (int32_t)num_kv_heads;
-    a.page = (int32_t)block_size;
+    a.num_rows = (uint32_t)(num_tokens * num_kv_heads);
+    a.kv_heads = (uint32_t)num_kv_heads;
+    a.page = (uint32_t)block_size;
     const int64_t groups = (num_tokens * threads_per_token + kInsThreads - 1) / kInsThreads;
     // a multiple of 8 workgroups, each XCD's a consecutive range (more than the grid's end: threads past the tokens leave)
-    a.blocks_per_xcd = groups >= 64 && groups < 0x7ffffff0LL ? (uint32_t)((groups + 7) / 8) : 0;
+    a.blocks_per_xcd = groups >= 64 ? (uint32_t)((groups + 7) / 8) : 0;
     const unsigned grid = a.blocks_per_xcd ? 8 * a.blocks_per_xcd : (unsigned)groups;
     const bool wide = aligned(k, 16) && aligned(v, 16) &&
                       ((k_stride_token | k_stride_head | v_stride_token | v_stride_head) & 7) == 0;
