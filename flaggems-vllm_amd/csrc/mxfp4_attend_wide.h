@@ -40,9 +40,7 @@ __device__ __forceinline__ bool half_holds(uint32_t byte, u32x4_t codes) {
 
 template <int D, int kPieces>
 struct WideShape {
-    static constexpr bool kFp16 = D <= 128;  // with both loops, more than registers hold of D = 256
     static constexpr int kChunks = D / 64;                // of 64 dims: one QK instruction per piece
-    static constexpr int kVChunks = D < 128 ? 1 : D / 128;  // of 128 dims: 16 bytes of codes a lane
     static constexpr int kVPitch = D == 64 ? 192 : 2 * D + 64;  // four rows of 64 bytes meet no bank twice
     static constexpr int kVBytes = kWideKeys * kVPitch;
     static constexpr int kOPitch = 2 * D + 16;
@@ -52,13 +50,13 @@ struct WideShape {
 template <int D>
 struct WideKeyTile {
     u32x4_t k[2][D / 64];
-    uint32_t ks[2][(D + 127) / 128];  // of 4 blocks, moved by h bytes: byte 0 or 2 is this lane's
+    uint32_t ks[2];  // the key's scales
 };
 
 template <int D>
 struct WideValueTile {
-    u32x4_t v[D < 128 ? 1 : D / 128];
-    uint32_t vs[D < 128 ? 1 : D / 128];  // of 4 blocks (2 where D = 64); `look` takes this lane's
+    u32x4_t v;    // 32 dims of a token
+    uint32_t vs;  // the token's scales; `look` takes this lane's
     int32_t key;  // of the first of the wave's 16 tokens, kNoKey: no block
 };
 
@@ -73,7 +71,7 @@ struct WidePlaces {
 template <int D>
 __device__ __forceinline__ WidePlaces find_wide_places(const AttArgs& a, int32_t b, int32_t h, int32_t key, int32_t end,
                                                        int lane) {
-    const Places p = find_places<4>(a, b, h, mx_token_bytes(D), key, kWideKeys, end, lane);
+    const Places p = find_places<4>(a, b, h, mx_token_bytes(D), key, kWideKeys, end, end, lane);
     const uint64_t head = (uint64_t)a.cache + (uint64_t)p.base;
     const uint32_t first = (uint32_t)max(p.place, 0);
     WidePlaces w;
@@ -133,9 +131,7 @@ __device__ __forceinline__ void load_keys(const WideKeyAt& at, int lane, WideKey
 #pragma unroll
         for (int i = 0; i < D / 64; ++i)
             out.k[t][i] = *global<u32x4_t>(codes + 32 * i);
-#pragma unroll
-        for (int i = 0; i < (D + 127) / 128; ++i)
-            out.ks[t][i] = scales_of<D>(scales + 4 * i);
+        out.ks[t] = scales_of<D>(scales);
     }
 }
 
@@ -147,11 +143,8 @@ __device__ __forceinline__ void load_values(const AttArgs& a, const WidePlaces& 
     const uint64_t codes = from_uniform(p.codes, from) + (uint64_t)mx_part(1, a.page, D);
     const uint64_t scales = from_uniform(p.scales, from) + (uint64_t)a.page * (D / kMxBlock);
     out.key = p.live >> from & 1 ? key0 + 16 * wave : kNoKey;
-#pragma unroll
-    for (int c = 0; c < (D < 128 ? 1 : D / 128); ++c) {
-        out.v[c] = *global<u32x4_t>(codes + (uint32_t)(r * (D / 2) + 64 * c + 16 * g));
-        out.vs[c] = scales_of<D>(scales + (uint32_t)(r * (D / kMxBlock) + 4 * c));
-    }
+    out.v = *global<u32x4_t>(codes + (uint32_t)(r * (D / 2) + 16 * g));
+    out.vs = scales_of<D>(scales + (uint32_t)(r * (D / kMxBlock)));
 }
 
 // The query rows as the B operand: piece p of 64 dims c in step p * kChunks + c.
@@ -159,7 +152,7 @@ __device__ __forceinline__ void load_values(const AttArgs& a, const WidePlaces& 
 // be too many for them, in LDS.
 template <int D, int kPieces>
 struct WideQuery {
-    static constexpr int kHeld = D == 256 ? 1 : 2;
+    static constexpr int kHeld = 2;
     static constexpr int kInLds = (kPieces - kHeld) * D / 32;  // 16 bytes of each lane
     v8i_t q[D / 64 * kHeld];
     int scale;  // of the first piece
@@ -281,12 +274,12 @@ struct Yes { static constexpr bool value = true; };
 struct No { static constexpr bool value = false; };
 
 template <int D, int kPieces>
-__global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wide_kernel(AttArgs a) {
+__global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttArgs a) {
     using S = WideShape<D, kPieces>;
     constexpr bool kHalf = kPieces == 3;
     __shared__ __align__(16) uint8_t turned[2][S::kVBytes];
     __shared__ __align__(16) uint32_t held_by[2][kAttWaves];  // whether fp16 holds each wave's values
-    __shared__ uint64_t nan_of[2][kAttWaves][S::kVChunks];    // which of its value blocks are NaN, bit by lane
+    __shared__ uint64_t nan_of[2][kAttWaves];                 // which of its value blocks are NaN, bit by lane
     using Rows = WideQuery<D, kPieces>;
     __shared__ uint4 more_query[kAttWaves][Rows::kInLds ? 64 * Rows::kInLds : 1];  // the pieces not in registers
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -344,8 +337,7 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
         if (tiles > 0) {
             load_keys<D>(find_keys<D>(places, 0, lane), lane, keys);
             load_values<D>(a, places, 0, wave, lane, begin, now);
-            if constexpr (S::kFp16)
-                load_values<D>(a, places, min(1, tiles - 1), wave, lane, begin + kWideKeys, next);
+            load_values<D>(a, places, min(1, tiles - 1), wave, lane, begin + kWideKeys, next);
         }
         Rows query;
         split_wide_query<D, kPieces, kHalf>(a, raw_query, query, more_query[wave], lane);
@@ -359,39 +351,61 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
 
         // A token that no row sees may hold anything: its values are taken as finite.
         auto look = [&](WideValueTile<D>& t, int buffer) {
-            bool held = true;
-#pragma unroll
-            for (int c = 0; c < S::kVChunks; ++c) {
-                t.vs[c] = any(t.key + r) ? t.vs[c] >> (8 * (D < 128 ? g & 1 : g)) & 255u : 127;
-                held = held & half_holds(t.vs[c], t.v[c]);
-            }
-            if constexpr (S::kFp16)
-                held_by[buffer][wave] = __all(held);
+            t.vs = any(t.key + r) ? t.vs >> (8 * (D < 128 ? g & 1 : g)) & 255u : 127;
+            held_by[buffer][wave] = __all(half_holds(t.vs, t.v));
         };
         uint32_t live_next = (uint32_t)places.live & 15u;  // which of the next tile's subtiles have a block
         bool all_held = false;  // by fp16, the next tile's values
         auto read_held = [&](int buffer) { return *reinterpret_cast<const uint4*>(held_by[buffer]); };
         auto set_held = [&](uint4 f) { all_held = __builtin_amdgcn_readfirstlane(f.x & f.y & f.z & f.w) != 0; };
 
+        // This wave's 16 tokens into LDS: the scale they are converted with, and their 8-dim parts 0..3.
+        auto scale_values = [&](auto kind, int buffer) {
+            uint32_t byte = now.vs;
+            if constexpr (decltype(kind)::value) {
+                byte = max(byte, (uint32_t)kHalfShift) - kHalfShift;
+            } else {
+                nan_of[buffer][wave] = __ballot(byte == 255u);
+                byte = byte == 255u ? 0 : byte;
+            }
+            return __uint_as_float(byte << 23);
+        };
+        auto put_values = [&](auto kind, int buffer, int part, float scale) {
+            // (D = 64: both halves of the wave write the same)
+            *reinterpret_cast<uint4*>(turned[0] + (((uint32_t)(buffer * S::kVBytes) + write_at) ^ (16 * part))) =
+                wide_values<decltype(kind)::value>(now.v[part], scale);
+        };
+        auto find_ahead = [&](int32_t i) {
+            if (i + 2 < tiles && ((i + 2) & 15) == 0)
+                places = find_wide_places<D>(a, w.b, h, begin + (i + 2) * kWideKeys, end, lane);
+        };
+        auto load_ahead = [&](int32_t i) {
+            load_values<D>(a, places, min(i + 2, tiles - 1), wave, lane, begin + (i + 2) * kWideKeys, next);
+        };
+
+        // A wave without rows has its part in V only.
+        auto idle_step = [&](auto kind, int32_t i) {
+            find_ahead(i);
+            const float scale = scale_values(kind, i & 1);
+#pragma unroll
+            for (int part = 0; part < 4; ++part)
+                put_values(kind, i & 1, part, scale);
+            now = next;
+            look(now, (i & 1) ^ 1);
+            load_ahead(i);
+            lds_barrier();
+            set_held(read_held((i & 1) ^ 1));
+        };
+
         auto step = [&](auto kind, int32_t i) {
             constexpr bool kFast = decltype(kind)::value;
             constexpr int kPPieces = kFast && kPieces == 2 ? 1 : 2;
             const int buffer = i & 1;
             const int32_t key = begin + i * kWideKeys;
-            constexpr int kAheadOf = S::kFp16 ? 2 : 1;  // tiles that V is loaded ahead
-            auto refresh = [&] {
-                if (i + kAheadOf < tiles && ((i + kAheadOf) & 15) == 0)
-                    places = find_wide_places<D>(a, w.b, h, key + kAheadOf * kWideKeys, end, lane);
-            };
-            if constexpr (!S::kFp16) {
-                look(now, buffer);
-                refresh();
-            }
             const WideKeyAt next_keys = find_keys<D>(places, min(i + 1, tiles - 1), lane);
             const uint32_t live = live_next;
             live_next = (uint32_t)(places.live >> (4 * ((i + 1) & 15))) & 15u;
-            if constexpr (S::kFp16)
-                refresh();
+            find_ahead(i);
             // ---- scores; between the matrix instructions this tile's V into LDS
             __builtin_amdgcn_s_setprio(1);
             f32x16_t s[2];
@@ -400,19 +414,7 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
                     s[t][j] = 0.f;
-            const uint32_t to = (uint32_t)(buffer * S::kVBytes) + write_at;
-            float v_scale[S::kVChunks];
-#pragma unroll
-            for (int c = 0; c < S::kVChunks; ++c) {
-                uint32_t byte = now.vs[c];
-                if constexpr (kFast) {
-                    byte = max(byte, (uint32_t)kHalfShift) - kHalfShift;
-                } else {
-                    nan_of[buffer][wave][c] = __ballot(byte == 255u);
-                    byte = byte == 255u ? 0 : byte;
-                }
-                v_scale[c] = __uint_as_float(byte << 23);
-            }
+            const float v_scale = scale_values(kind, buffer);
 #pragma unroll
             for (int q = 0; q < S::kChunks * kPieces; ++q) {
                 const int c = q % S::kChunks, piece = q / S::kChunks;
@@ -427,169 +429,159 @@ __global__ void __launch_bounds__(kAttThreads, D == 256 ? 1 : 2) mxfp4_attend_wi
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const v8i_t k = key_operand(__builtin_bit_cast(uint4, keys.k[t][c]));
-                    const int scales = (int)(keys.ks[t][c / 2] >> 8 * hh), q_scale = piece_scale(query.scale, piece);
+                    const int scales = (int)(keys.ks[t] >> 8 * hh), q_scale = piece_scale(query.scale, piece);
                     s[t] = c & 1 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, rows_q, s[t], 4, 0, 2, scales, 0, q_scale)
                                  : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, rows_q, s[t], 4, 0, 0, scales, 0, q_scale);
-                    const int part = 2 * q + t;
-                    if (part < 4 * S::kVChunks) {
-                        // (D = 64: both halves of the wave write the same values)
-                        const uint32_t words[4] = {now.v[part / 4].x, now.v[part / 4].y, now.v[part / 4].z, now.v[part / 4].w};
-                        *reinterpret_cast<uint4*>(turned[0] + (to ^ (16 * (part % 4))) + 256 * (part / 4)) =
-                            wide_values<kFast>(words[part % 4], v_scale[part / 4]);
-                    }
+                    if (2 * q + t < 4)
+                        put_values(kind, buffer, 2 * q + t, v_scale);
                     __builtin_amdgcn_sched_barrier(kLdsRead);
                 }
             }
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (S::kFp16) {
-                now = next;
-                look(now, buffer ^ 1);
-            }
+            now = next;
+            look(now, buffer ^ 1);
             // ---- the next tile of K, and the one after it of V
             load_keys<D>(next_keys, lane, keys);
-            load_values<D>(a, places, min(i + kAheadOf, tiles - 1), wave, lane, key + kAheadOf * kWideKeys,
-                           S::kFp16 ? next : now);
+            load_ahead(i);
             lds_barrier();
-            uint4 held = {};
-            if constexpr (S::kFp16)
-                held = read_held(buffer ^ 1);
+            const uint4 held = read_held(buffer ^ 1);
 
-            {
-                const bool plain = (key + kWideKeys - 1 <= min(wave_first, end - 1)) &
-                                   ((a.window == 0) | (key > wave_last - a.window)) & (live == 15u);
-                if (!plain) {
+            const bool plain = (key + kWideKeys - 1 <= min(wave_first, end - 1)) &
+                               ((a.window == 0) | (key > wave_last - a.window)) & (live == 15u);
+            if (!plain) {
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            int32_t base = (live >> (2 * t + u) & 1 ? key + 32 * t + 16 * u : kNoKey) + 4 * hh;
-                            asm("" : "+v"(base));  // one register in all, not one for each key
+                    for (int u = 0; u < 2; ++u) {
+                        int32_t base = (live >> (2 * t + u) & 1 ? key + 32 * t + 16 * u : kNoKey) + 4 * hh;
+                        asm("" : "+v"(base));  // one register in all, not one for each key
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                s[t][8 * u + j] = seen(base + 8 * (j / 4) + j % 4) ? s[t][8 * u + j] : -INFINITY;
-                        }
-                }
-                float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    most[j & 1] = fmaxf(most[j & 1], s[0][j]);
-                    most[2 + (j & 1)] = fmaxf(most[2 + (j & 1)], s[1][j]);
-                }
-                const float top = pair_max(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * a.scale_f;
-                if (__any(top > m_run)) {
-                    const float m_new = top > m_run ? top + kAhead : m_run;
-                    const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
-                    l_run *= alpha;
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d)
-                        acc[d] *= alpha;
-                    m_run = m_new;
-                }
-                float m_use = (m_run == -INFINITY ? 0.f : m_run) - (kFast ? (float)kHalfShift : 0.f);
-                float times = a.scale_f;
-                if (__any(fabsf(m_use) > kFar)) {
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            s[t][j] = s[t][j] * a.scale_f - m_use;
-                    times = 1.f;
-                    m_use = 0.f;
-                }
-                // Products of the first 32 keys' values go between the second's exponentials, and those
-                // between the sums; operands are read kFetch products ahead.
-                constexpr int kOps = 2 * (D / 32), kFetch = D == 128 ? 3 : 2;
-                const uint32_t from0 = (uint32_t)(buffer * S::kVBytes) + read_at;
-                const uint32_t from1 = (from0 + 8 * S::kVPitch) ^ 32;
-                float p[32];
-                uint4 pw[2][kPPieces][2];  // by 16 keys: keys 4h..4h+3 and 8+4h..8+4h+3 of them
-                uint4 v[2 * kOps];
-                auto fetch = [&](int q) {
-                    if (q < 2 * kOps) {
-                        const uint8_t* at = turned[0] + 16 * (q / (D / 32)) * S::kVPitch + 64 * (q % (D / 32));
-                        const uint2 x = read_turned(at + from0), y = read_turned(at + from1);
-                        v[q] = make_uint4(x.x, x.y, y.x, y.y);
+                        for (int j = 0; j < 8; ++j)
+                            s[t][8 * u + j] = seen(base + 8 * (j / 4) + j % 4) ? s[t][8 * u + j] : -INFINITY;
                     }
-                };
-                auto weigh = [&](int j) {
-                    p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 16][j % 16], times, -m_use));
-                    if (j & 1) {
-                        const uint32_t hi = pack_pair<kFast>(p[j - 1], p[j]);
-                        uint32_t* to = &pw[j / 16][0][j / 8 % 2].x;
-                        to[j / 2 % 4] = hi;
-                        if constexpr (kPPieces == 2)
-                            (&pw[j / 16][1][j / 8 % 2].x)[j / 2 % 4] =
-                                pack_pair<kFast>(p[j - 1] - first_of<kFast>(hi), p[j] - second_of<kFast>(hi));
-                    }
-                };
-                auto product = [&](int q) {
-                    const int t = q / kOps, u = q / (D / 32) % 2, d = q % (D / 32);
+            }
+            float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int piece = 0; piece < kPPieces; ++piece)
-                        acc[d] = wide_product<kFast>(v[q], pw[t][piece][u], acc[d]);
-                };
+            for (int j = 0; j < 16; ++j) {
+                most[j & 1] = fmaxf(most[j & 1], s[0][j]);
+                most[2 + (j & 1)] = fmaxf(most[2 + (j & 1)], s[1][j]);
+            }
+            const float top = pair_max(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * a.scale_f;
+            if (__any(top > m_run)) {
+                const float m_new = top > m_run ? top + kAhead : m_run;
+                const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+                l_run *= alpha;
 #pragma unroll
-                for (int q = 0; q < kFetch; ++q)
-                    fetch(q);
+                for (int d = 0; d < D / 32; ++d)
+                    acc[d] *= alpha;
+                m_run = m_new;
+            }
+            float m_use = (m_run == -INFINITY ? 0.f : m_run) - (kFast ? (float)kHalfShift : 0.f);
+            float times = a.scale_f;
+            if (__any(fabsf(m_use) > kFar)) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        s[t][j] = s[t][j] * a.scale_f - m_use;
+                times = 1.f;
+                m_use = 0.f;
+            }
+            // Products of the first 32 keys' values go between the second's exponentials, and those
+            // between the sums; operands are read kFetch products ahead.
+            constexpr int kOps = 2 * (D / 32), kFetch = D == 128 && kPPieces == 1 ? 3 : 2;
+            const uint32_t from0 = (uint32_t)(buffer * S::kVBytes) + read_at;
+            const uint32_t from1 = (from0 + 8 * S::kVPitch) ^ 32;
+            float p[32];
+            uint4 pw[2][kPPieces][2];  // by 16 keys: keys 4h..4h+3 and 8+4h..8+4h+3 of them
+            uint4 v[2 * kOps];
+            auto fetch = [&](int q) {
+                if (q < 2 * kOps) {
+                    const uint8_t* at = turned[0] + 16 * (q / (D / 32)) * S::kVPitch + 64 * (q % (D / 32));
+                    const uint2 x = read_turned(at + from0), y = read_turned(at + from1);
+                    v[q] = make_uint4(x.x, x.y, y.x, y.y);
+                }
+            };
+            auto weigh = [&](int j) {
+                p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 16][j % 16], times, -m_use));
+                if (j & 1) {
+                    const uint32_t hi = pack_pair<kFast>(p[j - 1], p[j]);
+                    uint32_t* to = &pw[j / 16][0][j / 8 % 2].x;
+                    to[j / 2 % 4] = hi;
+                    if constexpr (kPPieces == 2)
+                        (&pw[j / 16][1][j / 8 % 2].x)[j / 2 % 4] =
+                            pack_pair<kFast>(p[j - 1] - first_of<kFast>(hi), p[j] - second_of<kFast>(hi));
+                }
+            };
+            auto product = [&](int q) {
+                const int t = q / kOps, u = q / (D / 32) % 2, d = q % (D / 32);
+#pragma unroll
+                for (int piece = 0; piece < kPPieces; ++piece)
+                    acc[d] = wide_product<kFast>(v[q], pw[t][piece][u], acc[d]);
+            };
+#pragma unroll
+            for (int q = 0; q < kFetch; ++q)
+                fetch(q);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                weigh(j);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int q = 0; q < kOps; ++q) {
+                fetch(q + kFetch);
+                product(q);
+#pragma unroll
+                for (int j = 16 + q * 16 / kOps; j < 16 + (q + 1) * 16 / kOps; ++j)
                     weigh(j);
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            float sum = 0.f;
 #pragma unroll
-                for (int q = 0; q < kOps; ++q) {
-                    fetch(q + kFetch);
-                    product(q);
+            for (int q = kOps; q < 2 * kOps; ++q) {
+                fetch(q + kFetch);
+                product(q);
 #pragma unroll
-                    for (int j = 16 + q * 16 / kOps; j < 16 + (q + 1) * 16 / kOps; ++j)
-                        weigh(j);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                float sum = 0.f;
+                for (int j = (q - kOps) * 32 / kOps; j < (q + 1 - kOps) * 32 / kOps; ++j)
+                    sum += p[j];
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            l_run += kFast ? sum * (1.0f / (1 << kHalfShift)) : sum;
+            if constexpr (!kFast) {
+                // value blocks that are NaN, for the rows that see them
 #pragma unroll
-                for (int q = kOps; q < 2 * kOps; ++q) {
-                    fetch(q + kFetch);
-                    product(q);
+                for (int u = 0; u < 4; ++u) {
+                    const uint64_t nan = nan_of[buffer][u];
+                    const uint32_t half[2] = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)nan),
+                                              (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(nan >> 32))};
 #pragma unroll
-                    for (int j = (q - kOps) * 32 / kOps; j < (q + 1 - kOps) * 32 / kOps; ++j)
-                        sum += p[j];
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                l_run += kFast ? sum * (1.0f / (1 << kHalfShift)) : sum;
-                if constexpr (!kFast) {
-                    // value blocks that are NaN, for the rows that see them
-#pragma unroll
-                    for (int u = 0; u < 4; ++u)
-#pragma unroll
-                        for (int c = 0; c < S::kVChunks; ++c) {
-                            const uint64_t nan = nan_of[buffer][u][c];
-                            const uint32_t half[2] = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)nan),
-                                                      (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(nan >> 32))};
-#pragma unroll
-                            for (int b = 0; b < (D < 128 ? 2 : 4); ++b) {
-                                float add = 0.f;
-                                for (uint32_t bits = half[b / 2] >> (16 * (b & 1)) & 0xffffu; bits; bits &= bits - 1)
-                                    add = seen(key + 16 * u + __builtin_ctz(bits)) ? NAN : add;
-                                acc[4 * c + b] += add;
-                            }
-                        }
+                    for (int b = 0; b < D / 32; ++b) {
+                        float add = 0.f;
+                        for (uint32_t bits = half[b / 2] >> (16 * (b & 1)) & 0xffffu; bits; bits &= bits - 1)
+                            add = seen(key + 16 * u + __builtin_ctz(bits)) ? NAN : add;
+                        acc[b] += add;
+                    }
                 }
             }
             set_held(held);
         };
 
         if (tiles > 0) {
-            if constexpr (S::kFp16) {
-                look(now, 0);
-                lds_barrier();
-                set_held(read_held(0));
-            }
+            look(now, 0);
+            lds_barrier();
+            set_held(read_held(0));
             int32_t i = 0;
-            if constexpr (S::kFp16)
+            if (idle) {
+                for (; i < tiles && all_held; ++i)
+                    idle_step(Yes{}, i);
+                for (; i < tiles; ++i)
+                    idle_step(No{}, i);
+            } else {
                 for (; i < tiles && all_held; ++i)
                     step(Yes{}, i);
-            for (; i < tiles; ++i)
-                step(No{}, i);
+                for (; i < tiles; ++i)
+                    step(No{}, i);
+            }
         }
 
         l_run += __shfl_xor(l_run, 32);

@@ -129,7 +129,12 @@ __device__ __forceinline__ Request request_of(const AttArgs& a, int32_t b) {
 
 // The first tile boundary in front of what a row at position `pos` sees.
 __device__ __forceinline__ int32_t keys_begin(const AttArgs& a, int32_t pos) {
-    return a.window > 0 ? max(pos - a.window + 1, 0) & ~(kTileKeys - 1) : 0;
+    int32_t begin = 0;
+    if (a.window > 0) {
+        asm volatile("");  // a branch: without a window nothing waits for the request's length here
+        begin = max(pos - a.window + 1, 0) & ~(kTileKeys - 1);
+    }
+    return begin;
 }
 
 // A request and its tiles of rows, `units` units of keys each, dealt out as `cost`.
@@ -186,6 +191,18 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 // more; then nothing is computed.)
 __device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int32_t rows_per_tile, int32_t unit_keys,
                                            Start& start) {
+    if (a.workers == 0 && (a.num_reqs == 1 || !a.query_start_loc)) {
+        // requests of equally many tiles need no scan (1 x 518 keys, 32 heads: 10.0 us with it, 9.3 without)
+        const uint32_t each = (uint32_t)(a.group + rows_per_tile - 1) / (uint32_t)rows_per_tile;
+        start.b = a.num_reqs == 1 ? 0 : (int32_t)(index / each);
+        if (start.b >= a.num_reqs)
+            return false;
+        start.tiles = tiles_of(a, start.b, rows_per_tile, unit_keys);
+        start.tile = start.tiles.count - 1 - (int32_t)(index - start.b * each);
+        start.at = 0;
+        start.take = start.each = 1;
+        return start.tile >= 0;
+    }
     __shared__ uint32_t part[kAttWaves];
     __shared__ int32_t found[8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -432,7 +449,7 @@ struct RawTile {
     int32_t place[kSub];  // of its first token in the block, negative: there is none
 };
 
-// Where a wave's next 64 subtiles lie: lane kSub i + t has subtile t of the i-th
+// Where a wave's next 64 subtiles below `end` lie (entries are read up to `limit`): lane kSub i + t has subtile t of the i-th
 // tile, the head's block at `base` and the first of its tokens at `place`
 // (negative: no block).  Tiles of a wave are `stride` keys apart.
 struct Places {
@@ -442,13 +459,13 @@ struct Places {
 
 template <int kSub>
 __device__ __forceinline__ Places find_places(const AttArgs& a, int32_t b, int32_t h, int32_t token_bytes, int32_t key0,
-                                              int32_t stride, int32_t end, int lane) {
+                                              int32_t stride, int32_t limit, int32_t end, int lane) {
     const int64_t key = (int64_t)key0 + (int64_t)(lane / kSub) * stride + 16 * (lane % kSub);
     Places p = {0, -1};
-    if (key < end) {
+    if (key < limit) {
         const int32_t column = (int32_t)key / a.page;
         const int32_t id = a.block_table[(int64_t)b * a.bt_stride + column];
-        if (id >= 0 && id < a.num_blocks) {
+        if (id >= 0 && id < a.num_blocks && key < end) {
             p.base = (int64_t)id * a.block_stride + (int64_t)h * a.page * token_bytes;
             p.place = (int32_t)key - column * a.page;
         }
@@ -779,10 +796,11 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
 
         const int32_t key0 = begin + wave * kKeys;
         const int32_t tiles = end > key0 ? (end - key0 + kUnit - 1) / kUnit : 0;
-        // in the order in which they are waited for: the query's values are split while the first tiles come
+        // in the order in which they are waited for (the table has its columns whatever the request's length, so that
+        // one does not wait for the other): the query's values are split while the first tiles come
         RawQuery<D> raw_query;
         load_query<D>(a, (req.first + token) * a.q_st + head * a.q_sh, valid, g, raw_query);
-        Places places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0, kUnit, end, lane);
+        Places places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0, kUnit, a.table_keys, end, lane);
         // kDepth tiles are on their way: a tile's registers take another as soon as they are free
         RawTile<kSub, S::kChunks> raw[kDepth];
 #pragma unroll
@@ -803,7 +821,7 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
                 const int32_t next = i + kDepth;
                 if (next < tiles) {
                     if (next % kBatch == 0)
-                        places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0 + next * kUnit, kUnit, end, lane);
+                        places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0 + next * kUnit, kUnit, end, end, lane);
                     load_tile<D, kSub>(a, places, next, lane, now);
                 }
             };
@@ -1004,16 +1022,19 @@ struct Dealing {
 };
 
 // One launch takes all requests, or two share them by their rows: 16-row tiles for
-// up to kFewRows, 128-row tiles (whose waves would have nothing to do) for more.
+// up to kFewRows, 128-row tiles (whose waves would have nothing to do: 56 rows
+// 49 us with the first, 68 with the others) for more, where D is at most 128 (D =
+// 256 leaves 128-row tiles one workgroup to a CU; they took 842 us where the others
+// take 735, 2048 tokens behind 8192 keys).
 constexpr int kFewRows = 64;
 
 struct Call {
     int64_t tokens, heads, kv_heads, dim, reqs, max_query, max_seq;
-    bool wide() const { return max_query * (heads / kv_heads) > kFewRows; }
+    bool wide() const { return dim <= 128 && max_query * (heads / kv_heads) > kFewRows; }
     bool few() const { return !wide() || reqs > 1; }
 };
 
-int per_cu(int dim, bool wide) { return wide ? (dim == 256 ? 1 : 2) : groups_per_cu(dim); }
+int per_cu(int dim, bool wide) { return wide ? 2 : groups_per_cu(dim); }
 
 Dealing dealing_of(const Call& c, bool wide) {
     const int64_t group = c.heads / c.kv_heads, tile_rows = wide ? kWideRows : kRows;
@@ -1064,16 +1085,17 @@ void launch_part(const Dealing& d, uint8_t* workspace, int64_t unit, hipStream_t
 
 template <int D, int kPieces>
 void launch_attend(const Call& c, uint8_t* workspace, hipStream_t st, AttArgs a) {
-    const bool both = c.wide() && c.few();
     a.rows_from = 0;
     a.rows_to = 0x7fffffff;
-    if (c.wide()) {
-        const Dealing d = dealing_of(c, true);
-        a.rows_from = both ? kFewRows + 1 : 0;
-        launch_part<D, kPieces, kWideRows>(d, workspace, kWideKeys, st, a);
-        workspace = workspace ? workspace + d.bytes : nullptr;
-        a.rows_from = 0;
-        a.rows_to = kFewRows;
+    if constexpr (D <= 128) {
+        if (c.wide()) {
+            const Dealing d = dealing_of(c, true);
+            a.rows_from = c.few() ? kFewRows + 1 : 0;
+            launch_part<D, kPieces, kWideRows>(d, workspace, kWideKeys, st, a);
+            workspace = workspace ? workspace + d.bytes : nullptr;
+            a.rows_from = 0;
+            a.rows_to = kFewRows;
+        }
     }
     if (c.few())
         launch_part<D, kPieces, kRows>(dealing_of(c, false), workspace, unit_keys(D), st, a);
