@@ -941,20 +941,52 @@ __device__ __forceinline__ void write_row(const AttArgs& a, const CutTile& tile,
         a.lse[t * a.lse_st + head] = e.lse;
 }
 
-// Joins the cuts of the tile that begins in a worker, for one head (blockIdx.x) and the
-// rows of blockIdx.y.  kWide: a workgroup per row, its waves share out the cuts
-// (few rows, of many cuts); otherwise a wave per row.  (The grid has as many rows
-// as the host was told of; there may be more.)
+// The worker in which the index-th of the cut tiles begins (in some order); -1: there
+// are fewer.
+__device__ __forceinline__ int32_t find_cut(const AttArgs& a, int32_t index) {
+    __shared__ int32_t found, in_front[kAttWaves];
+    const int wave = threadIdx.x >> 6;
+    if (threadIdx.x == 0)
+        found = -1;
+    for (int32_t base = 0; base < a.workers; base += kAttThreads) {
+        const int32_t worker = base + (int32_t)threadIdx.x;
+        const bool cut = worker < a.workers && a.cut_tiles[worker].count > 0;
+        const uint64_t cuts = __ballot(cut);
+        if (base > 0)
+            __syncthreads();  // the last turn's counts were read
+        in_front[wave] = __popcll(cuts);
+        __syncthreads();
+        int32_t rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(cuts >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)cuts, 0));
+        int32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < kAttWaves; ++w) {
+            rank += w < wave ? in_front[w] : 0;
+            all += in_front[w];
+        }
+        if (cut && rank == index)
+            found = worker;
+        index -= all;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(found);
+}
+
+// Joins the cuts of a tile, for one head (both blockIdx.x) and the rows of blockIdx.y.
+// kWide: a workgroup per row, its waves share out the cuts (few rows, of many
+// cuts); otherwise a wave per row.  (The grid has as many rows as the host was told
+// of; there may be more.)  Workgroups are launched for tiles, which the host knows
+// better than how many workers there will be (875 rows of one request, 2 heads: 5.4 us;
+// for each worker, most of them with nothing to join, 8.4).
 template <int D, bool kHalf, int kTileRows, bool kWide>
 __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
     constexpr int kLanes = D / 4, kGroups = 64 / kLanes;  // lanes per row, cuts that a wave takes at a time
     constexpr int kRowsAtOnce = kWide ? 1 : kAttWaves;
     __shared__ f32x4_t sums[kWide ? kAttWaves : 1][kLanes];
     __shared__ float factors[kAttWaves][64];
-    const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads), h = (int32_t)(blockIdx.x % a.kv_heads);
-    const CutTile tile = a.cut_tiles[worker];
-    if (tile.count == 0)
+    const int32_t h = (int32_t)(blockIdx.x % a.kv_heads), worker = find_cut(a, (int32_t)(blockIdx.x / a.kv_heads));
+    if (worker < 0)
         return;
+    const CutTile tile = a.cut_tiles[worker];
     const int32_t rows = min(tile.rows - tile.first_row, kTileRows);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int part = lane % kLanes, group = lane / kLanes;
@@ -1076,10 +1108,10 @@ void launch_part(const Dealing& d, uint8_t* workspace, int64_t unit, hipStream_t
     // a wave per row where that fills the chip (4 x 256 rows)
     const int64_t cut_tiles = (d.tiles < a.workers ? d.tiles : a.workers) * a.kv_heads;
     if (cut_tiles * d.rows >= 1024)
-        hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, kTileRows, false>), dim3(grid, (d.rows + 3) / 4),
-                           dim3(kAttThreads), 0, st, a);
+        hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, kTileRows, false>),
+                           dim3((unsigned)cut_tiles, (d.rows + 3) / 4), dim3(kAttThreads), 0, st, a);
     else
-        hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, kTileRows, true>), dim3(grid, d.rows),
+        hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, kTileRows, true>), dim3((unsigned)cut_tiles, d.rows),
                            dim3(kAttThreads), 0, st, a);
 }
 

@@ -622,3 +622,20 @@ def test_c_abi_refusals(kw, code):
 def test_c_abi_nothing_to_do():
     assert call_c(tokens=0, reqs=0, q=None, out=None, lse=None) == 0
     assert call_c(heads=0, kv=0, q=None, out=None, lse=None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts", [[0, 9, 2, 9], [9, 0, 9, 0], [-5, 4, 2 ** 31 - 1, 3]])
+def test_gpu_starts_that_fall(starts):
+    """No request should have such starts: rows outside of them stay, and the next call is as ever."""
+    c = Case(25, [3000, 64, 500], [3, 3, 3])
+    want = c.check(max_query_len=3)
+    out = torch.full_like(torch.cat([c.q, c.q]), 7.0)
+    for most in (3, 100):
+        fv.mxfp4_paged_attention(torch.cat([c.q, c.q]), c.cache, c.table, c.lens, c.scale, max_query_len=most, out=out,
+                                 query_start_loc=torch.tensor(starts, dtype=torch.int32, device=DEV))
+        torch.cuda.synchronize()
+        if max(starts[1:]) <= 9:
+            assert bool((out[9:] == 7).all())
+    for x, y in zip(c.run(max_query_len=3), want):
+        assert torch.equal(x, y)
