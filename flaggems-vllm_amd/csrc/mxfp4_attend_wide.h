@@ -16,6 +16,14 @@
 // again, and a second piece another half of PV's time.  Value blocks beyond
 // fp16's range (half_holds) are left to a second loop in bf16 with two pieces,
 // which the first one enters at the first tile that holds one.
+//
+// A wave's matrix instructions of a tile take 1026 cycles (D = 128, bf16 calls), its
+// vector instructions 1180 (exp2 among them), and the two overlap only where other
+// instructions stand between them in the stream: so V's conversion goes between
+// QK's, the second half's exponentials between PV's for the first, loads are asked
+// for a tile (V: two) ahead.  2048 tokens behind 14336 keys, 32 heads of 128: 497 us,
+// 515 GFLOP at 1040 TFLOP/s, matrix units busy 46 %, vector issue 54 %; QK, softmax
+// and PV one after the other took 610, 16-row tiles 1083.
 #pragma once
 
 namespace fgv {

@@ -31,8 +31,15 @@
 // PV: v_cvt_scalef32_pk_bf16_fp4 gives V in bf16 exactly (codes have two
 // bits), token by token; LDS turns it, written by tokens and read by
 // ds_read_b64_tr_b16.  P goes in as two bf16 pieces (16 bits): one alone would
-// put its own 2^-9 beside the output's.  A value block under byte 255 (NaN) makes the outputs of those
-// rows NaN that see it.
+// put its own 2^-9 beside the output's.  A value block under byte 255 (NaN) makes
+// the outputs of those rows NaN that see it.
+//
+// Two kernels: 16-row tiles, whose waves share out the keys (here; single tokens,
+// a few of them, and D = 256), and 128-row tiles, whose waves share out the rows
+// (mxfp4_attend_wide.h).  Single tokens are bound by the cache's bytes, once there
+// are many: 64 requests of up to 8191 keys, 199 MB, 50 us, of it 5 for joining
+// cuts; 1 x 131072 keys, 143 MB, 39 us.  In front of that stand some 10 us of latency:
+// launch, lengths, block table and first keys each wait for the one before.
 #include <math.h>
 
 #include "fgv_device.h"
