@@ -114,6 +114,9 @@ struct CutTile {
     int32_t first_token, first_row, rows, count;
 };
 
+// Longer requests are taken as this long: twice a table's keys, which windows are below.
+constexpr int32_t kLongest = 0x7ff00000;
+
 // A request's query tokens [first, first + count) and lengths.
 struct Request {
     int32_t first, count, len;
@@ -130,7 +133,7 @@ __device__ __forceinline__ Request request_of(const AttArgs& a, int32_t b) {
         r.first = b;
         r.count = 1;
     }
-    r.len = max(a.seq_lens[b], 0);
+    r.len = min(max(a.seq_lens[b], 0), kLongest);
     return r;
 }
 
@@ -245,7 +248,7 @@ __device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int
         // 20000 keys, D = 256: 285 workgroups with 7 each 27.5 us, 333 with 6 32.5, as most CUs had one and some two)
         uint32_t to = (uint32_t)a.workers;
         for (int32_t k = a.per_cu - 1; k > 0; --k)
-            to = total < to * (uint32_t)kLeastCost ? (uint32_t)(a.workers * k / a.per_cu) : to;
+            to = total < to * (uint32_t)kLeastCost ? (uint32_t)max(a.workers * k / a.per_cu, 1) : to;
         each = max((total + to - 1) / to, (uint32_t)kLeastCost);
     }
     uint64_t first = (uint64_t)each * index;
@@ -533,7 +536,7 @@ struct Seen {
     uint32_t count;
     __device__ bool operator()(int32_t key) const { return (uint32_t)(key - first) < count; }
 };
-constexpr int32_t kNoKey = -0x40000000;  // seen by nobody: keys are below 2^30
+constexpr int32_t kNoKey = 0x7ff80000;  // seen by nobody: behind the longest request's last position
 
 // Attends the tile's keys, from key0 on, for the wave's 16 rows.  `plain`: all of
 // them are seen by all rows; otherwise some may be hidden, hold anything or be NaN.
@@ -1073,6 +1076,11 @@ struct Call {
     bool few() const { return !wide() || reqs > 1; }
 };
 
+Call call_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t reqs, int64_t max_query,
+             int64_t max_seq) {
+    return {tokens, heads, kv_heads, dim, reqs, max_query < tokens ? max_query : tokens, max_seq};
+}
+
 int per_cu(int dim, bool wide) { return wide ? 2 : groups_per_cu(dim); }
 
 Dealing dealing_of(const Call& c, bool wide) {
@@ -1085,10 +1093,10 @@ Dealing dealing_of(const Call& c, bool wide) {
     // no request has more tiles than its rows' share, rounded up
     d.tiles = c.tokens * group / tile_rows + c.reqs;
     int64_t workers = slots / c.kv_heads;
-    workers = workers < 1 ? 1 : workers > kMostWorkers ? kMostWorkers : workers;
+    workers = workers > kMostWorkers ? kMostWorkers : workers;
     // Nothing to cut; or two 128-row tiles a workgroup and more.  Their partial results are 66 KB at D = 128: prompts
     // of 1140 tiles on 512 workgroups took 151 us with cuts, which leave no workgroup idle, and 108 without.
-    if (c.max_seq <= kWholeUnits * unit || (wide && (d.tiles - c.reqs) * c.kv_heads >= 2 * slots))
+    if (workers < 2 || c.max_seq <= kWholeUnits * unit || (wide && (d.tiles - c.reqs) * c.kv_heads >= 2 * slots))
         return d;
     d.workers = (int32_t)workers;
     d.cut_tiles_at = 2 * workers * c.kv_heads * (int64_t)slot_floats((int)c.dim, (int)tile_rows) * 4;
@@ -1223,7 +1231,7 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
     a.window = (int32_t)(window_size < 0x3fffffffLL ? window_size : 0);
     a.q_wide = aligned(q, 16) && ((q_stride_token | q_stride_head) & 7) == 0;
     a.o_wide = aligned(out, 8) && ((out_stride_token | out_stride_head) & 3) == 0;
-    const Call call = {num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len};
+    const Call call = call_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len);
     if ((num_tokens * a.group / kRows + num_reqs) * num_kv_heads > 0x7fffffffLL)
         return fail(FGV_E_TOO_LARGE, "too many row tiles");
     const int64_t bytes = workspace_of(call);
@@ -1245,5 +1253,6 @@ extern "C" int64_t fgv_mxfp4_paged_attention_workspace_bytes(int64_t num_tokens,
     if (num_tokens <= 0 || num_reqs <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || num_heads > 65536 ||
         num_tokens * num_heads > 0x3fffffffLL || num_reqs > 0x3fffffffLL)
         return 0;
-    return fgv::workspace_of({num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len});
+    return fgv::workspace_of(
+        fgv::call_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len));
 }

@@ -639,3 +639,34 @@ def test_gpu_starts_that_fall(starts):
             assert bool((out[9:] == 7).all())
     for x, y in zip(c.run(max_query_len=3), want):
         assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("query", [None, [1, 90]])
+def test_gpu_lengths_and_windows_at_their_ends(query):
+    """Lengths up to int32's end are the table's keys, pages without a block among them; a window near 2^30 is none."""
+    c = Case(26, [320, 320], query)
+    c.table = c.table[:, :20].contiguous()
+    c.table[0, 3], c.table[1, 7] = -1, len(c.cache)
+    want = c.check()
+    for window in (2 ** 30 - 2, 2 ** 30 - 1, 2 ** 62):
+        for x, y in zip(c.run(window_size=window), want):
+            assert torch.equal(x, y)
+    if query is None:
+        for n in (2 ** 31 - 1, 2 ** 31 - 2 ** 13, 2 ** 30):
+            c.lens.fill_(n)
+            for x, y in zip(c.run(), want):
+                assert torch.equal(x, y)
+        out, lse = c.run(window_size=1000)  # a window behind the table
+        assert not bool(out.any()) and bool(torch.isposinf(lse).all())
+    for most in (2 ** 62, 2 ** 31):
+        c.run(max_query_len=most, max_seq_len=most)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_heads", [257, 600])
+def test_gpu_many_key_heads(kv_heads):
+    """More key heads than there are workgroups to deal work out to."""
+    c = Case(27, [1500, 3], [2, 1], heads=kv_heads, kv_heads=kv_heads, dim=64)
+    c.check()
+    Case(28, [1100], [70], heads=kv_heads, kv_heads=kv_heads, dim=64).check()
