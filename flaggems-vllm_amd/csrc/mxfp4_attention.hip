@@ -806,11 +806,12 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
 
         const int32_t key0 = begin + wave * kKeys;
         const int32_t tiles = end > key0 ? (end - key0 + kUnit - 1) / kUnit : 0;
-        // in the order in which they are waited for (the table has its columns whatever the request's length, so that
-        // one does not wait for the other): the query's values are split while the first tiles come
+        // in the order in which they are waited for (without cuts the length is not known yet: the table has its columns
+        // whatever it is, so that one does not wait for the other): the query's values are split while the first tiles come
         RawQuery<D> raw_query;
         load_query<D>(a, (req.first + token) * a.q_st + head * a.q_sh, valid, g, raw_query);
-        Places places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0, kUnit, a.table_keys, end, lane);
+        Places places = find_places<kSub>(a, w.b, h, mx_token_bytes(D), key0, kUnit,
+                                           a.workers > 0 ? end : a.table_keys, end, lane);
         // kDepth tiles are on their way: a tile's registers take another as soon as they are free
         RawTile<kSub, S::kChunks> raw[kDepth];
 #pragma unroll
