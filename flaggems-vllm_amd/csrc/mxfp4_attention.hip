@@ -1007,9 +1007,21 @@ __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
     };
     for (int32_t r = (int32_t)blockIdx.y * kRowsAtOnce + (kWide ? 0 : wave); r < rows;
          r += (int32_t)gridDim.y * kRowsAtOnce) {
+        // the first sums are asked for before their factors are known
+        constexpr int kEarly = 4, kStep = kWide ? kAttWaves * kGroups : kGroups;
+        const int32_t mine = kWide ? wave * kGroups + group : group;
+        f32x4_t early[kEarly];
+#pragma unroll
+        for (int e = 0; e < kEarly; ++e)
+            early[e] = *reinterpret_cast<const f32x4_t*>(slot_at(min(mine + e * kStep, tile.count - 1)) + r * D + 4 * part);
         // every wave finds the reference for itself
-        float m = -INFINITY;
-        for (int32_t i = lane; i < tile.count; i += 64)
+        float m_first = -INFINITY, l_first = 0.f;  // of the cut with this lane's number
+        if (lane < tile.count) {
+            m_first = slot_at(lane)[kTileRows * D + r];
+            l_first = slot_at(lane)[kTileRows * D + kTileRows + r];
+        }
+        float m = m_first;
+        for (int32_t i = lane + 64; i < tile.count; i += 64)
             m = fmaxf(m, slot_at(i)[kTileRows * D + r]);
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1)
@@ -1019,15 +1031,27 @@ __global__ void __launch_bounds__(kAttThreads) mxfp4_combine_kernel(AttArgs a) {
         f32x4_t o = {0.f, 0.f, 0.f, 0.f};
         for (int32_t base = 0; base < tile.count; base += 64) {
             float f = 0.f;
-            if (base + lane < tile.count) {
+            if (base == 0) {
+                f = __builtin_amdgcn_exp2f(m_first - m_use);
+                l = f * l_first;
+            } else if (base + lane < tile.count) {
                 const float* slot = slot_at(base + lane) + kTileRows * D + r;
                 f = __builtin_amdgcn_exp2f(slot[0] - m_use);
                 l += f * slot[kTileRows];
             }
             const int32_t n = min(tile.count - base, 64);
             factors[wave][lane] = f;  // read by this wave alone
+            int32_t i = mine;
+            if (base == 0) {
+#pragma unroll
+                for (int e = 0; e < kEarly; ++e) {
+                    if (i < n)
+                        o += factors[wave][i] * early[e];
+                    i += kStep;
+                }
+            }
 #pragma unroll 8
-            for (int32_t i = kWide ? wave * kGroups + group : group; i < n; i += kWide ? kAttWaves * kGroups : kGroups)
+            for (; i < n; i += kStep)
                 o += factors[wave][i] * *reinterpret_cast<const f32x4_t*>(slot_at(base + i) + r * D + 4 * part);
         }
 #pragma unroll
