@@ -65,8 +65,9 @@ constexpr int kMostWorkers = 1024;  // per head
 // much as this many more, so that a worker of many short tiles gets fewer units.
 constexpr int kTileCost = 4;
 constexpr int kLeastCost = kTileCost + 1;  // what a worker takes at least
-// Tiles of no more units than this are not cut: joining cuts takes a launch, 5 us.
-constexpr int kWholeUnits = 8;
+// Tiles of no more units than this are not cut: joining cuts takes a launch, 4 us (128 windows of 1000 keys, 9 units:
+// 27.7 us whole, 30.4 cut).
+constexpr int kWholeUnits = 10;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // A row's reference is raised when a score exceeds it, and then to this much
@@ -1096,14 +1097,21 @@ struct Dealing {
 constexpr int kFewRows = 64;
 
 struct Call {
-    int64_t tokens, heads, kv_heads, dim, reqs, max_query, max_seq;
+    int64_t tokens, heads, kv_heads, dim, reqs, max_query;
+    int64_t max_keys;  // of a tile's rows
     bool wide() const { return dim <= 128 && max_query * (heads / kv_heads) > kFewRows; }
-    bool few() const { return !wide() || reqs > 1; }
+    // Short requests, if they are a few, are better off in the others' tiles than in two launches more, whether there
+    // are any or not (6 prompts 109 us with the launches, 104 without).
+    bool few() const {
+        return !wide() || (reqs > 1 && (max_keys > kWholeUnits * unit_keys((int)dim) || reqs * kv_heads > cu_count() / 4));
+    }
 };
 
 Call call_of(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t reqs, int64_t max_query,
-             int64_t max_seq) {
-    return {tokens, heads, kv_heads, dim, reqs, max_query < tokens ? max_query : tokens, max_seq};
+             int64_t max_seq, int64_t window) {
+    // (a window's tile: its rows' tokens apart, and the boundary before its first key)
+    const int64_t most = window > 0 && window < max_seq ? window + kTileKeys + 128 * kv_heads / heads : max_seq;
+    return {tokens, heads, kv_heads, dim, reqs, max_query < tokens ? max_query : tokens, most < max_seq ? most : max_seq};
 }
 
 int per_cu(int dim, bool wide) { return wide ? 2 : groups_per_cu(dim); }
@@ -1121,7 +1129,7 @@ Dealing dealing_of(const Call& c, bool wide) {
     workers = workers > kMostWorkers ? kMostWorkers : workers;
     // Nothing to cut; or two 128-row tiles a workgroup and more.  Their partial results are 66 KB at D = 128: prompts
     // of 1140 tiles on 512 workgroups took 151 us with cuts, which leave no workgroup idle, and 108 without.
-    if (workers < 2 || c.max_seq <= kWholeUnits * unit || (wide && (d.tiles - c.reqs) * c.kv_heads >= 2 * slots))
+    if (workers < 2 || c.max_keys <= kWholeUnits * unit || (wide && (d.tiles - c.reqs) * c.kv_heads >= 2 * slots))
         return d;
     d.workers = (int32_t)workers;
     d.cut_tiles_at = 2 * workers * c.kv_heads * (int64_t)slot_floats((int)c.dim, (int)tile_rows) * 4;
@@ -1256,7 +1264,8 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
     a.window = (int32_t)(window_size < 0x3fffffffLL ? window_size : 0);
     a.q_wide = aligned(q, 16) && ((q_stride_token | q_stride_head) & 7) == 0;
     a.o_wide = aligned(out, 8) && ((out_stride_token | out_stride_head) & 3) == 0;
-    const Call call = call_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len);
+    const Call call = call_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len,
+                              window_size);
     if ((num_tokens * a.group / kRows + num_reqs) * num_kv_heads > 0x7fffffffLL)
         return fail(FGV_E_TOO_LARGE, "too many row tiles");
     const int64_t bytes = workspace_of(call);
@@ -1279,5 +1288,5 @@ extern "C" int64_t fgv_mxfp4_paged_attention_workspace_bytes(int64_t num_tokens,
         num_tokens * num_heads > 0x3fffffffLL || num_reqs > 0x3fffffffLL)
         return 0;
     return fgv::workspace_of(
-        fgv::call_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len));
+        fgv::call_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len, 0));
 }

@@ -14,9 +14,11 @@ What the kernels may be off, row by row (``bounds``), counted before their first
   behind the first, 2^-4 as large at least, any may be;
 * scores are scaled and exp2 taken in 32 bits: 2^-20 (1 + |s|) together covers the
   scaling, the subtraction and two ulp of the exponential;
-* P enters as two bf16 pieces (2^-16).  Where a request has more than 64 rows for a key head (or
-  is alone) and D is at most 128, bf16 calls have one fp16 piece of it, 2^-11, and both types lose of P times 2^7 what lies
-  below fp16's least step, half of 2^-24: under a reference of at most 2^4 times the row's largest
+* P enters as two bf16 pieces (2^-16).  Where D is at most 128 and a request has more than 64 rows for a
+  key head (or is alone, or among so few that all their key heads together are at most a quarter of the
+  CUs: such may share the others' tiles), bf16 calls have one fp16 piece of it, half a step of its 11
+  bits or 2^-11, an eighth of what the output's rounding takes, and both types lose of P times 2^7 what
+  lies below fp16's least step, half of 2^-24: under a reference of at most 2^4 times the row's largest
   that is 2^(-25 - 7 + 4) = 2^-28 of the row's largest a key;
 * P below 2^-126 is nothing in 32 bits (the first run showed that this had been left out: a dim
   where all keys but such ones hold zeros came out as 0 instead of 4e-39).  P is taken under a
@@ -149,7 +151,9 @@ def reference(q, cache, table, lens, start, scale, window=None, sink=None):
             weight = p @ torch.where(nan, 0.0, vh).abs() * share[:, None]
             o = o * share[:, None]
             half = torch.finfo(q.dtype).eps / 2
-            many = dim <= 128 and ((t1 - t0) * group > 64 or len(lens) == 1)
+            cus = torch.cuda.get_device_properties(q.device).multi_processor_count
+            many = dim <= 128 and ((t1 - t0) * group > 64 or len(lens) == 1
+                                 or (len(q) * group > 64 and len(lens) * kv_heads <= cus // 4))
             ob = weight * ((2.0 ** -11 if many and not three else 2.0 ** -16) + 2.5 * d + steps)[:, None] * (1 + half)
             if many:
                 ob = ob + 2.0 ** -28 * (p.amax(1) * share)[:, None] * torch.where(nan, 0.0, vh).abs().sum(0)
