@@ -1124,12 +1124,17 @@ Dealing dealing_of(const Call& c, bool wide) {
     const int64_t rows = group * (c.max_query < 1 ? 1 : c.max_query < tile_rows ? c.max_query : tile_rows);
     d.rows = (int32_t)(rows < tile_rows ? rows : tile_rows);
     // no request has more tiles than its rows' share, rounded up
-    d.tiles = c.tokens * group / tile_rows + c.reqs;
+    d.tiles = c.reqs == 1 ? (c.tokens * group + tile_rows - 1) / tile_rows : c.tokens * group / tile_rows + c.reqs;
     int64_t workers = slots / c.kv_heads;
     workers = workers > kMostWorkers ? kMostWorkers : workers;
     // Nothing to cut; or two 128-row tiles a workgroup and more.  Their partial results are 66 KB at D = 128: prompts
     // of 1140 tiles on 512 workgroups took 151 us with cuts, which leave no workgroup idle, and 108 without.
     if (workers < 2 || c.max_keys <= kWholeUnits * unit || (wide && (d.tiles - c.reqs) * c.kv_heads >= 2 * slots))
+        return d;
+    // One request's tiles, much alike, in (nearly) whole turns of the chip (2048 tokens behind 14336 keys, 512 tiles on as
+    // many workgroups: 502 us dealt out, 10 of it for finding nothing to join; 472 whole, the longest first).
+    const int64_t turns = (d.tiles * c.kv_heads + slots - 1) / slots;
+    if (wide && c.reqs == 1 && 20 * d.tiles * c.kv_heads >= 19 * turns * slots)
         return d;
     d.workers = (int32_t)workers;
     d.cut_tiles_at = 2 * workers * c.kv_heads * (int64_t)slot_floats((int)c.dim, (int)tile_rows) * 4;
@@ -1155,12 +1160,16 @@ void launch_part(const Dealing& d, uint8_t* workspace, int64_t unit, hipStream_t
         return;
     // a wave per row where that fills the chip (4 x 256 rows)
     const int64_t cut_tiles = (d.tiles < a.workers ? d.tiles : a.workers) * a.kv_heads;
-    if (cut_tiles * d.rows >= 1024)
+    if (cut_tiles * d.rows >= 1024) {
+        // (4096 workgroups at most, if each has a tile: they take more rows then)
+        const int64_t most = 4096 / cut_tiles, rows = (d.rows + 3) / 4;
         hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, kTileRows, false>),
-                           dim3((unsigned)cut_tiles, (d.rows + 3) / 4), dim3(kAttThreads), 0, st, a);
-    else
+                           dim3((unsigned)cut_tiles, (unsigned)(most < 1 ? 1 : most < rows ? most : rows)),
+                           dim3(kAttThreads), 0, st, a);
+    } else {
         hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, kTileRows, true>), dim3((unsigned)cut_tiles, d.rows),
                            dim3(kAttThreads), 0, st, a);
+    }
 }
 
 template <int D, int kPieces>
