@@ -432,7 +432,8 @@ __device__ __forceinline__ void split_query(const AttArgs& a, const RawQuery<D>&
                     out.q[s][4 * half + i] = 2 * s + half >= kPieces ? 0
                                              : (int)(s + half == 0 ? take_piece<true>(&x[0][4 * i])
                                                                    : take_piece<false>(&x[0][4 * i]));
-            out.scale[s] = q.bad ? 255 : q.byte - 4 * (2 * s + (g >> 1));
+            // (a piece that is not there, zeros, takes the last one's scale: one more step down might be no byte, or NaN's)
+            out.scale[s] = q.bad ? 255 : q.byte - 4 * min(2 * s + (g >> 1), kPieces - 1);
         }
     } else {
 #pragma unroll

@@ -1,0 +1,50 @@
+"""The 4-bit cache's ops at the ends of what they take: softmax scales and queries of any size, value blocks whose sums
+pass 32 bits' range, against the formula in 64 bits within the bounds of test_mxfp4_attention.py.
+"""
+import pytest
+import torch
+
+from .test_mxfp4_attention import BF, FP, Case
+from .test_mxfp4_kv_cache import parts
+
+QUERIES = [None, [70, 3, 1]]  # single tokens (16-row tiles), and a request whose rows take 128-row tiles up to D = 128
+
+
+def small(seed, query, dtype, dim, exponent):
+    """Rows whose largest value is in [2^exponent, 2^(exponent + 1))."""
+    c = Case(seed, [150, 40, 9], query, dtype=dtype, dim=dim)
+    x = c.q.double()
+    x = x / x.abs().amax(2, keepdim=True) * 1.5 * 2.0 ** exponent
+    c.q = x.to(dtype)
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("query", QUERIES)
+def test_gpu_tiny_softmax_scales(dtype, dim, query):
+    """Scores of nothing, row maximum times scale from 2^-96 to 2^-140: the mean of the values, lse the keys' logarithm."""
+    for exponent in (0, -9, -14):
+        c = small(40, query, dtype, dim, exponent)
+        for s in range(96, 140):
+            c.scale = 2.0 ** (-s - exponent)
+            c.check(max_query_len=70)
+    for scale, exponent in ((1e-31, -9), (1e-28, -16), (1e-30, 0), (-1e-31, -9), (1e-45, 3)):
+        c = small(41, query, dtype, dim, max(exponent, -14) if dtype == FP else exponent)
+        c.scale = scale
+        c.check(max_query_len=70)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("query", [None, [50, 1, 20]])
+def test_gpu_queries_that_are_not_finite(dtype, dim, query):
+    """Their rows are NaN and no others, at the head sizes beside 128 too."""
+    c = Case(42, [77, 0, 200], query, dtype=dtype, dim=dim)
+    c.q[0, 0, 3], c.q[0, 5, 60], c.q[-1, 2, dim - 1], c.q[1, 1, 0] = torch.nan, torch.inf, -torch.inf, torch.nan
+    for scale in (c.scale, 1e-31):
+        c.scale = scale
+        out, lse = c.check(max_query_len=50)
+        assert bool(torch.isnan(out[0, 0]).all()) and bool(torch.isnan(lse[0, 5])) and not bool(torch.isnan(out[0, 1]).any())
