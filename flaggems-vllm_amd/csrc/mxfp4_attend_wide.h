@@ -43,7 +43,7 @@ constexpr int kWideKeys = 64;   // keys of a tile, and of a unit
 constexpr int kHalfShift = 7;
 __device__ __forceinline__ bool half_holds(uint32_t byte, u32x4_t codes) {
     const bool zeros = ((codes.x | codes.y | codes.z | codes.w) & 0x77777777u) == 0;
-    return (byte - (104u + kHalfShift) <= 36u) | (zeros & (byte != 255u));
+    return (byte - (104u + kHalfShift) <= 36u) | (zeros & (byte <= kMostByte));
 }
 
 template <int D, int kPieces>
@@ -373,8 +373,8 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
             if constexpr (decltype(kind)::value) {
                 byte = max(byte, (uint32_t)kHalfShift) - kHalfShift;
             } else {
-                nan_of[buffer][wave] = __ballot(byte == 255u);
-                byte = byte == 255u ? 0 : byte;
+                nan_of[buffer][wave] = __ballot(byte > kMostByte);
+                byte = byte > kMostByte ? 0 : byte;
             }
             return __uint_as_float(byte << 23);
         };

@@ -32,7 +32,8 @@
 // bits), token by token; LDS turns it, written by tokens and read by
 // ds_read_b64_tr_b16.  P goes in as two bf16 pieces (16 bits): one alone would
 // put its own 2^-9 beside the output's.  A value block under byte 255 (NaN) makes
-// the outputs of those rows NaN that see it.
+// the outputs of those rows NaN that see it, and so do 253 and 254, whose values
+// bf16 does not hold (their infinities would make any row NaN in whose tile they lie).
 //
 // Two kernels: 16-row tiles, whose waves share out the keys (here; single tokens,
 // a few of them, and D = 256), and 128-row tiles, whose waves share out the rows
@@ -76,6 +77,9 @@ constexpr float kAhead = 4.0f;
 // References farther from 0 are rounded by more than the one below which a score that is not
 // rounded may lie: there both are.
 constexpr float kFar = 1 << 20;
+
+// The last scale byte of values: above it they are NaN.
+constexpr uint32_t kMostByte = 252;
 
 // 16-key subtiles that a wave takes at a time: two such tiles have to fit its registers.
 __host__ __device__ constexpr int key_subtiles(int) { return 2; }
@@ -513,7 +517,7 @@ __device__ __forceinline__ void load_tile(const AttArgs& a, const Places& p, int
     }
 }
 
-// 8 codes times 2^(byte - 127) in bf16, exact below byte 253; byte 255 gives NaN.
+// 8 codes times 2^(byte - 127) in bf16, exact up to byte kMostByte; byte 255 gives NaN.
 __device__ __forceinline__ uint4 values_of(uint32_t codes, float scale) {
     return make_uint4(
         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
@@ -577,11 +581,17 @@ __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>
             for (int c = 0; c < S::kChunks; ++c) {
                 // a token that no row sees may hold anything; a NaN that some rows see is dealt with at the end
                 const uint32_t byte = any(key_of[t] + r) ? raw.vs[t][c] : 0;
-                nan[t][c] = __ballot(byte == 255u);
+                nan[t][c] = __ballot(byte > kMostByte);
                 any_nan |= nan[t][c] != 0;
-                raw.vs[t][c] = byte == 255u ? 0 : byte;
+                raw.vs[t][c] = byte > kMostByte ? 0 : byte;
             }
         }
+    } else {
+#pragma unroll
+        for (int t = 0; t < kSub; ++t)
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+                raw.vs[t][c] = raw.vs[t][c] > kMostByte ? 255 : raw.vs[t][c];
     }
 
     // V into LDS while the scores are on their way

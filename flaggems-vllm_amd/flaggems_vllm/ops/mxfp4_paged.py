@@ -137,8 +137,9 @@ def mxfp4_paged_attention(
     Returns:
         out [T, Hq, D] in q's type and lse [T, Hq] float32, the natural logarithm
         of each row's sum.  A row that sees no key has out 0 and lse +inf.  NaN
-        where a row sees a key or value block that is NaN, or its query holds a
-        NaN or an infinity.
+        where a row sees a key or value block that is NaN (byte 255; of values
+        253 and 254 too, which no op here writes), or its query holds a NaN or
+        an infinity.
     """
     rc, out, lse = _native.torch_ext().mxfp4_attention(
         q, kv_cache, block_table, seq_lens, float(softmax_scale), query_start_loc, max_query_len, max_seq_len,

@@ -776,8 +776,10 @@ int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t 
  *   lse = ln sum_j exp(softmax_scale q . k_j)
  *   out = sum_j exp(softmax_scale q . k_j) v_j / (exp(lse) + exp(attn_sink[h]))
  * (attn_sink NULL: none; it does not enter lse).  A row that sees nothing gets out 0
- * and lse +inf.  A row that sees a key or value block of byte 255, or whose
- * query holds a NaN or an infinity and that sees a key, gets NaN.  Rows of q
+ * and lse +inf.  A row that sees a key block of byte 255 or a value block of byte
+ * 253 and up (bf16 does not hold such values, and fgv_mxfp4_kv_quant_and_cache
+ * writes none), or whose query holds a NaN or an infinity and that sees a key,
+ * gets NaN (of values: in that block's dims).  Rows of q
  * outside query_start_loc's ranges are not written.
  *
  *   q, out  [num_tokens, num_heads, D] bf16 (dtype 0) or fp16 (1), unit last

@@ -48,3 +48,28 @@ def test_gpu_queries_that_are_not_finite(dtype, dim, query):
         c.scale = scale
         out, lse = c.check(max_query_len=50)
         assert bool(torch.isnan(out[0, 0]).all()) and bool(torch.isnan(lse[0, 5])) and not bool(torch.isnan(out[0, 1]).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens,query", [([300, 80, 190], [1, 1, 1]), ([300, 80, 190], [100, 9, 190]), ([300, 64], [5, 3])])
+def test_gpu_value_bytes_past_the_range(dtype, dim, lens, query):
+    """Value blocks under bytes 253 and 254, which no op here writes, are NaN as under 255: for the rows that see them,
+    and for no other row of their tile."""
+    for byte in (253, 254):
+        for at in (0, 70, 189, 295):
+            print(f"\n[case] byte {byte} {dtype} {dim} {query} {at}", flush=True)
+            c = Case(50, lens, query, dim=dim, dtype=dtype)
+            codes, scales = parts(c.cache)[1], parts(c.cache)[3]
+            where = [(int(c.table[b, at // 16]), b) for b, n in enumerate(lens) if at < n]
+            for block, _ in where:
+                codes[block, :, at % 16] = 0x7F  # 6 and -6
+            got = []
+            for x in (byte, 255):
+                for block, _ in where:
+                    scales[block, 1, at % 16, dim // 64] = x
+                got.append((c.run(max_query_len=max(query)), c.run(max_query_len=max(query), window_size=40)))
+            c.check(got=got[0][0])
+            c.check(40, got=got[0][1])
+            c.check(got=got[1][0])
