@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
     __shared__ __align__(16) uint8_t turned[2][S::kVBytes];
     __shared__ __align__(16) uint32_t held_by[2][kAttWaves];  // whether fp16 holds each wave's values
     __shared__ uint64_t nan_of[2][kAttWaves];                 // which of its value blocks are NaN, bit by lane
+    __shared__ __align__(16) uint32_t large_of[2][kAttWaves];  // whether it has values under bytes past kLargeByte
     using Rows = WideQuery<D, kPieces>;
     __shared__ uint4 more_query[kAttWaves][Rows::kInLds ? 64 * Rows::kInLds : 1];  // the pieces not in registers
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -356,6 +357,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
             for (int i = 0; i < 16; ++i)
                 acc[d][i] = 0.f;
         float m_run = -INFINITY, l_run = 0.f;
+        Margin margin = kUsual;  // the large values', which only the second loop meets, from the first of them on
 
         // A token that no row sees may hold anything: its values are taken as finite.
         auto look = [&](WideValueTile<D>& t, int buffer) {
@@ -375,6 +377,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
             } else {
                 nan_of[buffer][wave] = __ballot(byte > kMostByte);
                 byte = byte > kMostByte ? 0 : byte;
+                large_of[buffer][wave] = __any(byte > kLargeByte);
             }
             return __uint_as_float(byte << 23);
         };
@@ -475,9 +478,15 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
                 most[j & 1] = fmaxf(most[j & 1], s[0][j]);
                 most[2 + (j & 1)] = fmaxf(most[2 + (j & 1)], s[1][j]);
             }
-            const float top = pair_max(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * a.scale_f;
+            float top = pair_max(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * a.scale_f;
+            if constexpr (!kFast) {
+                const uint4 large = *reinterpret_cast<const uint4*>(large_of[buffer]);
+                if (__builtin_amdgcn_readfirstlane(large.x | large.y | large.z | large.w))
+                    margin = large_margin(keys_seen(a, req));
+                top += margin.margin;
+            }
             if (__any(top > m_run)) {
-                const float m_new = top > m_run ? top + kAhead : m_run;
+                const float m_new = top > m_run ? top + (kFast ? kAhead : margin.ahead) : m_run;
                 const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
                 l_run *= alpha;
 #pragma unroll

@@ -74,6 +74,18 @@ constexpr float kLn2 = 0.6931471805599453f;
 // A row's reference is raised when a score exceeds it, and then to this much
 // above the score (base 2), so that most tiles rescale nothing.  P is at most 1.
 constexpr float kAhead = 4.0f;
+// Sums of P v over 2^30 keys stay finite with P at most 1 for values under bytes up to kLargeByte
+// (6 * 2^89).  Once a wave meets larger ones, up to 6 * 2^125, its references keep `margin` above the
+// scores instead: P is below 1 / n, n the keys that a row may see.  (Nothing is P below 2^-126:
+// below n 2^-126 of the row's largest there, 2^-122 otherwise.)
+constexpr uint32_t kLargeByte = 216;
+struct Margin {
+    float margin, ahead;
+};
+constexpr Margin kUsual = {0.f, kAhead};
+__device__ __forceinline__ Margin large_margin(int32_t keys) {
+    return Margin{(float)(32 - __builtin_clz((uint32_t)keys | 1u)), 0.f};
+}
 // References farther from 0 are rounded by more than the one below which a score that is not
 // rounded may lie: there both are.
 constexpr float kFar = 1 << 20;
@@ -150,6 +162,12 @@ __device__ __forceinline__ int32_t keys_begin(const AttArgs& a, int32_t pos) {
         begin = max(pos - a.window + 1, 0) & ~(kTileKeys - 1);
     }
     return begin;
+}
+
+// The most keys that a row of a request sees.
+__device__ __forceinline__ int32_t keys_seen(const AttArgs& a, const Request& r) {
+    const int32_t keys = min(r.len, a.table_keys);
+    return a.window > 0 ? min(keys, a.window) : keys;
 }
 
 // A request and its tiles of rows, `units` units of keys each, dealt out as `cost`.
@@ -548,13 +566,15 @@ constexpr int32_t kNoKey = 0x7ff80000;  // seen by nobody: behind the longest re
 // them are seen by all rows; otherwise some may be hidden, hold anything or be NaN.
 // (One body for both: with two, the compiler keeps two sets of sums.)
 //
+// `margin` is the large values' from the first of them on; a row sees `most_keys` at most.
+//
 // `refill` loads the next tile into `raw` as soon as this one has left it, for
 // the matrix instruction and for LDS.
 template <int D, int kPieces, int kSub, class Refill>
 __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>& raw, int32_t key0, bool plain,
                                        Seen any, Seen seen, float scale_f, const Query<D, kPieces>& query,
                                        uint8_t* turned, int lane, f32x4_t (&acc)[D / 16], float& m_run, float& l_run,
-                                       Refill refill) {
+                                       Margin& margin, int32_t most_keys, Refill refill) {
     using S = Shape<D, kPieces>;
     const int r = lane & 15, g = lane >> 4;
     f32x4_t s[kSub];
@@ -586,7 +606,15 @@ __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>
                 raw.vs[t][c] = byte > kMostByte ? 0 : byte;
             }
         }
-    } else {
+    }
+    uint32_t largest = 0;
+#pragma unroll
+    for (int t = 0; t < kSub; ++t)
+#pragma unroll
+        for (int c = 0; c < S::kChunks; ++c)
+            largest = max(largest, raw.vs[t][c]);
+    if (__any(largest > kLargeByte)) {
+        margin = large_margin(most_keys);
 #pragma unroll
         for (int t = 0; t < kSub; ++t)
 #pragma unroll
@@ -626,9 +654,9 @@ __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             most = fmaxf(most, s[t][i]);
-    most = group4_max(most) * scale_f;
+    most = __builtin_fmaf(group4_max(most), scale_f, margin.margin);
     if (__any(most > m_run)) {
-        const float m_new = most > m_run ? most + kAhead : m_run;
+        const float m_new = most > m_run ? most + margin.ahead : m_run;
         const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
         l_run *= alpha;
 #pragma unroll
@@ -838,6 +866,8 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
         for (int d = 0; d < D / 16; ++d)
             acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         float m_run = -INFINITY, l_run = 0.f;
+        Margin margin = kUsual;
+        const int32_t most_keys = keys_seen(a, req);
 
         auto step = [&](int32_t i, RawTile<kSub, S::kChunks>& now) {
             auto refill = [&]() {
@@ -854,7 +884,7 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
             for (int t = 0; t < kSub; ++t)
                 plain = plain & (now.place[t] >= 0);
             attend<D, kPieces, kSub>(now, key, plain, any, seen, a.scale_f, query, turned[wave], lane, acc, m_run, l_run,
-                                     refill);
+                                     margin, most_keys, refill);
         };
         for (int32_t i = 0; i < tiles; i += kDepth) {
 #pragma unroll

@@ -73,3 +73,48 @@ def test_gpu_value_bytes_past_the_range(dtype, dim, lens, query):
             c.check(got=got[0][0])
             c.check(40, got=got[0][1])
             c.check(got=got[1][0])
+
+
+SIZES = [  # lengths, query tokens, heads, key heads, dim
+    ([700, 64, 23], None, 8, 2, 128), ([700, 64, 23], None, 16, 1, 256), ([700, 64, 23], None, 8, 8, 64),
+    ([700, 300], [700, 70], 8, 2, 128), ([700, 300], [650, 1], 2, 1, 64), ([700, 300], [90, 70], 8, 2, 256),
+    ([9000], None, 8, 1, 128), ([9000], [130], 4, 4, 64), ([9000, 5000], [3, 200], 8, 2, 128), ([9000], None, 4, 1, 256)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lens,query,heads,kv_heads,dim", SIZES)
+def test_gpu_large_values_of_one_sign(dtype, lens, query, heads, kv_heads, dim):
+    """Scores all alike over values all alike, the largest that a cache is written with among them: their mean is that
+    value, though their sum is past 32 bits' range; tiles whole and cut."""
+    for byte in (252, 245, 230, 217, 216, 215, 127) if dtype == BF else (252, 217, 140, 127):
+        print(f"\n[case] one sign {dtype} {lens} {query} {dim} {byte}", flush=True)
+        c = Case(44, lens, query, heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype)
+        codes, scales = parts(c.cache)[1], parts(c.cache)[3]
+        codes.fill_(0x77)
+        codes[:, :, :, 1] = 0xFF
+        scales[scales != 255] = byte
+        for shrink in (0.0, 1.0):  # scores all alike, and the usual ones
+            c.q = c.q * shrink if shrink else Case(45, lens, query, heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype).q
+            out, _ = c.check(max_query_len=max(query or [1]))
+            if dtype == BF:
+                want = torch.full_like(out, 6 * 2.0 ** (byte - 127))
+                want[..., 2:4] *= -1
+                assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lens,query,heads,kv_heads,dim", SIZES)
+def test_gpu_large_values_here_and_there(dtype, lens, query, heads, kv_heads, dim):
+    """The largest values at some tokens only, early, late and throughout, of both signs, beside ordinary ones."""
+    for seed, where in enumerate([slice(0, 1), slice(600, 640), slice(20, 5000, 37), slice(0, 9000)]):
+        print(f"\n[case] here and there {dtype} {lens} {query} {dim} {where}", flush=True)
+        c = Case(46 + seed, lens, query, heads=heads, kv_heads=kv_heads, dim=dim, dtype=dtype)
+        at = torch.arange(lens[0], device=c.cache.device)[where]
+        block = c.table[0, at // 16].long()
+        for h in range(kv_heads):
+            byte = torch.randint(205, 253, (len(at), dim // 32), generator=c.g).to(torch.uint8).to(at.device)
+            parts(c.cache)[3][block, h, at % 16] = byte
+        c.check(max_query_len=max(query or [1]))
+        c.check(window=333, sink=torch.randn(heads, device=at.device), max_query_len=max(query or [1]))
