@@ -406,17 +406,18 @@ __device__ __forceinline__ void load_query(const AttArgs& a, int64_t at, bool va
 // How a row with largest magnitude `most` (its bits) enters: q 2^scale_e = x 2^e,
 // x = q * down with its maximum in [128, 256).  The softmax scale's power of two
 // goes in here, so that scores leave binary32's range only where scaled ones
-// would.  -118 leaves room for the pieces' smaller scales.
+// would.  -118 leaves room for the pieces' smaller scales: rows whose largest value is below
+// 2^-111 under the scale lose bits, which only keys of 2^100 and more would show.
 struct QueryScale {
-    bool bad;  // not finite: the scale says NaN
+    bool bad;  // not finite, or not under the scale (2^135 and more): the scale says NaN
     int byte;
     float down;
 };
 
 __device__ __forceinline__ QueryScale query_scale(const AttArgs& a, uint32_t most) {
-    const int e = min(max((int)(most >> 23) - 127 - 7 + a.scale_e, -118), 127);
+    const int exact = (int)(most >> 23) - 127 - 7 + a.scale_e, e = min(max(exact, -118), 127);
     QueryScale q;
-    q.bad = most >= 0x7f800000u;
+    q.bad = most >= 0x7f800000u || exact > 127;
     q.byte = e + 127;
     q.down = __uint_as_float((uint32_t)min(max(127 - e + a.scale_e, 1), 254) << 23) * a.scale_sign;
     return q;

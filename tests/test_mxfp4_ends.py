@@ -118,3 +118,25 @@ def test_gpu_large_values_here_and_there(dtype, lens, query, heads, kv_heads, di
             parts(c.cache)[3][block, h, at % 16] = byte
         c.check(max_query_len=max(query or [1]))
         c.check(window=333, sink=torch.randn(heads, device=at.device), max_query_len=max(query or [1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("query", QUERIES)
+def test_gpu_scaled_queries_past_the_range(dim, query):
+    """A row whose largest value times the scale (and log2 e) is 2^135 or more counts as one that holds an infinity, whatever its
+    keys are; below that scores are what they are."""
+    c = Case(43, [90, 40, 9], query, dim=dim, dtype=BF)
+    parts(c.cache)[2].masked_fill_(parts(c.cache)[2] != 255, 1)  # keys of at most 6 * 2^-126
+    c.q = (c.q.double() / c.q.double().abs().amax(2, keepdim=True) * 1.5).to(BF)
+    c.q[:, 1::2] *= 2.0 ** 116
+    c.q[:, 0::2] *= 2.0 ** 110
+    c.scale = 2.0 ** 18  # 2^134 is inside, 2^128 well so
+    c.check(max_query_len=70)
+    c.scale = 2.0 ** 19
+    out, lse = c.run(max_query_len=70)
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(out[:, 1::2]).all()) and bool(torch.isnan(lse[:, 1::2]).all())
+    assert not bool(torch.isnan(out[:, 0::2]).any()) and not bool(torch.isnan(lse[:, 0::2]).any())
+    c.scale = -2.0 ** 22
+    assert bool(torch.isnan(c.run(max_query_len=70)[0][:, 1::2]).all())
