@@ -1273,7 +1273,7 @@ extern "C" int fgv_mxfp4_paged_attention(const void* q, int64_t q_stride_token, 
     if (!(softmax_scale >= -1e30 && softmax_scale <= 1e30))
         return fail(FGV_E_BAD_SHAPE, "softmax_scale must be finite");
     if (num_heads > 65536 || block_size > 4096 || num_reqs > 0x3fffffffLL || num_blocks > 0x7fffffffLL ||
-        num_tokens * num_heads > 0x3fffffffLL || max_blocks_per_req > (0x3fffffffLL / block_size))
+        num_tokens > 0x3fffffffLL / num_heads || max_blocks_per_req > (0x3fffffffLL / block_size))
         return fail(FGV_E_TOO_LARGE, "at most 65536 heads, 4096 tokens per block, 2^30 - 1 query rows and table keys");
     if (!q || !out || !lse || !seq_lens || (max_blocks_per_req > 0 && !block_table) || (num_blocks > 0 && !kv_cache))
         return fail(FGV_E_NULL_POINTER, "null pointer argument");
@@ -1336,7 +1336,7 @@ extern "C" int64_t fgv_mxfp4_paged_attention_workspace_bytes(int64_t num_tokens,
                                                              int64_t num_kv_heads, int64_t head_dim, int64_t num_reqs,
                                                              int64_t max_query_len, int64_t max_seq_len) {
     if (num_tokens <= 0 || num_reqs <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || num_heads > 65536 ||
-        num_tokens * num_heads > 0x3fffffffLL || num_reqs > 0x3fffffffLL)
+        num_tokens > 0x3fffffffLL / num_heads || num_reqs > 0x3fffffffLL)
         return 0;
     return fgv::workspace_of(
         fgv::call_of(num_tokens, num_heads, num_kv_heads, head_dim, num_reqs, max_query_len, max_seq_len, 0));

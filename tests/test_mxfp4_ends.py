@@ -4,6 +4,8 @@ pass 32 bits' range, against the formula in 64 bits within the bounds of test_mx
 import pytest
 import torch
 
+from flaggems_vllm import _native
+
 from .test_mxfp4_attention import BF, FP, Case
 from .test_mxfp4_kv_cache import parts
 
@@ -140,3 +142,18 @@ def test_gpu_scaled_queries_past_the_range(dim, query):
     assert not bool(torch.isnan(out[:, 0::2]).any()) and not bool(torch.isnan(lse[:, 0::2]).any())
     c.scale = -2.0 ** 22
     assert bool(torch.isnan(c.run(max_query_len=70)[0][:, 1::2]).all())
+
+
+def call_c(tokens, heads, reqs, start=16):
+    return _native.lib().fgv_mxfp4_paged_attention(
+        16, 64 * heads, 64, 0, tokens, heads, heads, 64, 16, heads * 16 * 68, 5, 16, 16, 4, 4, 16, start, reqs, 1, 64, 0.1,
+        0, None, 16, 64 * heads, 64, 16, heads, None, 0, None)
+
+
+@pytest.mark.parametrize("tokens,heads", [(1 << 48, 65536), (1 << 62, 4), ((1 << 58) + 1, 64), (1 << 30, 1), (1 << 29, 3)])
+def test_c_abi_refuses_rows_whose_number_wraps(tokens, heads):
+    """tokens * heads past 64 bits is too large, not small."""
+    assert call_c(tokens, heads, 3) == -5
+    assert b"2^30 - 1 query rows" in _native.lib().fgv_last_error()
+    assert call_c(tokens, heads, 1 << 62) == -5
+    assert _native.lib().fgv_mxfp4_paged_attention_workspace_bytes(tokens, heads, heads, 64, 3, 100, 100000) == 0
