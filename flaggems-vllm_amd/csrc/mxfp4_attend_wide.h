@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hh = lane >> 5, r = lane & 15, g = lane >> 4;
     const int h = (int)blockIdx.x % a.kv_heads;
-    const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads);
+    const int32_t worker = a.first_worker + (int32_t)(blockIdx.x / a.kv_heads);
     // Where this lane writes its first 16-byte piece of V, and reads V turned: piece i of a 64-byte run
     // lies at i ^ (row / 4 % 4), so that neither the lanes of a write nor of a read meet a bank twice.
     static_assert(S::kVPitch % 64 == 0 && S::kVBytes % 64 == 0, "pieces are found by xor");

@@ -122,6 +122,7 @@ struct AttArgs {
     int32_t rows_from, rows_to;  // requests of other numbers of rows are another launch's
     // Stream mode (workers > 0): workers per head, and the workspace's parts.
     int32_t workers, per_cu, tile_cost;
+    int32_t first_worker;  // of this launch
     float* partials;
     struct CutTile* cut_tiles;
 };
@@ -809,7 +810,7 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
     __shared__ float wave_m[kAttWaves][kRows], wave_l[kAttWaves][kRows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = (int)blockIdx.x % a.kv_heads;
-    const int32_t worker = (int32_t)(blockIdx.x / a.kv_heads);
+    const int32_t worker = a.first_worker + (int32_t)(blockIdx.x / a.kv_heads);
     const int r = lane & 15, g = lane >> 4;
     const int orow = threadIdx.x >> 4, part = threadIdx.x & 15;  // of the end: 16 threads per row
     Start w;
@@ -1184,6 +1185,9 @@ Dealing dealing_of(const Call& c, bool wide) {
     return d;
 }
 
+// Workgroups of a launch: one of 2^32 threads and more is cut to the low 32 bits without an error.
+constexpr int64_t kMostGroups = (1LL << 31) / kAttThreads;
+
 template <int D, int kPieces, int kTileRows>
 void launch_part(const Dealing& d, uint8_t* workspace, int64_t unit, hipStream_t st, AttArgs a) {
     // (the cost of all tiles has to fit 31 bits: with more of it there is nothing to gain either)
@@ -1193,20 +1197,24 @@ void launch_part(const Dealing& d, uint8_t* workspace, int64_t unit, hipStream_t
     a.per_cu = per_cu(D, kTileRows == kWideRows);
     a.partials = reinterpret_cast<float*>(workspace);
     a.cut_tiles = reinterpret_cast<CutTile*>(workspace + d.cut_tiles_at);
-    const unsigned grid = (unsigned)((stream ? d.workers : d.tiles) * a.kv_heads);
-    if constexpr (kTileRows == kRows)
-        hipLaunchKernelGGL((mxfp4_attend_kernel<D, kPieces>), dim3(grid), dim3(kAttThreads), 0, st, a);
-    else
-        hipLaunchKernelGGL((mxfp4_attend_wide_kernel<D, kPieces>), dim3(grid), dim3(kAttThreads), 0, st, a);
+    const int64_t workers = stream ? d.workers : d.tiles, most = kMostGroups / a.kv_heads;
+    for (int64_t first = 0; first < workers; first += most) {
+        a.first_worker = (int32_t)first;
+        const unsigned grid = (unsigned)((workers - first < most ? workers - first : most) * a.kv_heads);
+        if constexpr (kTileRows == kRows)
+            hipLaunchKernelGGL((mxfp4_attend_kernel<D, kPieces>), dim3(grid), dim3(kAttThreads), 0, st, a);
+        else
+            hipLaunchKernelGGL((mxfp4_attend_wide_kernel<D, kPieces>), dim3(grid), dim3(kAttThreads), 0, st, a);
+    }
     if (!stream)
         return;
     // a wave per row where that fills the chip (4 x 256 rows)
     const int64_t cut_tiles = (d.tiles < a.workers ? d.tiles : a.workers) * a.kv_heads;
     if (cut_tiles * d.rows >= 1024) {
         // (4096 workgroups at most, if each has a tile: they take more rows then)
-        const int64_t most = 4096 / cut_tiles, rows = (d.rows + 3) / 4;
+        const int64_t share = 4096 / cut_tiles, rows = (d.rows + 3) / 4;
         hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, kTileRows, false>),
-                           dim3((unsigned)cut_tiles, (unsigned)(most < 1 ? 1 : most < rows ? most : rows)),
+                           dim3((unsigned)cut_tiles, (unsigned)(share < 1 ? 1 : share < rows ? share : rows)),
                            dim3(kAttThreads), 0, st, a);
     } else {
         hipLaunchKernelGGL((mxfp4_combine_kernel<D, kPieces == 3, kTileRows, true>), dim3((unsigned)cut_tiles, d.rows),

@@ -26,6 +26,8 @@ namespace fgv {
 namespace {
 
 constexpr int kInsThreads = 256;
+// Threads of a launch: one of 2^32 and more is cut to the low 32 bits without an error.
+constexpr int64_t kInsMostThreads = 1LL << 31;
 
 struct InsertArgs {
     const void* k;
@@ -143,8 +145,11 @@ __global__ void __launch_bounds__(kInsThreads) mxfp4_insert_kernel(InsertArgs a)
 }
 
 template <int D>
-void launch_insert(bool half, bool wide, unsigned grid, hipStream_t st, const InsertArgs& a) {
-    const dim3 g(grid), b(kInsThreads);
+void launch_insert(bool half, bool wide, hipStream_t st, InsertArgs a) {
+    const int64_t groups = (a.num_rows + kInsThreads / (D / 8) - 1) / (kInsThreads / (D / 8));
+    // a multiple of 8 workgroups, each XCD's a consecutive range (more than the grid's end: threads past the tokens leave)
+    a.blocks_per_xcd = groups >= 64 ? (uint32_t)((groups + 7) / 8) : 0;
+    const dim3 g(a.blocks_per_xcd ? 8 * a.blocks_per_xcd : (unsigned)groups), b(kInsThreads);
     if (half && wide)
         hipLaunchKernelGGL((mxfp4_insert_kernel<D, true, true>), g, b, 0, st, a);
     else if (half)
@@ -188,8 +193,6 @@ extern "C" int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_toke
     if (!aligned(kv_cache, 16) || !aligned(slot_mapping, 8) || !aligned(k, 2) || !aligned(v, 2))
         return fail(FGV_E_MISALIGNED, "kv_cache must be 16-byte aligned, slot_mapping 8, k and v by element");
     InsertArgs a;
-    a.k = k;
-    a.v = v;
     a.k_st = k_stride_token;
     a.k_sh = k_stride_head;
     a.v_st = v_stride_token;
@@ -197,21 +200,22 @@ extern "C" int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_toke
     a.cache = kv_cache;
     a.block_stride = cache_block_stride;
     a.num_slots = num_blocks * block_size;
-    a.slots = slot_mapping;
-    a.num_rows = (uint32_t)(num_tokens * num_kv_heads);
     a.kv_heads = (uint32_t)num_kv_heads;
     a.page = (uint32_t)block_size;
-    const int64_t groups = (num_tokens * threads_per_token + kInsThreads - 1) / kInsThreads;
-    // a multiple of 8 workgroups, each XCD's a consecutive range (more than the grid's end: threads past the tokens leave)
-    a.blocks_per_xcd = groups >= 64 ? (uint32_t)((groups + 7) / 8) : 0;
-    const unsigned grid = a.blocks_per_xcd ? 8 * a.blocks_per_xcd : (unsigned)groups;
     const bool wide = aligned(k, 16) && aligned(v, 16) &&
                       ((k_stride_token | k_stride_head | v_stride_token | v_stride_head) & 7) == 0;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    switch (head_dim) {
-        case 64: launch_insert<64>(dtype == 1, wide, grid, st, a); break;
-        case 128: launch_insert<128>(dtype == 1, wide, grid, st, a); break;
-        default: launch_insert<256>(dtype == 1, wide, grid, st, a); break;
+    const int64_t most = kInsMostThreads / threads_per_token;  // 2^10 tokens at least
+    for (int64_t first = 0; first < num_tokens; first += most) {
+        a.k = static_cast<const uint16_t*>(k) + first * k_stride_token;
+        a.v = static_cast<const uint16_t*>(v) + first * v_stride_token;
+        a.slots = slot_mapping + first;
+        a.num_rows = (uint32_t)((num_tokens - first < most ? num_tokens - first : most) * num_kv_heads);
+        switch (head_dim) {
+            case 64: launch_insert<64>(dtype == 1, wide, st, a); break;
+            case 128: launch_insert<128>(dtype == 1, wide, st, a); break;
+            default: launch_insert<256>(dtype == 1, wide, st, a); break;
+        }
     }
     return launch_status();
 }

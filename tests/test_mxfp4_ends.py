@@ -4,10 +4,11 @@ pass 32 bits' range, against the formula in 64 bits within the bounds of test_mx
 import pytest
 import torch
 
+import flaggems_vllm as fv
 from flaggems_vllm import _native
 
 from .test_mxfp4_attention import BF, FP, Case
-from .test_mxfp4_kv_cache import parts
+from .test_mxfp4_kv_cache import empty_cache, expected, parts, rows, values
 
 QUERIES = [None, [70, 3, 1]]  # single tokens (16-row tiles), and a request whose rows take 128-row tiles up to D = 128
 
@@ -157,3 +158,41 @@ def test_c_abi_refuses_rows_whose_number_wraps(tokens, heads):
     assert b"2^30 - 1 query rows" in _native.lib().fgv_last_error()
     assert call_c(tokens, heads, 1 << 62) == -5
     assert _native.lib().fgv_mxfp4_paged_attention_workspace_bytes(tokens, heads, heads, 64, 3, 100, 100000) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("query_heads", [64, 128])
+def test_gpu_attention_in_more_workgroups_than_a_launch_has(query_heads):
+    """2^18 + 1 requests of one token and 64 key heads: 2^24 + 64 workgroups of 256 threads, of which a launch of 2^32
+    and more has only what is left of 32 bits."""
+    reqs, heads, dim = 2 ** 18 + 1, 64, 64
+    c = Case(51, [16] * 40, heads=query_heads, kv_heads=heads, dim=dim, dtype=BF)
+    g = torch.Generator().manual_seed(52)
+    live = c.table[:, 0]
+    table = live[torch.randint(0, 40, (reqs,), generator=g).to(live.device)][:, None]
+    lens = torch.ones(reqs, dtype=torch.int32, device=live.device)
+    lens[77::1000] = 0
+    out, lse = fv.mxfp4_paged_attention(c.q[:1].expand(reqs, -1, -1), c.cache, table, lens, c.scale)
+    first = values(parts(c.cache)[1][live.long(), :, 0], parts(c.cache)[3][live.long(), :, 0])  # [40, heads, dim]
+    want = first.to(BF).repeat_interleave(query_heads // heads, 1)
+    at = torch.empty(len(c.cache), dtype=torch.long, device=live.device)
+    at[live.long()] = torch.arange(40, device=live.device)
+    for b in range(0, reqs, 1 << 14):
+        mine = want[at[table[b:b + (1 << 14), 0].long()]] * (lens[b:b + (1 << 14)] > 0)[:, None, None]
+        assert torch.equal(out[b:b + (1 << 14)], mine), b
+    assert bool((torch.isposinf(lse) == (lens == 0)[:, None]).all())
+
+
+@pytest.mark.gpu
+def test_gpu_insert_in_more_workgroups_than_a_launch_has():
+    """2^24 + 3 tokens of 8 heads of 256, a workgroup each."""
+    tokens, heads, dim, page = 2 ** 24 + 3, 8, 256, 16
+    k, v = rows(53, 1, heads, dim, dtype=BF), rows(54, 1, heads, dim, dtype=BF)
+    cache = empty_cache(4, heads, page, dim)
+    slots = torch.full((tokens,), -1, dtype=torch.int64)
+    at = torch.tensor([0, 5, 2 ** 21 - 1, 2 ** 21, 2 ** 23 - 1, 2 ** 23, 2 ** 23 + 1, 2 ** 24 - 1, 2 ** 24, tokens - 1])
+    slots[at] = torch.arange(len(at)) * 5 + 3
+    want = expected(cache, k.expand(len(at), -1, -1), v.expand(len(at), -1, -1), slots[at])
+    fv.mxfp4_kv_quant_and_cache(k.expand(tokens, -1, -1), v.expand(tokens, -1, -1), cache, slots.to(k.device))
+    torch.cuda.synchronize()
+    assert torch.equal(cache.cpu(), want)
