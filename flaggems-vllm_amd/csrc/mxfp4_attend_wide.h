@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
             for (int i = 0; i < 16; ++i)
                 acc[d][i] = 0.f;
         float m_run = -INFINITY, l_run = 0.f;
-        Margin margin = kUsual;  // the large values', which only the second loop meets, from the first of them on
+        float margin = 0.f;  // as in attend(): from the first large values on, which only the second loop meets
 
         // A token that no row sees may hold anything: its values are taken as finite.
         auto look = [&](WideValueTile<D>& t, int buffer) {
@@ -478,15 +478,20 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
                 most[j & 1] = fmaxf(most[j & 1], s[0][j]);
                 most[2 + (j & 1)] = fmaxf(most[2 + (j & 1)], s[1][j]);
             }
-            float top = pair_max(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * a.scale_f;
+            const float top = pair_max(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * a.scale_f;
             if constexpr (!kFast) {
                 const uint4 large = *reinterpret_cast<const uint4*>(large_of[buffer]);
-                if (__builtin_amdgcn_readfirstlane(large.x | large.y | large.z | large.w))
+                if (margin == 0.f && __builtin_amdgcn_readfirstlane(large.x | large.y | large.z | large.w)) {
                     margin = large_margin(keys_seen(a, req));
-                top += margin.margin;
+                    const float down = __builtin_amdgcn_exp2f(-margin);
+                    l_run *= down;
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d)
+                        acc[d] *= down;
+                }
             }
             if (__any(top > m_run)) {
-                const float m_new = top > m_run ? top + (kFast ? kAhead : margin.ahead) : m_run;
+                const float m_new = top > m_run ? top + kAhead : m_run;
                 const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
                 l_run *= alpha;
 #pragma unroll
@@ -494,7 +499,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
                     acc[d] *= alpha;
                 m_run = m_new;
             }
-            float m_use = (m_run == -INFINITY ? 0.f : m_run) - (kFast ? (float)kHalfShift : 0.f);
+            float m_use = (m_run == -INFINITY ? 0.f : m_run) + (kFast ? -(float)kHalfShift : margin);
             float times = a.scale_f;
             if (__any(fabsf(m_use) > kFar)) {
 #pragma unroll
@@ -602,6 +607,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
         }
 
         l_run += __shfl_xor(l_run, 32);
+        m_run += margin;
         lds_barrier();  // V was read
         int lane_again = lane;
         asm("" : "+v"(lane_again));  // what follows from it takes no registers in the loops

@@ -75,17 +75,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 // above the score (base 2), so that most tiles rescale nothing.  P is at most 1.
 constexpr float kAhead = 4.0f;
 // Sums of P v over 2^30 keys stay finite with P at most 1 for values under bytes up to kLargeByte
-// (6 * 2^89).  Once a wave meets larger ones, up to 6 * 2^125, its references keep `margin` above the
-// scores instead: P is below 1 / n, n the keys that a row may see.  (Nothing is P below 2^-126:
-// below n 2^-126 of the row's largest there, 2^-122 otherwise.)
+// (6 * 2^89).  Once a wave meets larger ones, up to 6 * 2^125, P and its sums are taken under a
+// reference that is large_margin higher: P is below 1 / n, n the keys that a row may see.  (Nothing
+// is P below 2^-126: below n 2^-121 of the row's largest there, 2^-122 otherwise.)
 constexpr uint32_t kLargeByte = 216;
-struct Margin {
-    float margin, ahead;
-};
-constexpr Margin kUsual = {0.f, kAhead};
-__device__ __forceinline__ Margin large_margin(int32_t keys) {
-    return Margin{(float)(32 - __builtin_clz((uint32_t)keys | 1u)), 0.f};
-}
+__device__ __forceinline__ float large_margin(int32_t keys) { return (float)(32 - __builtin_clz((uint32_t)keys | 1u)); }
 // References farther from 0 are rounded by more than the one below which a score that is not
 // rounded may lie: there both are.
 constexpr float kFar = 1 << 20;
@@ -118,11 +112,11 @@ struct AttArgs {
     int32_t scale_e;
     float scale_sign;
     int32_t num_reqs, num_tokens, kv_heads, group, page, table_keys, window;
-    int32_t q_wide, o_wide;
+    int32_t first_worker;        // of this launch
     int32_t rows_from, rows_to;  // requests of other numbers of rows are another launch's
     // Stream mode (workers > 0): workers per head, and the workspace's parts.
     int32_t workers, per_cu, tile_cost;
-    int32_t first_worker;  // of this launch
+    int32_t q_wide, o_wide;
     float* partials;
     struct CutTile* cut_tiles;
 };
@@ -565,10 +559,11 @@ struct Seen {
 constexpr int32_t kNoKey = 0x7ff80000;  // seen by nobody: behind the longest request's last position
 
 // Attends the tile's keys, from key0 on, for the wave's 16 rows.  `plain`: all of
-// them are seen by all rows; otherwise some may be hidden, hold anything or be NaN.
-// (One body for both: with two, the compiler keeps two sets of sums.)
+// them are seen by all rows; otherwise, and where values are large or NaN, some may be
+// hidden, hold anything or be NaN.  (One body for both: with two, the compiler keeps two sets of sums.)
 //
-// `margin` is the large values' from the first of them on; a row sees `most_keys` at most.
+// `margin` is 0, and from the first large values on large_margin of `most_keys`, which a row
+// sees at most; sums are under the reference m_run + margin.
 //
 // `refill` loads the next tile into `raw` as soon as this one has left it, for
 // the matrix instruction and for LDS.
@@ -576,7 +571,7 @@ template <int D, int kPieces, int kSub, class Refill>
 __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>& raw, int32_t key0, bool plain,
                                        Seen any, Seen seen, float scale_f, const Query<D, kPieces>& query,
                                        uint8_t* turned, int lane, f32x4_t (&acc)[D / 16], float& m_run, float& l_run,
-                                       Margin& margin, int32_t most_keys, Refill refill) {
+                                       float& margin, int32_t most_keys, Refill refill) {
     using S = Shape<D, kPieces>;
     const int r = lane & 15, g = lane >> 4;
     f32x4_t s[kSub];
@@ -595,7 +590,15 @@ __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>
     uint64_t nan[kSub][S::kChunks];  // which value blocks are NaN, bit by lane
     int32_t key_of[kSub];            // each subtile's first key
     bool any_nan = false;
+    uint32_t largest = 0;
+#pragma unroll
+    for (int t = 0; t < kSub; ++t)
+#pragma unroll
+        for (int c = 0; c < S::kChunks; ++c)
+            largest = max(largest, raw.vs[t][c]);
+    plain = plain & !__any(largest > kLargeByte);
     if (!plain) {
+        largest = 0;
 #pragma unroll
         for (int t = 0; t < kSub; ++t) {
             key_of[t] = raw.place[t] >= 0 ? key0 + 16 * t : kNoKey;
@@ -606,22 +609,17 @@ __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>
                 nan[t][c] = __ballot(byte > kMostByte);
                 any_nan |= nan[t][c] != 0;
                 raw.vs[t][c] = byte > kMostByte ? 0 : byte;
+                largest = max(largest, raw.vs[t][c]);
             }
         }
-    }
-    uint32_t largest = 0;
+        if (margin == 0.f && __any(largest > kLargeByte)) {
+            margin = large_margin(most_keys);
+            const float down = __builtin_amdgcn_exp2f(-margin);
+            l_run *= down;
 #pragma unroll
-    for (int t = 0; t < kSub; ++t)
-#pragma unroll
-        for (int c = 0; c < S::kChunks; ++c)
-            largest = max(largest, raw.vs[t][c]);
-    if (__any(largest > kLargeByte)) {
-        margin = large_margin(most_keys);
-#pragma unroll
-        for (int t = 0; t < kSub; ++t)
-#pragma unroll
-            for (int c = 0; c < S::kChunks; ++c)
-                raw.vs[t][c] = raw.vs[t][c] > kMostByte ? 255 : raw.vs[t][c];
+            for (int d = 0; d < D / 16; ++d)
+                acc[d] *= down;
+        }
     }
 
     // V into LDS while the scores are on their way
@@ -656,9 +654,9 @@ __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             most = fmaxf(most, s[t][i]);
-    most = __builtin_fmaf(group4_max(most), scale_f, margin.margin);
+    most = group4_max(most) * scale_f;
     if (__any(most > m_run)) {
-        const float m_new = most > m_run ? most + margin.ahead : m_run;
+        const float m_new = most > m_run ? most + kAhead : m_run;
         const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
         l_run *= alpha;
 #pragma unroll
@@ -668,7 +666,7 @@ __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>
     }
     // (here, not earlier: behind the branch above the products above have left K's registers)
     refill();
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;
+    const float m_use = (m_run == -INFINITY ? 0.f : m_run) + margin;
     float p[4 * kSub];
     float sum = 0.f;
 #pragma unroll
@@ -868,8 +866,7 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
         for (int d = 0; d < D / 16; ++d)
             acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         float m_run = -INFINITY, l_run = 0.f;
-        Margin margin = kUsual;
-        const int32_t most_keys = keys_seen(a, req);
+        float margin = 0.f;
 
         auto step = [&](int32_t i, RawTile<kSub, S::kChunks>& now) {
             auto refill = [&]() {
@@ -886,7 +883,7 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
             for (int t = 0; t < kSub; ++t)
                 plain = plain & (now.place[t] >= 0);
             attend<D, kPieces, kSub>(now, key, plain, any, seen, a.scale_f, query, turned[wave], lane, acc, m_run, l_run,
-                                     margin, most_keys, refill);
+                                     margin, keys_seen(a, req), refill);
         };
         for (int32_t i = 0; i < tiles; i += kDepth) {
 #pragma unroll
@@ -900,7 +897,7 @@ __global__ void __launch_bounds__(kAttThreads, groups_per_cu(D)) mxfp4_attend_ke
         for (int d = 0; d < D / 16; ++d)
             *reinterpret_cast<f32x4_t*>(turned[wave] + r * S::kOPitch + 64 * d + 16 * g) = acc[d];
         if (g == 0) {
-            wave_m[wave][r] = m_run;
+            wave_m[wave][r] = m_run + margin;
             wave_l[wave][r] = l_run;
         }
         __syncthreads();

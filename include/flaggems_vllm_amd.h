@@ -781,7 +781,7 @@ int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t 
  * writes none), or whose query holds a NaN or an infinity (or, times softmax_scale
  * log2 e, a value of about 2^135 and more) and that sees a key, gets NaN (of values: in
  * that block's dims).  Keys count whose weight is above
- * 2^-122 of the row's largest, and where values pass 6 * 2^89 above n 2^-126 of
+ * 2^-122 of the row's largest, and where values pass 6 * 2^89 above n 2^-121 of
  * it, n the keys that a row sees; sums of values of any size stay finite.  Rows of q
  * outside query_start_loc's ranges are not written.
  *
