@@ -215,8 +215,9 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 // all tiles, one after the other, is dealt out evenly, so that workgroups have
 // the same to do whatever the lengths are; a tile that is longer than the
 // rest of its worker's share goes on with the next.  Otherwise a worker is a tile.
-// (The host sees to it that the cost fits 31 bits.  Starts that fall could make it
-// more; then nothing is computed.)
+// (The host sees to it that the cost fits 31 bits, and that whole tiles have a
+// workgroup each, for requests whose rows are their own.  Of requests that share rows
+// the cost may be more: past 31 bits nothing is computed, nor are more tiles than there are workgroups.)
 __device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int32_t rows_per_tile, int32_t unit_keys,
                                            Start& start) {
     if (a.workers == 0 && (a.num_reqs == 1 || !a.query_start_loc)) {
@@ -270,7 +271,7 @@ __device__ __forceinline__ bool find_start(const AttArgs& a, uint32_t index, int
         each = max((total + to - 1) / to, (uint32_t)kLeastCost);
     }
     uint64_t first = (uint64_t)each * index;
-    if (first >= total || total == ~0u)
+    if (first >= total || total > 0x7fffffffu)
         return false;
     if (a.workers == 0)
         first = total - 1 - first;  // from the end: of a prompt's tiles the last have the most keys

@@ -124,7 +124,10 @@ def mxfp4_paged_attention(
         seq_lens: int32 [R], each request's keys, the step's own tokens among them.
         softmax_scale: factor of q . k.
         query_start_loc: int32 [R + 1], the rows of q that are each request's: its
-            last tokens.  None: one token per request (T = R).
+            last tokens.  An end before its start is a request without tokens;
+            requests must not share rows (if some do, out and lse are undefined
+            in all rows of requests; nothing else is written).  None: one token
+            per request (T = R).
         max_query_len, max_seq_len: the most query tokens and keys of a request,
             as far as the caller knows them (T and W * block_size otherwise); they
             only choose how the work is cut.

@@ -769,7 +769,9 @@ int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t 
 /*
  * Causal attention of grouped heads over that cache.  Request b's query tokens are
  * q[query_start_loc[b] .. query_start_loc[b + 1]), the last of its seq_lens[b]
- * tokens (query_start_loc NULL: one token per request, num_tokens = num_reqs);
+ * tokens (query_start_loc NULL: one token per request, num_tokens = num_reqs).  A
+ * range that ends before it begins is empty, and ranges are cut to q's rows; they
+ * must not share rows (if they do, all rows of theirs may hold anything).  The
  * token at position p sees the keys j, p - window_size < j <= p (window_size 0: all
  * j <= p), j < max_blocks_per_req * block_size, whose block in block_table lies
  * in [0, num_blocks).  Head h reads key/value head h / (num_heads / num_kv_heads):
@@ -779,11 +781,11 @@ int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t 
  * and lse +inf.  A row that sees a key block of byte 255 or a value block of byte
  * 253 and up (bf16 does not hold such values, and fgv_mxfp4_kv_quant_and_cache
  * writes none), or whose query holds a NaN or an infinity (or, times softmax_scale
- * log2 e, a value of about 2^135 and more) and that sees a key, gets NaN (of values: in
- * that block's dims).  Keys count whose weight is above
- * 2^-122 of the row's largest, and where values pass 6 * 2^89 above n 2^-121 of
- * it, n the keys that a row sees; sums of values of any size stay finite.  Rows of q
- * outside query_start_loc's ranges are not written.
+ * log2 e, a value of about 2^135 and more) and that sees a key, gets NaN (of a value
+ * block: in its dims).  Keys count whose weight is above 2^-122 of the row's
+ * largest, and where values pass 6 * 2^89 above n 2^-121 of it, n the keys that a
+ * row sees; sums of values of any size stay finite.  Rows of q outside
+ * query_start_loc's ranges are not written.
  *
  *   q, out  [num_tokens, num_heads, D] bf16 (dtype 0) or fp16 (1), unit last
  *         stride; lse [num_tokens, num_heads] float32, unit last stride.

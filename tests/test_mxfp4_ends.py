@@ -196,3 +196,38 @@ def test_gpu_insert_in_more_workgroups_than_a_launch_has():
     fv.mxfp4_kv_quant_and_cache(k.expand(tokens, -1, -1), v.expand(tokens, -1, -1), cache, slots.to(k.device))
     torch.cuda.synchronize()
     assert torch.equal(cache.cpu(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("starts", [[20, 120, 70, 170], [20, 170, 20, 170, 20, 170], [170, 20, 170, 20, 100, 60, 170]])
+def test_gpu_requests_that_share_rows(dim, starts):
+    """More tiles than the launch has workgroups for, whole and dealt out: rows of no request stay, and the next call is as
+    ever."""
+    reqs = len(starts) - 1
+    for lens in ([60] * reqs, [5000] * reqs):
+        c = Case(55, lens, [50] * reqs, heads=8, kv_heads=2, dim=dim)
+        want = c.check(max_query_len=50)
+        q = torch.cat([c.q, c.q])[:190].contiguous()
+        out = torch.full_like(q, 7.0)
+        for most in (1, 50, 190):
+            print(f"\n[case] shared rows {dim} {starts} {lens[0]} {most}", flush=True)
+            fv.mxfp4_paged_attention(q, c.cache, c.table, c.lens, c.scale, max_query_len=most, out=out,
+                                     query_start_loc=torch.tensor(starts, dtype=torch.int32, device=q.device))
+            torch.cuda.synchronize()
+            assert bool((out[:20] == 7).all()) and bool((out[170:] == 7).all())
+        for x, y in zip(c.run(max_query_len=50), want):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_gpu_starts_that_fall_to_nothing():
+    """A batch padded with starts of 0, or of any row: those requests have no tokens, and the others what is theirs."""
+    c = Case(56, [300, 64, 500], [30, 2, 70])
+    want = c.check(max_query_len=70)
+    for pad in ([0, 0, 0], [101, 3, 3], [102, 0, 0]):
+        table = torch.cat([c.table, c.table])
+        out, lse = fv.mxfp4_paged_attention(
+            c.q, c.cache, table, torch.cat([c.lens, c.lens]), c.scale, max_query_len=70,
+            query_start_loc=torch.cat([c.start, torch.tensor(pad, dtype=torch.int32, device=table.device)]))
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
