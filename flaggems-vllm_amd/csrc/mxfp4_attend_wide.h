@@ -15,15 +15,17 @@
 // bf16's 8 bits of P would put as large an error beside the output's rounding
 // again, and a second piece another half of PV's time.  Value blocks beyond
 // fp16's range (half_holds) are left to a second loop in bf16 with two pieces,
-// which the first one enters at the first tile that holds one.
+// which the first one enters at the first 64 keys that hold one, for all keys
+// behind them: a single block among 16384 keys takes the call below from 487 us to
+// 660 if it stands in the middle, and to 854 at the first key.
 //
 // A wave's matrix instructions of a tile take 1026 cycles (D = 128, bf16 calls), its
 // vector instructions 1180 (exp2 among them), and the two overlap only where other
 // instructions stand between them in the stream: so V's conversion goes between
 // QK's, the second half's exponentials between PV's for the first, loads are asked
-// for a tile (V: two) ahead.  2048 tokens behind 14336 keys, 32 heads of 128: 472 us,
-// 515 GFLOP at 1090 TFLOP/s, matrix units busy half of the time, vector issue somewhat
-// more; QK, softmax and PV one after the other took 610, 16-row tiles 1083.
+// for a tile (V: two) ahead.  2048 tokens behind 14336 keys, 32 heads of 128: 484 to 495 us
+// (by the card), 515 GFLOP at 1040 to 1065 TFLOP/s, matrix units busy half of the time, vector
+// issue somewhat more; QK, softmax and PV one after the other took 610, 16-row tiles 1083.
 #pragma once
 
 namespace fgv {

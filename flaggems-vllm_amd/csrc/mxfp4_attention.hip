@@ -19,10 +19,14 @@
 // QK: the matrix instruction reads the cache's own format.  K's codes go from
 // memory into the A registers of v_mfma_scale_f32_16x16x128_f8f6f4, the UE8M0
 // bytes are its scales, and nothing is dequantised.  The query is the B
-// operand in e4m3, exactly: divided by a power of two per row that puts the
-// row's maximum into [128, 256), its 8 (bf16) or 11 (fp16) bits split into 2
-// or 3 e4m3 pieces of 4, each under a scale 2^-4 smaller.  What values far
-// below their row's maximum lose is under 2^-16 (2^-20) of that maximum.  Register
+// operand in e4m3: divided by a power of two per row that puts the row's
+// maximum into [128, 256), its 8 (bf16) or 11 (fp16) bits split into 2 or 3
+// e4m3 pieces of 4, each under a scale 2^-4 smaller.  Values near their row's
+// maximum are held whole; what values far below it lose is under 2^-16 (2^-20) of
+// that maximum.  With the products that the instruction cuts (take_piece) that
+// leaves scores of normal queries and keys an error of 1e-6 to 5e-6 rms (fp16: 1e-7 to
+// 4e-7; D = 256 to 64), which lse carries: up to 2.2e-4 of 5 to 8 in 128 windows of
+// 1000 keys, heads of 64; 3e-5 in 64 requests, heads of 128.  Register
 // images (measured; the tests pin them through the results): lane (r, g) =
 // (l % 16, l / 16) holds of A k = 32g..32g+31 of key r, of B k = 16g..16g+15
 // and 64+16g..64+16g+15 of row r; scales apply to k = 32g..32g+31; D holds
@@ -38,9 +42,10 @@
 // Two kernels: 16-row tiles, whose waves share out the keys (here; single tokens,
 // a few of them, and D = 256), and 128-row tiles, whose waves share out the rows
 // (mxfp4_attend_wide.h).  Single tokens are bound by the cache's bytes, once there
-// are many: 64 requests of up to 8191 keys, 199 MB, 50 us, of it 5 for joining
-// cuts; 1 x 131072 keys, 143 MB, 39 us.  In front of that stand some 10 us of latency:
-// launch, lengths, block table and first keys each wait for the one before.
+// are many: 64 requests of up to 8191 keys, 199 MB, 51 us, of it 4 to 5 for joining
+// cuts; 1 x 131072 keys, 143 MB, 38.4 us, of it 5 to 6.  In front of the bytes stand some 6 us
+// of latency (1 x 16 keys takes 6.2 us in all, 64 requests of 16 keys, with the plan,
+// 7.9): launch, lengths, block table and first keys each wait for the one before.
 #include <math.h>
 
 #include "fgv_device.h"
@@ -66,8 +71,11 @@ constexpr int kMostWorkers = 1024;  // per head
 // much as this many more, so that a worker of many short tiles gets fewer units.
 constexpr int kTileCost = 4;
 constexpr int kLeastCost = kTileCost + 1;  // what a worker takes at least
-// Tiles of no more units than this are not cut: joining cuts takes a launch, 4 us (128 windows of 1000 keys, 9 units:
-// 27.7 us whole, 30.4 cut).
+// Tiles of no more units than this are not cut: joining cuts takes a launch, 4 us.  Cut and whole, D = 128, 4 query heads
+// to a key head: 8 tiles of 8 units 14.0 and 11.9 us, of 10 14.0 and 13.7, of 12 14.0 and 15.4; 64 tiles of 10 14.8 and
+// 15.0, of 12 14.9 and 16.7; 512 tiles of 10 23.4 and 21.2, of 16 35.3 and 32.9.  D = 64: 8 tiles of 10 13.1 and 12.3, of 12
+// 13.2 and 14.1.  D = 256: 8 tiles of 8 20.5 and 19.5, of 10 20.5 and 22.0; 128 tiles of 10 25.9 and 23.1.  128 windows of
+// 1000 keys, 1024 tiles of 9, D = 64: 30.4 and 27.8.  (Few tiles of D = 256 would be cut from 9 units on, many of any D later.)
 constexpr int kWholeUnits = 10;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -1172,8 +1180,10 @@ Dealing dealing_of(const Call& c, bool wide) {
     // of 1140 tiles on 512 workgroups took 151 us with cuts, which leave no workgroup idle, and 108 without.
     if (workers < 2 || c.max_keys <= kWholeUnits * unit || (wide && (d.tiles - c.reqs) * c.kv_heads >= 2 * slots))
         return d;
-    // One request's tiles, much alike, in (nearly) whole turns of the chip (2048 tokens behind 14336 keys, 512 tiles on as
-    // many workgroups: 502 us dealt out, 10 of it for finding nothing to join; 472 whole, the longest first).
+    // One request's tiles, much alike, in (nearly) whole turns of the chip, the longest first.  Dealt out and whole, 32 heads
+    // of 128, 512 workgroups: behind 14336 keys 512 tiles (2048 tokens) 500 and 483 us, 488 tiles 511 and 472, 472 tiles 491
+    // and 461, 384 tiles 394 and 437, 520 tiles 545 and 726, 960 tiles 1038 and 953.  Behind 2048 keys whole is ahead at any
+    // number (256 tiles 79 and 76, 384 119 and 92, 512 128 and 112, 576 183 and 165), which this rule does not know.
     const int64_t turns = (d.tiles * c.kv_heads + slots - 1) / slots;
     if (wide && c.reqs == 1 && 20 * d.tiles * c.kv_heads >= 19 * turns * slots)
         return d;

@@ -726,7 +726,9 @@ int64_t fgv_int8_scaled_mm_workspace_bytes(const int8_t* a, int64_t a_stride, co
  *       ceil(context / page) .. ceil(seq_len / page) - 1, as far as they are below
  *       W, get blocks from the top of the stack free_blocks[0 .. num_free), in the
  *       order of requests and columns (free_blocks[num_free - 1] first), and -1
- *       once it is empty; other columns are left as they are;
+ *       once it is empty; other columns are left as they are (a later call counts
+ *       a column of -1 among those that the context holds and does not fill it, and
+ *       no call puts blocks back on the stack: both are the caller's);
  *   positions [max_num_tokens] int64: context + i of token i of a request;
  *   slot_mapping [max_num_tokens] int64: block * page + position % page, block out
  *       of the table; pad_id where that is negative or the column is not below W;
@@ -786,6 +788,12 @@ int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t 
  * largest, and where values pass 6 * 2^89 above n 2^-121 of it, n the keys that a
  * row sees; sums of values of any size stay finite.  Rows of q outside
  * query_start_loc's ranges are not written.
+ * Scores, and with them lse, have fewer than 32 bits: a bf16 query is held to 2^-16
+ * of its row's largest value (fp16: 2^-20), and of 32 products that are added at
+ * once bits below 2^-13 of the largest are cut, which for normal queries and keys is
+ * an error of 1e-6 to 5e-6 rms (fp16: 1e-7 to 4e-7).  A weight has 16 bits, in bf16
+ * calls 11 where a request has more than 64 rows (tokens times heads of a key head)
+ * and head_dim is at most 128; weights below 2^-28 of the row's largest are nothing there.
  *
  *   q, out  [num_tokens, num_heads, D] bf16 (dtype 0) or fp16 (1), unit last
  *         stride; lse [num_tokens, num_heads] float32, unit last stride.
