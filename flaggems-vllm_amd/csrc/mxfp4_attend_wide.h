@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
     __shared__ __align__(16) uint8_t turned[2][S::kVBytes];
     __shared__ __align__(16) uint32_t held_by[2][kAttWaves];  // whether fp16 holds each wave's values
     __shared__ uint64_t nan_of[2][kAttWaves];                 // which of its value blocks are NaN, bit by lane
-    __shared__ __align__(16) uint32_t large_of[2][kAttWaves];  // whether it has values under bytes past kLargeByte
+    __shared__ __align__(16) uint32_t large_of[2][kAttWaves];  // their largest byte, if it is past kLargeByte
     using Rows = WideQuery<D, kPieces>;
     __shared__ uint4 more_query[kAttWaves][Rows::kInLds ? 64 * Rows::kInLds : 1];  // the pieces not in registers
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
             } else {
                 nan_of[buffer][wave] = __ballot(byte > kMostByte);
                 byte = byte > kMostByte ? 0 : byte;
-                large_of[buffer][wave] = __any(byte > kLargeByte);
+                large_of[buffer][wave] = __any(byte > kLargeByte) ? wave_largest(byte) : 0;
             }
             return __uint_as_float(byte << 23);
         };
@@ -483,9 +483,11 @@ __global__ void __launch_bounds__(kAttThreads, 2) mxfp4_attend_wide_kernel(AttAr
             const float top = pair_max(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]))) * a.scale_f;
             if constexpr (!kFast) {
                 const uint4 large = *reinterpret_cast<const uint4*>(large_of[buffer]);
-                if (margin == 0.f && __builtin_amdgcn_readfirstlane(large.x | large.y | large.z | large.w)) {
-                    margin = large_margin(keys_seen(a, req));
-                    const float down = __builtin_amdgcn_exp2f(-margin);
+                const uint32_t largest = __builtin_amdgcn_readfirstlane(max(max(large.x, large.y), max(large.z, large.w)));
+                const float more = largest > 0 ? large_margin(keys_seen(a, req), largest) : 0.f;
+                if (more > margin) {
+                    const float down = __builtin_amdgcn_exp2f(margin - more);
+                    margin = more;
                     l_run *= down;
 #pragma unroll
                     for (int d = 0; d < D / 32; ++d)

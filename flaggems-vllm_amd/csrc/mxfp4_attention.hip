@@ -82,18 +82,27 @@ constexpr float kLn2 = 0.6931471805599453f;
 // A row's reference is raised when a score exceeds it, and then to this much
 // above the score (base 2), so that most tiles rescale nothing.  P is at most 1.
 constexpr float kAhead = 4.0f;
+// The last scale byte of values: above it they are NaN.
+constexpr uint32_t kMostByte = 252;
 // Sums of P v over 2^30 keys stay finite with P at most 1 for values under bytes up to kLargeByte
 // (6 * 2^89).  Once a wave meets larger ones, up to 6 * 2^125, P and its sums are taken under a
-// reference that is large_margin higher: P is below 1 / n, n the keys that a row may see.  (Nothing
-// is P below 2^-126: below n 2^-121 of the row's largest there, 2^-122 otherwise.)
+// reference that is large_margin higher: by as many binades as a sum over the `keys` that a row
+// may see could pass 6 * 2^125 by.  (Nothing is P below 2^-126: 2^-122 of the row's largest, and so much more there.)
 constexpr uint32_t kLargeByte = 216;
-__device__ __forceinline__ float large_margin(int32_t keys) { return (float)(32 - __builtin_clz((uint32_t)keys | 1u)); }
+__device__ __forceinline__ float large_margin(int32_t keys, uint32_t byte) {
+    return (float)max(32 - __builtin_clz((uint32_t)keys | 1u) + (int)byte - (int)kMostByte, 0);
+}
+// The wave's largest byte, some being past kLargeByte (step by step: such tiles are rare, and what
+// moves between lanes would take registers in all of them).
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
+    uint32_t most = kMostByte;
+    while (most > kLargeByte && !__any(v >= most))
+        --most;
+    return most;
+}
 // References farther from 0 are rounded by more than the one below which a score that is not
 // rounded may lie: there both are.
 constexpr float kFar = 1 << 20;
-
-// The last scale byte of values: above it they are NaN.
-constexpr uint32_t kMostByte = 252;
 
 // 16-key subtiles that a wave takes at a time: two such tiles have to fit its registers.
 __host__ __device__ constexpr int key_subtiles(int) { return 2; }
@@ -571,8 +580,8 @@ constexpr int32_t kNoKey = 0x7ff80000;  // seen by nobody: behind the longest re
 // them are seen by all rows; otherwise, and where values are large or NaN, some may be
 // hidden, hold anything or be NaN.  (One body for both: with two, the compiler keeps two sets of sums.)
 //
-// `margin` is 0, and from the first large values on large_margin of `most_keys`, which a row
-// sees at most; sums are under the reference m_run + margin.
+// `margin` is large_margin of the largest values so far and `most_keys`, which a row sees at
+// most; sums are under the reference m_run + margin.
 //
 // `refill` loads the next tile into `raw` as soon as this one has left it, for
 // the matrix instruction and for LDS.
@@ -621,13 +630,16 @@ __device__ __forceinline__ void attend(RawTile<kSub, Shape<D, kPieces>::kChunks>
                 largest = max(largest, raw.vs[t][c]);
             }
         }
-        if (margin == 0.f && __any(largest > kLargeByte)) {
-            margin = large_margin(most_keys);
-            const float down = __builtin_amdgcn_exp2f(-margin);
-            l_run *= down;
+        if (__any(largest > kLargeByte)) {
+            const float more = large_margin(most_keys, wave_largest(largest));
+            if (more > margin) {
+                const float down = __builtin_amdgcn_exp2f(margin - more);
+                margin = more;
+                l_run *= down;
 #pragma unroll
-            for (int d = 0; d < D / 16; ++d)
-                acc[d] *= down;
+                for (int d = 0; d < D / 16; ++d)
+                    acc[d] *= down;
+            }
         }
     }
 

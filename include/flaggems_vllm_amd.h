@@ -785,9 +785,9 @@ int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t 
  * writes none), or whose query holds a NaN or an infinity (or, times softmax_scale
  * log2 e, a value of about 2^135 and more) and that sees a key, gets NaN (of a value
  * block: in its dims).  Keys count whose weight is above 2^-122 of the row's
- * largest, and where values pass 6 * 2^89 above n 2^-121 of it, n the keys that a
- * row sees; sums of values of any size stay finite.  Rows of q outside
- * query_start_loc's ranges are not written.
+ * largest; where the row's number of keys times the largest value passes 2^127, above
+ * 2^-122 times as much as it passes it by, so that sums of values of any size stay
+ * finite.  Rows of q outside query_start_loc's ranges are not written.
  * Scores, and with them lse, have fewer than 32 bits: a bf16 query is held to 2^-16
  * of its row's largest value (fp16: 2^-20), and of 32 products that are added at
  * once bits below 2^-13 of the largest are cut, which for normal queries and keys is

@@ -231,3 +231,23 @@ def test_gpu_starts_that_fall_to_nothing():
             c.q, c.cache, table, torch.cat([c.lens, c.lens]), c.scale, max_query_len=70,
             query_start_loc=torch.cat([c.start, torch.tensor(pad, dtype=torch.int32, device=table.device)]))
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("query", [None, [70]])
+def test_gpu_small_weights_of_large_values(dtype, dim, query):
+    """One key's score 118 binades above all others, and its values 0: what the others' weights leave of values of 6 * 2^103 is
+    the output, also where their sum could never pass the range."""
+    c = Case(57, [700], query, heads=2, kv_heads=2, dim=dim, dtype=dtype)
+    kc, vc, ks, vs = parts(c.cache)
+    live = c.table[0, :-(-700 // 16)].long()
+    kc[live], vc[live], ks[live], vs[live] = 0, 0x77, 127, 230
+    one = int(c.table[0, 0])
+    kc[one, :, 5, 0], vc[one, :, 5] = 0x07, 0  # 6 in dim 0
+    c.q.zero_()
+    c.q[:, :, 0] = 13.625  # 6 * 13.625 = 117.9 ln 2
+    c.scale = 1.0
+    out, _ = c.check(max_query_len=max(query or [1]))
+    assert bool((out > 0.1).all())
