@@ -251,3 +251,22 @@ def test_gpu_small_weights_of_large_values(dtype, dim, query):
     c.scale = 1.0
     out, _ = c.check(max_query_len=max(query or [1]))
     assert bool((out > 0.1).all())
+
+
+@pytest.mark.gpu
+def test_gpu_columns_without_a_block_stay_and_blocks_come_back_by_the_caller():
+    """What a step that ran out leaves behind, as the next steps see it; a finished request's blocks put back on the stack."""
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    table, free = torch.full((2, 6), -1, dtype=torch.int32, device="cuda"), i32(10, 11, 12, 13)
+    _, lens, _, slots, left = fv.build_block_tables(i32(0, 0), i32(40, 40), table, free, i32(4), 16, 80)
+    assert table[:, :3].tolist() == [[13, 12, 11], [10, -1, -1]] and left.tolist() == [-2]
+    assert (slots >= 0).sum().item() == 56
+    # the first request ends: its blocks go back behind what is left (a negative count as 0)
+    free[:3], left = table[0, :3].clone(), i32(3)
+    _, lens, _, slots, left = fv.build_block_tables(i32(0, 40), i32(0, 9), table, free, left, 16, 9)
+    assert table[1].tolist() == [10, -1, -1, 11, -1, -1] and left.tolist() == [2] and lens.tolist() == [0, 49]
+    assert slots.tolist() == [-1] * 8 + [11 * 16]
+    # taken back to the length that its blocks hold, it goes on
+    _, lens, _, slots, left = fv.build_block_tables(i32(0, 16), i32(0, 20), table, free, left, 16, 20)
+    assert table[1, :3].tolist() == [10, 12, 13] and left.tolist() == [0]
+    assert slots.tolist() == [12 * 16 + i for i in range(16)] + [13 * 16 + i for i in range(4)]
