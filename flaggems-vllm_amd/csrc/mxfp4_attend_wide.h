@@ -23,8 +23,8 @@
 // vector instructions 1180 (exp2 among them), and the two overlap only where other
 // instructions stand between them in the stream: so V's conversion goes between
 // QK's, the second half's exponentials between PV's for the first, loads are asked
-// for a tile (V: two) ahead.  2048 tokens behind 14336 keys, 32 heads of 128: 484 to 495 us
-// (by the card), 515 GFLOP at 1040 to 1065 TFLOP/s, matrix units busy half of the time, vector
+// for a tile (V: two) ahead.  2048 tokens behind 14336 keys, 32 heads of 128: 475 to 495 us
+// (by the card), 515 GFLOP at 1040 to 1085 TFLOP/s, matrix units busy half of the time, vector
 // issue somewhat more; QK, softmax and PV one after the other took 610, 16-row tiles 1083.
 #pragma once
 

@@ -774,8 +774,8 @@ int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t 
  * tokens (query_start_loc NULL: one token per request, num_tokens = num_reqs).  A
  * range that ends before it begins is empty, and ranges are cut to q's rows; they
  * must not share rows (if they do, all rows of theirs may hold anything).  The
- * token at position p sees the keys j, p - window_size < j <= p (window_size 0: all
- * j <= p), j < max_blocks_per_req * block_size, whose block in block_table lies
+ * token at position p sees the keys j, p - window_size < j <= p (window_size 0, or
+ * 2^30 - 1 and more: all j <= p), j < max_blocks_per_req * block_size, whose block in block_table lies
  * in [0, num_blocks).  Head h reads key/value head h / (num_heads / num_kv_heads):
  *   lse = ln sum_j exp(softmax_scale q . k_j)
  *   out = sum_j exp(softmax_scale q . k_j) v_j / (exp(lse) + exp(attn_sink[h]))
@@ -788,7 +788,8 @@ int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t 
  * largest; where the row's number of keys times the largest value passes 2^127, above
  * 2^-122 times as much as it passes it by, so that sums of values of any size stay
  * finite.  Rows of q outside query_start_loc's ranges are not written.
- * Scores, and with them lse, have fewer than 32 bits: a bf16 query is held to 2^-16
+ * Scores have to lie in binary32's range (one past it, with its sign, makes the row
+ * NaN or counts for nothing).  They, and lse with them, have fewer than 32 bits: a bf16 query is held to 2^-16
  * of its row's largest value (fp16: 2^-20), and of 32 products that are added at
  * once bits below 2^-13 of the largest are cut, which for normal queries and keys is
  * an error of 1e-6 to 5e-6 rms (fp16: 1e-7 to 4e-7).  A weight has 16 bits, in bf16
