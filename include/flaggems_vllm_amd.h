@@ -775,8 +775,9 @@ int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t 
  * range that ends before it begins is empty, and ranges are cut to q's rows; they
  * must not share rows (if they do, all rows of theirs may hold anything).  The
  * token at position p sees the keys j, p - window_size < j <= p (window_size 0, or
- * 2^30 - 1 and more: all j <= p), j < max_blocks_per_req * block_size, whose block in block_table lies
- * in [0, num_blocks).  Head h reads key/value head h / (num_heads / num_kv_heads):
+ * 2^30 - 1 and more: all j <= p), j < max_blocks_per_req * block_size, whose block
+ * in block_table lies in [0, num_blocks).  Head h reads key/value head
+ * h / (num_heads / num_kv_heads):
  *   lse = ln sum_j exp(softmax_scale q . k_j)
  *   out = sum_j exp(softmax_scale q . k_j) v_j / (exp(lse) + exp(attn_sink[h]))
  * (attn_sink NULL: none; it does not enter lse).  A row that sees nothing gets out 0
@@ -789,12 +790,14 @@ int fgv_mxfp4_kv_quant_and_cache(const void* k, int64_t k_stride_token, int64_t 
  * 2^-122 times as much as it passes it by, so that sums of values of any size stay
  * finite.  Rows of q outside query_start_loc's ranges are not written.
  * Scores have to lie in binary32's range (one past it, with its sign, makes the row
- * NaN or counts for nothing).  They, and lse with them, have fewer than 32 bits: a bf16 query is held to 2^-16
- * of its row's largest value (fp16: 2^-20), and of 32 products that are added at
- * once bits below 2^-13 of the largest are cut, which for normal queries and keys is
- * an error of 1e-6 to 5e-6 rms (fp16: 1e-7 to 4e-7).  A weight has 16 bits, in bf16
- * calls 11 where a request has more than 64 rows (tokens times heads of a key head)
- * and head_dim is at most 128; weights below 2^-28 of the row's largest are nothing there.
+ * NaN or counts for nothing).  They, and lse with them, have fewer than 32 bits: a
+ * bf16 query is held to 2^-16 of its row's largest value (fp16: 2^-20), and of 32
+ * products that are added at once bits below 2^-13 of the largest are cut, which for
+ * normal queries and keys is an error of 1e-6 to 5e-6 rms (fp16: 1e-7 to 4e-7).
+ * Weights have 16 bits.  Where head_dim is at most 128 and a request has more than 64
+ * rows (tokens times heads of a key head; the others of a call of few requests
+ * share its tiles), they have 11 in bf16 calls, and in both types those below 2^-28
+ * of the row's largest may be nothing.
  *
  *   q, out  [num_tokens, num_heads, D] bf16 (dtype 0) or fp16 (1), unit last
  *         stride; lse [num_tokens, num_heads] float32, unit last stride.
